@@ -412,7 +412,8 @@ def _err_word() -> torch.Tensor:
     return torch.zeros(1, dtype=torch.int32, device=device())
 
 
-_ERRORS = {1: "a lookup index outside its table", 2: "a softmax row sum of zero (round_div by zero)"}
+_ERRORS = {1: "a lookup index outside its table", 2: "a softmax row sum of zero (round_div by zero)",
+           8: "a value outside the range of the single-token kernels", 16: "a full key / value cache"}
 
 
 def _check_err(err: torch.Tensor, what: str):

@@ -1,0 +1,830 @@
+// decode.cu -- the forward of single tokens: what a step of generation needs
+// of the op layer, for a few rows instead of a whole sequence, with every
+// result bit-identical to the same row of the graph's forward_ops.
+//
+// - k_q4_pack / k_q4_project: Op::Projection and Op::MatMul for a few rows by
+//   a weight in 4 bits with group scales (q4.cuh), the rounding, bias,
+//   activation table and residual in its epilogue;
+// - k_kv_append / k_kv_attend: one new token per sequence against a cache of
+//   the keys and values (Scale, MatMul, Scale, StableSoftmaxIndex, Softmax,
+//   MatMul, Scale of one row);
+// - k_choose_token: penalties, bias and mask on the logits and Op::Argmax.
+//
+// Tensors are rows of field elements as everywhere in the op layer.  Data
+// outside what a kernel takes sets a bit of the caller's error word
+// (kErrIndex, kErrDivide, kErrRange, kErrFull) and the pass carries on.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/zkie2.h"
+#include "common.cuh"
+#include "fixed.cuh"
+#include "gl64.cuh"
+#include "q4.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace zk {
+
+namespace {
+
+constexpr uint32_t kErrIndex = 1u;
+constexpr uint32_t kErrDivide = 2u;
+constexpr uint32_t kErrFull = 16u;  // a cache without room for the new token
+constexpr int kSms = 148;
+constexpr size_t kMaxShared = 227 * 1024;
+
+// ---- the weight ---------------------------------------------------------------------------
+// codes (e x k x n, int8) and scales (e x rows x n, int32; ceil(k_seg / G)
+// rows to a segment) into blocks: one thread per output word
+__global__ void k_q4_pack(const int8_t* __restrict__ codes, const int32_t* __restrict__ scales, uint32_t experts,
+                          Q4Shape s, uint32_t* __restrict__ packed, uint32_t* __restrict__ pscales,
+                          uint32_t* __restrict__ err) {
+    const uint64_t stride = (uint64_t)gridDim.x * blockDim.x, first = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t per = (uint64_t)s.tiles * s.blocks * 128;
+    const uint32_t seg_blocks = s.kp_seg / 64;
+    bool bad = false;
+    for (uint64_t i = first; i < per * experts; i += stride) {
+        const uint64_t ex = i / per;
+        uint64_t r = i % per;
+        const uint32_t q = r & 3, lane = (r >> 2) & 31;
+        r >>= 7;
+        const uint32_t block = (uint32_t)(r % s.blocks), tile = (uint32_t)(r / s.blocks);
+        const uint32_t g = lane >> 2, t = lane & 3, n = tile * 16 + g + 8 * (q & 1);
+        const uint32_t seg = block / seg_blocks;
+        uint32_t word = 0;
+        for (int j = 0; j < 4; j++)
+            for (int h = 0; h < 2; h++) {
+                const uint32_t k = (block % seg_blocks) * 64 + 32 * h + 8 * t + 4 * (q >> 1) + j;
+                int c = 0;
+                if (k < s.k_seg && n < s.n) c = codes[(ex * s.k + (uint64_t)seg * s.k_seg + k) * s.n + n];
+                if (c < -8 || c > 7) {
+                    bad = true;
+                    c = 0;
+                }
+                word |= (uint32_t)(c & 15) << (8 * j + 4 * h);
+            }
+        packed[i] = word;
+    }
+    const uint64_t sper = (uint64_t)s.tiles * s.groups * 8;
+    const uint32_t seg_groups = s.kp_seg / s.group, rows = (s.k_seg + s.group - 1) / s.group;
+    for (uint64_t i = first; i < sper * experts; i += stride) {
+        const uint64_t ex = i / sper, r = i % sper;
+        const uint32_t g = r & 7, grp = (uint32_t)((r >> 3) % s.groups), tile = (uint32_t)((r >> 3) / s.groups);
+        const uint32_t seg = grp / seg_groups, in = grp % seg_groups;
+        uint32_t word = 0;
+        for (int h = 0; h < 2; h++) {
+            const uint32_t n = tile * 16 + g + 8 * h;
+            int64_t v = 0;
+            if (in < rows && n < s.n) v = scales[(ex * s.segs * rows + (uint64_t)seg * rows + in) * s.n + n];
+            if (v < 0 || v > 0xFFFF) {
+                bad = true;
+                v = 0;
+            }
+            word |= (uint32_t)v << (16 * h);
+        }
+        pscales[i] = word;
+    }
+    if (bad) atomicOr(err, kErrRange);
+}
+
+// ---- the product ----------------------------------------------------------------------------
+constexpr int kProjThreads = 256;
+constexpr int kProjWarps = kProjThreads / 32;
+
+struct ProjectArgs {
+    const uint64_t* x;
+    uint64_t ldx;
+    uint32_t m;
+    const uint4* codes;
+    const uint32_t* scales;
+    Q4Shape s;
+    uint32_t shift;
+    const uint64_t* bias;
+    const uint64_t* table;
+    uint64_t table_len;
+    int64_t offset;
+    const uint64_t* residual;
+    uint64_t ldr;
+    uint64_t* out;
+    uint32_t* err;
+    uint32_t split;   // warps that share a tile of 16 columns
+    uint32_t stride;  // bytes of a digit row in shared memory
+};
+
+// One block: 2 NT rows of x as digits in shared memory; its warps stream the
+// tiles of 16 columns, `split` warps to a tile, each a part of K (whole
+// segments where each segment is rounded by itself); their 64-bit sums meet
+// in shared memory, and a thread per output rounds and finishes it.
+template <int G, int NT, bool SEG>
+__global__ void __launch_bounds__(kProjThreads, 2) k_q4_project(const ProjectArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int kRows = 2 * NT;
+    const uint32_t row0 = blockIdx.y * kRows, rows = min((uint32_t)kRows, p.m - row0);
+    uint8_t* digits = smem;
+    long long* red = reinterpret_cast<long long*>(smem + (size_t)kRows * 4 * p.stride);
+    const uint32_t kp = p.s.blocks * 64, quads = kp / 4;
+    bool bad = false;
+    for (uint32_t i = threadIdx.x; i < rows * quads; i += kProjThreads) {
+        const uint32_t r = i / quads, k0 = (i % quads) * 4;
+        const uint32_t seg = SEG ? k0 / p.s.kp_seg : 0, in = SEG ? k0 % p.s.kp_seg : k0;
+        const uint64_t* xr = p.x + (row0 + r) * p.ldx + seg * p.s.k_seg + in;
+        uint32_t d[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t v = in + j < p.s.k_seg ? fx_to_i64(__ldg(xr + j)) : 0;
+            bad |= !q4_digits(v, &d[j]);
+        }
+        uint8_t* to = digits + (size_t)r * 4 * p.stride + q4_pos(k0);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t lo = __byte_perm(d[0], d[1], q | ((4 + q) << 4));
+            const uint32_t hi = __byte_perm(d[2], d[3], q | ((4 + q) << 4));
+            *reinterpret_cast<uint32_t*>(to + (size_t)q * p.stride) = __byte_perm(lo, hi, 0x5410);
+        }
+    }
+    if (bad) atomicOr(p.err, kErrRange);
+    __syncthreads();
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t per = kProjWarps / p.split, mine = warp / p.split, part = warp % p.split;
+    const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
+    const uint32_t b0 = part * units / p.split * unit, b1 = (part + 1) * units / p.split * unit;
+    const uint8_t* from = digits + (size_t)g * p.stride + 16 * t;  // column g: digit g % 4 of row g / 4
+    uint32_t flip = 0;
+    for (uint32_t group = blockIdx.x; group * per < p.s.tiles; group += gridDim.x, flip ^= 1) {
+        const uint32_t tile = group * per + mine;
+        if (tile < p.s.tiles) {
+            const uint4* codes = p.codes + (uint64_t)tile * p.s.blocks * 32 + lane;
+            const uint32_t* scales = p.scales + (uint64_t)tile * p.s.groups * 8;
+            Q4Sum<NT> sum;
+            sum.clear();
+            long long total[NT][2];
+#pragma unroll
+            for (int i = 0; i < NT; i++) total[i][0] = total[i][1] = 0;
+            for (uint32_t b = b0; b < b1; b += 4) {
+                uint4 w[4];
+                uint32_t s0[4], s1[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (b + j < b1) {
+                        w[j] = ldg_stream(codes + (uint64_t)(b + j) * 32);
+                        q4_scales<G>(scales, b + j, g, &s0[j], &s1[j]);
+                    }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (b + j < b1) {
+                        uint4 x[NT];
+#pragma unroll
+                        for (int i = 0; i < NT; i++)
+                            x[i] = *reinterpret_cast<const uint4*>(from + (size_t)i * 8 * p.stride + (b + j) * 64);
+                        q4_block<G, NT>(sum, w[j], s0[j], s1[j], x, (b + j) & 1);
+                        if (SEG && (b + j + 1) % unit == 0) {
+#pragma unroll
+                            for (int i = 0; i < NT; i++) {
+                                long long v0, v1;
+                                sum.finish(i, &v0, &v1);
+                                total[i][0] += fx_round_div_pow2(v0, p.shift);
+                                total[i][1] += fx_round_div_pow2(v1, p.shift);
+                            }
+                            sum.clear();
+                        }
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                if (!SEG) sum.finish(i, &total[i][0], &total[i][1]);
+                if (!(t & 1)) {
+                    long long* to = red + ((size_t)(flip * kProjWarps + warp) * kRows + 2 * i + (t >> 1)) * 16;
+                    to[g] = total[i][0];
+                    to[g + 8] = total[i][1];
+                }
+            }
+        }
+        __syncthreads();
+        for (uint32_t o = threadIdx.x; o < per * rows * 16; o += kProjThreads) {
+            const uint32_t c = o & 15, which = (o >> 4) % per, r = (o >> 4) / per;
+            const uint64_t n = (uint64_t)(group * per + which) * 16 + c;
+            if (n >= p.s.n) continue;
+            uint64_t v = 0;
+            for (uint32_t w = 0; w < p.split; w++)
+                v += (uint64_t)red[((size_t)(flip * kProjWarps + which * p.split + w) * kRows + r) * 16 + c];
+            int64_t y = SEG ? (int64_t)v : fx_round_div_pow2((int64_t)v, p.shift);
+            if (p.bias) y = fx_wadd(y, fx_to_i64(__ldg(p.bias + n)));
+            uint64_t f = p.table ? gl_canon(table_at(p.table, p.table_len, y, p.offset)) : fx_from_i64(y);
+            if (p.residual) f = gl_canon(gl_add(f, gl_canon(__ldg(p.residual + (row0 + r) * p.ldr + n))));
+            p.out[(row0 + r) * (uint64_t)p.s.n + n] = f;
+        }
+    }
+}
+
+uint32_t digit_stride(uint32_t blocks) {
+    const uint32_t kp = blocks * 64;
+    return kp % 128 ? kp : kp + 64;  // 64 mod 128: the eight lanes of a phase read 128 different bytes
+}
+
+template <int G, int NT, bool SEG>
+int project_launch(ProjectArgs p, cudaStream_t stream) {
+    const size_t shared = (size_t)2 * NT * 4 * p.stride + 2ull * kProjWarps * 2 * NT * 16 * 8;
+    auto* kernel = k_q4_project<G, NT, SEG>;
+    ZK_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared));
+    const uint32_t at_once = kSms * (shared > kMaxShared / 2 ? 1 : 2);
+    // Warps to a tile: the fewest steps of a block's warps, each with what a tile costs besides its blocks
+    const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
+    uint64_t least = ~0ull;
+    for (uint32_t split = 1; split <= (uint32_t)kProjWarps; split *= 2) {
+        const uint64_t groups = ceil_div(p.s.tiles, kProjWarps / split);
+        const uint64_t cost = ceil_div(groups, at_once) * (ceil_div(units, split) * unit + 3);
+        if (cost < least) {
+            least = cost;
+            p.split = split;
+        }
+    }
+    const uint64_t groups = ceil_div(p.s.tiles, kProjWarps / p.split);
+    const dim3 grid((unsigned)(groups < at_once ? groups : at_once), (unsigned)ceil_div(p.m, 2 * NT));
+    kernel<<<grid, kProjThreads, shared, stream>>>(p);
+    ZK_LAUNCH_CHECK();
+    return 0;
+}
+
+template <int G, int NT>
+int project_seg(const ProjectArgs& p, cudaStream_t stream) {
+    return p.s.segs > 1 ? project_launch<G, NT, true>(p, stream) : project_launch<G, NT, false>(p, stream);
+}
+
+template <int G>
+int project_rows(const ProjectArgs& p, cudaStream_t stream) {
+    // rows to a block: up to eight, as many as their digits leave room for
+    const uint64_t row = 4ull * p.stride, red = 2ull * kProjWarps * 16 * 8;
+    if (p.m > 4 && 8 * (row + red) <= kMaxShared) return project_seg<G, 4>(p, stream);
+    if (p.m > 2 && 4 * (row + red) <= kMaxShared) return project_seg<G, 2>(p, stream);
+    return project_seg<G, 1>(p, stream);
+}
+
+// ---- the cache ------------------------------------------------------------------------------
+// Keys lie in blocks of 32 tokens, four dimensions of each token side by side
+// (b, head, token / 32, dk / 4, token % 32, 4): a lane takes a token, its
+// loads are 16 bytes next to its neighbours', and a score needs no sum over
+// lanes.  Values are rows (b, head, token, dv).
+constexpr int kKvBlock = 32;
+constexpr int64_t kKeyLimit = 1ll << 27;  // |q|, |k| up to here: a score of 256 products stays below 2^62
+
+__device__ __forceinline__ uint64_t key_at(uint64_t head, uint64_t blocks, uint32_t dk, uint64_t tok, uint32_t d) {
+    return ((head * blocks + tok / kKvBlock) * (dk / 4) + d / 4) * (4 * kKvBlock) + (tok % kKvBlock) * 4 + d % 4;
+}
+
+struct KvCache {
+    int32_t* k;
+    int32_t* v;
+    const int32_t* lens;
+    uint32_t batch, heads, dk, dv, cap;
+};
+
+struct KvRows {
+    const uint64_t* k;
+    uint64_t ldk;
+    const uint64_t* v;
+    uint64_t ldv;
+    int64_t factor;
+    uint32_t shift;
+};
+
+// the d-th number of a new key (d < dk) or value (from dk on) into the cache
+__device__ __forceinline__ bool kv_store(const KvCache& c, const KvRows& rows, uint64_t row, uint32_t seq, uint32_t h,
+                                         uint64_t tok, uint32_t d) {
+    const uint64_t head = (uint64_t)seq * c.heads + h;
+    if (d < c.dk) {
+        const int64_t x = fx_to_i64(__ldg(rows.k + row * rows.ldk + (uint64_t)h * c.dk + d));
+        const int64_t y = fx_round_div_pow2(fx_wmul(x, rows.factor), rows.shift);
+        const bool ok = y >= -kKeyLimit && y <= kKeyLimit;
+        c.k[key_at(head, c.cap / kKvBlock, c.dk, tok, d)] = ok ? (int32_t)y : 0;
+        return ok;
+    }
+    d -= c.dk;
+    const int64_t y = fx_to_i64(__ldg(rows.v + row * rows.ldv + (uint64_t)h * c.dv + d));
+    const bool ok = y >= INT32_MIN && y <= INT32_MAX;
+    c.v[(head * c.cap + tok) * c.dv + d] = ok ? (int32_t)y : 0;
+    return ok;
+}
+
+// rows x: `tokens` rows of keys and values of sequence blockIdx.z, at the
+// positions from lens[seq] on
+__global__ void k_kv_append(KvCache c, KvRows rows, uint32_t tokens, uint32_t* __restrict__ err) {
+    const uint32_t seq = blockIdx.z, h = blockIdx.y, width = c.dk + c.dv;
+    const int64_t len = c.lens[seq];
+    if (len < 0) return;
+    bool bad = false, full = false;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (uint64_t)tokens * width;
+         i += (uint64_t)gridDim.x * blockDim.x) {
+        const uint64_t r = i / width, tok = len + r;
+        if (tok >= c.cap)
+            full = true;
+        else
+            bad |= !kv_store(c, rows, (uint64_t)seq * tokens + r, seq, h, tok, (uint32_t)(i % width));
+    }
+    if (bad) atomicOr(err, kErrRange);
+    if (full) atomicOr(err, kErrFull);
+}
+
+constexpr int kAttThreads = 256;
+constexpr int kAttWarps = kAttThreads / 32;
+
+struct AttendArgs {
+    KvCache c;
+    KvRows rows;  // the new token's key and value (null: none)
+    const uint64_t* q;
+    uint64_t ldq;
+    uint32_t each;    // query heads to a key head
+    uint32_t groups;  // blocks of EACH query heads to a key head
+    int64_t q_factor, s_factor;
+    uint32_t q_shift, s_shift, out_shift;
+    const uint64_t* table;
+    uint64_t table_len;
+    int64_t offset;
+    uint64_t* out;
+    uint32_t* err;
+    uint32_t chunk;  // tokens of a block's share of the scores
+};
+
+// One cluster per sequence, key head and EACH of its query heads; a block
+// takes an equal run of the token blocks.  The softmax's rounding needs the
+// row's maximum and then its sum before any weight is known, so the scores
+// stay in shared memory and the cluster meets twice, keys and values each
+// being read once; the blocks' value sums meet in a third exchange.
+template <int EACH>
+__global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ long long s_red[kAttWarps][EACH];
+    __shared__ long long s_max[EACH], s_sum[EACH];
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t seq = blockIdx.z, h = blockIdx.y / p.groups, e0 = (blockIdx.y % p.groups) * EACH;
+    const uint32_t heads = min((uint32_t)EACH, p.each - e0), dk = p.c.dk, dv = p.c.dv;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t* out = p.out + ((uint64_t)seq * p.c.heads * p.each + (uint64_t)h * p.each + e0) * dv;
+
+    const int64_t len = p.c.lens[seq];
+    const bool append = p.rows.k != nullptr && len >= 0 && len < p.c.cap;
+    if (p.rows.k != nullptr && len >= p.c.cap && threadIdx.x == 0) atomicOr(p.err, kErrFull);
+    const uint32_t n = (uint32_t)(len < 0 ? 0 : min(len + (append ? 1 : 0), (int64_t)p.c.cap));
+    if (n == 0) {  // the whole cluster's answer
+        for (uint32_t i = rank * kAttThreads + threadIdx.x; i < heads * dv; i += ranks * kAttThreads) out[i] = 0;
+        return;
+    }
+    const uint32_t blocks = (n + kKvBlock - 1) / kKvBlock;
+    const uint32_t b0 = (uint32_t)((uint64_t)rank * blocks / ranks), b1 = (uint32_t)((uint64_t)(rank + 1) * blocks / ranks);
+    const uint32_t t0 = b0 * kKvBlock, count = b1 > b0 ? min(b1 * kKvBlock, n) - t0 : 0;
+
+    long long* scores = reinterpret_cast<long long*>(smem);                               // EACH x chunk
+    unsigned long long* acc = reinterpret_cast<unsigned long long*>(scores + (size_t)EACH * p.chunk);  // EACH x dv
+    int* qs = reinterpret_cast<int*>(acc + (size_t)EACH * dv);                            // EACH x dk
+    bool bad = false;
+    for (uint32_t i = threadIdx.x; i < EACH * dv; i += kAttThreads) acc[i] = 0;
+    for (uint32_t i = threadIdx.x; i < EACH * dk; i += kAttThreads) {
+        int64_t y = 0;
+        if (i / dk < heads) {
+            const int64_t x = fx_to_i64(__ldg(p.q + seq * p.ldq + (uint64_t)(h * p.each + e0) * dk + i));
+            y = fx_round_div_pow2(fx_wmul(x, p.q_factor), p.q_shift);
+            if (y < -kKeyLimit || y > kKeyLimit) {
+                bad = true;
+                y = 0;
+            }
+        }
+        qs[i] = (int)y;
+    }
+    // The new token belongs to the block whose share holds it (blocks of other
+    // query heads of the same key head store the same numbers).
+    if (append && (uint32_t)len / kKvBlock >= b0 && (uint32_t)len / kKvBlock < b1)
+        for (uint32_t d = threadIdx.x; d < dk + dv; d += kAttThreads)
+            bad |= !kv_store(p.c, p.rows, seq, seq, h, (uint64_t)len, d);
+    __syncthreads();
+
+    const uint64_t head = (uint64_t)seq * p.c.heads + h;
+    long long top[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) top[e] = INT64_MIN;
+    for (uint32_t b = b0 + warp; b < b1; b += kAttWarps) {
+        const int32_t* kb = p.c.k + key_at(head, p.c.cap / kKvBlock, dk, (uint64_t)b * kKvBlock + lane, 0);
+        long long s[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) s[e] = 0;
+#pragma unroll 8
+        for (uint32_t d = 0; d < dk; d += 4) {
+            const int4 kv = __ldcg(reinterpret_cast<const int4*>(kb + (size_t)d * kKvBlock));
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                const int4 qv = *reinterpret_cast<const int4*>(qs + e * dk + d);
+                s[e] += (long long)qv.x * kv.x + (long long)qv.y * kv.y + (long long)qv.z * kv.z +
+                        (long long)qv.w * kv.w;
+            }
+        }
+        const uint32_t at = b * kKvBlock + lane - t0;
+        if (at < count) {
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                const long long z = fx_round_div_pow2(fx_wmul(s[e], p.s_factor), p.s_shift);
+                scores[(size_t)e * p.chunk + at] = z;
+                top[e] = z > top[e] ? z : top[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        for (int o = 16; o; o >>= 1) {
+            const long long other = __shfl_xor_sync(0xFFFFFFFFu, top[e], o);
+            top[e] = other > top[e] ? other : top[e];
+        }
+        if (lane == 0) s_red[warp][e] = top[e];
+    }
+    __syncthreads();
+    if (threadIdx.x < EACH) {
+        long long v = s_red[0][threadIdx.x];
+        for (int w = 1; w < kAttWarps; w++) v = max(v, s_red[w][threadIdx.x]);
+        s_max[threadIdx.x] = v;
+    }
+    cluster.sync();
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        top[e] = INT64_MIN;
+        for (uint32_t r = 0; r < ranks; r++) top[e] = max(top[e], *cluster.map_shared_rank(&s_max[e], r));
+    }
+
+    long long part[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) part[e] = 0;
+    for (uint32_t j = threadIdx.x; j < count; j += kAttThreads) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            int64_t v = fx_to_i64(
+                table_at(p.table, p.table_len, fx_wsub(scores[(size_t)e * p.chunk + j], top[e]), p.offset));
+            if (v < 0 || v > INT32_MAX) {
+                bad = true;
+                v = 0;
+            }
+            scores[(size_t)e * p.chunk + j] = v;
+            part[e] += v;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        for (int o = 16; o; o >>= 1) part[e] += __shfl_xor_sync(0xFFFFFFFFu, part[e], o);
+        if (lane == 0) s_red[warp][e] = part[e];
+    }
+    __syncthreads();
+    if (threadIdx.x < EACH) {
+        long long v = 0;
+        for (int w = 0; w < kAttWarps; w++) v += s_red[w][threadIdx.x];
+        s_sum[threadIdx.x] = v;
+    }
+    cluster.sync();
+    double inv[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        part[e] = 0;
+        for (uint32_t r = 0; r < ranks; r++) part[e] += *cluster.map_shared_rank(&s_sum[e], r);
+        if (part[e] == 0 && e < heads && rank == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDivide);
+        inv[e] = part[e] ? 1.0 / (double)part[e] : 0.0;
+    }
+    for (uint32_t j = threadIdx.x; j < count; j += kAttThreads) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const long long v = scores[(size_t)e * p.chunk + j];
+            scores[(size_t)e * p.chunk + j] = part[e] ? round_div_near(v << 16, part[e], inv[e]) : 0;
+        }
+    }
+    __syncthreads();
+
+    // A thread keeps four dimensions and takes every step-th token
+    const uint32_t wide = dv / 4, step = kAttThreads / wide, phase = threadIdx.x / wide, d4 = threadIdx.x % wide;
+    if (phase < step) {
+        long long y[EACH][4];
+#pragma unroll
+        for (int e = 0; e < EACH; e++) y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0;
+        const int32_t* vb = p.c.v + (head * p.c.cap + t0) * dv + d4 * 4;
+#pragma unroll 4
+        for (uint32_t j = phase; j < count; j += step) {
+            const int4 vv = __ldcg(reinterpret_cast<const int4*>(vb + (size_t)j * dv));
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                const int w = (int)scores[(size_t)e * p.chunk + j];
+                y[e][0] += (long long)w * vv.x;
+                y[e][1] += (long long)w * vv.y;
+                y[e][2] += (long long)w * vv.z;
+                y[e][3] += (long long)w * vv.w;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) atomicAdd(&acc[e * dv + d4 * 4 + i], (unsigned long long)y[e][i]);
+    }
+    if (bad) atomicOr(p.err, kErrRange);
+    cluster.sync();
+    for (uint32_t i = rank * kAttThreads + threadIdx.x; i < heads * dv; i += ranks * kAttThreads) {
+        unsigned long long v = 0;
+        for (uint32_t r = 0; r < ranks; r++) v += *cluster.map_shared_rank(&acc[i], r);
+        out[i] = fx_from_i64(fx_round_div_pow2((int64_t)v, p.out_shift));
+    }
+    cluster.sync();  // no block leaves while its sums may still be read
+}
+
+size_t attend_shared(uint32_t each, uint32_t chunk, uint32_t dk, uint32_t dv) {
+    return (size_t)each * (8ull * chunk + 8ull * dv + 4ull * dk);
+}
+
+template <int EACH>
+int attend_launch(AttendArgs p, uint32_t ranks, cudaStream_t stream) {
+    p.groups = (uint32_t)ceil_div(p.each, EACH);
+    p.chunk = (uint32_t)ceil_div(p.c.cap / kKvBlock, ranks) * kKvBlock;
+    const size_t shared = attend_shared(EACH, p.chunk, p.c.dk, p.c.dv);
+    auto* kernel = k_kv_attend<EACH>;
+    ZK_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(220 * 1024)));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ranks, p.c.heads * p.groups, p.c.batch);
+    cfg.blockDim = dim3(kAttThreads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    ZK_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
+    return 0;
+}
+
+// ---- the next token ---------------------------------------------------------------------------
+constexpr int kChooseThreads = 512;
+constexpr int kChooseWarps = kChooseThreads / 32;
+constexpr uint32_t kCounts = 8192;  // vocabulary entries counted at a time
+
+struct ChooseArgs {
+    const uint64_t* logits;
+    uint64_t v;
+    const int32_t* history;
+    uint64_t history_len;
+    const int32_t* history_lens;
+    int64_t repeat_pos, repeat_neg, presence, frequency;
+    const uint64_t* bias;
+    uint64_t bias_stride;
+    const uint32_t* allowed;
+    uint64_t allowed_stride;
+    int64_t mask_value;
+    uint64_t* out;
+    uint32_t* token;
+    uint32_t* err;
+};
+
+// One cluster per row, a block to an equal slice of the vocabulary: counts of
+// the history's tokens in shared memory, then one pass over the slice; the
+// blocks' maxima meet in the first block.
+__global__ void __launch_bounds__(kChooseThreads) k_choose_token(const ChooseArgs p) {
+    __shared__ uint32_t counts[kCounts];
+    __shared__ long long s_v[kChooseWarps];
+    __shared__ unsigned long long s_j[kChooseWarps];
+    __shared__ long long best_v;
+    __shared__ unsigned long long best_j;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint64_t row = blockIdx.y, lo = p.v * rank / ranks, hi = p.v * (rank + 1) / ranks;
+    uint64_t past = 0;
+    if (p.history) {
+        past = p.history_len;
+        if (p.history_lens) {
+            const int64_t l = p.history_lens[row];
+            past = l < 0 ? 0 : (l < (int64_t)past ? l : past);
+        }
+    }
+    long long bv = INT64_MIN;
+    unsigned long long bj = UINT64_MAX;
+    bool bad = false;
+    for (uint64_t s0 = lo; s0 < hi; s0 += kCounts) {
+        const uint64_t s1 = s0 + kCounts < hi ? s0 + kCounts : hi;
+        if (past) {
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < s1 - s0; i += kChooseThreads) counts[i] = 0;
+            __syncthreads();
+            for (uint64_t i = threadIdx.x; i < past; i += kChooseThreads) {
+                const int64_t tok = __ldg(p.history + row * p.history_len + i);
+                if (tok < 0 || tok >= (int64_t)p.v)
+                    bad = true;
+                else if ((uint64_t)tok >= s0 && (uint64_t)tok < s1)
+                    atomicAdd(&counts[tok - s0], 1u);
+            }
+            __syncthreads();
+        }
+        for (uint64_t j = s0 + threadIdx.x; j < s1; j += kChooseThreads) {
+            int64_t y = fx_to_i64(__ldg(p.logits + row * p.v + j));
+            const uint32_t c = past ? counts[j - s0] : 0;
+            if (c) {
+                y = fx_round_div_pow2(fx_wmul(y, y > 0 ? p.repeat_pos : p.repeat_neg), 16);
+                y = fx_wsub(fx_wsub(y, p.presence), fx_wmul(p.frequency, c));
+            }
+            if (p.bias) y = fx_wadd(y, fx_to_i64(__ldg(p.bias + row * p.bias_stride + j)));
+            if (p.allowed && !((__ldg(p.allowed + row * p.allowed_stride + j / 32) >> (j % 32)) & 1))
+                y = fx_wadd(y, p.mask_value);
+            const uint64_t f = fx_from_i64(y);
+            p.out[row * p.v + j] = f;
+            if (y > bv || bj == UINT64_MAX) {
+                bv = y;
+                bj = j;
+            }
+        }
+    }
+    if (bad && rank == 0) atomicOr(p.err, kErrIndex);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto take = [&](long long ov, unsigned long long oj) {
+        if (oj != UINT64_MAX && (bj == UINT64_MAX || ov > bv || (ov == bv && oj < bj))) {
+            bv = ov;
+            bj = oj;
+        }
+    };
+    for (int o = 16; o; o >>= 1) {
+        const long long ov = __shfl_xor_sync(0xFFFFFFFFu, bv, o);
+        const unsigned long long oj = __shfl_xor_sync(0xFFFFFFFFu, bj, o);
+        take(ov, oj);
+    }
+    if (lane == 0) {
+        s_v[warp] = bv;
+        s_j[warp] = bj;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kChooseWarps; w++) take(s_v[w], s_j[w]);
+        best_v = bv;
+        best_j = bj;
+    }
+    cluster.sync();
+    if (rank == 0 && threadIdx.x == 0) {
+        for (uint32_t r = 1; r < ranks; r++)
+            take(*cluster.map_shared_rank(&best_v, r), *cluster.map_shared_rank(&best_j, r));
+        p.token[row] = (uint32_t)bj;
+    }
+    cluster.sync();
+}
+
+}  // namespace
+
+}  // namespace zk
+
+using namespace zk;
+
+extern "C" {
+
+uint64_t zkie2_q4_code_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment) {
+    Q4Shape s;
+    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, segment, &s)) return 0;
+    return experts * s.tiles * s.blocks * 128ull;
+}
+
+uint64_t zkie2_q4_scale_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment) {
+    Q4Shape s;
+    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, segment, &s)) return 0;
+    return experts * s.tiles * s.groups * 8ull;
+}
+
+int zkie2_q4_pack(const int8_t* d_codes, const int32_t* d_scales, uint64_t experts, uint64_t k, uint64_t n,
+                  uint32_t group, uint64_t segment, uint32_t* d_packed, uint32_t* d_packed_scales, uint32_t* d_err,
+                  cudaStream_t stream) {
+    Q4Shape s;
+    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, segment, &s) || !d_codes || !d_scales || !d_packed ||
+        !d_packed_scales || !d_err)
+        return (int)cudaErrorInvalidValue;
+    const uint64_t words = experts * s.tiles * s.blocks * 128ull, blocks = ceil_div(words, 256);
+    k_q4_pack<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), 256, 0, stream>>>(
+        d_codes, d_scales, (uint32_t)experts, s, d_packed, d_packed_scales, d_err);
+    ZK_LAUNCH_CHECK();
+    return 0;
+}
+
+int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32_t* d_packed,
+                     const uint32_t* d_packed_scales, uint64_t k, uint64_t n, uint32_t group, uint64_t segment,
+                     uint32_t shift, const uint64_t* d_bias, const uint64_t* d_table, uint64_t table_len,
+                     int64_t offset, const uint64_t* d_residual, uint64_t ldr, uint64_t* d_out, uint32_t* d_err,
+                     cudaStream_t stream) {
+    ProjectArgs p{};
+    if (!q4_shape(k, n, group, segment, &p.s) || shift > 62 || m > 65535 || !d_packed || !d_packed_scales || !d_err ||
+        (d_table && table_len == 0) || (m > 1 && ldx < k) || (d_residual && m > 1 && ldr < n) ||
+        ((uintptr_t)d_packed & 15))
+        return (int)cudaErrorInvalidValue;
+    if (m == 0) return 0;
+    if (!d_x || !d_out) return (int)cudaErrorInvalidValue;
+    p.x = d_x;
+    p.ldx = ldx;
+    p.m = (uint32_t)m;
+    p.codes = reinterpret_cast<const uint4*>(d_packed);
+    p.scales = d_packed_scales;
+    p.shift = shift;
+    p.bias = d_bias;
+    p.table = d_table;
+    p.table_len = table_len;
+    p.offset = offset;
+    p.residual = d_residual;
+    p.ldr = ldr;
+    p.out = d_out;
+    p.err = d_err;
+    p.stride = digit_stride(p.s.blocks);
+    return group == 32 ? project_rows<32>(p, stream) : group == 64 ? project_rows<64>(p, stream)
+                                                                    : project_rows<128>(p, stream);
+}
+
+int zkie2_kv_append(const uint64_t* d_k, uint64_t ldk, const uint64_t* d_v, uint64_t ldv, uint64_t tokens,
+                    int64_t k_factor, uint32_t k_shift, int32_t* d_cache_k, int32_t* d_cache_v, const int32_t* d_lens,
+                    uint64_t batch, uint64_t heads, uint64_t dk, uint64_t dv, uint64_t capacity, uint32_t* d_err,
+                    cudaStream_t stream) {
+    if (!d_cache_k || !d_cache_v || !d_lens || !d_err || batch == 0 || batch > 65535 || heads == 0 || heads > 65535 ||
+        dk == 0 || dk > 256 || dk % 4 || dv == 0 || dv > 256 || dv % 4 || capacity == 0 || capacity % kKvBlock ||
+        capacity > (1u << 17) || tokens > (1u << 17) || k_shift > 62 || ldk < heads * dk || ldv < heads * dv)
+        return (int)cudaErrorInvalidValue;
+    if (tokens == 0) return 0;
+    if (!d_k || !d_v) return (int)cudaErrorInvalidValue;
+    const KvCache c{d_cache_k, d_cache_v, d_lens, (uint32_t)batch, (uint32_t)heads, (uint32_t)dk, (uint32_t)dv,
+                    (uint32_t)capacity};
+    const KvRows rows{d_k, ldk, d_v, ldv, k_factor, k_shift};
+    const uint64_t blocks = ceil_div(tokens * (dk + dv), 256);
+    k_kv_append<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)heads, (unsigned)batch), 256, 0, stream>>>(
+        c, rows, (uint32_t)tokens, d_err);
+    ZK_LAUNCH_CHECK();
+    return 0;
+}
+
+int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t q_factor, uint32_t q_shift,
+                    const uint64_t* d_k, uint64_t ldk, const uint64_t* d_v, uint64_t ldv, int64_t k_factor,
+                    uint32_t k_shift, int32_t* d_cache_k, int32_t* d_cache_v, const int32_t* d_lens, uint64_t batch,
+                    uint64_t heads, uint64_t dk, uint64_t dv, uint64_t capacity, int64_t s_factor, uint32_t s_shift,
+                    const uint64_t* d_table, uint64_t table_len, int64_t offset, uint32_t out_shift, uint64_t* d_out,
+                    uint32_t* d_err, cudaStream_t stream) {
+    if (!d_q || !d_cache_k || !d_cache_v || !d_lens || !d_table || !d_out || !d_err || batch == 0 || batch > 65535 ||
+        heads == 0 || q_heads == 0 || q_heads % heads || q_heads > 65535 || dk == 0 || dk > 256 || dk % 4 || dv == 0 ||
+        dv > 256 || dv % 4 || capacity == 0 || capacity % kKvBlock || capacity > (1u << 17) || q_shift > 62 ||
+        k_shift > 62 || s_shift > 62 || out_shift > 62 || table_len == 0 || (batch > 1 && ldq < q_heads * dk) ||
+        !d_k != !d_v || (d_k && batch > 1 && (ldk < heads * dk || ldv < heads * dv)) ||
+        (((uintptr_t)d_cache_k | (uintptr_t)d_cache_v) & 15))
+        return (int)cudaErrorInvalidValue;
+    AttendArgs p{};
+    p.c = KvCache{d_cache_k, d_cache_v, d_lens, (uint32_t)batch, (uint32_t)heads, (uint32_t)dk, (uint32_t)dv,
+                  (uint32_t)capacity};
+    p.rows = KvRows{d_k, ldk, d_v, ldv, k_factor, k_shift};
+    p.q = d_q;
+    p.ldq = ldq;
+    p.each = (uint32_t)(q_heads / heads);
+    p.q_factor = q_factor;
+    p.q_shift = q_shift;
+    p.s_factor = s_factor;
+    p.s_shift = s_shift;
+    p.out_shift = out_shift;
+    p.table = d_table;
+    p.table_len = table_len;
+    p.offset = offset;
+    p.out = d_out;
+    p.err = d_err;
+    // Query heads to a block: those that share a key head, up to four (their
+    // sums stay in registers); fewer where their scores do not fit.  Blocks to
+    // a cluster: enough to fill the device, more where the scores need it.
+    const uint32_t most = 8, blocks = (uint32_t)(capacity / kKvBlock);
+    for (uint32_t each = p.each >= 3 ? 4 : p.each;; each /= 2) {
+        const uint64_t rows = batch * heads * ceil_div(p.each, each);
+        uint32_t ranks = 1;
+        while (ranks < most && rows * ranks < 2 * kSms && ranks < blocks) ranks *= 2;
+        while (ranks < most &&
+               attend_shared(each, (uint32_t)ceil_div(blocks, ranks) * kKvBlock, p.c.dk, p.c.dv) > 220 * 1024)
+            ranks *= 2;
+        if (attend_shared(each, (uint32_t)ceil_div(blocks, ranks) * kKvBlock, p.c.dk, p.c.dv) > 220 * 1024 && each > 1)
+            continue;
+        return each == 4 ? attend_launch<4>(p, ranks, stream) : each == 2 ? attend_launch<2>(p, ranks, stream)
+                                                                          : attend_launch<1>(p, ranks, stream);
+    }
+}
+
+int zkie2_choose_token(const uint64_t* d_logits, uint64_t batch, uint64_t vocab, const int32_t* d_history,
+                       uint64_t history_len, const int32_t* d_history_lens, int64_t repeat_pos, int64_t repeat_neg,
+                       int64_t presence, int64_t frequency, const uint64_t* d_bias, uint64_t bias_stride,
+                       const uint32_t* d_allowed, uint64_t allowed_stride, int64_t mask_value, uint64_t* d_out,
+                       uint32_t* d_token, uint32_t* d_err, cudaStream_t stream) {
+    if (vocab == 0 || vocab > 0x7FFFFFFFull || batch > 65535 || (d_history_lens && !d_history) || !d_err ||
+        history_len > 0x7FFFFFFFull)
+        return (int)cudaErrorInvalidValue;
+    if (batch == 0) return 0;
+    if (!d_logits || !d_out || !d_token) return (int)cudaErrorInvalidValue;
+    const ChooseArgs p{d_logits, vocab, d_history, history_len, d_history_lens, repeat_pos, repeat_neg, presence,
+                       frequency, d_bias, bias_stride, d_allowed, allowed_stride, mask_value, d_out, d_token, d_err};
+    uint32_t ranks = 1;
+    while (ranks < 8 && vocab > (uint64_t)ranks * kChooseThreads * 2) ranks *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ranks, (unsigned)batch);
+    cfg.blockDim = dim3(kChooseThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    ZK_TRY(cudaLaunchKernelEx(&cfg, k_choose_token, p));
+    return 0;
+}
+
+}  // extern "C"

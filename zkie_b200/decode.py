@@ -1,0 +1,472 @@
+"""The forward of single tokens on the device: what a step of generation needs
+of the op layer, for a few rows instead of a whole, fixed-length sequence.
+
+``compose.forward_ops`` computes the witness of a whole sequence, ending in
+the Argmax arm (models/gpt2/src/lib.rs:321-436).  Answering token by token
+needs one row at a time; these operators compute it, and since every value is
+a whole number the row is the graph's own row, bit for bit: the answer that is
+generated is the answer the proof is about.
+
+- ``QuantWeight`` and ``project``: Projection / MatMul of a few rows by a
+  weight held in 4 bits with group scales.  Its numbers codes x scales are the
+  model's weights; ``QuantWeight.dense()`` is the tensor the Store gets.
+- ``KvCache`` and ``attend``: one new token per sequence over the keys and
+  values of the earlier ones, held exactly in 32 bits.
+- ``MoeBlock``: build_moe (models/deepseek-v2-lite/src/lib.rs:252-470) for a
+  few tokens in two kernels.
+- ``choose_token``: penalties for repeated tokens, biases and masks on the
+  logits, and the Argmax arm.
+
+Every call takes rows of field elements (torch.uint64, unit stride within a
+row) on the current device and enqueues on the current stream.  ``err`` is the
+device error word of ``forward_ops``: given, the caller reads it when it
+likes (``check_err``); not given, the call reads its own, which synchronises,
+and raises ValueError.  Besides the op layer's bits, 8 is a value outside the
+32-bit range the kernels take (computed on as zero) and 16 a full cache.
+"""
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .compose import _check_err, _err_word
+from .device import P, device
+
+GROUPS = (32, 64, 128)
+KV_BLOCK = 32
+MASKED = -(1 << 41)  # the graph's vocabulary mask (models/gpt2/src/lib.rs:410-418)
+
+
+def check_err(err: torch.Tensor, what: str = "decode"):
+    """Read an error word (synchronises) and raise ValueError if a bit is set."""
+    _check_err(err, what)
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _on_device(t: torch.Tensor, name: str, dtype) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor of {dtype} is wanted")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t
+
+
+def _rows(t: torch.Tensor, name: str, cols: int) -> torch.Tensor:
+    """A matrix of field elements with rows of ``cols`` of unit stride."""
+    _on_device(t, name, torch.uint64)
+    if t.dim() != 2 or t.shape[1] != cols:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, {cols} columns are wanted")
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name}: rows of unit stride that do not overlap are wanted")
+    return t
+
+
+def _flat(t: torch.Tensor, name: str, dtype, shape=None) -> torch.Tensor:
+    _on_device(t, name, dtype)
+    if not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name}: a contiguous tensor{'' if shape is None else f' of shape {tuple(shape)}'} is wanted")
+    return t
+
+
+def _word(err: Optional[torch.Tensor]) -> torch.Tensor:
+    if err is None:
+        return _err_word()
+    return _flat(err, "err", torch.int32, (1,))
+
+
+def _out(out, shape) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.uint64, device=torch.device("cuda", torch.cuda.current_device()))
+    return _flat(out, "out", torch.uint64, shape)
+
+
+def _signed(t: torch.Tensor) -> torch.Tensor:
+    """Field elements (or whole numbers) as int64: fixed_point.rs to_i64."""
+    if t.dtype == torch.uint64:
+        t = t.view(torch.int64)
+        return torch.where(t < 0, t + ((1 << 64) - P), t)
+    return t.to(torch.int64)
+
+
+def _field(t: torch.Tensor) -> torch.Tensor:
+    """int64 as field elements: fixed_point.rs from_i64."""
+    return torch.where(t < 0, t - ((1 << 64) - P), t).view(torch.uint64)
+
+
+# ---- 4-bit weights ------------------------------------------------------------------------------
+def _scale_rows(k: int, group: int, segment: int) -> int:
+    return k // segment * -(-segment // group) if segment else -(-k // group)
+
+
+def _group_of(k: int, group: int, segment: int, dev) -> torch.Tensor:
+    """The row of scales that each of the k rows of codes has."""
+    at = torch.arange(k, device=dev)
+    return at // segment * -(-segment // group) + at % segment // group if segment else at // group
+
+
+def quantise(w: torch.Tensor, group: int = 64, segment: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The nearest 4-bit form of a weight (k x n or experts x k x n, field
+    elements or whole numbers): codes (int8, in [-8, 7]) and scales (int32),
+    the smallest whole scale that covers each group of ``group`` rows of a
+    column.  Raises where a weight needs a scale above 65535."""
+    if group not in GROUPS or segment < 0 or w.dim() not in (2, 3) or (segment and w.shape[-2] % segment):
+        raise ValueError("quantise: group 32, 64 or 128, and segments that divide the rows, are wanted")
+    w = _signed(w)
+    k, n = w.shape[-2:]
+    row = _group_of(k, group, segment, w.device)
+    at = row[:, None].expand(k, n).expand(w.shape)
+    lo = torch.zeros(w.shape[:-2] + (_scale_rows(k, group, segment), n), dtype=torch.int64, device=w.device)
+    hi = lo.clone().scatter_reduce_(-2, at, w, "amax")
+    lo = lo.scatter_reduce_(-2, at, w, "amin")
+    scales = torch.maximum(torch.maximum((hi + 6) // 7, (7 - lo) // 8), torch.ones_like(lo))
+    if int(scales.max()) > 65535:
+        raise ValueError("quantise: a weight needs a scale above 65535")
+    s = scales[..., row, :]
+    codes = torch.div(2 * w + s, 2 * s, rounding_mode="floor").clamp(-8, 7)
+    return codes.to(torch.int8), scales.to(torch.int32)
+
+
+class QuantWeight:
+    """A weight w[k][n] = codes[k][n] scales[row of k][n] in 4 bits, laid out
+    once for the kernels (``packed``, ``packed_scales``).
+
+    codes: int8, k x n or experts x k x n, in [-8, 7]; scales: whole numbers in
+    [0, 65535], one for each ``group`` (32, 64 or 128) rows of a column, as
+    many rows of them as groups begin.  ``segment`` splits the rows into runs
+    (the heads of an output projection) that the product rounds one by one and
+    adds, as the graph's Projection per head and its Adds do; groups begin
+    anew in each run.  At most 8192 rows, each run counted as a multiple of 64
+    (128 for group 128)."""
+
+    def __init__(self, codes, scales, group: int = 64, segment: int = 0):
+        codes, scales = torch.as_tensor(codes).to(device()), torch.as_tensor(scales).to(device())
+        if codes.dtype != torch.int8 or codes.dim() not in (2, 3) or scales.is_floating_point():
+            raise ValueError("QuantWeight: codes int8 (k x n or experts x k x n) and whole scales are wanted")
+        if group not in GROUPS or segment < 0:
+            raise ValueError("QuantWeight: group 32, 64 or 128 is wanted")
+        self.experts = codes.shape[0] if codes.dim() == 3 else 1
+        self.k, self.n = int(codes.shape[-2]), int(codes.shape[-1])
+        self.group, self.segment = group, segment
+        words = lib.zkie2_q4_code_words(self.experts, self.k, self.n, group, segment)
+        if words == 0:
+            raise ValueError(f"QuantWeight: {self.experts} x {self.k} x {self.n} with group {group} and segment "
+                             f"{segment} is not taken (at most 8192 padded rows, segments that divide them)")
+        want = tuple(codes.shape[:-2]) + (_scale_rows(self.k, group, segment), self.n)
+        if tuple(scales.shape) != want:
+            raise ValueError(f"QuantWeight: scales of shape {tuple(scales.shape)}, {want} is wanted")
+        if int(codes.min()) < -8 or int(codes.max()) > 7 or int(scales.min()) < 0 or int(scales.max()) > 65535:
+            raise ValueError("QuantWeight: a code outside [-8, 7] or a scale outside [0, 65535]")
+        codes, scales = codes.contiguous(), scales.to(torch.int32).contiguous()
+        dev = codes.device
+        self.packed = torch.empty(words, dtype=torch.int32, device=dev)
+        self.packed_scales = torch.empty(lib.zkie2_q4_scale_words(self.experts, self.k, self.n, group, segment),
+                                         dtype=torch.int32, device=dev)
+        err = _err_word()
+        check(lib.zkie2_q4_pack(codes.data_ptr(), scales.data_ptr(), self.experts, self.k, self.n, group, segment,
+                                self.packed.data_ptr(), self.packed_scales.data_ptr(), err.data_ptr(), _stream()),
+              "zkie2_q4_pack")
+        _check_err(err, "QuantWeight")
+
+    def codes(self) -> torch.Tensor:
+        """The codes back (experts x k x n)."""
+        tiles, unit = -(-self.n // 16), 128 if self.group == 128 else 64
+        seg = self.segment or self.k
+        b = self.packed.view(torch.uint8).reshape(self.experts, tiles, -1, 8, 4, 2, 2, 4)
+        both = torch.stack([b & 15, b >> 4], dim=-1).to(torch.int8)  # expert tile block g t q/2 q%2 j half
+        both = torch.where(both > 7, both - 16, both)
+        full = both.permute(0, 2, 8, 4, 5, 7, 1, 6, 3).reshape(self.experts, -1, tiles * 16)
+        full = full.reshape(self.experts, self.k // seg, -(-seg // unit) * unit, tiles * 16)
+        return full[:, :, :seg, :self.n].reshape(self.experts, self.k, self.n)
+
+    def scales(self) -> torch.Tensor:
+        """The scales back (experts x rows x n)."""
+        tiles, seg = -(-self.n // 16), self.segment or self.k
+        w = self.packed_scales.reshape(self.experts, tiles, -1, 8)
+        both = torch.stack([w & 0xFFFF, (w >> 16) & 0xFFFF], dim=-1)  # expert tile group g half
+        full = both.permute(0, 2, 1, 4, 3).reshape(self.experts, self.k // seg, -1, tiles * 16)
+        return full[:, :, :-(-seg // self.group), :self.n].reshape(self.experts, -1, self.n)
+
+    def dense(self) -> torch.Tensor:
+        """The weights as field elements, flat and row-major (experts one after
+        another): the tensor of a Store."""
+        row = _group_of(self.k, self.group, self.segment, self.packed.device)
+        return _field(self.codes().to(torch.int64) * self.scales().to(torch.int64)[:, row]).reshape(-1)
+
+
+def project(x: torch.Tensor, weight: QuantWeight, shift: int, *, bias: Optional[torch.Tensor] = None,
+            table: Optional[torch.Tensor] = None, offset: Optional[int] = None,
+            residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+            err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The Projection arm's out for the rows of x (m x k -> m x n):
+    round_div(x w, 2^shift), one rounding per segment of the weight, + bias (n);
+    then ``table[clamp(y + offset, 0, len - 1)]`` (GeluIndex and Lookup; offset
+    defaults to the table's middle) and ``+ residual`` (m x n; Add) where
+    given.  shift 0 without a bias is the MatMul arm.  |x| <= 0x7F7F7F7F."""
+    if weight.experts != 1:
+        raise ValueError("project: one weight is wanted, not a stack of experts")
+    x = _rows(x, "x", weight.k)
+    m, n = x.shape[0], weight.n
+    if not 0 <= shift <= 62 or m > 65535:
+        raise ValueError("project: shift 0 .. 62 and at most 65535 rows are wanted")
+    if bias is not None:
+        _flat(bias, "bias", torch.uint64, (n,))
+    if table is not None:
+        _flat(table, "table", torch.uint64)
+        if table.numel() == 0:
+            raise ValueError("project: an empty table")
+        offset = table.numel() // 2 if offset is None else offset
+    if residual is not None:
+        _rows(residual, "residual", n)
+        if residual.shape[0] != m:
+            raise ValueError(f"residual: {residual.shape[0]} rows, {m} are wanted")
+    out, word = _out(out, (m, n)), _word(err)
+    check(lib.zkie2_q4_project(x.data_ptr(), x.stride(0), m, weight.packed.data_ptr(),
+                               weight.packed_scales.data_ptr(), weight.k, n, weight.group, weight.segment, shift,
+                               None if bias is None else bias.data_ptr(), None if table is None else table.data_ptr(),
+                               0 if table is None else table.numel(), offset or 0,
+                               None if residual is None else residual.data_ptr(),
+                               0 if residual is None else residual.stride(0), out.data_ptr(), word.data_ptr(),
+                               _stream()), "zkie2_q4_project")
+    if err is None:
+        _check_err(word, "project")
+    return out
+
+
+# ---- attention over a cache -----------------------------------------------------------------------
+class KvCache:
+    """The keys and values of ``batch`` sequences, exact in 32 bits.
+
+    k: int32 (batch, heads, capacity / 32, dk / 4, 32, 4) -- blocks of 32
+    tokens, four dimensions of a token side by side; v: int32 (batch, heads,
+    capacity, dv); lens: int32 (batch), tokens held (negative: an inactive
+    sequence).  The layers of a model may share one ``lens``.  dk and dv are
+    multiples of 4 up to 256, the capacity a multiple of 32 up to 131072."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor):
+        _flat(k, "k", torch.int32)
+        _flat(v, "v", torch.int32)
+        _flat(lens, "lens", torch.int32)
+        if k.dim() != 6 or v.dim() != 4 or k.shape[4:] != (KV_BLOCK, 4):
+            raise ValueError("KvCache: k (batch, heads, capacity / 32, dk / 4, 32, 4) and v (batch, heads, capacity, "
+                             "dv) are wanted")
+        self.batch, self.heads, self.capacity, self.dv = v.shape
+        self.dk = k.shape[3] * 4
+        if tuple(k.shape[:3]) != (self.batch, self.heads, self.capacity // KV_BLOCK) or \
+                tuple(lens.shape) != (self.batch,):
+            raise ValueError("KvCache: k, v and lens do not match")
+        if self.capacity % KV_BLOCK or not 0 < self.capacity <= 1 << 17 or not 0 < self.dk <= 256 or self.dv % 4 or \
+                not 0 < self.dv <= 256 or not 0 < self.batch <= 65535 or not 0 < self.heads <= 65535:
+            raise ValueError("KvCache: head sizes in multiples of 4 up to 256 and a capacity in multiples of 32 up to "
+                             "131072 are wanted")
+        if (k.data_ptr() | v.data_ptr()) & 15:
+            raise ValueError("KvCache: 16-byte aligned buffers are wanted")
+        self.k, self.v, self.lens = k, v, lens
+
+    @classmethod
+    def zeros(cls, batch: int, heads: int, dk: int, dv: int, capacity: int,
+              lens: Optional[torch.Tensor] = None) -> "KvCache":
+        """An empty cache; the capacity is rounded up to whole blocks."""
+        blocks, dev = -(-capacity // KV_BLOCK), device()
+        if dk % 4:
+            raise ValueError("KvCache: head sizes in multiples of 4 are wanted")
+        return cls(torch.zeros((batch, heads, blocks, dk // 4, KV_BLOCK, 4), dtype=torch.int32, device=dev),
+                   torch.zeros((batch, heads, blocks * KV_BLOCK, dv), dtype=torch.int32, device=dev),
+                   torch.zeros(batch, dtype=torch.int32, device=dev) if lens is None else lens)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, k_scale: Tuple[int, int] = (1, 0),
+               err: Optional[torch.Tensor] = None):
+        """Store rows of a prompt from position lens on (lens stays: see
+        ``advance``): k (batch, tokens, heads dk) and v (batch, tokens, heads
+        dv) field elements, the keys through Scale by k_scale = (factor,
+        shift).  |key| <= 2^27, values in 32 bits."""
+        _on_device(k, "k", torch.uint64)
+        _on_device(v, "v", torch.uint64)
+        if k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or k.shape[0] != self.batch or \
+                k.shape[2] != self.heads * self.dk or v.shape[2] != self.heads * self.dv:
+            raise ValueError("append: k (batch, tokens, heads dk) and v (batch, tokens, heads dv) are wanted")
+        if k.shape[1] > 1 << 17 or not 0 <= k_scale[1] <= 62:
+            raise ValueError("append: at most 131072 tokens and a shift 0 .. 62 are wanted")
+        k, v, word = k.contiguous(), v.contiguous(), _word(err)
+        check(lib.zkie2_kv_append(k.data_ptr(), k.shape[2], v.data_ptr(), v.shape[2], k.shape[1], k_scale[0],
+                                  k_scale[1], self.k.data_ptr(), self.v.data_ptr(), self.lens.data_ptr(), self.batch,
+                                  self.heads, self.dk, self.dv, self.capacity, word.data_ptr(), _stream()),
+              "zkie2_kv_append")
+        if err is None:
+            _check_err(word, "append")
+
+    def advance(self, tokens: int = 1):
+        """Count ``tokens`` more in every active sequence."""
+        self.lens.add_((self.lens >= 0).to(torch.int32), alpha=tokens)
+
+
+def attend(q: torch.Tensor, cache: KvCache, table: torch.Tensor, *, k: Optional[torch.Tensor] = None,
+           v: Optional[torch.Tensor] = None, q_scale: Tuple[int, int] = (1, 0), k_scale: Tuple[int, int] = (1, 0),
+           score_scale: Tuple[int, int] = (1, 16), offset: Optional[int] = None, out_shift: int = 16,
+           out: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query row per sequence (batch x heads dk, as many query heads as a
+    multiple of the cache's) over its cache -> batch x (query heads dv): the
+    row of Scale (q_scale), MatMul, Scale (score_scale), StableSoftmaxIndex
+    (offset, the table's length if not given), Softmax over ``table``, MatMul
+    and Scale (1, out_shift) in a causal graph.  With k (batch x heads dk) and
+    v (batch x heads dv) the new token is stored at position lens first, its
+    key through Scale (k_scale), and attended to; ``cache.advance`` then counts
+    it.  Rows may be columns of a wider matrix.  A graph's masked columns count
+    table[0] each in its softmax's sum: the rows agree where that is zero, as
+    in the models' tables.  A sequence without tokens answers zeros.  Scaled
+    queries and keys |q|, |k| <= 2^27; table values in [0, 2^31)."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (cache.heads * cache.dk):
+        raise ValueError("q: batch x (query heads dk) with a multiple of the cache's heads is wanted")
+    q = _rows(q, "q", q.shape[1])
+    heads = q.shape[1] // cache.dk
+    if q.shape[0] != cache.batch or (k is None) != (v is None):
+        raise ValueError("attend: a row per sequence, and k and v together, are wanted")
+    if k is not None:
+        _rows(k, "k", cache.heads * cache.dk)
+        _rows(v, "v", cache.heads * cache.dv)
+        if k.shape[0] != cache.batch or v.shape[0] != cache.batch:
+            raise ValueError("attend: a row of k and v per sequence is wanted")
+    _flat(table, "table", torch.uint64)
+    for s in (q_scale[1], k_scale[1], score_scale[1], out_shift):
+        if not 0 <= s <= 62:
+            raise ValueError("attend: shifts 0 .. 62 are wanted")
+    if table.numel() == 0 or heads > 65535:
+        raise ValueError("attend: an empty table, or too many heads")
+    _on_device(cache.k, "cache", torch.int32)
+    out, word = _out(out, (cache.batch, heads * cache.dv)), _word(err)
+    check(lib.zkie2_kv_attend(q.data_ptr(), q.stride(0), heads, q_scale[0], q_scale[1],
+                              None if k is None else k.data_ptr(), 0 if k is None else k.stride(0),
+                              None if v is None else v.data_ptr(), 0 if v is None else v.stride(0), k_scale[0],
+                              k_scale[1], cache.k.data_ptr(), cache.v.data_ptr(), cache.lens.data_ptr(), cache.batch,
+                              cache.heads, cache.dk, cache.dv, cache.capacity, score_scale[0], score_scale[1],
+                              table.data_ptr(), table.numel(), table.numel() if offset is None else offset, out_shift,
+                              out.data_ptr(), word.data_ptr(), _stream()), "zkie2_kv_attend")
+    if err is None:
+        _check_err(word, "attend")
+    return out
+
+
+# ---- a mixture-of-experts layer -----------------------------------------------------------------------
+class MoeBlock:
+    """build_moe's layer for a few tokens: router (h x experts, field elements
+    of at most 32639 in size), the routed experts' gate, up (experts x h x f)
+    and down (experts x f x h) and the shared experts' gate, up (h x shared f)
+    and down weights, all of one group without segments, the exp and silu
+    tables (field elements; silu's middle is zero) and how many experts a token
+    takes."""
+
+    def __init__(self, router: torch.Tensor, gate: QuantWeight, up: QuantWeight, down: QuantWeight,
+                 shared_gate: QuantWeight, shared_up: QuantWeight, shared_down: QuantWeight, exp_table: torch.Tensor,
+                 silu_table: torch.Tensor, top_k: int, shift: int = 16):
+        self.h, self.f, self.shared_f = gate.k, gate.n, shared_gate.n
+        self.experts, self.group, self.top_k, self.shift = gate.experts, gate.group, top_k, shift
+        h, f, s, e = self.h, self.f, self.shared_f, self.experts
+        self.weights = (gate, up, down, shared_gate, shared_up, shared_down)
+        want = ((e, h, f), (e, h, f), (e, f, h), (1, h, s), (1, h, s), (1, s, h))
+        for w, shape in zip(self.weights, want):
+            if (w.experts, w.k, w.n) != shape or w.group != self.group or w.segment:
+                raise ValueError(f"MoeBlock: weight {w.experts} x {w.k} x {w.n}, group {w.group}, segment {w.segment}: "
+                                 f"{shape} with group {self.group} and no segments is wanted")
+        router = _flat(router, "router", torch.uint64, (h, e))
+        self.exp_table, self.silu_table = _flat(exp_table, "exp_table", torch.uint64), \
+            _flat(silu_table, "silu_table", torch.uint64)
+        if exp_table.numel() == 0 or silu_table.numel() == 0:
+            raise ValueError("MoeBlock: an empty table")
+        if not 1 <= top_k <= min(e, 16) or e > 256 or not 0 <= shift <= 62:
+            raise ValueError("MoeBlock: at most 256 experts, 1 .. 16 of them to a token, and a shift 0 .. 62 are wanted")
+        self.router = torch.empty(lib.zkie2_moe_router_words(h, e, self.group), dtype=torch.int32,
+                                  device=router.device)
+        err = _err_word()
+        check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self.group, self.router.data_ptr(), err.data_ptr(),
+                                        _stream()), "zkie2_moe_router_pack")
+        _check_err(err, "MoeBlock: router")
+        self._codes = (_lib.vp * 6)(*[w.packed.data_ptr() for w in self.weights])
+        self._scales = (_lib.vp * 6)(*[w.packed_scales.data_ptr() for w in self.weights])
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(out, gate) of the rows of x (m x h, m <= 65535; two launches to 16
+        rows): the layer's output (+ residual where given) and TopKSelect's
+        gate (m x experts).  |x| and |silu(gate) up| <= 0x7F7F7F7F."""
+        x = _rows(x, "x", self.h)
+        m = x.shape[0]
+        if m > 65535:
+            raise ValueError("MoeBlock: at most 65535 rows are wanted")
+        if residual is not None:
+            _rows(residual, "residual", self.h)
+            if residual.shape[0] != m:
+                raise ValueError(f"residual: {residual.shape[0]} rows, {m} are wanted")
+        _on_device(self.router, "MoeBlock", torch.int32)
+        out, word = _out(out, (m, self.h)), _word(err)
+        gate = torch.empty((m, self.experts), dtype=torch.uint64, device=x.device)
+        scratch = torch.empty(max(lib.zkie2_moe_rows_scratch_elems(m, self.h, self.experts, self.top_k, self.f,
+                                                                   self.shared_f, self.group), 1),
+                              dtype=torch.int64, device=x.device)
+        check(lib.zkie2_moe_rows(x.data_ptr(), x.stride(0), m, self.h, self.experts, self.top_k, self.f, self.shared_f,
+                                 self.group, self.router.data_ptr(), self._codes, self._scales,
+                                 self.exp_table.data_ptr(), self.exp_table.numel(), self.silu_table.data_ptr(),
+                                 self.silu_table.numel(), self.shift,
+                                 None if residual is None else residual.data_ptr(),
+                                 0 if residual is None else residual.stride(0), out.data_ptr(), gate.data_ptr(),
+                                 word.data_ptr(), scratch.data_ptr(), _stream()), "zkie2_moe_rows")
+        if err is None:
+            _check_err(word, "MoeBlock")
+        return out, gate
+
+
+# ---- the next token -----------------------------------------------------------------------------------
+def choose_token(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
+                 history_lens: Optional[torch.Tensor] = None, *, repeat: Tuple[int, int] = (1 << 16, 1 << 16),
+                 presence: int = 0, frequency: int = 0, bias: Optional[torch.Tensor] = None,
+                 allowed: Optional[torch.Tensor] = None, mask_value: int = MASKED,
+                 out: Optional[torch.Tensor] = None,
+                 err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(token, adjusted logits) of each row of logits (batch x vocab field
+    elements): the Argmax arm (the lowest index among equals) after, in
+    wrapping i64,
+
+    - for a token that occurs c > 0 times in its row of ``history`` (batch x
+      tokens, int32; the first ``history_lens`` of a row where given):
+      round_div(y repeat[0], 2^16) where y > 0, else round_div(y repeat[1],
+      2^16), then - presence - c frequency;
+    - ``+ bias`` (vocab, or batch x vocab, field elements);
+    - ``+ mask_value`` where bit v % 32 of word v / 32 of ``allowed`` (int32
+      words, ceil(vocab / 32), or batch x that) is clear.  With the graph's
+      mask value a row that allows nothing still has a maximum."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError("choose_token: logits batch x vocab are wanted")
+    b, v = logits.shape
+    _flat(logits, "logits", torch.uint64)
+    if b > 65535 or v > 0x7FFFFFFF:
+        raise ValueError("choose_token: at most 65535 rows are wanted")
+    for name, t, dtype, shapes in (("bias", bias, torch.uint64, ((v,), (b, v))),
+                                   ("allowed", allowed, torch.int32, ((-(-v // 32),), (b, -(-v // 32))))):
+        if t is not None and tuple(_flat(t, name, dtype).shape) not in shapes:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, one of {shapes} is wanted")
+    if history is not None:
+        _flat(history, "history", torch.int32)
+        if history.dim() != 2 or history.shape[0] != b:
+            raise ValueError("history: batch x tokens is wanted")
+        if history_lens is not None:
+            _flat(history_lens, "history_lens", torch.int32, (b,))
+    elif history_lens is not None:
+        raise ValueError("choose_token: history_lens without a history")
+    out, word = _out(out, (b, v)), _word(err)
+    if out.data_ptr() == logits.data_ptr():
+        raise ValueError("choose_token: out may not be the logits")
+    token = torch.empty(b, dtype=torch.uint32, device=logits.device)
+    check(lib.zkie2_choose_token(logits.data_ptr(), b, v, None if history is None else history.data_ptr(),
+                                 0 if history is None else history.shape[1],
+                                 None if history_lens is None else history_lens.data_ptr(), repeat[0], repeat[1],
+                                 presence, frequency, None if bias is None else bias.data_ptr(),
+                                 0 if bias is None or bias.dim() == 1 else v,
+                                 None if allowed is None else allowed.data_ptr(),
+                                 0 if allowed is None or allowed.dim() == 1 else allowed.shape[1], mask_value,
+                                 out.data_ptr(), token.data_ptr(), word.data_ptr(), _stream()), "zkie2_choose_token")
+    if err is None:
+        _check_err(word, "choose_token")
+    return token, out
