@@ -16,12 +16,14 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/zkie2.h"
 #include "common.cuh"
 #include "fixed.cuh"
 #include "gl64.cuh"
+#include "launch.cuh"
 #include "q4.cuh"
 
 namespace cg = cooperative_groups;
@@ -33,7 +35,6 @@ namespace {
 constexpr uint32_t kErrIndex = 1u;
 constexpr uint32_t kErrDivide = 2u;
 constexpr uint32_t kErrFull = 16u;  // a cache without room for the new token
-constexpr int kSms = 148;
 constexpr size_t kMaxShared = 227 * 1024;
 
 // ---- the weight ---------------------------------------------------------------------------
@@ -114,84 +115,99 @@ struct ProjectArgs {
     uint32_t stride;  // bytes of a digit row in shared memory
 };
 
+constexpr int kProjDepth = 8;                    // slots of a warp's ring
+constexpr uint32_t kProjSlot = 512 + 64;         // a block's codes and scales
+
 // One block: 2 NT rows of x as digits in shared memory; its warps stream the
 // tiles of 16 columns, `split` warps to a tile, each a part of K (whole
 // segments where each segment is rounded by itself); their 64-bit sums meet
 // in shared memory, and a thread per output rounds and finishes it.
 template <int G, int NT, bool SEG>
-__global__ void __launch_bounds__(kProjThreads, 2) k_q4_project(const ProjectArgs p) {
+__global__ void __launch_bounds__(kProjThreads, 2) k_q4_project(const __grid_constant__ ProjectArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int kRows = 2 * NT;
     const uint32_t row0 = blockIdx.y * kRows, rows = min((uint32_t)kRows, p.m - row0);
-    uint8_t* digits = smem;
-    long long* red = reinterpret_cast<long long*>(smem + (size_t)kRows * 4 * p.stride);
-    const uint32_t kp = p.s.blocks * 64, quads = kp / 4;
-    bool bad = false;
-    for (uint32_t i = threadIdx.x; i < rows * quads; i += kProjThreads) {
-        const uint32_t r = i / quads, k0 = (i % quads) * 4;
-        const uint32_t seg = SEG ? k0 / p.s.kp_seg : 0, in = SEG ? k0 % p.s.kp_seg : k0;
-        const uint64_t* xr = p.x + (row0 + r) * p.ldx + seg * p.s.k_seg + in;
-        uint32_t d[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t v = in + j < p.s.k_seg ? fx_to_i64(__ldg(xr + j)) : 0;
-            bad |= !q4_digits(v, &d[j]);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint8_t* ring = smem + (size_t)warp * kProjDepth * kProjSlot;
+    long long* red = reinterpret_cast<long long*>(smem + (size_t)kProjWarps * kProjDepth * kProjSlot);
+    uint8_t* digits = reinterpret_cast<uint8_t*>(red + 2 * kProjWarps * kRows * 16);
+    let_next_start();
+
+    // ---- this warp's stream of blocks, and the first of them on their way
+    const uint32_t per = kProjWarps / p.split, mine = warp / p.split, part = warp % p.split;
+    const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
+    const uint32_t b0 = part * units / p.split * unit, b1 = (part + 1) * units / p.split * unit;
+    uint32_t next_tile = blockIdx.x * per + mine, next_b = b0, next_slot = 0;
+    const uint32_t tile_step = gridDim.x * per;
+    auto issue = [&]() {
+        if (next_tile < p.s.tiles && b0 < b1) {
+            uint8_t* slot = ring + next_slot * kProjSlot;
+            copy16(slot + lane * 16, p.codes + ((uint64_t)next_tile * p.s.blocks + next_b) * 32 + lane);
+            copy_scales<G>(reinterpret_cast<uint32_t*>(slot + 512), p.scales + (uint64_t)next_tile * p.s.groups * 8,
+                           next_b, g, t);
+            next_slot = next_slot + 1 == kProjDepth ? 0 : next_slot + 1;
+            if (++next_b == b1) {
+                next_b = b0;
+                next_tile += tile_step;
+            }
         }
-        uint8_t* to = digits + (size_t)r * 4 * p.stride + q4_pos(k0);
+        copy_commit();
+    };
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t lo = __byte_perm(d[0], d[1], q | ((4 + q) << 4));
-            const uint32_t hi = __byte_perm(d[2], d[3], q | ((4 + q) << 4));
-            *reinterpret_cast<uint32_t*>(to + (size_t)q * p.stride) = __byte_perm(lo, hi, 0x5410);
+    for (int i = 0; i < kProjDepth - 1; i++) issue();
+
+    // ---- the rows' digits
+    wait_for_previous();
+    const uint32_t kp = p.s.blocks * 64;
+    bool bad = false;
+    for (uint32_t r = 0; r < rows; r++) {
+        for (uint32_t k0 = threadIdx.x * 4; k0 < kp; k0 += kProjThreads * 4) {
+            const uint32_t seg = SEG ? k0 / p.s.kp_seg : 0, in = SEG ? k0 % p.s.kp_seg : k0;
+            const uint64_t* xr = p.x + (row0 + r) * p.ldx + seg * p.s.k_seg + in;
+            uint32_t d[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) bad |= !q4_digits(in + j < p.s.k_seg ? fx_to_i64(__ldg(xr + j)) : 0, &d[j]);
+            q4_store_digits(digits + (size_t)r * 4 * p.stride + q4_pos(k0), p.stride, d);
         }
     }
     if (bad) atomicOr(p.err, kErrRange);
     __syncthreads();
 
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t per = kProjWarps / p.split, mine = warp / p.split, part = warp % p.split;
-    const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
-    const uint32_t b0 = part * units / p.split * unit, b1 = (part + 1) * units / p.split * unit;
     const uint8_t* from = digits + (size_t)g * p.stride + 16 * t;  // column g: digit g % 4 of row g / 4
-    uint32_t flip = 0;
+    uint32_t flip = 0, slot_at = 0;
     for (uint32_t group = blockIdx.x; group * per < p.s.tiles; group += gridDim.x, flip ^= 1) {
         const uint32_t tile = group * per + mine;
         if (tile < p.s.tiles) {
-            const uint4* codes = p.codes + (uint64_t)tile * p.s.blocks * 32 + lane;
-            const uint32_t* scales = p.scales + (uint64_t)tile * p.s.groups * 8;
             Q4Sum<NT> sum;
             sum.clear();
             long long total[NT][2];
 #pragma unroll
             for (int i = 0; i < NT; i++) total[i][0] = total[i][1] = 0;
-            for (uint32_t b = b0; b < b1; b += 4) {
-                uint4 w[4];
-                uint32_t s0[4], s1[4];
+            for (uint32_t b = b0; b < b1; b++) {
+                __syncwarp();  // every lane has read the slot that is filled next
+                issue();
+                copy_wait<kProjDepth - 1>();
+                __syncwarp();
+                const uint8_t* slot = ring + slot_at * kProjSlot;
+                slot_at = slot_at + 1 == kProjDepth ? 0 : slot_at + 1;
+                const uint4 w = *reinterpret_cast<const uint4*>(slot + lane * 16);
+                const uint32_t s0 = reinterpret_cast<const uint32_t*>(slot + 512)[g];
+                const uint32_t s1 = G == 32 ? reinterpret_cast<const uint32_t*>(slot + 512)[8 + g] : 0;
+                uint4 x[NT];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (b + j < b1) {
-                        w[j] = ldg_stream(codes + (uint64_t)(b + j) * 32);
-                        q4_scales<G>(scales, b + j, g, &s0[j], &s1[j]);
+                for (int i = 0; i < NT; i++)
+                    x[i] = *reinterpret_cast<const uint4*>(from + (size_t)i * 8 * p.stride + b * 64);
+                q4_block<G, NT>(sum, w, s0, s1, x, b & 1);
+                if (SEG && (b + 1) % unit == 0) {
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        long long v0, v1;
+                        sum.finish(i, &v0, &v1);
+                        total[i][0] += fx_round_div_pow2(v0, p.shift);
+                        total[i][1] += fx_round_div_pow2(v1, p.shift);
                     }
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (b + j < b1) {
-                        uint4 x[NT];
-#pragma unroll
-                        for (int i = 0; i < NT; i++)
-                            x[i] = *reinterpret_cast<const uint4*>(from + (size_t)i * 8 * p.stride + (b + j) * 64);
-                        q4_block<G, NT>(sum, w[j], s0[j], s1[j], x, (b + j) & 1);
-                        if (SEG && (b + j + 1) % unit == 0) {
-#pragma unroll
-                            for (int i = 0; i < NT; i++) {
-                                long long v0, v1;
-                                sum.finish(i, &v0, &v1);
-                                total[i][0] += fx_round_div_pow2(v0, p.shift);
-                                total[i][1] += fx_round_div_pow2(v1, p.shift);
-                            }
-                            sum.clear();
-                        }
-                    }
+                    sum.clear();
+                }
             }
 #pragma unroll
             for (int i = 0; i < NT; i++) {
@@ -220,16 +236,14 @@ __global__ void __launch_bounds__(kProjThreads, 2) k_q4_project(const ProjectArg
     }
 }
 
-uint32_t digit_stride(uint32_t blocks) {
-    const uint32_t kp = blocks * 64;
-    return kp % 128 ? kp : kp + 64;  // 64 mod 128: the eight lanes of a phase read 128 different bytes
-}
+constexpr size_t kProjRing = (size_t)kProjWarps * kProjDepth * kProjSlot;
 
 template <int G, int NT, bool SEG>
 int project_launch(ProjectArgs p, cudaStream_t stream) {
-    const size_t shared = (size_t)2 * NT * 4 * p.stride + 2ull * kProjWarps * 2 * NT * 16 * 8;
+    const size_t shared = kProjRing + (size_t)2 * NT * 4 * p.stride + 2ull * kProjWarps * 2 * NT * 16 * 8;
     auto* kernel = k_q4_project<G, NT, SEG>;
-    ZK_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxShared));
+    static std::atomic<uint64_t> set{0};
+    ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kMaxShared, &set));
     const uint32_t at_once = kSms * (shared > kMaxShared / 2 ? 1 : 2);
     // Warps to a tile: the fewest steps of a block's warps, each with what a tile costs besides its blocks
     const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
@@ -244,9 +258,7 @@ int project_launch(ProjectArgs p, cudaStream_t stream) {
     }
     const uint64_t groups = ceil_div(p.s.tiles, kProjWarps / p.split);
     const dim3 grid((unsigned)(groups < at_once ? groups : at_once), (unsigned)ceil_div(p.m, 2 * NT));
-    kernel<<<grid, kProjThreads, shared, stream>>>(p);
-    ZK_LAUNCH_CHECK();
-    return 0;
+    return launch(kernel, grid, kProjThreads, shared, 1, stream, p);
 }
 
 template <int G, int NT>
@@ -258,8 +270,8 @@ template <int G>
 int project_rows(const ProjectArgs& p, cudaStream_t stream) {
     // rows to a block: up to eight, as many as their digits leave room for
     const uint64_t row = 4ull * p.stride, red = 2ull * kProjWarps * 16 * 8;
-    if (p.m > 4 && 8 * (row + red) <= kMaxShared) return project_seg<G, 4>(p, stream);
-    if (p.m > 2 && 4 * (row + red) <= kMaxShared) return project_seg<G, 2>(p, stream);
+    if (p.m > 4 && kProjRing + 8 * (row + red) <= kMaxShared) return project_seg<G, 4>(p, stream);
+    if (p.m > 2 && kProjRing + 4 * (row + red) <= kMaxShared) return project_seg<G, 2>(p, stream);
     return project_seg<G, 1>(p, stream);
 }
 
@@ -330,6 +342,8 @@ __global__ void k_kv_append(KvCache c, KvRows rows, uint32_t tokens, uint32_t* _
 
 constexpr int kAttThreads = 256;
 constexpr int kAttWarps = kAttThreads / 32;
+constexpr uint32_t kMaxRanks = 16;
+constexpr size_t kAttShared = 220 * 1024;
 
 struct AttendArgs {
     KvCache c;
@@ -346,24 +360,29 @@ struct AttendArgs {
     uint64_t* out;
     uint32_t* err;
     uint32_t chunk;  // tokens of a block's share of the scores
+    uint32_t slice;  // outputs that a block of the cluster finishes
 };
 
 // One cluster per sequence, key head and EACH of its query heads; a block
 // takes an equal run of the token blocks.  The softmax's rounding needs the
 // row's maximum and then its sum before any weight is known, so the scores
 // stay in shared memory and the cluster meets twice, keys and values each
-// being read once; the blocks' value sums meet in a third exchange.
+// being read once; the blocks' value sums meet in a third exchange.  A block
+// writes what the others need into their shared memory before each meeting,
+// so that nothing is fetched from a neighbour after it.
 template <int EACH>
-__global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
+__global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_constant__ AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long s_red[kAttWarps][EACH];
-    __shared__ long long s_max[EACH], s_sum[EACH];
+    __shared__ long long s_max[kMaxRanks][EACH], s_sum[kMaxRanks][EACH];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t seq = blockIdx.z, h = blockIdx.y / p.groups, e0 = (blockIdx.y % p.groups) * EACH;
     const uint32_t heads = min((uint32_t)EACH, p.each - e0), dk = p.c.dk, dv = p.c.dv;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t* out = p.out + ((uint64_t)seq * p.c.heads * p.each + (uint64_t)h * p.each + e0) * dv;
+    let_next_start();
+    wait_for_previous();
 
     const int64_t len = p.c.lens[seq];
     const bool append = p.rows.k != nullptr && len >= 0 && len < p.c.cap;
@@ -373,15 +392,30 @@ __global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
         for (uint32_t i = rank * kAttThreads + threadIdx.x; i < heads * dv; i += ranks * kAttThreads) out[i] = 0;
         return;
     }
+    cluster_arrive();  // every block has started before another writes into its shared memory
     const uint32_t blocks = (n + kKvBlock - 1) / kKvBlock;
     const uint32_t b0 = (uint32_t)((uint64_t)rank * blocks / ranks), b1 = (uint32_t)((uint64_t)(rank + 1) * blocks / ranks);
     const uint32_t t0 = b0 * kKvBlock, count = b1 > b0 ? min(b1 * kKvBlock, n) - t0 : 0;
+    const uint64_t head = (uint64_t)seq * p.c.heads + h;
+    int32_t* const keys = p.c.k + key_at(head, p.c.cap / kKvBlock, dk, t0, 0);
+    int32_t* const values = p.c.v + (head * p.c.cap + t0) * dv;
+    // this block's keys and values, both in one piece, start for the second-level cache
+    {
+        constexpr uint32_t kPiece = 8192;
+        const uint64_t kb = (uint64_t)(b1 - b0) * kKvBlock * dk * 4, vb = (uint64_t)count * dv * 4;
+        const uint32_t kn = (uint32_t)((kb + kPiece - 1) / kPiece), vn = (uint32_t)((vb + kPiece - 1) / kPiece);
+        for (uint32_t i = threadIdx.x; i < kn + vn; i += kAttThreads) {
+            const uint64_t at = (uint64_t)(i < kn ? i : i - kn) * kPiece, left = (i < kn ? kb : vb) - at;
+            prefetch_l2(reinterpret_cast<const uint8_t*>(i < kn ? keys : values) + at,
+                        (uint32_t)(left < kPiece ? left : kPiece));
+        }
+    }
 
-    long long* scores = reinterpret_cast<long long*>(smem);                               // EACH x chunk
-    unsigned long long* acc = reinterpret_cast<unsigned long long*>(scores + (size_t)EACH * p.chunk);  // EACH x dv
-    int* qs = reinterpret_cast<int*>(acc + (size_t)EACH * dv);                            // EACH x dk
+    long long* scores = reinterpret_cast<long long*>(smem);                  // EACH x chunk
+    long long* sums = scores + (size_t)EACH * p.chunk;                       // EACH x 4 threads: value sums
+    unsigned long long* acc = reinterpret_cast<unsigned long long*>(sums + (size_t)EACH * 4 * kAttThreads);
+    int* qs = reinterpret_cast<int*>(acc + (((size_t)ranks * p.slice + 1) & ~(size_t)1));  // EACH x dk
     bool bad = false;
-    for (uint32_t i = threadIdx.x; i < EACH * dv; i += kAttThreads) acc[i] = 0;
     for (uint32_t i = threadIdx.x; i < EACH * dk; i += kAttThreads) {
         int64_t y = 0;
         if (i / dk < heads) {
@@ -401,26 +435,32 @@ __global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
             bad |= !kv_store(p.c, p.rows, seq, seq, h, (uint64_t)len, d);
     __syncthreads();
 
-    const uint64_t head = (uint64_t)seq * p.c.heads + h;
     long long top[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) top[e] = INT64_MIN;
-    for (uint32_t b = b0 + warp; b < b1; b += kAttWarps) {
-        const int32_t* kb = p.c.k + key_at(head, p.c.cap / kKvBlock, dk, (uint64_t)b * kKvBlock + lane, 0);
+    for (uint32_t b = warp; b < b1 - b0; b += kAttWarps) {
+        const int32_t* kb = keys + (size_t)b * kKvBlock * dk + lane * 4;
         long long s[EACH];
 #pragma unroll
         for (int e = 0; e < EACH; e++) s[e] = 0;
-#pragma unroll 8
-        for (uint32_t d = 0; d < dk; d += 4) {
-            const int4 kv = __ldcg(reinterpret_cast<const int4*>(kb + (size_t)d * kKvBlock));
+        constexpr int kAhead = 8;
+        for (uint32_t d0 = 0; d0 < dk; d0 += 4 * kAhead) {
+            int4 kv[kAhead];
 #pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                const int4 qv = *reinterpret_cast<const int4*>(qs + e * dk + d);
-                s[e] += (long long)qv.x * kv.x + (long long)qv.y * kv.y + (long long)qv.z * kv.z +
-                        (long long)qv.w * kv.w;
-            }
+            for (int i = 0; i < kAhead; i++)
+                if (d0 + 4 * i < dk) kv[i] = __ldcg(reinterpret_cast<const int4*>(kb + (size_t)(d0 + 4 * i) * kKvBlock));
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (d0 + 4 * i < dk) {
+#pragma unroll
+                    for (int e = 0; e < EACH; e++) {
+                        const int4 qv = *reinterpret_cast<const int4*>(qs + e * dk + d0 + 4 * i);
+                        s[e] += (long long)qv.x * kv[i].x + (long long)qv.y * kv[i].y + (long long)qv.z * kv[i].z +
+                                (long long)qv.w * kv[i].w;
+                    }
+                }
         }
-        const uint32_t at = b * kKvBlock + lane - t0;
+        const uint32_t at = b * kKvBlock + lane;
         if (at < count) {
 #pragma unroll
             for (int e = 0; e < EACH; e++) {
@@ -439,21 +479,21 @@ __global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
         if (lane == 0) s_red[warp][e] = top[e];
     }
     __syncthreads();
-    if (threadIdx.x < EACH) {
-        long long v = s_red[0][threadIdx.x];
-        for (int w = 1; w < kAttWarps; w++) v = max(v, s_red[w][threadIdx.x]);
-        s_max[threadIdx.x] = v;
+    cluster_wait();
+    for (uint32_t i = threadIdx.x; i < ranks * EACH; i += kAttThreads) {
+        const uint32_t r = i / EACH, e = i % EACH;
+        long long v = s_red[0][e];
+        for (int w = 1; w < kAttWarps; w++) v = max(v, s_red[w][e]);
+        *cluster.map_shared_rank(&s_max[rank][e], r) = v;
     }
     cluster.sync();
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        top[e] = INT64_MIN;
-        for (uint32_t r = 0; r < ranks; r++) top[e] = max(top[e], *cluster.map_shared_rank(&s_max[e], r));
-    }
-
     long long part[EACH];
 #pragma unroll
-    for (int e = 0; e < EACH; e++) part[e] = 0;
+    for (int e = 0; e < EACH; e++) {
+        top[e] = s_max[0][e];
+        for (uint32_t r = 1; r < ranks; r++) top[e] = max(top[e], s_max[r][e]);
+        part[e] = 0;
+    }
     for (uint32_t j = threadIdx.x; j < count; j += kAttThreads) {
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
@@ -473,17 +513,18 @@ __global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
         if (lane == 0) s_red[warp][e] = part[e];
     }
     __syncthreads();
-    if (threadIdx.x < EACH) {
+    for (uint32_t i = threadIdx.x; i < ranks * EACH; i += kAttThreads) {
+        const uint32_t r = i / EACH, e = i % EACH;
         long long v = 0;
-        for (int w = 0; w < kAttWarps; w++) v += s_red[w][threadIdx.x];
-        s_sum[threadIdx.x] = v;
+        for (int w = 0; w < kAttWarps; w++) v += s_red[w][e];
+        *cluster.map_shared_rank(&s_sum[rank][e], r) = v;
     }
     cluster.sync();
     double inv[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         part[e] = 0;
-        for (uint32_t r = 0; r < ranks; r++) part[e] += *cluster.map_shared_rank(&s_sum[e], r);
+        for (uint32_t r = 0; r < ranks; r++) part[e] += s_sum[r][e];
         if (part[e] == 0 && e < heads && rank == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDivide);
         inv[e] = part[e] ? 1.0 / (double)part[e] : 0.0;
     }
@@ -502,64 +543,68 @@ __global__ void __launch_bounds__(kAttThreads) k_kv_attend(const AttendArgs p) {
         long long y[EACH][4];
 #pragma unroll
         for (int e = 0; e < EACH; e++) y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0;
-        const int32_t* vb = p.c.v + (head * p.c.cap + t0) * dv + d4 * 4;
-#pragma unroll 4
-        for (uint32_t j = phase; j < count; j += step) {
-            const int4 vv = __ldcg(reinterpret_cast<const int4*>(vb + (size_t)j * dv));
+        const int32_t* vb = values + d4 * 4;
+        constexpr int kAhead = 8;
+        for (uint32_t j0 = phase; j0 < count; j0 += kAhead * step) {
+            int4 vv[kAhead];
 #pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                const int w = (int)scores[(size_t)e * p.chunk + j];
-                y[e][0] += (long long)w * vv.x;
-                y[e][1] += (long long)w * vv.y;
-                y[e][2] += (long long)w * vv.z;
-                y[e][3] += (long long)w * vv.w;
-            }
+            for (int i = 0; i < kAhead; i++)
+                if (j0 + i * step < count) vv[i] = __ldcg(reinterpret_cast<const int4*>(vb + (size_t)(j0 + i * step) * dv));
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (j0 + i * step < count) {
+#pragma unroll
+                    for (int e = 0; e < EACH; e++) {
+                        const int w = (int)scores[(size_t)e * p.chunk + j0 + i * step];
+                        y[e][0] += (long long)w * vv[i].x;
+                        y[e][1] += (long long)w * vv[i].y;
+                        y[e][2] += (long long)w * vv[i].z;
+                        y[e][3] += (long long)w * vv[i].w;
+                    }
+                }
         }
 #pragma unroll
         for (int e = 0; e < EACH; e++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) atomicAdd(&acc[e * dv + d4 * 4 + i], (unsigned long long)y[e][i]);
+            for (int i = 0; i < 4; i++) sums[((size_t)e * step + phase) * dv + d4 * 4 + i] = y[e][i];
     }
     if (bad) atomicOr(p.err, kErrRange);
-    cluster.sync();
-    for (uint32_t i = rank * kAttThreads + threadIdx.x; i < heads * dv; i += ranks * kAttThreads) {
+    __syncthreads();
+    // output i belongs to block i / slice: its part goes there
+    for (uint32_t i = threadIdx.x; i < heads * dv; i += kAttThreads) {
+        const uint32_t e = i / dv, d = i % dv;
         unsigned long long v = 0;
-        for (uint32_t r = 0; r < ranks; r++) v += *cluster.map_shared_rank(&acc[i], r);
-        out[i] = fx_from_i64(fx_round_div_pow2((int64_t)v, p.out_shift));
+        for (uint32_t s = 0; s < step; s++) v += (unsigned long long)sums[((size_t)e * step + s) * dv + d];
+        *cluster.map_shared_rank(&acc[(size_t)rank * p.slice + i % p.slice], i / p.slice) = v;
     }
-    cluster.sync();  // no block leaves while its sums may still be read
+    cluster.sync();
+    for (uint32_t i = threadIdx.x; i < p.slice && rank * p.slice + i < heads * dv; i += kAttThreads) {
+        unsigned long long v = 0;
+        for (uint32_t r = 0; r < ranks; r++) v += acc[(size_t)r * p.slice + i];
+        out[rank * p.slice + i] = fx_from_i64(fx_round_div_pow2((int64_t)v, p.out_shift));
+    }
 }
 
-size_t attend_shared(uint32_t each, uint32_t chunk, uint32_t dk, uint32_t dv) {
-    return (size_t)each * (8ull * chunk + 8ull * dv + 4ull * dk);
+size_t attend_shared(uint32_t each, uint32_t ranks, uint32_t blocks, uint32_t dk, uint32_t dv) {
+    const uint64_t chunk = ceil_div(blocks, ranks) * kKvBlock, slice = ceil_div(each * dv, ranks);
+    return each * (8 * chunk + 32ull * kAttThreads + 4ull * dk) + 8 * ((ranks * slice + 1) & ~1ull);
 }
 
 template <int EACH>
 int attend_launch(AttendArgs p, uint32_t ranks, cudaStream_t stream) {
     p.groups = (uint32_t)ceil_div(p.each, EACH);
     p.chunk = (uint32_t)ceil_div(p.c.cap / kKvBlock, ranks) * kKvBlock;
-    const size_t shared = attend_shared(EACH, p.chunk, p.c.dk, p.c.dv);
+    p.slice = (uint32_t)ceil_div(EACH * p.c.dv, ranks);
+    const size_t shared = attend_shared(EACH, ranks, p.c.cap / kKvBlock, p.c.dk, p.c.dv);
     auto* kernel = k_kv_attend<EACH>;
-    ZK_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(220 * 1024)));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ranks, p.c.heads * p.groups, p.c.batch);
-    cfg.blockDim = dim3(kAttThreads);
-    cfg.dynamicSmemBytes = shared;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    ZK_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
-    return 0;
+    static std::atomic<uint64_t> set{0};
+    ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kAttShared, &set, true));
+    return launch(kernel, dim3(ranks, p.c.heads * p.groups, p.c.batch), kAttThreads, shared, ranks, stream, p);
 }
 
 // ---- the next token ---------------------------------------------------------------------------
 constexpr int kChooseThreads = 512;
 constexpr int kChooseWarps = kChooseThreads / 32;
-constexpr uint32_t kCounts = 8192;  // vocabulary entries counted at a time
 
 struct ChooseArgs {
     const uint64_t* logits;
@@ -578,18 +623,25 @@ struct ChooseArgs {
     uint32_t* err;
 };
 
-// One cluster per row, a block to an equal slice of the vocabulary: counts of
-// the history's tokens in shared memory, then one pass over the slice; the
-// blocks' maxima meet in the first block.
-__global__ void __launch_bounds__(kChooseThreads) k_choose_token(const ChooseArgs p) {
-    __shared__ uint32_t counts[kCounts];
+constexpr int kChooseEach = 8;  // logits of a thread at a time
+
+// One cluster per row, a block to an equal slice of the vocabulary, a step of
+// 4096 at a time: the logits start for registers, the history's tokens are
+// counted in shared memory, then the logits are finished; the blocks' maxima
+// meet in the first block.
+__global__ void __launch_bounds__(kChooseThreads) k_choose_token(const __grid_constant__ ChooseArgs p) {
+    constexpr uint32_t kStep = kChooseThreads * kChooseEach;
+    __shared__ uint32_t counts[kStep];
     __shared__ long long s_v[kChooseWarps];
     __shared__ unsigned long long s_j[kChooseWarps];
-    __shared__ long long best_v;
-    __shared__ unsigned long long best_j;
+    __shared__ long long best_v[kMaxRanks];
+    __shared__ unsigned long long best_j[kMaxRanks];
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint64_t row = blockIdx.y, lo = p.v * rank / ranks, hi = p.v * (rank + 1) / ranks;
+    cluster_arrive();  // every block has started before another writes into its shared memory
+    let_next_start();
+    wait_for_previous();
     uint64_t past = 0;
     if (p.history) {
         past = p.history_len;
@@ -601,35 +653,50 @@ __global__ void __launch_bounds__(kChooseThreads) k_choose_token(const ChooseArg
     long long bv = INT64_MIN;
     unsigned long long bj = UINT64_MAX;
     bool bad = false;
-    for (uint64_t s0 = lo; s0 < hi; s0 += kCounts) {
-        const uint64_t s1 = s0 + kCounts < hi ? s0 + kCounts : hi;
+    for (uint64_t s0 = lo; s0 < hi; s0 += kStep) {
+        const uint64_t s1 = s0 + kStep < hi ? s0 + kStep : hi;
+        int64_t y[kChooseEach];
+#pragma unroll
+        for (int i = 0; i < kChooseEach; i++) {
+            const uint64_t j = s0 + i * kChooseThreads + threadIdx.x;
+            if (j < s1) y[i] = fx_to_i64(__ldg(p.logits + row * p.v + j));
+        }
         if (past) {
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < s1 - s0; i += kChooseThreads) counts[i] = 0;
+            for (uint32_t i = threadIdx.x; i < kStep; i += kChooseThreads) counts[i] = 0;
             __syncthreads();
-            for (uint64_t i = threadIdx.x; i < past; i += kChooseThreads) {
-                const int64_t tok = __ldg(p.history + row * p.history_len + i);
-                if (tok < 0 || tok >= (int64_t)p.v)
-                    bad = true;
-                else if ((uint64_t)tok >= s0 && (uint64_t)tok < s1)
-                    atomicAdd(&counts[tok - s0], 1u);
+            const int32_t* hist = p.history + row * p.history_len;
+            for (uint64_t i0 = threadIdx.x; i0 < past; i0 += kChooseThreads * 8) {
+                int32_t tok[8];
+#pragma unroll
+                for (int q = 0; q < 8; q++)
+                    if (i0 + q * kChooseThreads < past) tok[q] = __ldg(hist + i0 + q * kChooseThreads);
+#pragma unroll
+                for (int q = 0; q < 8; q++)
+                    if (i0 + q * kChooseThreads < past) {
+                        bad |= tok[q] < 0 || (uint64_t)tok[q] >= p.v;
+                        const uint64_t at = (uint64_t)tok[q] - s0;  // huge for a token before the step
+                        if (tok[q] >= 0 && at < s1 - s0) atomicAdd(&counts[at], 1u);
+                    }
             }
             __syncthreads();
         }
-        for (uint64_t j = s0 + threadIdx.x; j < s1; j += kChooseThreads) {
-            int64_t y = fx_to_i64(__ldg(p.logits + row * p.v + j));
+#pragma unroll
+        for (int i = 0; i < kChooseEach; i++) {
+            const uint64_t j = s0 + i * kChooseThreads + threadIdx.x;
+            if (j >= s1) continue;
+            int64_t z = y[i];
             const uint32_t c = past ? counts[j - s0] : 0;
             if (c) {
-                y = fx_round_div_pow2(fx_wmul(y, y > 0 ? p.repeat_pos : p.repeat_neg), 16);
-                y = fx_wsub(fx_wsub(y, p.presence), fx_wmul(p.frequency, c));
+                z = fx_round_div_pow2(fx_wmul(z, z > 0 ? p.repeat_pos : p.repeat_neg), 16);
+                z = fx_wsub(fx_wsub(z, p.presence), fx_wmul(p.frequency, c));
             }
-            if (p.bias) y = fx_wadd(y, fx_to_i64(__ldg(p.bias + row * p.bias_stride + j)));
+            if (p.bias) z = fx_wadd(z, fx_to_i64(__ldg(p.bias + row * p.bias_stride + j)));
             if (p.allowed && !((__ldg(p.allowed + row * p.allowed_stride + j / 32) >> (j % 32)) & 1))
-                y = fx_wadd(y, p.mask_value);
-            const uint64_t f = fx_from_i64(y);
-            p.out[row * p.v + j] = f;
-            if (y > bv || bj == UINT64_MAX) {
-                bv = y;
+                z = fx_wadd(z, p.mask_value);
+            p.out[row * p.v + j] = fx_from_i64(z);
+            if (z > bv || bj == UINT64_MAX) {
+                bv = z;
                 bj = j;
             }
         }
@@ -652,18 +719,17 @@ __global__ void __launch_bounds__(kChooseThreads) k_choose_token(const ChooseArg
         s_j[warp] = bj;
     }
     __syncthreads();
+    cluster_wait();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kChooseWarps; w++) take(s_v[w], s_j[w]);
-        best_v = bv;
-        best_j = bj;
+        *cluster.map_shared_rank(&best_v[rank], 0) = bv;
+        *cluster.map_shared_rank(&best_j[rank], 0) = bj;
     }
     cluster.sync();
     if (rank == 0 && threadIdx.x == 0) {
-        for (uint32_t r = 1; r < ranks; r++)
-            take(*cluster.map_shared_rank(&best_v, r), *cluster.map_shared_rank(&best_j, r));
+        for (uint32_t r = 0; r < ranks; r++) take(best_v[r], best_j[r]);
         p.token[row] = (uint32_t)bj;
     }
-    cluster.sync();
 }
 
 }  // namespace
@@ -726,7 +792,7 @@ int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32
     p.ldr = ldr;
     p.out = d_out;
     p.err = d_err;
-    p.stride = digit_stride(p.s.blocks);
+    p.stride = q4_digit_stride(p.s.blocks);
     return group == 32 ? project_rows<32>(p, stream) : group == 64 ? project_rows<64>(p, stream)
                                                                     : project_rows<128>(p, stream);
 }
@@ -784,16 +850,13 @@ int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t
     // Query heads to a block: those that share a key head, up to four (their
     // sums stay in registers); fewer where their scores do not fit.  Blocks to
     // a cluster: enough to fill the device, more where the scores need it.
-    const uint32_t most = 8, blocks = (uint32_t)(capacity / kKvBlock);
+    const uint32_t blocks = (uint32_t)(capacity / kKvBlock);
     for (uint32_t each = p.each >= 3 ? 4 : p.each;; each /= 2) {
         const uint64_t rows = batch * heads * ceil_div(p.each, each);
         uint32_t ranks = 1;
-        while (ranks < most && rows * ranks < 2 * kSms && ranks < blocks) ranks *= 2;
-        while (ranks < most &&
-               attend_shared(each, (uint32_t)ceil_div(blocks, ranks) * kKvBlock, p.c.dk, p.c.dv) > 220 * 1024)
-            ranks *= 2;
-        if (attend_shared(each, (uint32_t)ceil_div(blocks, ranks) * kKvBlock, p.c.dk, p.c.dv) > 220 * 1024 && each > 1)
-            continue;
+        while (ranks < kMaxRanks && rows * ranks * 2 <= 2 * kSms && ranks < blocks) ranks *= 2;
+        while (ranks < kMaxRanks && attend_shared(each, ranks, blocks, p.c.dk, p.c.dv) > kAttShared) ranks *= 2;
+        if (attend_shared(each, ranks, blocks, p.c.dk, p.c.dv) > kAttShared && each > 1) continue;
         return each == 4 ? attend_launch<4>(p, ranks, stream) : each == 2 ? attend_launch<2>(p, ranks, stream)
                                                                           : attend_launch<1>(p, ranks, stream);
     }
@@ -811,20 +874,13 @@ int zkie2_choose_token(const uint64_t* d_logits, uint64_t batch, uint64_t vocab,
     if (!d_logits || !d_out || !d_token) return (int)cudaErrorInvalidValue;
     const ChooseArgs p{d_logits, vocab, d_history, history_len, d_history_lens, repeat_pos, repeat_neg, presence,
                        frequency, d_bias, bias_stride, d_allowed, allowed_stride, mask_value, d_out, d_token, d_err};
+    // Blocks to a row: one step of the vocabulary each, fewer once the rows fill the device
     uint32_t ranks = 1;
-    while (ranks < 8 && vocab > (uint64_t)ranks * kChooseThreads * 2) ranks *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ranks, (unsigned)batch);
-    cfg.blockDim = dim3(kChooseThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    ZK_TRY(cudaLaunchKernelEx(&cfg, k_choose_token, p));
-    return 0;
+    while (ranks < kMaxRanks && vocab > (uint64_t)ranks * kChooseThreads * kChooseEach && batch * ranks < 2 * kSms)
+        ranks *= 2;
+    static std::atomic<uint64_t> set{0};
+    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_choose_token), 0, &set, true));
+    return launch(k_choose_token, dim3(ranks, (unsigned)batch), kChooseThreads, 0, ranks, stream, p);
 }
 
 }  // extern "C"

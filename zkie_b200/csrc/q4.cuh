@@ -72,6 +72,20 @@ __device__ __forceinline__ bool q4_digits(int64_t v, uint32_t* d) {
     return ok;
 }
 
+// the digits of four consecutive k, one word to each of the four digit rows
+__device__ __forceinline__ void q4_store_digits(uint8_t* to, size_t stride, const uint32_t (&d)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const uint32_t lo = __byte_perm(d[0], d[1], q | ((4 + q) << 4));
+        const uint32_t hi = __byte_perm(d[2], d[3], q | ((4 + q) << 4));
+        *reinterpret_cast<uint32_t*>(to + q * stride) = __byte_perm(lo, hi, 0x5410);
+    }
+}
+
+// bytes of a digit row: 64 mod 128, so that the eight lanes that read at once
+// (two rows, 64 bytes each) meet no shared-memory bank twice
+inline uint32_t q4_digit_stride(uint32_t blocks) { return blocks % 2 ? blocks * 64 : blocks * 64 + 64; }
+
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
     asm volatile(
@@ -80,12 +94,52 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
+// ---- asynchronous copies: a warp's ring of slots in shared memory ---------------------------
+// A lane copies the 16 bytes that it will read itself (scales: a few lanes,
+// for all), so a slot is ready when the lane's own copies are and the warp has
+// met once; the bytes in flight do not depend on registers, and the stream of
+// a warp's blocks runs on across tiles, sums and barriers.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// wait until at most n (< N + 1) of the groups asked for are still on their way
+template <int N>
+__device__ __forceinline__ void copy_wait_upto(uint32_t n) {
+    if constexpr (N == 0) {
+        copy_wait<0>();
+    } else {
+        if (n >= N)
+            copy_wait<N>();
+        else
+            copy_wait_upto<N - 1>(n);
+    }
+}
+
+// ---- overlap with the kernel before (programmatic dependent launch) --------------------------
+// Every kernel here lets its successor start early and waits, before it reads
+// or writes anything that an earlier kernel may have written or may still
+// read, until all earlier kernels are done.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// the two halves of a cluster's barrier
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+// a run of bytes (16-byte aligned, a multiple of 16) into the second-level cache
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 // Running sums of one tile of 16 columns against NT pairs of rows: c the
@@ -102,10 +156,11 @@ struct Q4Sum {
             a[i][0] = a[i][1] = 0;
         }
     }
+    template <int N>
     __device__ __forceinline__ void scale_group(uint32_t s) {
         const int s0 = (int)(s & 0xFFFFu), s1 = (int)(s >> 16);
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
+        for (int i = 0; i < N; i++) {
             a[i][0] += (long long)(c[i][0] + (c[i][1] << 8)) * s0;
             a[i][1] += (long long)(c[i][2] + (c[i][3] << 8)) * s1;
             c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0;
@@ -128,11 +183,11 @@ struct Q4Sum {
     }
 };
 
-// One block of 64 k: w the lane's codes, s0 (and s1 for G = 32) the scales of
+// One block of 64 k for NT of the MAX pairs: w the lane's codes, s0 (and s1 for G = 32) the scales of
 // the block's group(s), b the lane's digits; `last` where a group of 128 ends.
-template <int G, int NT>
-__device__ __forceinline__ void q4_block(Q4Sum<NT>& sum, const uint4& w, uint32_t s0, uint32_t s1,
-                                         const uint4 (&b)[NT], bool last) {
+template <int G, int NT, int MAX>
+__device__ __forceinline__ void q4_block_n(Q4Sum<MAX>& sum, const uint4& w, uint32_t s0, uint32_t s1,
+                                           const uint4 (&b)[MAX], bool last) {
     constexpr uint32_t kHigh = 0xF0F0F0F0u;  // a code in a byte's high half is sixteen times itself
     {
         const uint32_t a0 = (w.x << 4) & kHigh, a1 = (w.y << 4) & kHigh, a2 = (w.z << 4) & kHigh,
@@ -140,30 +195,34 @@ __device__ __forceinline__ void q4_block(Q4Sum<NT>& sum, const uint4& w, uint32_
 #pragma unroll
         for (int i = 0; i < NT; i++) mma_s8(sum.c[i], a0, a1, a2, a3, b[i].x, b[i].y);
     }
-    if (G == 32) sum.scale_group(s0);
+    if (G == 32) sum.template scale_group<NT>(s0);
     {
         const uint32_t a0 = w.x & kHigh, a1 = w.y & kHigh, a2 = w.z & kHigh, a3 = w.w & kHigh;
 #pragma unroll
         for (int i = 0; i < NT; i++) mma_s8(sum.c[i], a0, a1, a2, a3, b[i].z, b[i].w);
     }
     if (G == 32)
-        sum.scale_group(s1);
+        sum.template scale_group<NT>(s1);
     else if (G == 64)
-        sum.scale_group(s0);
+        sum.template scale_group<NT>(s0);
     else if (last)
-        sum.scale_group(s0);
+        sum.template scale_group<NT>(s0);
 }
 
-// The scale words of block b of a tile (lane's own): s0, and s1 for G = 32.
+template <int G, int NT>
+__device__ __forceinline__ void q4_block(Q4Sum<NT>& sum, const uint4& w, uint32_t s0, uint32_t s1,
+                                         const uint4 (&b)[NT], bool last) {
+    q4_block_n<G, NT, NT>(sum, w, s0, s1, b, last);
+}
+
+// The scale words of block b of a tile into a slot (16 words): lanes t = 0,
+// and t = 1 for G = 32 with its second group.
 template <int G>
-__device__ __forceinline__ void q4_scales(const uint32_t* __restrict__ tile_scales, uint32_t b, uint32_t g,
-                                          uint32_t* s0, uint32_t* s1) {
-    if (G == 32) {
-        *s0 = __ldg(tile_scales + (2 * b) * 8 + g);
-        *s1 = __ldg(tile_scales + (2 * b + 1) * 8 + g);
-    } else {
-        *s0 = __ldg(tile_scales + (G == 64 ? b : b / 2) * 8 + g);
-        *s1 = 0;
+__device__ __forceinline__ void copy_scales(uint32_t* to, const uint32_t* tile_scales, uint32_t b, uint32_t g,
+                                            uint32_t t) {
+    if (t < (G == 32 ? 2 : 1)) {
+        const uint32_t group = G == 32 ? 2 * b + t : (G == 64 ? b : b / 2);
+        copy4(to + 8 * t + g, tile_scales + (uint64_t)group * 8 + g);
     }
 }
 
