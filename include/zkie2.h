@@ -637,32 +637,28 @@ int zkie2_eq_combine(const uint64_t *h_points, const uint64_t *h_coeffs, uint32_
  * a whole sequence; every result equals the same row of the arms named with
  * it, bit for bit.  Beside the bits of *d_err above: 8, a value outside the
  * range that the kernels take (it is replaced by zero); 16, a cache without
- * room.  None of these synchronizes; row strides (ld*) are in elements. */
+ * room; 32, a copy that did not arrive (the call's results are void).  None of these synchronizes; row strides (ld*) are in elements. */
 
 /* A weight in 4 bits: w[k][n] = codes[k][n] * scales[row(k)][n] with codes in
  * [-8, 7] and scales in [0, 65535], one scale to `group` (32, 64 or 128) rows
  * of a column.  segment > 0 splits the k rows into k / segment runs, each
  * with ceil(segment / group) rows of scales and rounded by itself in the
- * product.  At most 8192 rows, each run counted as a multiple of 64 (128 for
- * group = 128).  `experts` weights of one shape lie one after another.
- * codes: experts x k x n; scales: experts x rows x n; the packed forms hold
- * the numbers of u32 words that the queries give (0: refused shape), the
- * codes 16-byte aligned. */
-uint64_t zkie2_q4_code_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment);
-uint64_t zkie2_q4_scale_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment);
+ * product.  At most 8192 rows, each run counted as a multiple of 64.
+ * `experts` weights of one shape lie one after another.  codes: experts x k x
+ * n; scales: experts x rows x n; packed: the number of u32 words that the
+ * query gives (0: refused shape), 16-byte aligned. */
+uint64_t zkie2_q4_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment);
 int zkie2_q4_pack(const int8_t *d_codes, const int32_t *d_scales, uint64_t experts, uint64_t k, uint64_t n,
-                  uint32_t group, uint64_t segment, uint32_t *d_packed, uint32_t *d_packed_scales, uint32_t *d_err,
-                  zkie_stream_t stream);
+                  uint32_t group, uint64_t segment, uint32_t *d_packed, uint32_t *d_err, zkie_stream_t stream);
 /* Op::Projection's out (Op::MatMul for shift = 0 and no bias) of m rows by one
  * packed weight: y = sum over segments of round_div(x w, 2^shift), + bias (n
  * values); with a table then table[clamp(y + offset, 0, table_len - 1)]
  * (Op::GeluIndex, Op::Lookup); with a residual (m x n) + residual
  * (Op::Add).  |x| <= 0x7F7F7F7F.  out: m x n. */
-int zkie2_q4_project(const uint64_t *d_x, uint64_t ldx, uint64_t m, const uint32_t *d_packed,
-                     const uint32_t *d_packed_scales, uint64_t k, uint64_t n, uint32_t group, uint64_t segment,
-                     uint32_t shift, const uint64_t *d_bias, const uint64_t *d_table, uint64_t table_len,
-                     int64_t offset, const uint64_t *d_residual, uint64_t ldr, uint64_t *d_out, uint32_t *d_err,
-                     zkie_stream_t stream);
+int zkie2_q4_project(const uint64_t *d_x, uint64_t ldx, uint64_t m, const uint32_t *d_packed, uint64_t k, uint64_t n,
+                     uint32_t group, uint64_t segment, uint32_t shift, const uint64_t *d_bias,
+                     const uint64_t *d_table, uint64_t table_len, int64_t offset, const uint64_t *d_residual,
+                     uint64_t ldr, uint64_t *d_out, uint32_t *d_err, zkie_stream_t stream);
 
 /* A cache of `batch` sequences: keys int32 (batch, heads, capacity / 32, dk /
  * 4, 32, 4), values int32 (batch, heads, capacity, dv), lens int32 (batch);
@@ -692,22 +688,22 @@ int zkie2_kv_attend(const uint64_t *d_q, uint64_t ldq, uint64_t q_heads, int64_t
 
 /* build_moe (models/deepseek-v2-lite/src/lib.rs:252-470) of m rows, two
  * launches to 16 rows: h wide, `experts` routed (top_k of them, hidden f) and
- * the shared experts (hidden shared_f) with weights of one group; h_codes and
- * h_scales: host arrays of 6 device pointers (packed gate, up, down, shared
+ * the shared experts (hidden shared_f) with weights of one group;
+ * h_weights: a host array of 6 device pointers (packed gate, up, down, shared
  * gate, up, down); the router packed from h x experts field elements of at
  * most 32639 in size.  Every Scale divides by 2^shift; the silu table is
  * indexed from its middle.  experts <= 256, top_k <= 16, |x| and |silu(gate)
  * up| <= 0x7F7F7F7F.  out: m x h (+ residual); gate (may be null): m x
  * experts, TopKSelect's gate.  d_scratch: 16-byte aligned. */
-uint64_t zkie2_moe_router_words(uint64_t h, uint64_t experts, uint32_t group);
-int zkie2_moe_router_pack(const uint64_t *d_w, uint64_t h, uint64_t experts, uint32_t group, uint32_t *d_packed,
-                          uint32_t *d_err, zkie_stream_t stream);
+uint64_t zkie2_moe_router_words(uint64_t h, uint64_t experts);
+int zkie2_moe_router_pack(const uint64_t *d_w, uint64_t h, uint64_t experts, uint32_t *d_packed, uint32_t *d_err,
+                          zkie_stream_t stream);
 uint64_t zkie2_moe_rows_scratch_elems(uint64_t m, uint64_t h, uint64_t experts, uint64_t top_k, uint64_t f,
                                       uint64_t shared_f, uint32_t group);
 int zkie2_moe_rows(const uint64_t *d_x, uint64_t ldx, uint64_t m, uint64_t h, uint64_t experts, uint64_t top_k,
                    uint64_t f, uint64_t shared_f, uint32_t group, const uint32_t *d_router,
-                   const uint32_t *const *h_codes, const uint32_t *const *h_scales, const uint64_t *d_exp_table,
-                   uint64_t exp_len, const uint64_t *d_silu_table, uint64_t silu_len, uint32_t shift,
+                   const uint32_t *const *h_weights, const uint64_t *d_exp_table, uint64_t exp_len,
+                   const uint64_t *d_silu_table, uint64_t silu_len, uint32_t shift,
                    const uint64_t *d_residual, uint64_t ldr, uint64_t *d_out, uint64_t *d_gate, uint32_t *d_err,
                    uint64_t *d_scratch, zkie_stream_t stream);
 

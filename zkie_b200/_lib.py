@@ -171,18 +171,17 @@ SIGNATURES = {
     "zkie2_expert_open": (i64, [vp, u64, vp, vp, u64, vp, u64, vp, vp, vp]),
     "zkie2_eq_combine_scratch_elems": (u64, [u32, u32]),
     "zkie2_eq_combine": (i64, [pu64, pu64, u32, u32, vp, vp, vp]),
-    "zkie2_q4_code_words": (u64, [u64, u64, u64, u32, u64]),
-    "zkie2_q4_scale_words": (u64, [u64, u64, u64, u32, u64]),
-    "zkie2_q4_pack": (i64, [vp, vp, u64, u64, u64, u32, u64, vp, vp, vp, vp]),
-    "zkie2_q4_project": (i64, [vp, u64, u64, vp, vp, u64, u64, u32, u64, u32, vp, vp, u64, s64, vp, u64, vp, vp, vp]),
+    "zkie2_q4_words": (u64, [u64, u64, u64, u32, u64]),
+    "zkie2_q4_pack": (i64, [vp, vp, u64, u64, u64, u32, u64, vp, vp, vp]),
+    "zkie2_q4_project": (i64, [vp, u64, u64, vp, u64, u64, u32, u64, u32, vp, vp, u64, s64, vp, u64, vp, vp, vp]),
     "zkie2_kv_append": (i64, [vp, u64, vp, u64, u64, s64, u32, vp, vp, vp, u64, u64, u64, u64, u64, vp, vp]),
     "zkie2_kv_attend": (i64, [vp, u64, u64, s64, u32, vp, u64, vp, u64, s64, u32, vp, vp, vp, u64, u64, u64, u64, u64,
                               s64, u32, vp, u64, s64, u32, vp, vp, vp]),
-    "zkie2_moe_router_words": (u64, [u64, u64, u32]),
-    "zkie2_moe_router_pack": (i64, [vp, u64, u64, u32, vp, vp, vp]),
+    "zkie2_moe_router_words": (u64, [u64, u64]),
+    "zkie2_moe_router_pack": (i64, [vp, u64, u64, vp, vp, vp]),
     "zkie2_moe_rows_scratch_elems": (u64, [u64, u64, u64, u64, u64, u64, u32]),
-    "zkie2_moe_rows": (i64, [vp, u64, u64, u64, u64, u64, u64, u64, u32, vp, C.POINTER(vp), C.POINTER(vp), vp, u64, vp,
-                             u64, u32, vp, u64, vp, vp, vp, vp, vp]),
+    "zkie2_moe_rows": (i64, [vp, u64, u64, u64, u64, u64, u64, u64, u32, vp, C.POINTER(vp), vp, u64, vp, u64,
+                             u32, vp, u64, vp, vp, vp, vp, vp]),
     "zkie2_choose_token": (i64, [vp, u64, u64, vp, u64, vp, s64, s64, s64, s64, vp, u64, vp, u64, s64, vp, vp, vp, vp]),
     "zkie2_mg_available": (i64, []),
     "zkie2_mg_unique_id": (i64, [C.c_char_p]),

@@ -413,7 +413,8 @@ def _err_word() -> torch.Tensor:
 
 
 _ERRORS = {1: "a lookup index outside its table", 2: "a softmax row sum of zero (round_div by zero)",
-           8: "a value outside the range of the single-token kernels", 16: "a full key / value cache"}
+           8: "a value outside the range of the single-token kernels", 16: "a full key / value cache",
+           32: "a copy that did not arrive (the results are void)"}
 
 
 def _check_err(err: torch.Tensor, what: str):

@@ -35,72 +35,63 @@ namespace {
 constexpr uint32_t kErrIndex = 1u;
 constexpr uint32_t kErrDivide = 2u;
 constexpr uint32_t kErrFull = 16u;  // a cache without room for the new token
-constexpr size_t kMaxShared = 227 * 1024;
+constexpr size_t kMaxShared = 226 * 1024;  // dynamic, next to what is declared
 
 // ---- the weight ---------------------------------------------------------------------------
 // codes (e x k x n, int8) and scales (e x rows x n, int32; ceil(k_seg / G)
 // rows to a segment) into blocks: one thread per output word
 __global__ void k_q4_pack(const int8_t* __restrict__ codes, const int32_t* __restrict__ scales, uint32_t experts,
-                          Q4Shape s, uint32_t* __restrict__ packed, uint32_t* __restrict__ pscales,
-                          uint32_t* __restrict__ err) {
+                          Q4Shape s, uint32_t* __restrict__ packed, uint32_t* __restrict__ err) {
     const uint64_t stride = (uint64_t)gridDim.x * blockDim.x, first = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const uint64_t per = (uint64_t)s.tiles * s.blocks * 128;
-    const uint32_t seg_blocks = s.kp_seg / 64;
+    const uint32_t words = s.bytes / 4, seg_blocks = s.kp_seg / 64, rows = (s.k_seg + s.group - 1) / s.group;
+    const uint64_t per = (uint64_t)s.tiles * s.blocks * words;
     bool bad = false;
     for (uint64_t i = first; i < per * experts; i += stride) {
-        const uint64_t ex = i / per;
-        uint64_t r = i % per;
-        const uint32_t q = r & 3, lane = (r >> 2) & 31;
-        r >>= 7;
-        const uint32_t block = (uint32_t)(r % s.blocks), tile = (uint32_t)(r / s.blocks);
-        const uint32_t g = lane >> 2, t = lane & 3, n = tile * 16 + g + 8 * (q & 1);
-        const uint32_t seg = block / seg_blocks;
+        const uint64_t ex = i / per, r = i % per;
+        const uint32_t at = (uint32_t)(r % words), block = (uint32_t)(r / words % s.blocks);
+        const uint32_t tile = (uint32_t)(r / words / s.blocks), seg = block / seg_blocks;
+        const uint32_t k0 = block % seg_blocks * 64;  // within the segment
         uint32_t word = 0;
-        for (int j = 0; j < 4; j++)
-            for (int h = 0; h < 2; h++) {
-                const uint32_t k = (block % seg_blocks) * 64 + 32 * h + 8 * t + 4 * (q >> 1) + j;
-                int c = 0;
-                if (k < s.k_seg && n < s.n) c = codes[(ex * s.k + (uint64_t)seg * s.k_seg + k) * s.n + n];
-                if (c < -8 || c > 7) {
-                    bad = true;
-                    c = 0;
+        if (at < 128) {
+            const uint32_t q = at & 3, lane = at >> 2, t = lane & 3, n = tile * 16 + (lane >> 2) + 8 * (q & 1);
+            for (int j = 0; j < 4; j++)
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t k = k0 + 32 * h + 8 * t + 4 * (q >> 1) + j;
+                    int c = 0;
+                    if (k < s.k_seg && n < s.n) c = codes[(ex * s.k + (uint64_t)seg * s.k_seg + k) * s.n + n];
+                    if (c < -8 || c > 7) {
+                        bad = true;
+                        c = 0;
+                    }
+                    word |= (uint32_t)(c & 15) << (8 * j + 4 * h);
                 }
-                word |= (uint32_t)(c & 15) << (8 * j + 4 * h);
+        } else {
+            const uint32_t in = (k0 + 32 * ((at - 128) >> 3)) / s.group;  // row of scales within the segment
+            for (int h = 0; h < 2; h++) {
+                const uint32_t n = tile * 16 + (at & 7) + 8 * h;
+                int64_t v = 0;
+                if (in < rows && n < s.n) v = scales[(ex * s.segs * rows + (uint64_t)seg * rows + in) * s.n + n];
+                if (v < 0 || v > 0xFFFF) {
+                    bad = true;
+                    v = 0;
+                }
+                word |= (uint32_t)v << (16 * h);
             }
-        packed[i] = word;
-    }
-    const uint64_t sper = (uint64_t)s.tiles * s.groups * 8;
-    const uint32_t seg_groups = s.kp_seg / s.group, rows = (s.k_seg + s.group - 1) / s.group;
-    for (uint64_t i = first; i < sper * experts; i += stride) {
-        const uint64_t ex = i / sper, r = i % sper;
-        const uint32_t g = r & 7, grp = (uint32_t)((r >> 3) % s.groups), tile = (uint32_t)((r >> 3) / s.groups);
-        const uint32_t seg = grp / seg_groups, in = grp % seg_groups;
-        uint32_t word = 0;
-        for (int h = 0; h < 2; h++) {
-            const uint32_t n = tile * 16 + g + 8 * h;
-            int64_t v = 0;
-            if (in < rows && n < s.n) v = scales[(ex * s.segs * rows + (uint64_t)seg * rows + in) * s.n + n];
-            if (v < 0 || v > 0xFFFF) {
-                bad = true;
-                v = 0;
-            }
-            word |= (uint32_t)v << (16 * h);
         }
-        pscales[i] = word;
+        packed[i] = word;
     }
     if (bad) atomicOr(err, kErrRange);
 }
 
 // ---- the product ----------------------------------------------------------------------------
-constexpr int kProjThreads = 256;
+constexpr int kProjThreads = 512;
 constexpr int kProjWarps = kProjThreads / 32;
 
 struct ProjectArgs {
     const uint64_t* x;
     uint64_t ldx;
     uint32_t m;
-    const uint4* codes;
-    const uint32_t* scales;
+    const uint8_t* w;
     Q4Shape s;
     uint32_t shift;
     const uint64_t* bias;
@@ -111,168 +102,205 @@ struct ProjectArgs {
     uint64_t ldr;
     uint64_t* out;
     uint32_t* err;
-    uint32_t split;   // warps that share a tile of 16 columns
     uint32_t stride;  // bytes of a digit row in shared memory
+    uint32_t run;     // blocks to a slot of a ring
 };
 
-constexpr int kProjDepth = 8;                    // slots of a warp's ring
-constexpr uint32_t kProjSlot = 512 + 64;         // a block's codes and scales
+constexpr int kProjDepth = 3;           // slots of a warp's ring
+constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 
-// One block: 2 NT rows of x as digits in shared memory; its warps stream the
-// tiles of 16 columns, `split` warps to a tile, each a part of K (whole
-// segments where each segment is rounded by itself); their 64-bit sums meet
-// in shared memory, and a thread per output rounds and finishes it.
-template <int G, int NT, bool SEG>
-__global__ void __launch_bounds__(kProjThreads, 2) k_q4_project(const __grid_constant__ ProjectArgs p) {
+// A block takes an equal run of the tiles of 16 columns, in batches; of a
+// batch every warp takes an equal run of blocks (of whole segments where each
+// is rounded by itself), whatever tiles they belong to, against the digits of
+// 2 NT rows in shared memory.  The 64-bit sums meet in shared memory; a thread
+// per output then rounds and finishes it.
+template <bool TWO, int NT, bool SEG>
+__global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_constant__ ProjectArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    constexpr int kRows = 2 * NT;
-    const uint32_t row0 = blockIdx.y * kRows, rows = min((uint32_t)kRows, p.m - row0);
+    __shared__ __align__(8) uint64_t s_bar[kProjWarps * kProjDepth];
+    constexpr uint32_t kRows = 2 * NT, kBytes = TWO ? 576 : 544;
+    const uint32_t row0 = blockIdx.y * kRows, rows = min(kRows, p.m - row0);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = smem + (size_t)warp * kProjDepth * kProjSlot;
-    long long* red = reinterpret_cast<long long*>(smem + (size_t)kProjWarps * kProjDepth * kProjSlot);
-    uint8_t* digits = reinterpret_cast<uint8_t*>(red + 2 * kProjWarps * kRows * 16);
+    const uint32_t slot_bytes = p.run * kBytes;
+    uint8_t* ring = smem + (size_t)warp * kProjDepth * slot_bytes;
+    constexpr uint32_t kCells = kProjBatch * kRows * 16;  // (tile, row, column)
+    const Limbs acc{reinterpret_cast<uint32_t*>(smem + (size_t)kProjWarps * kProjDepth * slot_bytes), kCells};
+    uint8_t* digits = reinterpret_cast<uint8_t*>(acc.w + 3 * kCells);
+    const uint32_t bar = shared_addr(&s_bar[warp * kProjDepth]);
     let_next_start();
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < kProjDepth; i++) barrier_init(bar + 8 * i);
+        barrier_init_done();
+    }
+    __syncwarp();
 
     // ---- this warp's stream of blocks, and the first of them on their way
-    const uint32_t per = kProjWarps / p.split, mine = warp / p.split, part = warp % p.split;
-    const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
-    const uint32_t b0 = part * units / p.split * unit, b1 = (part + 1) * units / p.split * unit;
-    uint32_t next_tile = blockIdx.x * per + mine, next_b = b0, next_slot = 0;
-    const uint32_t tile_step = gridDim.x * per;
-    auto issue = [&]() {
-        if (next_tile < p.s.tiles && b0 < b1) {
-            uint8_t* slot = ring + next_slot * kProjSlot;
-            copy16(slot + lane * 16, p.codes + ((uint64_t)next_tile * p.s.blocks + next_b) * 32 + lane);
-            copy_scales<G>(reinterpret_cast<uint32_t*>(slot + 512), p.scales + (uint64_t)next_tile * p.s.groups * 8,
-                           next_b, g, t);
-            next_slot = next_slot + 1 == kProjDepth ? 0 : next_slot + 1;
-            if (++next_b == b1) {
-                next_b = b0;
-                next_tile += tile_step;
-            }
-        }
-        copy_commit();
+    const uint32_t tile0 = (uint32_t)((uint64_t)blockIdx.x * p.s.tiles / gridDim.x);
+    const uint32_t tile1 = (uint32_t)((uint64_t)(blockIdx.x + 1) * p.s.tiles / gridDim.x);
+    const uint32_t blocks = p.s.blocks, unit = SEG ? p.s.kp_seg / 64 : 1;
+    // blocks of a batch, counted from its first tile, that the warp takes
+    auto first_of = [&](uint32_t batch, uint32_t w) {
+        const uint32_t units = min(kProjBatch, tile1 - batch) * blocks / unit;
+        return (uint32_t)((uint64_t)w * units / kProjWarps) * unit;
     };
-#pragma unroll
-    for (int i = 0; i < kProjDepth - 1; i++) issue();
+    uint32_t next_batch = tile0, next_at = first_of(tile0, warp), next_end = first_of(tile0, warp + 1), next_slot = 0;
+    auto ask = [&]() {  // lane 0 only
+        while (next_at == next_end) {
+            next_batch += kProjBatch;
+            if (next_batch >= tile1) {
+                next_batch = tile1;
+                return;
+            }
+            next_at = first_of(next_batch, warp);
+            next_end = first_of(next_batch, warp + 1);
+        }
+        const uint32_t bytes = min(p.run, next_end - next_at) * kBytes;
+        barrier_expect(bar + 8 * next_slot, bytes);
+        bulk_copy(shared_addr(ring + next_slot * slot_bytes), p.w + ((uint64_t)next_batch * blocks + next_at) * kBytes, bytes,
+                  bar + 8 * next_slot);
+        next_at = min(next_at + p.run, next_end);
+        next_slot = next_slot + 1 == kProjDepth ? 0 : next_slot + 1;
+    };
+    if (lane == 0)
+        for (int i = 0; i < kProjDepth; i++)
+            if (next_batch < tile1) ask();
 
     // ---- the rows' digits
+    for (uint32_t i = threadIdx.x; i < 3 * kCells; i += kProjThreads) acc.w[i] = 0;
     wait_for_previous();
-    const uint32_t kp = p.s.blocks * 64;
-    bool bad = false;
-    for (uint32_t r = 0; r < rows; r++) {
-        for (uint32_t k0 = threadIdx.x * 4; k0 < kp; k0 += kProjThreads * 4) {
-            const uint32_t seg = SEG ? k0 / p.s.kp_seg : 0, in = SEG ? k0 % p.s.kp_seg : k0;
-            const uint64_t* xr = p.x + (row0 + r) * p.ldx + seg * p.s.k_seg + in;
-            uint32_t d[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) bad |= !q4_digits(in + j < p.s.k_seg ? fx_to_i64(__ldg(xr + j)) : 0, &d[j]);
-            q4_store_digits(digits + (size_t)r * 4 * p.stride + q4_pos(k0), p.stride, d);
-        }
-    }
-    if (bad) atomicOr(p.err, kErrRange);
+    if (!q4_digitise<kProjThreads>(p.x + (uint64_t)row0 * p.ldx, p.ldx, rows, p.s.segs, p.s.k_seg, p.s.kp_seg, digits,
+                                   p.stride))
+        atomicOr(p.err, kErrRange);
     __syncthreads();
 
     const uint8_t* from = digits + (size_t)g * p.stride + 16 * t;  // column g: digit g % 4 of row g / 4
-    uint32_t flip = 0, slot_at = 0;
-    for (uint32_t group = blockIdx.x; group * per < p.s.tiles; group += gridDim.x, flip ^= 1) {
-        const uint32_t tile = group * per + mine;
-        if (tile < p.s.tiles) {
-            Q4Sum<NT> sum;
-            sum.clear();
-            long long total[NT][2];
+    Patience patience;
+    uint32_t slot = 0, phase = 0;
+    for (uint32_t batch = tile0; batch < tile1; batch += kProjBatch) {
+        uint32_t at = first_of(batch, warp);
+        const uint32_t end = first_of(batch, warp + 1);
+        uint32_t tile = at / blocks, b = at % blocks;
+        Q4Sum<NT> sum;
+        sum.clear();
+        long long total[NT];  // of the tile's segments, each rounded
 #pragma unroll
-            for (int i = 0; i < NT; i++) total[i][0] = total[i][1] = 0;
-            for (uint32_t b = b0; b < b1; b++) {
-                __syncwarp();  // every lane has read the slot that is filled next
-                issue();
-                copy_wait<kProjDepth - 1>();
-                __syncwarp();
-                const uint8_t* slot = ring + slot_at * kProjSlot;
-                slot_at = slot_at + 1 == kProjDepth ? 0 : slot_at + 1;
-                const uint4 w = *reinterpret_cast<const uint4*>(slot + lane * 16);
-                const uint32_t s0 = reinterpret_cast<const uint32_t*>(slot + 512)[g];
-                const uint32_t s1 = G == 32 ? reinterpret_cast<const uint32_t*>(slot + 512)[8 + g] : 0;
-                uint4 x[NT];
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-                    x[i] = *reinterpret_cast<const uint4*>(from + (size_t)i * 8 * p.stride + b * 64);
-                q4_block<G, NT>(sum, w, s0, s1, x, b & 1);
-                if (SEG && (b + 1) % unit == 0) {
-#pragma unroll
-                    for (int i = 0; i < NT; i++) {
-                        long long v0, v1;
-                        sum.finish(i, &v0, &v1);
-                        total[i][0] += fx_round_div_pow2(v0, p.shift);
-                        total[i][1] += fx_round_div_pow2(v1, p.shift);
-                    }
-                    sum.clear();
-                }
-            }
+        for (int i = 0; i < NT; i++) total[i] = 0;
+        auto flush = [&]() {
 #pragma unroll
             for (int i = 0; i < NT; i++) {
-                if (!SEG) sum.finish(i, &total[i][0], &total[i][1]);
-                if (!(t & 1)) {
-                    long long* to = red + ((size_t)(flip * kProjWarps + warp) * kRows + 2 * i + (t >> 1)) * 16;
-                    to[g] = total[i][0];
-                    to[g + 8] = total[i][1];
+                if (!SEG) total[i] = sum.finish(i);
+                const uint32_t r = 2 * i + (t >> 1);
+                if (r < rows) acc.add((tile * kRows + r) * 16 + g + 8 * (t & 1), total[i]);
+                total[i] = 0;
+            }
+            if (!SEG) sum.clear();
+        };
+        while (at < end) {
+            const uint32_t run = min(p.run, end - at);
+            barrier_wait(bar + 8 * slot, phase, patience);
+            const uint8_t* block = ring + slot * slot_bytes;
+            for (uint32_t j = 0; j < run;) {
+                // blocks up to the end of the tile (or segment)
+                const uint32_t n = min(run - j, (SEG ? unit - b % unit : blocks - b));
+#pragma unroll 2
+                for (uint32_t q = 0; q < n; q++) {
+                    uint4 x[NT];
+#pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        x[i] = *reinterpret_cast<const uint4*>(from + (size_t)i * 8 * p.stride + (b + q) * 64);
+                    q4_block<TWO, NT, NT>(sum, block + q * kBytes, x);
                 }
+                j += n;
+                b += n;
+                block += n * kBytes;
+                if (SEG && b % unit == 0) {
+#pragma unroll
+                    for (int i = 0; i < NT; i++) total[i] += round_shift(sum.finish(i), p.shift);
+                    sum.clear();
+                }
+                if (b == blocks) {
+                    flush();
+                    b = 0;
+                    tile++;
+                }
+            }
+            at += run;
+            __syncwarp();  // every lane has read the slot
+            if (lane == 0 && next_batch < tile1) ask();
+            if (++slot == kProjDepth) {
+                slot = 0;
+                phase ^= 1;
+            }
+        }
+        if (b) flush();
+        __syncthreads();
+        const uint32_t tiles = min(kProjBatch, tile1 - batch);
+        constexpr int kOuts = 4;  // outputs of a thread whose operands are under way together
+        for (uint32_t o0 = threadIdx.x; o0 < tiles * kRows * 16; o0 += kProjThreads * kOuts) {
+            uint64_t bias[kOuts], residual[kOuts];
+#pragma unroll
+            for (int u = 0; u < kOuts; u++) {
+                const uint32_t o = o0 + u * kProjThreads, r = o / 16 % kRows, n = (batch + o / (kRows * 16)) * 16 + o % 16;
+                const bool on = o < tiles * kRows * 16 && r < rows && n < p.s.n;
+                bias[u] = on && p.bias ? __ldg(p.bias + n) : 0;
+                residual[u] = on && p.residual ? __ldg(p.residual + (row0 + r) * p.ldr + n) : 0;
+            }
+            int64_t y[kOuts];
+#pragma unroll
+            for (int u = 0; u < kOuts; u++) {
+                const uint32_t o = o0 + u * kProjThreads;
+                if (o >= tiles * kRows * 16) continue;
+                y[u] = SEG ? acc.get(o) : round_shift(acc.get(o), p.shift);
+                acc.clear(o);
+                y[u] = fx_wadd(y[u], fx_to_i64(bias[u]));
+            }
+            uint64_t f[kOuts];
+#pragma unroll
+            for (int u = 0; u < kOuts; u++)
+                f[u] = o0 + u * kProjThreads >= tiles * kRows * 16 ? 0
+                       : p.table ? gl_canon(table_at(p.table, p.table_len, y[u], p.offset)) : fx_from_i64(y[u]);
+#pragma unroll
+            for (int u = 0; u < kOuts; u++) {
+                const uint32_t o = o0 + u * kProjThreads, r = o / 16 % kRows, n = (batch + o / (kRows * 16)) * 16 + o % 16;
+                if (o < tiles * kRows * 16 && r < rows && n < p.s.n)
+                    p.out[(row0 + r) * (uint64_t)p.s.n + n] = p.residual ? gl_canon(gl_add(f[u], gl_canon(residual[u]))) : f[u];
             }
         }
         __syncthreads();
-        for (uint32_t o = threadIdx.x; o < per * rows * 16; o += kProjThreads) {
-            const uint32_t c = o & 15, which = (o >> 4) % per, r = (o >> 4) / per;
-            const uint64_t n = (uint64_t)(group * per + which) * 16 + c;
-            if (n >= p.s.n) continue;
-            uint64_t v = 0;
-            for (uint32_t w = 0; w < p.split; w++)
-                v += (uint64_t)red[((size_t)(flip * kProjWarps + which * p.split + w) * kRows + r) * 16 + c];
-            int64_t y = SEG ? (int64_t)v : fx_round_div_pow2((int64_t)v, p.shift);
-            if (p.bias) y = fx_wadd(y, fx_to_i64(__ldg(p.bias + n)));
-            uint64_t f = p.table ? gl_canon(table_at(p.table, p.table_len, y, p.offset)) : fx_from_i64(y);
-            if (p.residual) f = gl_canon(gl_add(f, gl_canon(__ldg(p.residual + (row0 + r) * p.ldr + n))));
-            p.out[(row0 + r) * (uint64_t)p.s.n + n] = f;
-        }
     }
+    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
 }
 
-constexpr size_t kProjRing = (size_t)kProjWarps * kProjDepth * kProjSlot;
+// dynamic shared memory for blocks of `rows` rows and a ring of `run` blocks to a slot
+size_t project_shared(const Q4Shape& s, uint32_t rows, uint32_t run) {
+    return (size_t)kProjWarps * kProjDepth * run * s.bytes + (size_t)rows * (kProjBatch * 16 * 12 + 4 * q4_digit_stride(s.blocks));
+}
 
-template <int G, int NT, bool SEG>
-int project_launch(ProjectArgs p, cudaStream_t stream) {
-    const size_t shared = kProjRing + (size_t)2 * NT * 4 * p.stride + 2ull * kProjWarps * 2 * NT * 16 * 8;
-    auto* kernel = k_q4_project<G, NT, SEG>;
+template <bool TWO, int NT, bool SEG>
+int project_launch(const ProjectArgs& p, cudaStream_t stream) {
+    auto* kernel = k_q4_project<TWO, NT, SEG>;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kMaxShared, &set));
-    const uint32_t at_once = kSms * (shared > kMaxShared / 2 ? 1 : 2);
-    // Warps to a tile: the fewest steps of a block's warps, each with what a tile costs besides its blocks
-    const uint32_t unit = SEG ? p.s.kp_seg / 64 : (G == 128 ? 2 : 1), units = p.s.blocks / unit;
-    uint64_t least = ~0ull;
-    for (uint32_t split = 1; split <= (uint32_t)kProjWarps; split *= 2) {
-        const uint64_t groups = ceil_div(p.s.tiles, kProjWarps / split);
-        const uint64_t cost = ceil_div(groups, at_once) * (ceil_div(units, split) * unit + 3);
-        if (cost < least) {
-            least = cost;
-            p.split = split;
-        }
-    }
-    const uint64_t groups = ceil_div(p.s.tiles, kProjWarps / p.split);
-    const dim3 grid((unsigned)(groups < at_once ? groups : at_once), (unsigned)ceil_div(p.m, 2 * NT));
-    return launch(kernel, grid, kProjThreads, shared, 1, stream, p);
+    const dim3 grid(p.s.tiles < (uint32_t)kSms ? p.s.tiles : kSms, (unsigned)ceil_div(p.m, 2 * NT));
+    return launch(kernel, grid, kProjThreads, project_shared(p.s, 2 * NT, p.run), 1, stream, p);
 }
 
-template <int G, int NT>
+template <bool TWO, int NT>
 int project_seg(const ProjectArgs& p, cudaStream_t stream) {
-    return p.s.segs > 1 ? project_launch<G, NT, true>(p, stream) : project_launch<G, NT, false>(p, stream);
+    return p.s.segs > 1 ? project_launch<TWO, NT, true>(p, stream) : project_launch<TWO, NT, false>(p, stream);
 }
 
-template <int G>
-int project_rows(const ProjectArgs& p, cudaStream_t stream) {
-    // rows to a block: up to eight, as many as their digits leave room for
-    const uint64_t row = 4ull * p.stride, red = 2ull * kProjWarps * 16 * 8;
-    if (p.m > 4 && kProjRing + 8 * (row + red) <= kMaxShared) return project_seg<G, 4>(p, stream);
-    if (p.m > 2 && kProjRing + 4 * (row + red) <= kMaxShared) return project_seg<G, 2>(p, stream);
-    return project_seg<G, 1>(p, stream);
+template <bool TWO>
+int project_rows(ProjectArgs p, cudaStream_t stream) {
+    // Rows to a block: up to eight, as many as their digits leave room for; slots of four blocks
+    // (2 kB a copy) where there is room, else of two or one
+    for (uint32_t rows = p.m > 4 ? 8 : p.m > 2 ? 4 : 2;; rows /= 2)
+        for (p.run = 4; p.run; p.run /= 2)
+            if (project_shared(p.s, rows, p.run) <= kMaxShared)
+                return rows == 8   ? project_seg<TWO, 4>(p, stream)
+                       : rows == 4 ? project_seg<TWO, 2>(p, stream)
+                                   : project_seg<TWO, 1>(p, stream);
 }
 
 // ---- the cache ------------------------------------------------------------------------------
@@ -740,39 +768,31 @@ using namespace zk;
 
 extern "C" {
 
-uint64_t zkie2_q4_code_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment) {
+uint64_t zkie2_q4_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment) {
     Q4Shape s;
     if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, segment, &s)) return 0;
-    return experts * s.tiles * s.blocks * 128ull;
-}
-
-uint64_t zkie2_q4_scale_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment) {
-    Q4Shape s;
-    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, segment, &s)) return 0;
-    return experts * s.tiles * s.groups * 8ull;
+    return experts * s.tiles * s.blocks * (s.bytes / 4);
 }
 
 int zkie2_q4_pack(const int8_t* d_codes, const int32_t* d_scales, uint64_t experts, uint64_t k, uint64_t n,
-                  uint32_t group, uint64_t segment, uint32_t* d_packed, uint32_t* d_packed_scales, uint32_t* d_err,
-                  cudaStream_t stream) {
+                  uint32_t group, uint64_t segment, uint32_t* d_packed, uint32_t* d_err, cudaStream_t stream) {
     Q4Shape s;
     if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, segment, &s) || !d_codes || !d_scales || !d_packed ||
-        !d_packed_scales || !d_err)
+        !d_err)
         return (int)cudaErrorInvalidValue;
-    const uint64_t words = experts * s.tiles * s.blocks * 128ull, blocks = ceil_div(words, 256);
+    const uint64_t blocks = ceil_div(experts * s.tiles * s.blocks * (s.bytes / 4), 256);
     k_q4_pack<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), 256, 0, stream>>>(
-        d_codes, d_scales, (uint32_t)experts, s, d_packed, d_packed_scales, d_err);
+        d_codes, d_scales, (uint32_t)experts, s, d_packed, d_err);
     ZK_LAUNCH_CHECK();
     return 0;
 }
 
-int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32_t* d_packed,
-                     const uint32_t* d_packed_scales, uint64_t k, uint64_t n, uint32_t group, uint64_t segment,
-                     uint32_t shift, const uint64_t* d_bias, const uint64_t* d_table, uint64_t table_len,
-                     int64_t offset, const uint64_t* d_residual, uint64_t ldr, uint64_t* d_out, uint32_t* d_err,
-                     cudaStream_t stream) {
+int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32_t* d_packed, uint64_t k, uint64_t n,
+                     uint32_t group, uint64_t segment, uint32_t shift, const uint64_t* d_bias,
+                     const uint64_t* d_table, uint64_t table_len, int64_t offset, const uint64_t* d_residual,
+                     uint64_t ldr, uint64_t* d_out, uint32_t* d_err, cudaStream_t stream) {
     ProjectArgs p{};
-    if (!q4_shape(k, n, group, segment, &p.s) || shift > 62 || m > 65535 || !d_packed || !d_packed_scales || !d_err ||
+    if (!q4_shape(k, n, group, segment, &p.s) || shift > 62 || m > 65535 || !d_packed || !d_err ||
         (d_table && table_len == 0) || (m > 1 && ldx < k) || (d_residual && m > 1 && ldr < n) ||
         ((uintptr_t)d_packed & 15))
         return (int)cudaErrorInvalidValue;
@@ -781,8 +801,7 @@ int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32
     p.x = d_x;
     p.ldx = ldx;
     p.m = (uint32_t)m;
-    p.codes = reinterpret_cast<const uint4*>(d_packed);
-    p.scales = d_packed_scales;
+    p.w = reinterpret_cast<const uint8_t*>(d_packed);
     p.shift = shift;
     p.bias = d_bias;
     p.table = d_table;
@@ -793,8 +812,7 @@ int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32
     p.out = d_out;
     p.err = d_err;
     p.stride = q4_digit_stride(p.s.blocks);
-    return group == 32 ? project_rows<32>(p, stream) : group == 64 ? project_rows<64>(p, stream)
-                                                                    : project_rows<128>(p, stream);
+    return group == 32 ? project_rows<true>(p, stream) : project_rows<false>(p, stream);
 }
 
 int zkie2_kv_append(const uint64_t* d_k, uint64_t ldk, const uint64_t* d_v, uint64_t ldv, uint64_t tokens,

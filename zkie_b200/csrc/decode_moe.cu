@@ -21,7 +21,6 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
-#include <cmath>
 #include <cstdint>
 
 #include "../../include/zkie2.h"
@@ -49,8 +48,7 @@ constexpr size_t kMaxShared = 220 * 1024;
 constexpr int32_t kRouterLimit = 32639;  // two signed bytes
 
 struct Q4Weight {
-    const uint4* codes;
-    const uint32_t* scales;
+    const uint8_t* w;
     Q4Shape s;
 };
 
@@ -62,6 +60,7 @@ struct Items {
     uint8_t count[kMaxSlots];
     uint16_t first[kMaxSlots];  // into slot
     uint16_t slot[kMaxSlots];   // grouped by expert
+    uint8_t token[kMaxSlots];   // of slot[i]
     int32_t score[kMaxSlots];   // a slot's softmax value
 };
 static_assert(sizeof(Items) % 4 == 0, "copied in words");
@@ -82,16 +81,12 @@ struct MoeArgs {
     uint64_t* out;
     uint64_t* gate_out;  // m x experts (or null)
     Items* items;
-    uint8_t* act;        // (m top_k) x 4 x padded F digits
-    uint8_t* sact;       // m x 4 x padded shared F digits
+    uint8_t* act;        // the activation's digits: a slot's blocks of 64, in each its four digit rows
+    uint8_t* sact;       // the same of the shared experts, a token's blocks
     uint32_t* err;
     uint32_t stride;     // bytes of a digit row of x
-    uint32_t split;      // warps that share a tile of k_moe_up
+    uint32_t depth;      // slots of a ring of k_moe_down
 };
-
-__device__ __forceinline__ void group_sync(uint32_t id, uint32_t threads) {
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
 
 // The router's weights (h x experts, field elements) as two signed bytes in
 // blocks of 64 k and 16 experts: word q of lane (g, t) of half f and byte p
@@ -120,11 +115,11 @@ __global__ void k_moe_router_pack(const uint64_t* __restrict__ w, uint32_t h, ui
     if (bad) atomicOr(err, kErrRange);
 }
 
-// Logits of the 16 experts of a tile for 2 NT tokens, this warp's part of K,
-// added to raw (tokens x padded experts, 64-bit sums in shared memory)
+// Logits of the 16 experts of tile 2 i + rank for 2 NT tokens, this warp's
+// part of K, added to sums (tokens x this block's experts)
 template <int NT>
-__device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t tile, uint32_t tok0, uint32_t b0,
-                            uint32_t b1, unsigned long long* raw) {
+__device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t own, uint32_t rank, uint32_t tok0,
+                            uint32_t b0, uint32_t b1, const Limbs& sums, uint32_t pitch) {
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     int c[2][NT][4];
 #pragma unroll
@@ -133,7 +128,7 @@ __device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t ti
         for (int i = 0; i < NT; i++) c[w][i][0] = c[w][i][1] = c[w][i][2] = c[w][i][3] = 0;
 #pragma unroll 2
     for (uint32_t b = b0; b < b1; b++) {
-        const uint4* r = p.router + ((uint64_t)tile * p.gate.s.blocks + b) * 128 + lane;
+        const uint4* r = p.router + ((uint64_t)(2 * own + rank) * p.gate.s.blocks + b) * 128 + lane;
         const uint4 w00 = __ldg(r), w01 = __ldg(r + 32), w10 = __ldg(r + 64), w11 = __ldg(r + 96);
 #pragma unroll
         for (int i = 0; i < NT; i++) {
@@ -145,7 +140,6 @@ __device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t ti
             mma_s8(c[1][i], w11.x, w11.y, w11.z, w11.w, x.z, x.w);
         }
     }
-    const uint32_t pitch = p.etiles * 16;
 #pragma unroll
     for (int i = 0; i < NT; i++) {
         const uint32_t tok = tok0 + 2 * i + (t >> 1);
@@ -154,7 +148,7 @@ __device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t ti
             for (int q = 0; q < 2; q++) {
                 const long long v = ((long long)c[0][i][2 * q] + ((long long)c[0][i][2 * q + 1] << 8)) +
                                     (((long long)c[1][i][2 * q] << 8) + ((long long)c[1][i][2 * q + 1] << 16));
-                atomicAdd(&raw[tok * pitch + tile * 16 + g + 8 * q], (unsigned long long)v << (16 * (t & 1)));
+                sums.add(tok * pitch + own * 16 + g + 8 * q, (long long)((unsigned long long)v << (16 * (t & 1))));
             }
         }
     }
@@ -164,16 +158,16 @@ __device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t ti
 // of the pair's two blocks (tiles of experts alternate between them).  A key
 // holds an expert's value above its complement, so that the maximum is the
 // first in TopKSelect's order.
-__device__ void route_token(const MoeArgs& p, uint32_t r, const unsigned long long* even, const unsigned long long* odd,
+__device__ void route_token(const MoeArgs& p, uint32_t r, const long long* even, const long long* odd, uint32_t pitch,
                             uint32_t* s_sel, int32_t* s_score, uint32_t* s_mask) {
-    const uint32_t lane = threadIdx.x & 31, pitch = p.etiles * 16;
+    const uint32_t lane = threadIdx.x & 31;
     long long z[kMaxExperts / 32], top = INT64_MIN;
 #pragma unroll
     for (int i = 0; i < (int)kMaxExperts / 32; i++) {
         const uint32_t e = i * 32 + lane;
         z[i] = INT64_MIN;
         if (e < p.experts) {
-            z[i] = fx_round_div_pow2((int64_t)((e / 16) % 2 ? odd : even)[r * pitch + e], p.shift);
+            z[i] = round_shift((e / 16 % 2 ? odd : even)[r * pitch + e / 32 * 16 + e % 16], p.shift);
             top = max(top, z[i]);
         }
     }
@@ -253,6 +247,7 @@ __device__ void list_items(const MoeArgs& p, const uint32_t* s_sel, const uint32
             uint32_t place = 0;
             while (s_sel[tok * p.top_k + place] != e) place++;
             it->slot[at + j] = (uint16_t)(tok * p.top_k + place);
+            it->token[at + j] = (uint8_t)tok;
         }
         slot += __shfl_sync(0xFFFFFFFFu, sc, 31);
         item += __shfl_sync(0xFFFFFFFFu, si, 31);
@@ -260,97 +255,86 @@ __device__ void list_items(const MoeArgs& p, const uint32_t* s_sel, const uint32
     if (lane == 0) it->n = item;
 }
 
-constexpr uint32_t kUpSlot = 2 * (512 + 64);                         // gate and up: codes, codes, scales, scales
-constexpr size_t kUpRed = (size_t)kWarps * 2 * kTile * 16 * 8;       // every warp's sums of a tile
+constexpr uint32_t kUpBatch = 16;                                       // tiles whose sums are held at a time
+constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile, gate or up, token, column)
 
-template <int G, int NT>
-__device__ __forceinline__ void up_block(Q4Sum<2> (&sum)[2], const uint8_t* slot, const uint8_t* const (&from)[2],
-                                         uint32_t b) {
-    const uint32_t lane = threadIdx.x & 31, g = lane >> 2;
-    uint4 x[2];
-#pragma unroll
-    for (int i = 0; i < NT; i++) x[i] = *reinterpret_cast<const uint4*>(from[i] + b * 64);
-#pragma unroll
-    for (int q = 0; q < 2; q++) {
-        const uint4 w = *reinterpret_cast<const uint4*>(slot + q * 512 + lane * 16);
-        const uint32_t* sc = reinterpret_cast<const uint32_t*>(slot + 1024 + q * 64);
-        q4_block_n<G, NT>(sum[q], w, sc[g], G == 32 ? sc[8 + g] : 0, x, b & 1);
-    }
-}
-
-template <int G, int DEPTH>
+// The tiles of 16 hidden columns that a block takes, u = blockIdx.x + i
+// gridDim.x for i = 0, 1, ..: first those of the shared experts (four tokens
+// to each), then those of the chosen experts' items; in batches, of which
+// every warp takes an equal run of blocks of 64 k (gate and up together).
+template <bool TWO, int DEPTH>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Items items;
     __shared__ uint32_t s_mask[kMaxExperts], s_sel[kMaxSlots];
+    __shared__ __align__(8) uint64_t s_bar[kWarps * DEPTH];
+    constexpr uint32_t kBytes = TWO ? 576 : 544, kSlot = 2 * kBytes;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t pitch = p.etiles * 16, rank = cluster.block_rank();
-    uint8_t* ring = smem + (size_t)warp * DEPTH * kUpSlot;
-    long long* red = reinterpret_cast<long long*>(smem + (size_t)kWarps * DEPTH * kUpSlot);
-    unsigned long long* raw = reinterpret_cast<unsigned long long*>(reinterpret_cast<uint8_t*>(red) + kUpRed);
-    uint8_t* digits = reinterpret_cast<uint8_t*>(raw + 2 * p.m * pitch);
+    const uint32_t pitch = (p.etiles + 1) / 2 * 16, rank = cluster.block_rank();
+    uint8_t* ring = smem + (size_t)warp * DEPTH * kSlot;
+    const Limbs acc{reinterpret_cast<uint32_t*>(smem + (size_t)kWarps * DEPTH * kSlot), kUpCells};
+    const Limbs sums{acc.w, p.m * pitch};  // of the logits, before the tiles': at most kUpCells
+    long long* logits = reinterpret_cast<long long*>(acc.w + 3 * kUpCells);  // of the pair's even tiles, then the odd ones
+    uint8_t* digits = reinterpret_cast<uint8_t*>(logits + 2 * p.m * pitch);
+    const uint32_t bar = shared_addr(&s_bar[warp * DEPTH]);
     cluster_arrive();  // both blocks have started before one writes into the other's shared memory
     let_next_start();
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; i++) barrier_init(bar + 8 * i);
+        barrier_init_done();
+    }
+    __syncwarp();
 
-    // ---- the warp's tiles, of the shared experts first: its stream of blocks
+    // ---- the block's tiles and the warp's stream of blocks; until the routing is known, the
+    // shared experts' first batch
     const uint32_t ft = p.gate.s.tiles, st = p.sgate.s.tiles, stiles = st * ((p.m + kTile - 1) / kTile);
-    const uint32_t blocks = p.gate.s.blocks, unit = G == 128 ? 2 : 1;
-    const uint32_t per = kWarps / p.split, mine = warp / p.split, part = warp % p.split;
-    const uint32_t b0 = part * (blocks / unit) / p.split * unit, b1 = (part + 1) * (blocks / unit) / p.split * unit;
-    const uint32_t u0 = blockIdx.x + gridDim.x * mine, step = gridDim.x * per;
-    uint32_t known = stiles;  // tiles that may be asked for
-    uint32_t next_u = u0, next_b = b0, next_slot = 0;
-    uint64_t next_tile = 0;
-    const Q4Weight *next_g = nullptr, *next_w = nullptr;
-    auto issue = [&]() {
-        if (next_u < known && b0 < b1) {
-            if (next_b == b0) {
-                const bool shared = next_u < stiles;
-                next_g = shared ? &p.sgate : &p.gate;
-                next_w = shared ? &p.sup : &p.up;
-                next_tile = shared ? next_u % st
-                                   : (uint64_t)items.expert[(next_u - stiles) / ft] * ft + (next_u - stiles) % ft;
-            }
-            uint8_t* slot = ring + next_slot * kUpSlot;
-            const uint64_t block = (next_tile * blocks + next_b) * 32 + lane, groups = next_tile * p.gate.s.groups * 8;
-            copy16(slot + lane * 16, next_g->codes + block);
-            copy16(slot + 512 + lane * 16, next_w->codes + block);
-            uint32_t* sc = reinterpret_cast<uint32_t*>(slot + 1024);
-            copy_scales<G>(sc, next_g->scales + groups, next_b, g, t);
-            copy_scales<G>(sc + 16, next_w->scales + groups, next_b, g, t);
-            next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
-            if (++next_b == b1) {
-                next_b = b0;
-                next_u += step;
-            }
-        }
+    const uint32_t blocks = p.gate.s.blocks;
+    auto tiles_below = [&](uint32_t u) { return u > blockIdx.x ? (u - blockIdx.x + gridDim.x - 1) / gridDim.x : 0u; };
+    const uint32_t early = min(tiles_below(stiles), kUpBatch);  // tiles of the batch before the routing
+    uint32_t known = early;                                     // tiles of this block that may be asked for
+    uint32_t next_first = 0, next_n = early, next_at = warp * (early * blocks) / kWarps, next_end = (warp + 1) * (early * blocks) / kWarps;
+    uint32_t next_slot = 0, asked = 0, taken = 0;
+    const uint8_t *next_g = nullptr, *next_u = nullptr;
+    auto point = [&]() {  // at block next_at of the batch
+        const uint32_t i = next_first + next_at / blocks, u = blockIdx.x + i * gridDim.x;
+        const bool shared = u < stiles;
+        const uint64_t tile = shared ? u % st : (uint64_t)items.expert[(u - stiles) / ft] * ft + (u - stiles) % ft;
+        const uint64_t at = (tile * blocks + next_at % blocks) * kBytes;
+        next_g = (shared ? p.sgate.w : p.gate.w) + at;
+        next_u = (shared ? p.sup.w : p.up.w) + at;
     };
-    // Copies that could not be asked for before the routing are made up after it: a group to
-    // each block, counted ahead of the blocks taken.
-    uint32_t asked = 0, taken = 0;
-    auto ask = [&]() {
-        while (asked < taken + DEPTH && next_u < known && b0 < b1) {
-            issue();
-            copy_commit();
+    auto ask = [&]() {  // lane 0 only: fill the ring
+        while (asked < taken + DEPTH) {
+            while (next_at == next_end) {
+                if (next_first + next_n >= known) return;  // at the end, or of what is known
+                next_first += next_n;
+                next_n = min(kUpBatch, known - next_first);
+                next_at = warp * (next_n * blocks) / kWarps;
+                next_end = (warp + 1) * (next_n * blocks) / kWarps;
+                next_g = nullptr;
+            }
+            if (next_g == nullptr || next_at % blocks == 0) point();
+            const uint32_t b = bar + 8 * next_slot, to = shared_addr(ring + next_slot * kSlot);
+            barrier_expect(b, kSlot);
+            bulk_copy(to, next_g, kBytes, b);
+            bulk_copy(to + kBytes, next_u, kBytes, b);
+            next_g += kBytes;
+            next_u += kBytes;
+            next_at++;
             asked++;
+            next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
         }
     };
-    ask();
+    if (lane == 0) ask();
 
     // ---- the rows' digits and the logits
-    for (uint32_t i = threadIdx.x; i < p.m * pitch; i += kThreads) raw[i] = 0;
+    for (uint32_t i = threadIdx.x; i < 3 * kUpCells; i += kThreads) acc.w[i] = 0;
     for (uint32_t i = threadIdx.x; i < p.experts; i += kThreads) s_mask[i] = 0;
     wait_for_previous();
     bool bad = false;
-    for (uint32_t r = 0; r < p.m; r++)
-        for (uint32_t k0 = threadIdx.x * 4; k0 < blocks * 64; k0 += kThreads * 4) {
-            const uint64_t* xr = p.x + r * p.ldx + k0;
-            uint32_t d[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) bad |= !q4_digits(k0 + j < p.h ? fx_to_i64(__ldg(xr + j)) : 0, &d[j]);
-            q4_store_digits(digits + (size_t)r * 4 * p.stride + q4_pos(k0), p.stride, d);
-        }
+    bad |= !q4_digitise<kThreads>(p.x, p.ldx, p.m, 1, p.h, blocks * 64, digits, p.stride);
     __syncthreads();
     {
         // tiles of 16 experts, every other one this block's; eight (or sixteen) warps to a tile
@@ -358,219 +342,229 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
         for (uint32_t i = warp / wide; i < own; i += kWarps / wide) {
             const uint32_t w = warp % wide, r0 = w * blocks / wide, r1 = (w + 1) * blocks / wide;
             if (p.m <= 2)
-                router_part<1>(p, digits, 2 * i + rank, 0, r0, r1, raw);
+                router_part<1>(p, digits, i, rank, 0, r0, r1, sums, pitch);
             else
-                for (uint32_t tok = 0; tok < p.m; tok += 8) router_part<4>(p, digits, 2 * i + rank, tok, r0, r1, raw);
+                for (uint32_t tok = 0; tok < p.m; tok += 8) router_part<4>(p, digits, i, rank, tok, r0, r1, sums, pitch);
         }
     }
     __syncthreads();
     cluster_wait();
-    unsigned long long* other = raw + p.m * pitch;
     {
-        unsigned long long* there = cluster.map_shared_rank(other, rank ^ 1);
-        for (uint32_t i = threadIdx.x; i < p.m * pitch; i += kThreads)
-            if ((i % pitch / 16) % 2 == rank) there[i] = raw[i];
+        long long* mine = logits + rank * p.m * pitch;
+        long long* there = cluster.map_shared_rank(mine, rank ^ 1);
+        for (uint32_t i = threadIdx.x; i < p.m * pitch; i += kThreads) {
+            mine[i] = there[i] = sums.get(i);
+            sums.clear(i);
+        }
     }
-    cluster.sync();
+    __syncthreads();
+    cluster_arrive();  // the neighbour's logits: waited for after the first batch
+
+    Patience patience;
+    uint32_t slot = 0, phase = 0;
+    auto token_of = [&](bool shared, uint32_t first, uint32_t j) { return shared ? first + j : items.token[first + j]; };
+    // one batch of the block's tiles, from number `first` on: sums into acc, then the activations
+    auto run = [&](uint32_t first, uint32_t n) {
+        uint32_t at = warp * (n * blocks) / kWarps;
+        const uint32_t end = (warp + 1) * (n * blocks) / kWarps;
+        while (at < end) {
+            const uint32_t i = at / blocks, u = blockIdx.x + (first + i) * gridDim.x;
+            const bool shared = u < stiles;
+            const uint32_t item = shared ? u / st : (u - stiles) / ft;
+            const uint32_t tok0 = shared ? item * kTile : items.first[item];
+            const uint32_t count = shared ? min(kTile, p.m - tok0) : items.count[item];
+            const uint8_t* from[2];
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                from[q] = digits + (size_t)(token_of(shared, tok0, min(2 * q + (g >> 2), count - 1)) * 4 + (g & 3)) * p.stride + 16 * t;
+            Q4Sum<2> sum[2];
+            sum[0].clear();
+            sum[1].clear();
+            uint32_t b = at % blocks;
+            const uint32_t stop = min(blocks, b + end - at);
+            at += stop - b;
+            for (; b < stop; b++) {
+                barrier_wait(bar + 8 * slot, phase, patience);
+                const uint8_t* w = ring + slot * kSlot;
+                uint4 x[2];
+                x[0] = *reinterpret_cast<const uint4*>(from[0] + b * 64);
+                if (count > 2) {
+                    x[1] = *reinterpret_cast<const uint4*>(from[1] + b * 64);
+                    q4_block<TWO, 2>(sum[0], w, x);
+                    q4_block<TWO, 2>(sum[1], w + kBytes, x);
+                } else {
+                    q4_block<TWO, 1>(sum[0], w, x);
+                    q4_block<TWO, 1>(sum[1], w + kBytes, x);
+                }
+                taken++;
+                __syncwarp();  // every lane has read the slot
+                if (lane == 0) ask();
+                if (++slot == DEPTH) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+                if (2 * q < count) {
+                    const uint32_t j = 2 * q + (t >> 1);
+#pragma unroll
+                    for (int mat = 0; mat < 2; mat++) {
+                        const long long v = sum[mat].finish(q);
+                        if (j < count) acc.add(((i * 2 + mat) * kTile + j) * 16 + g + 8 * (t & 1), v);
+                    }
+                }
+        }
+        __syncthreads();
+        for (uint32_t o = threadIdx.x; o < n * kTile * 16; o += kThreads) {
+            const uint32_t i = o / (kTile * 16), j = o / 16 % kTile, c = o % 16, u = blockIdx.x + (first + i) * gridDim.x;
+            const bool shared = u < stiles;
+            const uint32_t item = shared ? u / st : (u - stiles) / ft, f = (shared ? u % st : (u - stiles) % ft) * 16 + c;
+            const uint32_t tok0 = shared ? item * kTile : items.first[item];
+            const uint32_t count = shared ? min(kTile, p.m - tok0) : items.count[item];
+            if (j >= count) continue;  // its sums are zero
+            const uint32_t cell = (i * 2 * kTile + j) * 16 + c;
+            const int64_t gi = round_shift(acc.get(cell), p.shift), ui = round_shift(acc.get(cell + kTile * 16), p.shift);
+            acc.clear(cell);
+            acc.clear(cell + kTile * 16);
+            if (f >= (shared ? p.sgate.s.n : p.gate.s.n)) continue;
+            const int64_t s = fx_to_i64(table_at(p.silu, p.silu_len, gi, (int64_t)(p.silu_len / 2)));
+            uint32_t d;
+            bad |= !q4_digits(round_shift(fx_wmul(s, ui), p.shift), &d);
+            uint8_t* to = (shared ? p.sact + (uint64_t)(tok0 + j) * p.sdown.s.blocks * 256
+                                  : p.act + (uint64_t)items.slot[tok0 + j] * p.down.s.blocks * 256) +
+                          f / 64 * 256 + q4_pos(f % 64);
+#pragma unroll
+            for (int q = 0; q < 4; q++) to[64 * q] = (uint8_t)(d >> (8 * q));
+        }
+        __syncthreads();
+    };
+    run(0, early);
+
+    // ---- routing
+    cluster_wait();
     for (uint32_t r = warp; r < p.m; r += kWarps)
-        route_token(p, r, rank ? other : raw, rank ? raw : other, s_sel, items.score, s_mask);
+        route_token(p, r, logits, logits + p.m * pitch, pitch, s_sel, items.score, s_mask);
     __syncthreads();
     if (warp == 0) list_items(p, s_sel, s_mask, &items);
     __syncthreads();
+    known = tiles_below(stiles + ft * items.n);
+    if (lane == 0) ask();
     if (blockIdx.x == 0)
         for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
             reinterpret_cast<uint32_t*>(p.items)[i] = reinterpret_cast<const uint32_t*>(&items)[i];
-    known = stiles + ft * items.n;
-
-    // ---- gate and up
-    const uint64_t fp = (uint64_t)p.down.s.blocks * 64, sp = (uint64_t)p.sdown.s.blocks * 64;
-    // A tile's last step, the SiLU lookup and the activation's digits, is held
-    // over to the next tile, when its table entries have come.
-    uint64_t held_silu = 0, held_row = 0;
-    int64_t held_up = 0;
-    uint8_t* held_to = nullptr;
-    auto finish_held = [&]() {
-        if (held_to) {
-            uint32_t d;
-            bad |= !q4_digits(fx_round_div_pow2(fx_wmul(fx_to_i64(held_silu), held_up), p.shift), &d);
-#pragma unroll
-            for (int j = 0; j < 4; j++) held_to[j * held_row] = (uint8_t)(d >> (8 * j));
-            held_to = nullptr;
-        }
-    };
-    uint32_t slot_at = 0;
-    for (uint32_t u = u0; u < known; u += step) {
-        const bool shared = u < stiles;
-        const uint32_t item = shared ? u / st : (u - stiles) / ft, tile = shared ? u % st : (u - stiles) % ft;
-        const uint32_t first = shared ? item * kTile : items.first[item];
-        const uint32_t count = shared ? min(kTile, p.m - first) : items.count[item];
-        const uint8_t* from[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t at = min(2 * i + (g >> 2), count - 1);
-            const uint32_t tok = shared ? first + at : items.slot[first + at] / p.top_k;
-            from[i] = digits + (size_t)(tok * 4 + (g & 3)) * p.stride + 16 * t;
-        }
-        Q4Sum<2> sum[2];
-        sum[0].clear();
-        sum[1].clear();
-        for (uint32_t b = b0; b < b1; b++) {
-            __syncwarp();  // every lane has read the slot that is filled next
-            ask();
-            taken++;
-            copy_wait_upto<DEPTH - 1>(asked - taken);
-            __syncwarp();
-            const uint8_t* slot = ring + slot_at * kUpSlot;
-            slot_at = slot_at + 1 == DEPTH ? 0 : slot_at + 1;
-            if (count > 2)
-                up_block<G, 2>(sum, slot, from, b);
-            else
-                up_block<G, 1>(sum, slot, from, b);
-        }
-        long long* to = red + (size_t)warp * (2 * kTile * 16);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (2 * i < count) {
-                long long v0, v1, w0, w1;
-                sum[0].finish(i, &v0, &v1);
-                sum[1].finish(i, &w0, &w1);
-                if (!(t & 1)) {
-                    long long* q = to + (2 * i + (t >> 1)) * 16;
-                    q[g] = v0;
-                    q[g + 8] = v1;
-                    q[kTile * 16 + g] = w0;
-                    q[kTile * 16 + g + 8] = w1;
-                }
-            }
-        group_sync(1 + mine, p.split * 32);
-        finish_held();
-        const uint32_t o = part * 32 + lane, c = o & 15, j = o >> 4, f = tile * 16 + c;  // split >= 2: one each
-        if (j < count && f < (shared ? p.sgate.s.n : p.gate.s.n)) {
-            uint64_t gv = 0, uv = 0;
-            for (uint32_t w = 0; w < p.split; w++) {
-                const long long* r = red + (size_t)(mine * p.split + w) * (2 * kTile * 16) + j * 16 + c;
-                gv += (uint64_t)r[0];
-                uv += (uint64_t)r[kTile * 16];
-            }
-            held_silu = table_at(p.silu, p.silu_len, fx_round_div_pow2((int64_t)gv, p.shift), (int64_t)(p.silu_len / 2));
-            held_up = fx_round_div_pow2((int64_t)uv, p.shift);
-            held_row = shared ? sp : fp;
-            held_to = (shared ? p.sact + (first + j) * 4 * sp : p.act + items.slot[first + j] * 4 * fp) + q4_pos(f);
-        }
-        group_sync(1 + mine, p.split * 32);  // the sums have been read
-    }
-    finish_held();
+    for (uint32_t first = early; first < known; first += kUpBatch) run(first, min(kUpBatch, known - first));
     if (bad) atomicOr(p.err, kErrRange);
+    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
 }
 
 constexpr int kDownDepth = 4;
-constexpr uint32_t kDownSlot = 2 * 512 + 2 * 512 + 2 * 64;  // two tiles' codes, the digits of four rows, scales
 
 // Blocks of the stream that a warp of k_moe_down takes: the chosen experts'
 // items one after another, then the shared experts' runs of tokens
 struct DownAt {
-    uint32_t item, b, count, first;
+    uint32_t b, len, count, first;
     bool shared;
-    const Q4Weight* w;
-    uint64_t tile0, tile1;
-    const uint8_t* from[2];  // this lane's digits
+    const uint8_t *w0, *w1;  // block b of the two tiles
 };
 
-template <int G>
+template <bool TWO>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Items items;
+    __shared__ __align__(8) uint64_t s_bar[kWarps * kDownDepth];
+    constexpr uint32_t kBytes = TWO ? 576 : 544, kSlot = 2 * kBytes + 256 * kTile;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t rank = cluster.block_rank(), slots = p.m * p.top_k, cells = (slots + p.m) * 32;
-    uint8_t* ring = smem + (size_t)warp * kDownDepth * kDownSlot;
-    unsigned long long* raw = reinterpret_cast<unsigned long long*>(smem + (size_t)kWarps * kDownDepth * kDownSlot);
+    uint8_t* ring = smem + (size_t)warp * p.depth * kSlot;
+    const Limbs acc{reinterpret_cast<uint32_t*>(smem + (size_t)kWarps * p.depth * kSlot), cells};
+    const uint32_t bar = shared_addr(&s_bar[warp * kDownDepth]);
     let_next_start();
-    for (uint32_t i = threadIdx.x; i < cells; i += kThreads) raw[i] = 0;
-    const uint32_t tiles = p.down.s.tiles, t0 = (blockIdx.x / 2) * 2, t1 = min(t0 + 1, tiles - 1);
-    {   // the shared experts' codes of these columns start for the second-level cache
-        const uint32_t bytes = p.sdown.s.blocks * 512;
-        if (threadIdx.x < 2) prefetch_l2(p.sdown.codes + (uint64_t)(threadIdx.x ? t1 : t0) * p.sdown.s.blocks * 32, bytes);
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < kDownDepth; i++) barrier_init(bar + 8 * i);
+        barrier_init_done();
     }
+    __syncwarp();
+    for (uint32_t i = threadIdx.x; i < 3 * cells; i += kThreads) acc.w[i] = 0;
+    const uint32_t tiles = p.down.s.tiles, t0 = (blockIdx.x / 2) * 2, t1 = min(t0 + 1, tiles - 1);
+    if (threadIdx.x < 2)  // the shared experts' codes of these columns start for the second-level cache
+        prefetch_l2(p.sdown.w + (uint64_t)(threadIdx.x ? t1 : t0) * p.sdown.s.blocks * kBytes, p.sdown.s.blocks * kBytes);
     wait_for_previous();
     for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
         reinterpret_cast<uint32_t*>(&items)[i] = __ldcg(reinterpret_cast<const uint32_t*>(p.items) + i);
     __syncthreads();
 
-    const uint32_t unit = G == 128 ? 2 : 1, nf = p.down.s.blocks / unit, ns = p.sdown.s.blocks / unit;
+    const uint32_t nf = p.down.s.blocks, ns = p.sdown.s.blocks;
     const uint32_t stiles = (p.m + kTile - 1) / kTile, routed = nf * items.n, total = routed + ns * stiles;
-    const uint64_t fp = (uint64_t)p.down.s.blocks * 64, sp = (uint64_t)p.sdown.s.blocks * 64;
     const uint32_t who = rank * kWarps + warp;
-    uint32_t at = (uint32_t)((uint64_t)who * total / (2 * kWarps)) * unit;
-    const uint32_t end = (uint32_t)((uint64_t)(who + 1) * total / (2 * kWarps)) * unit;
+    uint32_t at = (uint32_t)((uint64_t)who * total / (2 * kWarps));
+    const uint32_t end = (uint32_t)((uint64_t)(who + 1) * total / (2 * kWarps));
     auto locate = [&](DownAt& d, uint32_t pos) {
-        const uint32_t split = routed * unit;
-        d.shared = pos >= split;
-        const uint32_t in = d.shared ? pos - split : pos, len = d.shared ? p.sdown.s.blocks : p.down.s.blocks;
-        d.item = in / len;
-        d.b = in % len;
-        d.first = d.shared ? d.item * kTile : items.first[d.item];
-        d.count = d.shared ? min(kTile, p.m - d.first) : items.count[d.item];
-        d.w = d.shared ? &p.sdown : &p.down;
-        const uint64_t base = d.shared ? 0 : (uint64_t)items.expert[d.item] * tiles;
-        d.tile0 = base + t0;
-        d.tile1 = base + t1;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t j = min(2 * i + (g >> 2), d.count - 1);
-            d.from[i] = (d.shared ? p.sact + ((uint64_t)(d.first + j) * 4 + (g & 3)) * sp
-                                  : p.act + ((uint64_t)items.slot[d.first + j] * 4 + (g & 3)) * fp) + 16 * t;
-        }
+        d.shared = pos >= routed;
+        const uint32_t in = d.shared ? pos - routed : pos;
+        d.len = d.shared ? ns : nf;
+        const uint32_t item = in / d.len;
+        d.b = in % d.len;
+        d.first = d.shared ? item * kTile : items.first[item];
+        d.count = d.shared ? min(kTile, p.m - d.first) : items.count[item];
+        const uint8_t* w = d.shared ? p.sdown.w : p.down.w + (uint64_t)items.expert[item] * tiles * nf * kBytes;
+        d.w0 = w + ((uint64_t)t0 * d.len + d.b) * kBytes;
+        d.w1 = w + ((uint64_t)t1 * d.len + d.b) * kBytes;
     };
     DownAt next, now;
     uint32_t next_at = at, next_slot = 0;
     if (at < end) {
-        locate(next, at);
-        now = next;
+        locate(now, at);
+        next = now;
     }
-    auto issue = [&]() {
-        if (next_at < end) {
-            uint8_t* slot = ring + next_slot * kDownSlot;
-            const uint64_t blocks = next.w->s.blocks, groups = next.w->s.groups * 8ull;
-            copy16(slot + lane * 16, next.w->codes + (next.tile0 * blocks + next.b) * 32 + lane);
-            copy16(slot + 512 + lane * 16, next.w->codes + (next.tile1 * blocks + next.b) * 32 + lane);
-            copy16(slot + 1024 + lane * 16, next.from[0] + next.b * 64);
-            if (next.count > 2) copy16(slot + 1536 + lane * 16, next.from[1] + next.b * 64);
-            uint32_t* sc = reinterpret_cast<uint32_t*>(slot + 2048);
-            copy_scales<G>(sc, next.w->scales + next.tile0 * groups, next.b, g, t);
-            copy_scales<G>(sc + 16, next.w->scales + next.tile1 * groups, next.b, g, t);
-            next_slot = next_slot + 1 == kDownDepth ? 0 : next_slot + 1;
-            next_at++;
-            if (++next.b == next.w->s.blocks && next_at < end) locate(next, next_at);
-        }
-        copy_commit();
+    auto ask = [&]() {  // lane 0 only
+        const uint32_t b = bar + 8 * next_slot, to = shared_addr(ring + next_slot * kSlot);
+        barrier_expect(b, 2 * kBytes + 256 * next.count);
+        bulk_copy(to, next.w0, kBytes, b);
+        bulk_copy(to + kBytes, next.w1, kBytes, b);
+        for (uint32_t j = 0; j < next.count; j++)
+            bulk_copy(to + 2 * kBytes + 256 * j,
+                      (next.shared ? p.sact + (uint64_t)(next.first + j) * ns * 256
+                                   : p.act + (uint64_t)items.slot[next.first + j] * nf * 256) + next.b * 256, 256, b);
+        next_slot = next_slot + 1 == p.depth ? 0 : next_slot + 1;
+        next_at++;
+        next.w0 += kBytes;
+        next.w1 += kBytes;
+        if (++next.b == next.len && next_at < end) locate(next, next_at);
     };
-#pragma unroll
-    for (int i = 0; i < kDownDepth - 1; i++) issue();
-    uint32_t slot_at = 0;
+    if (lane == 0)
+        for (uint32_t i = 0; i < p.depth; i++)
+            if (next_at < end) ask();
+    Patience patience;
+    uint32_t slot = 0, phase = 0;
     while (at < end) {
-        const uint32_t stop = min(end, at + now.w->s.blocks - now.b);
+        const uint32_t stop = min(end, at + now.len - now.b);
         Q4Sum<2> sum[2];
         sum[0].clear();
         sum[1].clear();
-        for (; at < stop; at++, now.b++) {
-            __syncwarp();
-            issue();
-            copy_wait<kDownDepth - 1>();
-            __syncwarp();
-            const uint8_t* slot = ring + slot_at * kDownSlot;
-            slot_at = slot_at + 1 == kDownDepth ? 0 : slot_at + 1;
+        // digits of columns g: digit row g % 4 of token g / 4 (and 2 + g / 4) of the item
+        const uint32_t x0 = 2 * kBytes + min(g >> 2, now.count - 1) * 256 + (g & 3) * 64 + 16 * t;
+        const uint32_t x1 = 2 * kBytes + min(2 + (g >> 2), now.count - 1) * 256 + (g & 3) * 64 + 16 * t;
+        for (; at < stop; at++) {
+            barrier_wait(bar + 8 * slot, phase, patience);
+            const uint8_t* s = ring + slot * kSlot;
             uint4 x[2];
-            x[0] = *reinterpret_cast<const uint4*>(slot + 1024 + lane * 16);
-            if (now.count > 2) x[1] = *reinterpret_cast<const uint4*>(slot + 1536 + lane * 16);
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const uint4 w = *reinterpret_cast<const uint4*>(slot + q * 512 + lane * 16);
-                const uint32_t* sc = reinterpret_cast<const uint32_t*>(slot + 2048 + q * 64);
-                if (now.count > 2)
-                    q4_block_n<G, 2>(sum[q], w, sc[g], G == 32 ? sc[8 + g] : 0, x, now.b & 1);
-                else
-                    q4_block_n<G, 1>(sum[q], w, sc[g], G == 32 ? sc[8 + g] : 0, x, now.b & 1);
+            x[0] = *reinterpret_cast<const uint4*>(s + x0);
+            if (now.count > 2) {
+                x[1] = *reinterpret_cast<const uint4*>(s + x1);
+                q4_block<TWO, 2>(sum[0], s, x);
+                q4_block<TWO, 2>(sum[1], s + kBytes, x);
+            } else {
+                q4_block<TWO, 1>(sum[0], s, x);
+                q4_block<TWO, 1>(sum[1], s + kBytes, x);
+            }
+            __syncwarp();  // every lane has read the slot
+            if (lane == 0 && next_at < end) ask();
+            if (++slot == p.depth) {
+                slot = 0;
+                phase ^= 1;
             }
         }
 #pragma unroll
@@ -579,48 +573,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
                 const uint32_t j = 2 * i + (t >> 1);
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
-                    long long v0, v1;
-                    sum[q].finish(i, &v0, &v1);
-                    if (!(t & 1) && j < now.count) {
-                        const uint32_t slot = now.shared ? slots + now.first + j : items.slot[now.first + j];
-                        atomicAdd(&raw[slot * 32 + q * 16 + g], (unsigned long long)v0);
-                        atomicAdd(&raw[slot * 32 + q * 16 + g + 8], (unsigned long long)v1);
-                    }
+                    const long long v = sum[q].finish(i);
+                    if (j < now.count)
+                        acc.add((now.shared ? slots + now.first + j : items.slot[now.first + j]) * 32 + q * 16 + g + 8 * (t & 1), v);
                 }
             }
         if (at < end) locate(now, at);
     }
+    __syncwarp();
     cluster.sync();
     // A block finishes 16 of the 32 columns, with its neighbour's part of the sums
-    const unsigned long long* there = cluster.map_shared_rank(raw, rank ^ 1);
+    const Limbs there{cluster.map_shared_rank(acc.w, rank ^ 1), cells};
     for (uint32_t o = threadIdx.x; o < p.m * 16; o += kThreads) {
         const uint32_t c = rank * 16 + (o & 15), r = o >> 4;
         const uint64_t n = (uint64_t)t0 * 16 + c;
         if (n >= p.h) continue;
         const uint32_t s = (slots + r) * 32 + c;
-        int64_t y = fx_round_div_pow2((int64_t)(raw[s] + there[s]), p.shift);
+        int64_t y = round_shift(fx_wadd(acc.get(s), there.get(s)), p.shift);
         for (uint32_t j = 0; j < p.top_k; j++) {
             const uint32_t k = (r * p.top_k + j) * 32 + c;
-            const int64_t d = fx_round_div_pow2((int64_t)(raw[k] + there[k]), p.shift);
-            y = fx_wadd(y, fx_round_div_pow2(fx_wmul(d, items.score[r * p.top_k + j]), 16));
+            const int64_t d = round_shift(fx_wadd(acc.get(k), there.get(k)), p.shift);
+            y = fx_wadd(y, round_shift(fx_wmul(d, items.score[r * p.top_k + j]), 16));
         }
         uint64_t f = fx_from_i64(y);
         if (p.residual) f = gl_canon(gl_add(f, gl_canon(__ldg(p.residual + r * p.ldr + n))));
         p.out[r * (uint64_t)p.h + n] = f;
     }
+    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
     cluster.sync();  // no block leaves while its sums may still be read
 }
 
 // Dynamic shared memory of k_moe_up
-size_t up_shared(uint32_t m, uint32_t stride, uint32_t etiles, uint32_t depth) {
-    return (size_t)kWarps * depth * kUpSlot + kUpRed + (size_t)m * (4 * stride + 2 * 16 * 8 * etiles);
+size_t up_shared(uint32_t m, uint32_t stride, uint32_t etiles, uint32_t bytes, uint32_t depth) {
+    return (size_t)kWarps * depth * 2 * bytes + 12 * kUpCells + (size_t)m * (4 * stride + 2 * 16 * 8 * ((etiles + 1) / 2));
 }
 
 constexpr uint32_t kUpShallow = 3, kUpDeep = 6;
 
-uint32_t tokens_at_once(uint32_t stride, uint32_t etiles) {
+uint32_t tokens_at_once(uint32_t stride, uint32_t etiles, uint32_t bytes) {
     uint32_t m = kMaxTokens;
-    while (m > 1 && up_shared(m, stride, etiles, kUpShallow) > kMaxShared) m--;
+    while (m > 1 && up_shared(m, stride, etiles, bytes, kUpShallow) > kMaxShared) m--;
     return m;
 }
 
@@ -635,43 +627,25 @@ bool moe_shapes(uint64_t h, uint64_t experts, uint64_t top_k, uint64_t f, uint64
            q4_shape(h, shared_f, group, 0, &s->sup) && q4_shape(shared_f, h, group, 0, &s->sdown);
 }
 
-// Warps to a tile of k_moe_up (at least two: a thread then finishes one
-// result): fewest steps of a block's warps, each
-// tile with what it costs besides its blocks, for the number of experts that
-// m tokens choose if all are alike
-uint32_t up_split(const MoeArgs& p, uint32_t unit) {
-    const double hit = p.experts * (1 - pow(1 - (double)p.top_k / p.experts, p.m));
-    const uint64_t tiles = (uint64_t)(hit * p.gate.s.tiles) + ceil_div(p.m, kTile) * p.sgate.s.tiles;
-    uint64_t least = ~0ull;
-    uint32_t split = 2;
-    for (uint32_t s = 2; s <= (uint32_t)kWarps; s *= 2) {
-        const uint64_t cost = ceil_div(tiles, (uint64_t)kSms * (kWarps / s)) *
-                              (ceil_div(p.gate.s.blocks / unit, s) * unit + 2);
-        if (cost < least) {
-            least = cost;
-            split = s;
-        }
-    }
-    return split;
-}
-
-template <int G, int DEPTH>
+template <bool TWO, int DEPTH>
 int up_launch(const MoeArgs& p, cudaStream_t stream) {
     static std::atomic<uint64_t> set{0};
-    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_up<G, DEPTH>), kMaxShared, &set));
-    return launch(k_moe_up<G, DEPTH>, dim3(kSms), kThreads, up_shared(p.m, p.stride, p.etiles, DEPTH), 2, stream, p);
+    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_up<TWO, DEPTH>), kMaxShared, &set));
+    return launch(k_moe_up<TWO, DEPTH>, dim3(kSms), kThreads, up_shared(p.m, p.stride, p.etiles, p.gate.s.bytes, DEPTH),
+                  2, stream, p);
 }
 
-template <int G>
+template <bool TWO>
 int moe_launch(MoeArgs p, cudaStream_t stream) {
-    p.split = up_split(p, G == 128 ? 2 : 1);
-    const int rc = up_shared(p.m, p.stride, p.etiles, kUpDeep) <= kMaxShared ? up_launch<G, kUpDeep>(p, stream)
-                                                                             : up_launch<G, kUpShallow>(p, stream);
+    const bool deep = up_shared(p.m, p.stride, p.etiles, p.gate.s.bytes, kUpDeep) <= kMaxShared;
+    const int rc = deep ? up_launch<TWO, kUpDeep>(p, stream) : up_launch<TWO, kUpShallow>(p, stream);
     if (rc) return rc;
     static std::atomic<uint64_t> set{0};
-    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_down<G>), kMaxShared, &set));
-    const size_t shared = (size_t)kWarps * kDownDepth * kDownSlot + 8ull * (p.m * p.top_k + p.m) * 32;
-    return launch(k_moe_down<G>, dim3((p.down.s.tiles + 1) / 2 * 2), kThreads, shared, 2, stream, p);
+    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_down<TWO>), kMaxShared, &set));
+    const size_t sums = 12ull * (p.m * p.top_k + p.m) * 32, slot = (size_t)kWarps * (2 * p.down.s.bytes + 256 * kTile);
+    p.depth = kDownDepth;
+    while (p.depth * slot + sums > kMaxShared) p.depth--;  // three at least: 104 and 105 kB
+    return launch(k_moe_down<TWO>, dim3((p.down.s.tiles + 1) / 2 * 2), kThreads, p.depth * slot + sums, 2, stream, p);
 }
 
 }  // namespace
@@ -682,20 +656,19 @@ using namespace zk;
 
 extern "C" {
 
-uint64_t zkie2_moe_router_words(uint64_t h, uint64_t experts, uint32_t group) {
+uint64_t zkie2_moe_router_words(uint64_t h, uint64_t experts) {
     Q4Shape s;
-    if (experts == 0 || experts > kMaxExperts || !q4_shape(h, 16, group, 0, &s)) return 0;
+    if (experts == 0 || experts > kMaxExperts || !q4_shape(h, 16, 64, 0, &s)) return 0;
     return ceil_div(experts, 16) * s.blocks * 512;
 }
 
-int zkie2_moe_router_pack(const uint64_t* d_w, uint64_t h, uint64_t experts, uint32_t group, uint32_t* d_packed,
-                          uint32_t* d_err, cudaStream_t stream) {
-    Q4Shape s;
-    if (experts == 0 || experts > kMaxExperts || !q4_shape(h, 16, group, 0, &s) || !d_w || !d_packed || !d_err)
-        return (int)cudaErrorInvalidValue;
-    const uint64_t blocks = ceil_div(ceil_div(experts, 16) * s.blocks * 512, 256);
+int zkie2_moe_router_pack(const uint64_t* d_w, uint64_t h, uint64_t experts, uint32_t* d_packed, uint32_t* d_err,
+                          cudaStream_t stream) {
+    const uint64_t words = zkie2_moe_router_words(h, experts);
+    if (words == 0 || !d_w || !d_packed || !d_err) return (int)cudaErrorInvalidValue;
+    const uint64_t blocks = ceil_div(words, 256);
     k_moe_router_pack<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), 256, 0, stream>>>(
-        d_w, (uint32_t)h, (uint32_t)experts, s.blocks, (uint32_t)ceil_div(experts, 16), d_packed, d_err);
+        d_w, (uint32_t)h, (uint32_t)experts, (uint32_t)ceil_div(h, 64), (uint32_t)ceil_div(experts, 16), d_packed, d_err);
     ZK_LAUNCH_CHECK();
     return 0;
 }
@@ -711,24 +684,24 @@ uint64_t zkie2_moe_rows_scratch_elems(uint64_t m, uint64_t h, uint64_t experts, 
 
 int zkie2_moe_rows(const uint64_t* d_x, uint64_t ldx, uint64_t m, uint64_t h, uint64_t experts, uint64_t top_k,
                    uint64_t f, uint64_t shared_f, uint32_t group, const uint32_t* d_router,
-                   const uint32_t* const* h_codes, const uint32_t* const* h_scales, const uint64_t* d_exp_table,
-                   uint64_t exp_len, const uint64_t* d_silu_table, uint64_t silu_len, uint32_t shift,
+                   const uint32_t* const* h_weights, const uint64_t* d_exp_table, uint64_t exp_len,
+                   const uint64_t* d_silu_table, uint64_t silu_len, uint32_t shift,
                    const uint64_t* d_residual, uint64_t ldr, uint64_t* d_out, uint64_t* d_gate, uint32_t* d_err,
                    uint64_t* d_scratch, cudaStream_t stream) {
     MoeShapes s;
-    if (!moe_shapes(h, experts, top_k, f, shared_f, group, &s) || m > 65535 || shift > 62 || !d_router || !h_codes ||
-        !h_scales || !d_exp_table || exp_len == 0 || !d_silu_table || silu_len == 0 || !d_err || (m > 1 && ldx < h) ||
+    if (!moe_shapes(h, experts, top_k, f, shared_f, group, &s) || m > 65535 || shift > 62 || !d_router || !h_weights ||
+        !d_exp_table || exp_len == 0 || !d_silu_table || silu_len == 0 || !d_err || (m > 1 && ldx < h) ||
         (d_residual && m > 1 && ldr < h) || ((uintptr_t)d_router & 15) || ((uintptr_t)d_scratch & 15))
         return (int)cudaErrorInvalidValue;
     for (int i = 0; i < 6; i++)
-        if (!h_codes[i] || !h_scales[i] || ((uintptr_t)h_codes[i] & 15)) return (int)cudaErrorInvalidValue;
+        if (!h_weights[i] || ((uintptr_t)h_weights[i] & 15)) return (int)cudaErrorInvalidValue;
     if (m == 0) return 0;
     if (!d_x || !d_out || !d_scratch) return (int)cudaErrorInvalidValue;
     MoeArgs p{};
     const Q4Shape* shape[6] = {&s.up, &s.up, &s.down, &s.sup, &s.sup, &s.sdown};
     Q4Weight* weight[6] = {&p.gate, &p.up, &p.down, &p.sgate, &p.sup, &p.sdown};
     for (int i = 0; i < 6; i++)
-        *weight[i] = Q4Weight{reinterpret_cast<const uint4*>(h_codes[i]), h_scales[i], *shape[i]};
+        *weight[i] = Q4Weight{reinterpret_cast<const uint8_t*>(h_weights[i]), *shape[i]};
     p.ldx = ldx;
     p.h = (uint32_t)h;
     p.experts = (uint32_t)experts;
@@ -743,7 +716,7 @@ int zkie2_moe_rows(const uint64_t* d_x, uint64_t ldx, uint64_t m, uint64_t h, ui
     p.ldr = ldr;
     p.err = d_err;
     p.stride = q4_digit_stride(s.up.blocks);
-    const uint32_t most = tokens_at_once(p.stride, p.etiles);
+    const uint32_t most = tokens_at_once(p.stride, p.etiles, s.up.bytes);
     const uint64_t slots = (m < kMaxTokens ? m : kMaxTokens) * top_k;
     p.items = reinterpret_cast<Items*>(d_scratch);
     p.act = reinterpret_cast<uint8_t*>(d_scratch) + ceil_div(sizeof(Items), 16) * 16;
@@ -754,8 +727,7 @@ int zkie2_moe_rows(const uint64_t* d_x, uint64_t ldx, uint64_t m, uint64_t h, ui
         p.residual = d_residual ? d_residual + r * ldr : nullptr;
         p.out = d_out + r * h;
         p.gate_out = d_gate ? d_gate + r * experts : nullptr;
-        const int rc = group == 32 ? moe_launch<32>(p, stream) : group == 64 ? moe_launch<64>(p, stream)
-                                                                              : moe_launch<128>(p, stream);
+        const int rc = group == 32 ? moe_launch<true>(p, stream) : moe_launch<false>(p, stream);
         if (rc) return rc;
     }
     return 0;

@@ -13,18 +13,21 @@
 // is a few per cent either way, so nothing is gained from accumulators in
 // tensor memory and a good deal of set-up is saved.
 //
-// The sums are exact: within a group 16 c d stays below 2^29 even with two
+// The sums are exact: within a block 16 c d stays below 2^29 even with two
 // digits joined, the scaled group sums are added in 64 bits, and a padded K
 // of at most kQ4MaxK keeps the whole sum below 2^63, where a sum of 64-bit
 // numbers and one in the field are the same number.
 //
-// Layout.  K is padded to blocks of 64 (128 for G = 128; within each segment
-// where the weight has segments), N to tiles of 16.  Block (tile, b) holds
-// for lane (g = lane / 4, t = lane % 4) four words; byte j of word q holds in
-// its low half the code of row 8 t + 4 (q / 2) + j and in its high half that
-// of row 32 + 8 t + 4 (q / 2) + j, both of column g + 8 (q % 2).  The scales
-// of (tile, group) are eight words: s[g] | s[g + 8] << 16.  Digits lie in the
-// order in which a lane reads them: q4_pos.
+// Layout.  K is padded to blocks of 64 (within each segment where the weight
+// has segments), N to tiles of 16; the blocks of a tile follow one another,
+// tile after tile.  A block holds for lane (g = lane / 4, t = lane % 4) four
+// words; byte j of word q holds in its low half the code of row 8 t + 4 (q / 2)
+// + j and in its high half that of row 32 + 8 t + 4 (q / 2) + j, both of column
+// g + 8 (q % 2).  After the codes come eight words of scales, s[g] | s[g + 8]
+// << 16 (for G = 32 a second eight, of the second 32 rows; for G = 128 two
+// blocks repeat theirs, 3 % of the bytes for blocks that stand alone).  Any
+// run of blocks is one piece of memory, so one bulk copy brings it.  Digits
+// lie in the order in which a lane reads them: q4_pos.
 #pragma once
 #include <cstdint>
 
@@ -37,26 +40,25 @@ constexpr uint32_t kQ4MaxK = 8192;
 constexpr uint32_t kErrRange = 8u;  // a value outside the range the single-token kernels take
 
 // Shape of a packed weight: k_seg rows to a segment (k itself without
-// segments), padded to kp_seg; blocks and groups per tile over all segments.
+// segments), padded to kp_seg; blocks per tile over all segments, bytes of one.
 struct Q4Shape {
-    uint32_t k, n, group, segs, k_seg, kp_seg, blocks, groups, tiles;
+    uint32_t k, n, group, segs, k_seg, kp_seg, blocks, tiles, bytes;
 };
 
 inline bool q4_shape(uint64_t k, uint64_t n, uint32_t group, uint64_t segment, Q4Shape* s) {
     if (k == 0 || n == 0 || k > kQ4MaxK || n > 0x7FFFFFF0ull) return false;
     if (group != 32 && group != 64 && group != 128) return false;
     if (segment && (segment > k || k % segment)) return false;
-    const uint32_t unit = group == 128 ? 128 : 64;
     s->k = (uint32_t)k;
     s->n = (uint32_t)n;
     s->group = group;
     s->k_seg = (uint32_t)(segment ? segment : k);
     s->segs = s->k / s->k_seg;
-    s->kp_seg = (s->k_seg + unit - 1) / unit * unit;
+    s->kp_seg = (s->k_seg + 63) / 64 * 64;
     if ((uint64_t)s->kp_seg * s->segs > kQ4MaxK) return false;
     s->blocks = s->kp_seg / 64 * s->segs;
-    s->groups = s->kp_seg / group * s->segs;
     s->tiles = (s->n + 15) / 16;
+    s->bytes = group == 32 ? 576 : 544;
     return true;
 }
 
@@ -72,6 +74,15 @@ __device__ __forceinline__ bool q4_digits(int64_t v, uint32_t* d) {
     return ok;
 }
 
+// the same from zero
+__device__ __forceinline__ void mma_s8_new(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                           uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+
 // the digits of four consecutive k, one word to each of the four digit rows
 __device__ __forceinline__ void q4_store_digits(uint8_t* to, size_t stride, const uint32_t (&d)[4]) {
 #pragma unroll
@@ -82,48 +93,107 @@ __device__ __forceinline__ void q4_store_digits(uint8_t* to, size_t stride, cons
     }
 }
 
+// The digits of `rows` rows of x (k_seg numbers to each of `segs` segments,
+// padded to kp_seg) into digit rows of `stride` bytes, four to a row; false in
+// a thread that met a number out of range.  A thread takes four numbers at a
+// time and has four such loads under way, whatever rows they belong to: one
+// after the other, eight rows would cost eight times the memory's latency.
+template <int THREADS>
+__device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint64_t ldx, uint32_t rows, uint32_t segs,
+                                            uint32_t k_seg, uint32_t kp_seg, uint8_t* digits, uint32_t stride) {
+    const uint32_t quads = segs * kp_seg / 4, total = rows * quads;
+    const bool wide = (((uintptr_t)x | (ldx * 8)) & 15) == 0 && k_seg % 4 == 0;  // 16-byte loads
+    bool ok = true;
+    for (uint32_t i0 = threadIdx.x; i0 < total; i0 += THREADS * 4) {
+        int64_t v[4][4];
+        uint32_t to[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const uint32_t i = i0 + u * THREADS;
+            const bool on = i < total;
+            const uint32_t r = on ? i / quads : 0, k0 = on ? (i % quads) * 4 : 0;
+            const uint32_t seg = segs > 1 ? k0 / kp_seg : 0, in = k0 - seg * kp_seg;
+            const uint64_t* from = x + r * ldx + seg * k_seg + in;
+            to[u] = on ? r * 4 * stride + q4_pos(k0) : ~0u;
+            if (wide) {
+                ulonglong2 lo = make_ulonglong2(0, 0), hi = lo;
+                if (on && in < k_seg) {
+                    lo = __ldg(reinterpret_cast<const ulonglong2*>(from));
+                    hi = __ldg(reinterpret_cast<const ulonglong2*>(from) + 1);
+                }
+                v[u][0] = (int64_t)lo.x, v[u][1] = (int64_t)lo.y, v[u][2] = (int64_t)hi.x, v[u][3] = (int64_t)hi.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[u][j] = on && in + j < k_seg ? (int64_t)__ldg(from + j) : 0;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (to[u] != ~0u) {
+                uint32_t d[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) ok &= q4_digits(fx_to_i64((uint64_t)v[u][j]), &d[j]);
+                q4_store_digits(digits + to[u], stride, d);
+            }
+    }
+    return ok;
+}
+
 // bytes of a digit row: 64 mod 128, so that the eight lanes that read at once
 // (two rows, 64 bytes each) meet no shared-memory bank twice
 inline uint32_t q4_digit_stride(uint32_t blocks) { return blocks % 2 ? blocks * 64 : blocks * 64 + 64; }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// ---- asynchronous copies: a warp's ring of slots in shared memory ---------------------------
-// A lane copies the 16 bytes that it will read itself (scales: a few lanes,
-// for all), so a slot is ready when the lane's own copies are and the warp has
-// met once; the bytes in flight do not depend on registers, and the stream of
-// a warp's blocks runs on across tiles, sums and barriers.
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
-                 : "memory");
-}
-__device__ __forceinline__ void copy4(void* to, const void* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
-                 : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// ---- a warp's ring of slots, filled by bulk copies ----------------------------------------
+// One lane asks for a run of blocks with one instruction; a barrier in shared
+// memory counts its bytes.  The bytes in flight depend on no register, and the
+// stream of a warp's blocks runs on across tiles, sums and block-wide waits.
+// A wait gives up after a bounded number of attempts (a second or so), says so
+// in the error word, and every later one then after a few.
+constexpr uint32_t kErrWait = 32u;
 
-// wait until at most n (< N + 1) of the groups asked for are still on their way
-template <int N>
-__device__ __forceinline__ void copy_wait_upto(uint32_t n) {
-    if constexpr (N == 0) {
-        copy_wait<0>();
-    } else {
-        if (n >= N)
-            copy_wait<N>();
-        else
-            copy_wait_upto<N - 1>(n);
+struct Patience {
+    uint32_t tries = 1u << 18;
+    bool failed = false;
+};
+
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void barrier_init(uint32_t bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+}
+// after the inits, before the first copy
+__device__ __forceinline__ void barrier_init_done() {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+                 "l"(from), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, Patience& patience) {  // the whole warp
+    for (uint32_t i = 0; i < patience.tries; i++) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (__all_sync(0xFFFFFFFFu, done)) return;
     }
+    patience.failed = true;
+    patience.tries = 64;
 }
 
 // ---- overlap with the kernel before (programmatic dependent launch) --------------------------
@@ -134,96 +204,96 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // the two halves of a cluster's barrier
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 
 // a run of bytes (16-byte aligned, a multiple of 16) into the second-level cache
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
-// Running sums of one tile of 16 columns against NT pairs of rows: c the
-// present group's, a the scaled groups' (row g and g + 8 of the tile; lane t
-// holds digits 2 (t % 2) and 2 (t % 2) + 1, joined, of row t / 2 of a pair).
+// Running sums of one tile of 16 columns against NT pairs of rows: the scaled
+// groups' (row g and g + 8 of the tile; lane t holds digits 2 (t % 2) and
+// 2 (t % 2) + 1, joined, of row t / 2 of a pair).
 template <int NT>
 struct Q4Sum {
-    int c[NT][4];
     long long a[NT][2];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0;
-            a[i][0] = a[i][1] = 0;
-        }
+        for (int i = 0; i < NT; i++) a[i][0] = a[i][1] = 0;
     }
+    // c: a group's products (N of the pairs), s: its scales
     template <int N>
-    __device__ __forceinline__ void scale_group(uint32_t s) {
+    __device__ __forceinline__ void add_group(const int (&c)[N][4], uint32_t s) {
         const int s0 = (int)(s & 0xFFFFu), s1 = (int)(s >> 16);
 #pragma unroll
         for (int i = 0; i < N; i++) {
             a[i][0] += (long long)(c[i][0] + (c[i][1] << 8)) * s0;
             a[i][1] += (long long)(c[i][2] + (c[i][3] << 8)) * s1;
-            c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0;
         }
     }
-    // The sums themselves: sixteenfold and split over two lanes until here.
-    // Valid in every lane: the number of row t / 2 of the pair.
-    __device__ __forceinline__ void finish(int i, long long* v0, long long* v1) const {
+    // The sum itself, sixteenfold and split over two lanes until here: in lane
+    // (g, t) that of column g + 8 (t % 2) of the tile and row t / 2 of pair i.
+    __device__ __forceinline__ long long finish(int i) const {
         const bool high = threadIdx.x & 1;
-        long long r[2];
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const long long mine = a[i][q] >> 4;
-            const long long other = __shfl_xor_sync(0xFFFFFFFFu, mine, 1);
-            const long long lo = high ? other : mine, hi = high ? mine : other;
-            r[q] = (long long)((unsigned long long)lo + ((unsigned long long)hi << 16));
-        }
-        *v0 = r[0];
-        *v1 = r[1];
+        const long long got = __shfl_xor_sync(0xFFFFFFFFu, high ? a[i][0] : a[i][1], 1) >> 4;
+        const long long mine = (high ? a[i][1] : a[i][0]) >> 4;
+        return (long long)((unsigned long long)(high ? got : mine) + ((unsigned long long)(high ? mine : got) << 16));
     }
 };
 
-// One block of 64 k for NT of the MAX pairs: w the lane's codes, s0 (and s1 for G = 32) the scales of
-// the block's group(s), b the lane's digits; `last` where a group of 128 ends.
-template <int G, int NT, int MAX>
-__device__ __forceinline__ void q4_block_n(Q4Sum<MAX>& sum, const uint4& w, uint32_t s0, uint32_t s1,
-                                           const uint4 (&b)[MAX], bool last) {
+// Sums of 64-bit numbers from several warps in shared memory: three words of
+// 22, 22 and 20 bits a number, each added by an atomic that returns nothing
+// (the 64-bit one is a loop of compare-and-swaps here, 9 to 240 cycles a warp).
+// Up to 1024 numbers to a sum; exact modulo 2^64.
+struct Limbs {
+    uint32_t* w;
+    uint32_t n;  // numbers
+    __device__ __forceinline__ void add(uint32_t at, long long v) const {
+        atomicAdd(w + at, (uint32_t)v & 0x3FFFFFu);
+        atomicAdd(w + n + at, (uint32_t)(v >> 22) & 0x3FFFFFu);
+        atomicAdd(w + 2 * n + at, (uint32_t)(v >> 44));
+    }
+    __device__ __forceinline__ long long get(uint32_t at) const {
+        return (long long)((unsigned long long)w[at] + ((unsigned long long)w[n + at] << 22) +
+                           ((unsigned long long)w[2 * n + at] << 44));
+    }
+    __device__ __forceinline__ void clear(uint32_t at) const { w[at] = w[n + at] = w[2 * n + at] = 0; }
+};
+
+// One block of 64 k at `block` in shared memory against NT of the MAX pairs of
+// rows, their digits in b.  TWO: two groups of 32 rows, else one.
+template <bool TWO, int NT, int MAX>
+__device__ __forceinline__ void q4_block(Q4Sum<MAX>& sum, const uint8_t* block, const uint4 (&b)[MAX]) {
     constexpr uint32_t kHigh = 0xF0F0F0F0u;  // a code in a byte's high half is sixteen times itself
+    const uint32_t lane = threadIdx.x & 31;
+    const uint4 w = *reinterpret_cast<const uint4*>(block + lane * 16);
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(block + 512) + (lane >> 2);
+    const uint32_t s0 = scales[0], s1 = TWO ? scales[8] : 0;
+    int c[NT][4];
     {
         const uint32_t a0 = (w.x << 4) & kHigh, a1 = (w.y << 4) & kHigh, a2 = (w.z << 4) & kHigh,
                        a3 = (w.w << 4) & kHigh;
 #pragma unroll
-        for (int i = 0; i < NT; i++) mma_s8(sum.c[i], a0, a1, a2, a3, b[i].x, b[i].y);
+        for (int i = 0; i < NT; i++) mma_s8_new(c[i], a0, a1, a2, a3, b[i].x, b[i].y);
     }
-    if (G == 32) sum.template scale_group<NT>(s0);
+    if (TWO) sum.template add_group<NT>(c, s0);
     {
         const uint32_t a0 = w.x & kHigh, a1 = w.y & kHigh, a2 = w.z & kHigh, a3 = w.w & kHigh;
 #pragma unroll
-        for (int i = 0; i < NT; i++) mma_s8(sum.c[i], a0, a1, a2, a3, b[i].z, b[i].w);
+        for (int i = 0; i < NT; i++) {
+            if (TWO)
+                mma_s8_new(c[i], a0, a1, a2, a3, b[i].z, b[i].w);
+            else
+                mma_s8(c[i], a0, a1, a2, a3, b[i].z, b[i].w);
+        }
     }
-    if (G == 32)
-        sum.template scale_group<NT>(s1);
-    else if (G == 64)
-        sum.template scale_group<NT>(s0);
-    else if (last)
-        sum.template scale_group<NT>(s0);
+    sum.template add_group<NT>(c, TWO ? s1 : s0);
 }
 
-template <int G, int NT>
-__device__ __forceinline__ void q4_block(Q4Sum<NT>& sum, const uint4& w, uint32_t s0, uint32_t s1,
-                                         const uint4 (&b)[NT], bool last) {
-    q4_block_n<G, NT, NT>(sum, w, s0, s1, b, last);
-}
-
-// The scale words of block b of a tile into a slot (16 words): lanes t = 0,
-// and t = 1 for G = 32 with its second group.
-template <int G>
-__device__ __forceinline__ void copy_scales(uint32_t* to, const uint32_t* tile_scales, uint32_t b, uint32_t g,
-                                            uint32_t t) {
-    if (t < (G == 32 ? 2 : 1)) {
-        const uint32_t group = G == 32 ? 2 * b + t : (G == 64 ? b : b / 2);
-        copy4(to + 8 * t + g, tile_scales + (uint64_t)group * 8 + g);
-    }
+// round_div(a, 2^s): the quotient rounded down, plus the highest bit shifted out
+__device__ __forceinline__ int64_t round_shift(int64_t a, uint32_t s) {
+    return s ? (a >> s) + ((a >> (s - 1)) & 1) : a;
 }
 
 // from_i64(to_i64(v)'s table entry): Op::GeluIndex and Op::Lookup on one value

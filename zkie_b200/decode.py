@@ -24,7 +24,6 @@ likes (``check_err``); not given, the call reads its own, which synchronises,
 and raises ValueError.  Besides the op layer's bits, 8 is a value outside the
 32-bit range the kernels take (computed on as zero) and 16 a full cache.
 """
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
@@ -33,6 +32,9 @@ from . import _lib
 from ._lib import check, lib
 from .compose import _check_err, _err_word
 from .device import P, device
+
+_q4_project, _kv_attend, _moe_rows = lib.zkie2_q4_project, lib.zkie2_kv_attend, lib.zkie2_moe_rows
+_choose = lib.zkie2_choose_token
 
 GROUPS = (32, 64, 128)
 KV_BLOCK = 32
@@ -44,45 +46,65 @@ def check_err(err: torch.Tensor, what: str = "decode"):
     _check_err(err, what)
 
 
+# A step makes a call per operator and layer, each of a few microseconds on the
+# device, so the checks below are written to cost less than that.
+_U64, _I32 = torch.uint64, torch.int32
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def _on_device(t: torch.Tensor, name: str, dtype) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
-        raise ValueError(f"{name}: a CUDA tensor of {dtype} is wanted")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return t
+def _device_of(t, name: str) -> int:
+    """The index of the device that ``t`` and the call are on."""
+    if isinstance(t, torch.Tensor):
+        dev = t.get_device()
+        if dev >= 0 and dev == _current_device():
+            return dev
+    _refuse(t, name, None, "a tensor on the current CUDA device")
 
 
-def _rows(t: torch.Tensor, name: str, cols: int) -> torch.Tensor:
-    """A matrix of field elements with rows of ``cols`` of unit stride."""
-    _on_device(t, name, torch.uint64)
-    if t.dim() != 2 or t.shape[1] != cols:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, {cols} columns are wanted")
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
-        raise ValueError(f"{name}: rows of unit stride that do not overlap are wanted")
-    return t
+def _refuse(t, name: str, dtype, what: str):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: {what} is wanted, not {type(t).__name__}")
+    if not t.is_cuda or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name}: {what} is wanted{'' if dtype is None else f' ({dtype}, CUDA)'}, not {t.dtype} on "
+                         f"{t.device}")
+    if t.get_device() != _current_device():
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{_current_device()}")
+    raise ValueError(f"{name}: {what} is wanted, not shape {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _flat(t: torch.Tensor, name: str, dtype, shape=None) -> torch.Tensor:
-    _on_device(t, name, dtype)
-    if not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{name}: a contiguous tensor{'' if shape is None else f' of shape {tuple(shape)}'} is wanted")
-    return t
+def _rows(t, name: str, cols: int, dev: int) -> Tuple[int, int]:
+    """(rows, row stride) of a matrix of field elements with rows of ``cols``
+    numbers of unit stride that do not overlap."""
+    if isinstance(t, torch.Tensor) and t.dtype is _U64 and t.get_device() == dev:
+        shape = t.shape
+        if len(shape) == 2 and shape[1] == cols:
+            s0, s1 = t.stride()
+            if (s1 == 1 or cols == 1) and (s0 >= cols or shape[0] < 2):
+                return shape[0], s0
+    _refuse(t, name, _U64, f"a matrix of {cols} columns, unit stride within its rows,")
 
 
-def _word(err: Optional[torch.Tensor]) -> torch.Tensor:
+def _flat(t, name: str, dtype, dev: int, shape=None) -> torch.Tensor:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and \
+            (shape is None or t.shape == shape):
+        return t
+    _refuse(t, name, dtype, "a contiguous tensor" + ("" if shape is None else f" of shape {tuple(shape)}"))
+
+
+def _word(err: Optional[torch.Tensor], dev: int) -> torch.Tensor:
     if err is None:
         return _err_word()
-    return _flat(err, "err", torch.int32, (1,))
+    if err.dtype is _I32 and err.get_device() == dev and err.numel() == 1:
+        return err
+    _refuse(err, "err", _I32, "an int32 word")
 
 
-def _out(out, shape) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=torch.uint64, device=torch.device("cuda", torch.cuda.current_device()))
-    return _flat(out, "out", torch.uint64, shape)
+def _out(out, like: torch.Tensor, shape, dev: int) -> torch.Tensor:
+    return like.new_empty(shape) if out is None else _flat(out, "out", _U64, dev, shape)
 
 
 def _signed(t: torch.Tensor) -> torch.Tensor:
@@ -133,15 +155,15 @@ def quantise(w: torch.Tensor, group: int = 64, segment: int = 0) -> Tuple[torch.
 
 class QuantWeight:
     """A weight w[k][n] = codes[k][n] scales[row of k][n] in 4 bits, laid out
-    once for the kernels (``packed``, ``packed_scales``).
+    once for the kernels (``packed``).
 
     codes: int8, k x n or experts x k x n, in [-8, 7]; scales: whole numbers in
     [0, 65535], one for each ``group`` (32, 64 or 128) rows of a column, as
     many rows of them as groups begin.  ``segment`` splits the rows into runs
     (the heads of an output projection) that the product rounds one by one and
     adds, as the graph's Projection per head and its Adds do; groups begin
-    anew in each run.  At most 8192 rows, each run counted as a multiple of 64
-    (128 for group 128)."""
+    anew in each run.  At most 8192 rows, each run counted as a multiple of
+    64."""
 
     def __init__(self, codes, scales, group: int = 64, segment: int = 0):
         codes, scales = torch.as_tensor(codes).to(device()), torch.as_tensor(scales).to(device())
@@ -152,7 +174,7 @@ class QuantWeight:
         self.experts = codes.shape[0] if codes.dim() == 3 else 1
         self.k, self.n = int(codes.shape[-2]), int(codes.shape[-1])
         self.group, self.segment = group, segment
-        words = lib.zkie2_q4_code_words(self.experts, self.k, self.n, group, segment)
+        words = lib.zkie2_q4_words(self.experts, self.k, self.n, group, segment)
         if words == 0:
             raise ValueError(f"QuantWeight: {self.experts} x {self.k} x {self.n} with group {group} and segment "
                              f"{segment} is not taken (at most 8192 padded rows, segments that divide them)")
@@ -164,31 +186,31 @@ class QuantWeight:
         codes, scales = codes.contiguous(), scales.to(torch.int32).contiguous()
         dev = codes.device
         self.packed = torch.empty(words, dtype=torch.int32, device=dev)
-        self.packed_scales = torch.empty(lib.zkie2_q4_scale_words(self.experts, self.k, self.n, group, segment),
-                                         dtype=torch.int32, device=dev)
+        self.device, self.pointer = self.packed.get_device(), self.packed.data_ptr()
         err = _err_word()
         check(lib.zkie2_q4_pack(codes.data_ptr(), scales.data_ptr(), self.experts, self.k, self.n, group, segment,
-                                self.packed.data_ptr(), self.packed_scales.data_ptr(), err.data_ptr(), _stream()),
-              "zkie2_q4_pack")
+                                self.packed.data_ptr(), err.data_ptr(), _stream()), "zkie2_q4_pack")
         _check_err(err, "QuantWeight")
+
+    def _blocks(self) -> torch.Tensor:
+        return self.packed.reshape(self.experts, -(-self.n // 16), -1, 144 if self.group == 32 else 136)
 
     def codes(self) -> torch.Tensor:
         """The codes back (experts x k x n)."""
-        tiles, unit = -(-self.n // 16), 128 if self.group == 128 else 64
-        seg = self.segment or self.k
-        b = self.packed.view(torch.uint8).reshape(self.experts, tiles, -1, 8, 4, 2, 2, 4)
+        tiles, seg = -(-self.n // 16), self.segment or self.k
+        b = self._blocks()[..., :128].contiguous().view(torch.uint8).reshape(self.experts, tiles, -1, 8, 4, 2, 2, 4)
         both = torch.stack([b & 15, b >> 4], dim=-1).to(torch.int8)  # expert tile block g t q/2 q%2 j half
         both = torch.where(both > 7, both - 16, both)
-        full = both.permute(0, 2, 8, 4, 5, 7, 1, 6, 3).reshape(self.experts, -1, tiles * 16)
-        full = full.reshape(self.experts, self.k // seg, -(-seg // unit) * unit, tiles * 16)
+        full = both.permute(0, 2, 8, 4, 5, 7, 1, 6, 3).reshape(self.experts, self.k // seg, -(-seg // 64) * 64, tiles * 16)
         return full[:, :, :seg, :self.n].reshape(self.experts, self.k, self.n)
 
     def scales(self) -> torch.Tensor:
         """The scales back (experts x rows x n)."""
         tiles, seg = -(-self.n // 16), self.segment or self.k
-        w = self.packed_scales.reshape(self.experts, tiles, -1, 8)
+        w = self._blocks()[..., 128:].reshape(self.experts, tiles, -1, 8)
         both = torch.stack([w & 0xFFFF, (w >> 16) & 0xFFFF], dim=-1)  # expert tile group g half
         full = both.permute(0, 2, 1, 4, 3).reshape(self.experts, self.k // seg, -1, tiles * 16)
+        full = full[:, :, ::2 if self.group == 128 else 1]  # two blocks repeat a group of 128
         return full[:, :, :-(-seg // self.group), :self.n].reshape(self.experts, -1, self.n)
 
     def dense(self) -> torch.Tensor:
@@ -207,31 +229,30 @@ def project(x: torch.Tensor, weight: QuantWeight, shift: int, *, bias: Optional[
     then ``table[clamp(y + offset, 0, len - 1)]`` (GeluIndex and Lookup; offset
     defaults to the table's middle) and ``+ residual`` (m x n; Add) where
     given.  shift 0 without a bias is the MatMul arm.  |x| <= 0x7F7F7F7F."""
-    if weight.experts != 1:
-        raise ValueError("project: one weight is wanted, not a stack of experts")
-    x = _rows(x, "x", weight.k)
-    m, n = x.shape[0], weight.n
+    dev = _device_of(x, "x")
+    n = weight.n
+    m, ldx = _rows(x, "x", weight.k, dev)
+    if weight.experts != 1 or weight.device != dev:
+        raise ValueError("project: one weight (no stack of experts) on the current device is wanted")
     if not 0 <= shift <= 62 or m > 65535:
         raise ValueError("project: shift 0 .. 62 and at most 65535 rows are wanted")
+    p_bias = p_table = p_residual = None
+    table_len = ldr = 0
     if bias is not None:
-        _flat(bias, "bias", torch.uint64, (n,))
+        p_bias = _flat(bias, "bias", _U64, dev, (n,)).data_ptr()
     if table is not None:
-        _flat(table, "table", torch.uint64)
-        if table.numel() == 0:
+        p_table, table_len = _flat(table, "table", _U64, dev).data_ptr(), table.numel()
+        if table_len == 0:
             raise ValueError("project: an empty table")
-        offset = table.numel() // 2 if offset is None else offset
     if residual is not None:
-        _rows(residual, "residual", n)
-        if residual.shape[0] != m:
-            raise ValueError(f"residual: {residual.shape[0]} rows, {m} are wanted")
-    out, word = _out(out, (m, n)), _word(err)
-    check(lib.zkie2_q4_project(x.data_ptr(), x.stride(0), m, weight.packed.data_ptr(),
-                               weight.packed_scales.data_ptr(), weight.k, n, weight.group, weight.segment, shift,
-                               None if bias is None else bias.data_ptr(), None if table is None else table.data_ptr(),
-                               0 if table is None else table.numel(), offset or 0,
-                               None if residual is None else residual.data_ptr(),
-                               0 if residual is None else residual.stride(0), out.data_ptr(), word.data_ptr(),
-                               _stream()), "zkie2_q4_project")
+        rows, ldr = _rows(residual, "residual", n, dev)
+        if rows != m:
+            raise ValueError(f"residual: {rows} rows, {m} are wanted")
+        p_residual = residual.data_ptr()
+    out, word = _out(out, x, (m, n), dev), _word(err, dev)
+    check(_q4_project(x.data_ptr(), ldx, m, weight.pointer, weight.k, n, weight.group, weight.segment, shift, p_bias,
+                      p_table, table_len, table_len // 2 if offset is None else offset, p_residual, ldr, out.data_ptr(),
+                      word.data_ptr(), _raw_stream(dev)), "zkie2_q4_project")
     if err is None:
         _check_err(word, "project")
     return out
@@ -248,9 +269,10 @@ class KvCache:
     multiples of 4 up to 256, the capacity a multiple of 32 up to 131072."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor):
-        _flat(k, "k", torch.int32)
-        _flat(v, "v", torch.int32)
-        _flat(lens, "lens", torch.int32)
+        self.device = dev = _device_of(k, "k")
+        _flat(k, "k", _I32, dev)
+        _flat(v, "v", _I32, dev)
+        _flat(lens, "lens", _I32, dev)
         if k.dim() != 6 or v.dim() != 4 or k.shape[4:] != (KV_BLOCK, 4):
             raise ValueError("KvCache: k (batch, heads, capacity / 32, dk / 4, 32, 4) and v (batch, heads, capacity, "
                              "dv) are wanted")
@@ -266,6 +288,8 @@ class KvCache:
         if (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("KvCache: 16-byte aligned buffers are wanted")
         self.k, self.v, self.lens = k, v, lens
+        self._args = (k.data_ptr(), v.data_ptr(), lens.data_ptr(), self.batch, self.heads, self.dk, self.dv,
+                      self.capacity)
 
     @classmethod
     def zeros(cls, batch: int, heads: int, dk: int, dv: int, capacity: int,
@@ -284,18 +308,16 @@ class KvCache:
         ``advance``): k (batch, tokens, heads dk) and v (batch, tokens, heads
         dv) field elements, the keys through Scale by k_scale = (factor,
         shift).  |key| <= 2^27, values in 32 bits."""
-        _on_device(k, "k", torch.uint64)
-        _on_device(v, "v", torch.uint64)
-        if k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or k.shape[0] != self.batch or \
-                k.shape[2] != self.heads * self.dk or v.shape[2] != self.heads * self.dv:
-            raise ValueError("append: k (batch, tokens, heads dk) and v (batch, tokens, heads dv) are wanted")
-        if k.shape[1] > 1 << 17 or not 0 <= k_scale[1] <= 62:
-            raise ValueError("append: at most 131072 tokens and a shift 0 .. 62 are wanted")
-        k, v, word = k.contiguous(), v.contiguous(), _word(err)
-        check(lib.zkie2_kv_append(k.data_ptr(), k.shape[2], v.data_ptr(), v.shape[2], k.shape[1], k_scale[0],
-                                  k_scale[1], self.k.data_ptr(), self.v.data_ptr(), self.lens.data_ptr(), self.batch,
-                                  self.heads, self.dk, self.dv, self.capacity, word.data_ptr(), _stream()),
-              "zkie2_kv_append")
+        dev = _device_of(k, "k")
+        for name, t, cols in (("k", k, self.heads * self.dk), ("v", v, self.heads * self.dv)):
+            if t.dtype is not _U64 or t.get_device() != dev or t.dim() != 3 or t.shape[0] != self.batch or \
+                    t.shape[1] != k.shape[1] or t.shape[2] != cols:
+                _refuse(t, name, _U64, f"a tensor of {self.batch} sequences, as many tokens each and {cols} columns,")
+        if self.device != dev or k.shape[1] > 1 << 17 or not 0 <= k_scale[1] <= 62:
+            raise ValueError("append: the cache's device, at most 131072 tokens and a shift 0 .. 62 are wanted")
+        k, v, word = k.contiguous(), v.contiguous(), _word(err, dev)
+        check(lib.zkie2_kv_append(k.data_ptr(), k.shape[2], v.data_ptr(), v.shape[2], k.shape[1], *k_scale,
+                                  *self._args, word.data_ptr(), _raw_stream(dev)), "zkie2_kv_append")
         if err is None:
             _check_err(word, "append")
 
@@ -319,32 +341,31 @@ def attend(q: torch.Tensor, cache: KvCache, table: torch.Tensor, *, k: Optional[
     table[0] each in its softmax's sum: the rows agree where that is zero, as
     in the models' tables.  A sequence without tokens answers zeros.  Scaled
     queries and keys |q|, |k| <= 2^27; table values in [0, 2^31)."""
-    if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % (cache.heads * cache.dk):
-        raise ValueError("q: batch x (query heads dk) with a multiple of the cache's heads is wanted")
-    q = _rows(q, "q", q.shape[1])
-    heads = q.shape[1] // cache.dk
-    if q.shape[0] != cache.batch or (k is None) != (v is None):
-        raise ValueError("attend: a row per sequence, and k and v together, are wanted")
+    dev = _device_of(q, "q")
+    batch, one, dk, dv = cache.batch, cache.heads, cache.dk, cache.dv
+    cols = q.shape[-1]
+    heads = cols // dk
+    if cols == 0 or cols % (one * dk) or heads > 65535:
+        raise ValueError(f"q: {cols} columns, a multiple of {one * dk} is wanted")
+    rows, ldq = _rows(q, "q", cols, dev)
+    if rows != batch or (k is None) != (v is None) or cache.device != dev:
+        raise ValueError("attend: a row per sequence, k and v together, and the cache's device are wanted")
+    p_k = p_v = None
+    ldk = ldv = 0
     if k is not None:
-        _rows(k, "k", cache.heads * cache.dk)
-        _rows(v, "v", cache.heads * cache.dv)
-        if k.shape[0] != cache.batch or v.shape[0] != cache.batch:
+        rk, ldk = _rows(k, "k", one * dk, dev)
+        rv, ldv = _rows(v, "v", one * dv, dev)
+        if rk != batch or rv != batch:
             raise ValueError("attend: a row of k and v per sequence is wanted")
-    _flat(table, "table", torch.uint64)
-    for s in (q_scale[1], k_scale[1], score_scale[1], out_shift):
-        if not 0 <= s <= 62:
-            raise ValueError("attend: shifts 0 .. 62 are wanted")
-    if table.numel() == 0 or heads > 65535:
-        raise ValueError("attend: an empty table, or too many heads")
-    _on_device(cache.k, "cache", torch.int32)
-    out, word = _out(out, (cache.batch, heads * cache.dv)), _word(err)
-    check(lib.zkie2_kv_attend(q.data_ptr(), q.stride(0), heads, q_scale[0], q_scale[1],
-                              None if k is None else k.data_ptr(), 0 if k is None else k.stride(0),
-                              None if v is None else v.data_ptr(), 0 if v is None else v.stride(0), k_scale[0],
-                              k_scale[1], cache.k.data_ptr(), cache.v.data_ptr(), cache.lens.data_ptr(), cache.batch,
-                              cache.heads, cache.dk, cache.dv, cache.capacity, score_scale[0], score_scale[1],
-                              table.data_ptr(), table.numel(), table.numel() if offset is None else offset, out_shift,
-                              out.data_ptr(), word.data_ptr(), _stream()), "zkie2_kv_attend")
+        p_k, p_v = k.data_ptr(), v.data_ptr()
+    table_len = _flat(table, "table", _U64, dev).numel()
+    if table_len == 0 or not (0 <= q_scale[1] <= 62 and 0 <= k_scale[1] <= 62 and 0 <= score_scale[1] <= 62 and
+                              0 <= out_shift <= 62):
+        raise ValueError("attend: a table and shifts 0 .. 62 are wanted")
+    out, word = _out(out, q, (batch, heads * dv), dev), _word(err, dev)
+    check(_kv_attend(q.data_ptr(), ldq, heads, *q_scale, p_k, ldk, p_v, ldv, *k_scale, *cache._args, *score_scale,
+                     table.data_ptr(), table_len, table_len if offset is None else offset, out_shift, out.data_ptr(),
+                     word.data_ptr(), _raw_stream(dev)), "zkie2_kv_attend")
     if err is None:
         _check_err(word, "attend")
     return out
@@ -371,48 +392,50 @@ class MoeBlock:
             if (w.experts, w.k, w.n) != shape or w.group != self.group or w.segment:
                 raise ValueError(f"MoeBlock: weight {w.experts} x {w.k} x {w.n}, group {w.group}, segment {w.segment}: "
                                  f"{shape} with group {self.group} and no segments is wanted")
-        router = _flat(router, "router", torch.uint64, (h, e))
-        self.exp_table, self.silu_table = _flat(exp_table, "exp_table", torch.uint64), \
-            _flat(silu_table, "silu_table", torch.uint64)
+        self.device = dev = _device_of(router, "router")
+        if any(w.device != dev for w in self.weights):
+            raise ValueError("MoeBlock: weights on the current device are wanted")
+        router = _flat(router, "router", _U64, dev, (h, e))
+        self.exp_table, self.silu_table = _flat(exp_table, "exp_table", _U64, dev), \
+            _flat(silu_table, "silu_table", _U64, dev)
         if exp_table.numel() == 0 or silu_table.numel() == 0:
             raise ValueError("MoeBlock: an empty table")
         if not 1 <= top_k <= min(e, 16) or e > 256 or not 0 <= shift <= 62:
             raise ValueError("MoeBlock: at most 256 experts, 1 .. 16 of them to a token, and a shift 0 .. 62 are wanted")
-        self.router = torch.empty(lib.zkie2_moe_router_words(h, e, self.group), dtype=torch.int32,
+        self.router = torch.empty(lib.zkie2_moe_router_words(h, e), dtype=torch.int32,
                                   device=router.device)
         err = _err_word()
-        check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self.group, self.router.data_ptr(), err.data_ptr(),
-                                        _stream()), "zkie2_moe_router_pack")
+        check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self.router.data_ptr(), err.data_ptr(), _stream()), "zkie2_moe_router_pack")
         _check_err(err, "MoeBlock: router")
-        self._codes = (_lib.vp * 6)(*[w.packed.data_ptr() for w in self.weights])
-        self._scales = (_lib.vp * 6)(*[w.packed_scales.data_ptr() for w in self.weights])
+        self._packed = (_lib.vp * 6)(*[w.pointer for w in self.weights])
+        self._shape = (h, e, top_k, f, s, self.group)
+        self._args = (self.router.data_ptr(), self._packed, exp_table.data_ptr(), exp_table.numel(),
+                      silu_table.data_ptr(), silu_table.numel(), shift)
+        self._scratch = {}  # elements by rows
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                 err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """(out, gate) of the rows of x (m x h, m <= 65535; two launches to 16
         rows): the layer's output (+ residual where given) and TopKSelect's
         gate (m x experts).  |x| and |silu(gate) up| <= 0x7F7F7F7F."""
-        x = _rows(x, "x", self.h)
-        m = x.shape[0]
-        if m > 65535:
-            raise ValueError("MoeBlock: at most 65535 rows are wanted")
+        dev = _device_of(x, "x")
+        m, ldx = _rows(x, "x", self.h, dev)
+        if m > 65535 or self.device != dev:
+            raise ValueError("MoeBlock: at most 65535 rows, on the weights' device, are wanted")
+        p_residual, ldr = None, 0
         if residual is not None:
-            _rows(residual, "residual", self.h)
-            if residual.shape[0] != m:
-                raise ValueError(f"residual: {residual.shape[0]} rows, {m} are wanted")
-        _on_device(self.router, "MoeBlock", torch.int32)
-        out, word = _out(out, (m, self.h)), _word(err)
-        gate = torch.empty((m, self.experts), dtype=torch.uint64, device=x.device)
-        scratch = torch.empty(max(lib.zkie2_moe_rows_scratch_elems(m, self.h, self.experts, self.top_k, self.f,
-                                                                   self.shared_f, self.group), 1),
-                              dtype=torch.int64, device=x.device)
-        check(lib.zkie2_moe_rows(x.data_ptr(), x.stride(0), m, self.h, self.experts, self.top_k, self.f, self.shared_f,
-                                 self.group, self.router.data_ptr(), self._codes, self._scales,
-                                 self.exp_table.data_ptr(), self.exp_table.numel(), self.silu_table.data_ptr(),
-                                 self.silu_table.numel(), self.shift,
-                                 None if residual is None else residual.data_ptr(),
-                                 0 if residual is None else residual.stride(0), out.data_ptr(), gate.data_ptr(),
-                                 word.data_ptr(), scratch.data_ptr(), _stream()), "zkie2_moe_rows")
+            rows, ldr = _rows(residual, "residual", self.h, dev)
+            if rows != m:
+                raise ValueError(f"residual: {rows} rows, {m} are wanted")
+            p_residual = residual.data_ptr()
+        out, word = _out(out, x, (m, self.h), dev), _word(err, dev)
+        gate = x.new_empty((m, self.experts))
+        elems = self._scratch.get(m)
+        if elems is None:
+            elems = self._scratch[m] = max(lib.zkie2_moe_rows_scratch_elems(m, *self._shape), 1)
+        scratch = x.new_empty(elems)  # this call's own: calls on other streams may run beside it
+        check(_moe_rows(x.data_ptr(), ldx, m, *self._shape, *self._args, p_residual, ldr, out.data_ptr(),
+                        gate.data_ptr(), word.data_ptr(), scratch.data_ptr(), _raw_stream(dev)), "zkie2_moe_rows")
         if err is None:
             _check_err(word, "MoeBlock")
         return out, gate
@@ -437,36 +460,35 @@ def choose_token(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     - ``+ mask_value`` where bit v % 32 of word v / 32 of ``allowed`` (int32
       words, ceil(vocab / 32), or batch x that) is clear.  With the graph's
       mask value a row that allows nothing still has a maximum."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.shape[1] == 0:
-        raise ValueError("choose_token: logits batch x vocab are wanted")
+    dev = _device_of(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] == 0 or logits.shape[0] > 65535 or logits.shape[1] > 0x7FFFFFFF:
+        raise ValueError(f"logits: shape {tuple(logits.shape)}, at most 65535 rows of a vocabulary are wanted")
     b, v = logits.shape
-    _flat(logits, "logits", torch.uint64)
-    if b > 65535 or v > 0x7FFFFFFF:
-        raise ValueError("choose_token: at most 65535 rows are wanted")
-    for name, t, dtype, shapes in (("bias", bias, torch.uint64, ((v,), (b, v))),
-                                   ("allowed", allowed, torch.int32, ((-(-v // 32),), (b, -(-v // 32))))):
-        if t is not None and tuple(_flat(t, name, dtype).shape) not in shapes:
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, one of {shapes} is wanted")
+    _flat(logits, "logits", _U64, dev)
+    p_bias = p_allowed = p_history = p_lens = None
+    bias_stride = allowed_stride = tokens = 0
+    if bias is not None:
+        bias_stride = 0 if bias.dim() == 1 else v
+        p_bias = _flat(bias, "bias", _U64, dev, (b, v) if bias_stride else (v,)).data_ptr()
+    if allowed is not None:
+        words = (v + 31) // 32
+        allowed_stride = 0 if allowed.dim() == 1 else words
+        p_allowed = _flat(allowed, "allowed", _I32, dev, (b, words) if allowed_stride else (words,)).data_ptr()
     if history is not None:
-        _flat(history, "history", torch.int32)
         if history.dim() != 2 or history.shape[0] != b:
-            raise ValueError("history: batch x tokens is wanted")
+            raise ValueError(f"history: shape {tuple(history.shape)}, {b} rows of tokens are wanted")
+        p_history, tokens = _flat(history, "history", _I32, dev).data_ptr(), history.shape[1]
         if history_lens is not None:
-            _flat(history_lens, "history_lens", torch.int32, (b,))
+            p_lens = _flat(history_lens, "history_lens", _I32, dev, (b,)).data_ptr()
     elif history_lens is not None:
         raise ValueError("choose_token: history_lens without a history")
-    out, word = _out(out, (b, v)), _word(err)
-    if out.data_ptr() == logits.data_ptr():
+    out, word = _out(out, logits, (b, v), dev), _word(err, dev)
+    if out is logits or (b and out.data_ptr() == logits.data_ptr()):
         raise ValueError("choose_token: out may not be the logits")
-    token = torch.empty(b, dtype=torch.uint32, device=logits.device)
-    check(lib.zkie2_choose_token(logits.data_ptr(), b, v, None if history is None else history.data_ptr(),
-                                 0 if history is None else history.shape[1],
-                                 None if history_lens is None else history_lens.data_ptr(), repeat[0], repeat[1],
-                                 presence, frequency, None if bias is None else bias.data_ptr(),
-                                 0 if bias is None or bias.dim() == 1 else v,
-                                 None if allowed is None else allowed.data_ptr(),
-                                 0 if allowed is None or allowed.dim() == 1 else allowed.shape[1], mask_value,
-                                 out.data_ptr(), token.data_ptr(), word.data_ptr(), _stream()), "zkie2_choose_token")
+    token = logits.new_empty(b, dtype=torch.uint32)
+    check(_choose(logits.data_ptr(), b, v, p_history, tokens, p_lens, *repeat, presence, frequency, p_bias, bias_stride,
+                  p_allowed, allowed_stride, mask_value, out.data_ptr(), token.data_ptr(), word.data_ptr(),
+                  _raw_stream(dev)), "zkie2_choose_token")
     if err is None:
         _check_err(word, "choose_token")
     return token, out
