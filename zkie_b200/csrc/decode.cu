@@ -333,18 +333,20 @@ struct KvRows {
 
 // the d-th number of a new key (d < dk) or value (from dk on) into the cache
 __device__ __forceinline__ bool kv_store(const KvCache& c, const KvRows& rows, uint64_t row, uint32_t seq, uint32_t h,
-                                         uint64_t tok, uint32_t d) {
+                                         uint64_t tok, uint32_t d, int* copy = nullptr) {
     const uint64_t head = (uint64_t)seq * c.heads + h;
     if (d < c.dk) {
         const int64_t x = fx_to_i64(__ldg(rows.k + row * rows.ldk + (uint64_t)h * c.dk + d));
         const int64_t y = fx_round_div_pow2(fx_wmul(x, rows.factor), rows.shift);
         const bool ok = y >= -kKeyLimit && y <= kKeyLimit;
+        if (copy) *copy = ok ? (int32_t)y : 0;
         c.k[key_at(head, c.cap / kKvBlock, c.dk, tok, d)] = ok ? (int32_t)y : 0;
         return ok;
     }
     d -= c.dk;
     const int64_t y = fx_to_i64(__ldg(rows.v + row * rows.ldv + (uint64_t)h * c.dv + d));
     const bool ok = y >= INT32_MIN && y <= INT32_MAX;
+    if (copy) *copy = ok ? (int32_t)y : 0;
     c.v[(head * c.cap + tok) * c.dv + d] = ok ? (int32_t)y : 0;
     return ok;
 }
@@ -370,8 +372,10 @@ __global__ void k_kv_append(KvCache c, KvRows rows, uint32_t tokens, uint32_t* _
 
 constexpr int kAttThreads = 256;
 constexpr int kAttWarps = kAttThreads / 32;
-constexpr uint32_t kMaxRanks = 16;
+constexpr uint32_t kMaxRanks = 16;   // blocks of a cluster
 constexpr size_t kAttShared = 220 * 1024;
+constexpr uint32_t kAttPiece = 4096;  // bytes of a ring's slot
+constexpr uint32_t kKeyDims = 32;     // dimensions of 32 keys to a slot
 
 struct AttendArgs {
     KvCache c;
@@ -387,20 +391,27 @@ struct AttendArgs {
     int64_t offset;
     uint64_t* out;
     uint32_t* err;
-    uint32_t chunk;  // tokens of a block's share of the scores
+    uint32_t chunk;  // scores that a block has room for
     uint32_t slice;  // outputs that a block of the cluster finishes
+    uint32_t depth;  // slots of a warp's ring
 };
 
 // One cluster per sequence, key head and EACH of its query heads; a block
-// takes an equal run of the token blocks.  The softmax's rounding needs the
-// row's maximum and then its sum before any weight is known, so the scores
-// stay in shared memory and the cluster meets twice, keys and values each
-// being read once; the blocks' value sums meet in a third exchange.  A block
-// writes what the others need into their shared memory before each meeting,
-// so that nothing is fetched from a neighbour after it.
-template <int EACH>
+// takes an equal run of the token blocks, a warp every eighth of them.  A warp
+// streams its blocks' keys and then their values through its ring, so that
+// values are on their way while the softmax is worked out.  The softmax's
+// rounding needs the row's maximum and then its sum before any weight is
+// known, so the scores stay in shared memory and the cluster meets twice, keys
+// and values each being read once; the blocks' value sums meet in a third
+// exchange.  A block writes what the others need into their shared memory
+// before each meeting, so that nothing is fetched from a neighbour after it.
+// The new token is taken from its rows, not from the cache it is stored to.
+// A product is one 32 x 32 + 64 bit multiply-add, 32 a clock on an SM, which
+// for four query heads to a key head costs about what the memory does.
+template <int EACH, int WIDE>
 __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_constant__ AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ __align__(8) uint64_t s_bar[kAttWarps * 4];
     __shared__ long long s_red[kAttWarps][EACH];
     __shared__ long long s_max[kMaxRanks][EACH], s_sum[kMaxRanks][EACH];
     cg::cluster_group cluster = cg::this_cluster();
@@ -409,46 +420,94 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     const uint32_t heads = min((uint32_t)EACH, p.each - e0), dk = p.c.dk, dv = p.c.dv;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t* out = p.out + ((uint64_t)seq * p.c.heads * p.each + (uint64_t)h * p.each + e0) * dv;
+    const uint32_t bar = shared_addr(&s_bar[warp * 4]);
     let_next_start();
+    if (lane == 0) {
+        for (uint32_t i = 0; i < p.depth; i++) barrier_init(bar + 8 * i);
+        barrier_init_done();
+    }
+    __syncwarp();
     wait_for_previous();
 
     const int64_t len = p.c.lens[seq];
     const bool append = p.rows.k != nullptr && len >= 0 && len < p.c.cap;
     if (p.rows.k != nullptr && len >= p.c.cap && threadIdx.x == 0) atomicOr(p.err, kErrFull);
-    const uint32_t n = (uint32_t)(len < 0 ? 0 : min(len + (append ? 1 : 0), (int64_t)p.c.cap));
-    if (n == 0) {  // the whole cluster's answer
+    const uint32_t n = (uint32_t)(len < 0 ? 0 : min(len, (int64_t)p.c.cap));  // tokens in the cache
+    if (n + append == 0) {  // the whole cluster's answer
         for (uint32_t i = rank * kAttThreads + threadIdx.x; i < heads * dv; i += ranks * kAttThreads) out[i] = 0;
         return;
     }
     cluster_arrive();  // every block has started before another writes into its shared memory
     const uint32_t blocks = (n + kKvBlock - 1) / kKvBlock;
     const uint32_t b0 = (uint32_t)((uint64_t)rank * blocks / ranks), b1 = (uint32_t)((uint64_t)(rank + 1) * blocks / ranks);
-    const uint32_t t0 = b0 * kKvBlock, count = b1 > b0 ? min(b1 * kKvBlock, n) - t0 : 0;
+    const uint32_t t0 = b0 * kKvBlock, cached = b1 > b0 ? min(b1 * kKvBlock, n) - t0 : 0;
+    const bool own = append && rank == ranks - 1;  // the new token's block: its score is number `cached`
+    const uint32_t count = cached + own;
     const uint64_t head = (uint64_t)seq * p.c.heads + h;
-    int32_t* const keys = p.c.k + key_at(head, p.c.cap / kKvBlock, dk, t0, 0);
-    int32_t* const values = p.c.v + (head * p.c.cap + t0) * dv;
-    // this block's keys and values, both in one piece, start for the second-level cache
-    {
-        constexpr uint32_t kPiece = 8192;
-        const uint64_t kb = (uint64_t)(b1 - b0) * kKvBlock * dk * 4, vb = (uint64_t)count * dv * 4;
-        const uint32_t kn = (uint32_t)((kb + kPiece - 1) / kPiece), vn = (uint32_t)((vb + kPiece - 1) / kPiece);
-        for (uint32_t i = threadIdx.x; i < kn + vn; i += kAttThreads) {
-            const uint64_t at = (uint64_t)(i < kn ? i : i - kn) * kPiece, left = (i < kn ? kb : vb) - at;
-            prefetch_l2(reinterpret_cast<const uint8_t*>(i < kn ? keys : values) + at,
-                        (uint32_t)(left < kPiece ? left : kPiece));
-        }
-    }
+    const int32_t* keys = p.c.k + key_at(head, p.c.cap / kKvBlock, dk, t0, 0);
+    const int32_t* values = p.c.v + (head * p.c.cap + t0) * dv;
 
-    long long* scores = reinterpret_cast<long long*>(smem);                  // EACH x chunk
-    long long* sums = scores + (size_t)EACH * p.chunk;                       // EACH x 4 threads: value sums
-    unsigned long long* acc = reinterpret_cast<unsigned long long*>(sums + (size_t)EACH * 4 * kAttThreads);
-    int* qs = reinterpret_cast<int*>(acc + (((size_t)ranks * p.slice + 1) & ~(size_t)1));  // EACH x dk
+    uint8_t* ring = smem + (size_t)warp * p.depth * kAttPiece;
+    long long* sums = reinterpret_cast<long long*>(smem);  // in the rings' place, once they are done
+    // chunk x EACH; a token's weights later take the first half of its scores' place, as 32-bit numbers
+    long long* scores = reinterpret_cast<long long*>(smem + (size_t)kAttWarps * p.depth * kAttPiece);
+    unsigned long long* acc = reinterpret_cast<unsigned long long*>(scores + (size_t)EACH * p.chunk);  // ranks x slice
+    int* qs = reinterpret_cast<int*>(acc + (((size_t)ranks * p.slice + 1) & ~(size_t)1));              // EACH x dk
+    int* fresh = qs + EACH * dk;                                                                       // dk + dv
+
+    // ---- the warp's stream: keys of its token blocks in pieces of 32 dimensions, then their
+    // values in pieces of a few tokens
+    const uint32_t kpieces = (dk + kKeyDims - 1) / kKeyDims;
+    const uint32_t vtokens = min((uint32_t)kKvBlock, kAttPiece / (4 * dv)), vpieces = (kKvBlock + vtokens - 1) / vtokens;
+    uint32_t next_b = warp, next_i = 0, next_slot = 0;
+    bool next_v = false;
+    auto piece_tokens = [&](uint32_t b, uint32_t i) {  // of piece i of a block's values
+        const uint32_t there = min((uint32_t)kKvBlock, cached - b * kKvBlock), at = i * vtokens;
+        return at < there ? min(vtokens, there - at) : 0u;
+    };
+    auto ask = [&]() {  // lane 0 only
+        if (next_b >= b1 - b0) {
+            if (next_v || warp >= b1 - b0) return;
+            next_v = true;
+            next_b = warp;
+        }
+        const void* from;
+        uint32_t bytes;
+        if (!next_v) {
+            from = keys + ((size_t)next_b * dk + next_i * kKeyDims) * kKvBlock;
+            bytes = min(kKeyDims, dk - next_i * kKeyDims) * kKvBlock * 4;
+        } else {
+            from = values + ((size_t)next_b * kKvBlock + next_i * vtokens) * dv;
+            bytes = piece_tokens(next_b, next_i) * dv * 4;
+        }
+        barrier_expect(bar + 8 * next_slot, bytes);
+        bulk_copy(shared_addr(ring + next_slot * kAttPiece), from, bytes, bar + 8 * next_slot);
+        next_slot = next_slot + 1 == p.depth ? 0 : next_slot + 1;
+        next_i++;
+        if (next_v ? next_i == vpieces || piece_tokens(next_b, next_i) == 0 : next_i == kpieces) {
+            next_i = 0;
+            next_b += kAttWarps;
+        }
+    };
+    if (lane == 0)
+        for (uint32_t i = 0; i < p.depth; i++) ask();
+    Patience patience;
+    uint32_t slot = 0, phase = 0;
+    auto step = [&]() {  // on to the next slot, this one being filled again
+        __syncwarp();
+        if (lane == 0) ask();
+        if (++slot == p.depth) {
+            slot = 0;
+            phase ^= 1;
+        }
+    };
+
     bool bad = false;
     for (uint32_t i = threadIdx.x; i < EACH * dk; i += kAttThreads) {
         int64_t y = 0;
         if (i / dk < heads) {
             const int64_t x = fx_to_i64(__ldg(p.q + seq * p.ldq + (uint64_t)(h * p.each + e0) * dk + i));
-            y = fx_round_div_pow2(fx_wmul(x, p.q_factor), p.q_shift);
+            y = round_shift(fx_wmul(x, p.q_factor), p.q_shift);
             if (y < -kKeyLimit || y > kKeyLimit) {
                 bad = true;
                 y = 0;
@@ -456,54 +515,60 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         }
         qs[i] = (int)y;
     }
-    // The new token belongs to the block whose share holds it (blocks of other
-    // query heads of the same key head store the same numbers).
-    if (append && (uint32_t)len / kKvBlock >= b0 && (uint32_t)len / kKvBlock < b1)
+    if (own)  // store the new token (blocks of other query heads of this key head store the same numbers)
         for (uint32_t d = threadIdx.x; d < dk + dv; d += kAttThreads)
-            bad |= !kv_store(p.c, p.rows, seq, seq, h, (uint64_t)len, d);
+            bad |= !kv_store(p.c, p.rows, seq, seq, h, (uint64_t)len, d, &fresh[d]);
     __syncthreads();
 
+    // ---- scores
     long long top[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) top[e] = INT64_MIN;
+    auto keep = [&](int e, uint32_t at, long long s) {
+        const long long z = round_shift(fx_wmul(s, p.s_factor), p.s_shift);
+        scores[at * EACH + e] = z;
+        top[e] = max(top[e], z);
+    };
     for (uint32_t b = warp; b < b1 - b0; b += kAttWarps) {
-        const int32_t* kb = keys + (size_t)b * kKvBlock * dk + lane * 4;
         long long s[EACH];
 #pragma unroll
         for (int e = 0; e < EACH; e++) s[e] = 0;
-        constexpr int kAhead = 8;
-        for (uint32_t d0 = 0; d0 < dk; d0 += 4 * kAhead) {
-            int4 kv[kAhead];
+        for (uint32_t d0 = 0; d0 < dk; d0 += kKeyDims) {
+            barrier_wait(bar + 8 * slot, phase, patience);
+            const int4* kv = reinterpret_cast<const int4*>(ring + slot * kAttPiece) + lane;
+            const uint32_t quads = min(kKeyDims, dk - d0) / 4;
+            const int* qd = qs + d0;
+#pragma unroll 4
+            for (uint32_t i = 0; i < quads; i++) {
+                const int4 x = kv[i * 32];
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (d0 + 4 * i < dk) kv[i] = __ldcg(reinterpret_cast<const int4*>(kb + (size_t)(d0 + 4 * i) * kKvBlock));
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (d0 + 4 * i < dk) {
-#pragma unroll
-                    for (int e = 0; e < EACH; e++) {
-                        const int4 qv = *reinterpret_cast<const int4*>(qs + e * dk + d0 + 4 * i);
-                        s[e] += (long long)qv.x * kv[i].x + (long long)qv.y * kv[i].y + (long long)qv.z * kv[i].z +
-                                (long long)qv.w * kv[i].w;
-                    }
+                for (int e = 0; e < EACH; e++) {
+                    const int4 qv = *reinterpret_cast<const int4*>(qd + e * dk + 4 * i);
+                    s[e] += (long long)qv.x * x.x;
+                    s[e] += (long long)qv.y * x.y;
+                    s[e] += (long long)qv.z * x.z;
+                    s[e] += (long long)qv.w * x.w;
                 }
-        }
-        const uint32_t at = b * kKvBlock + lane;
-        if (at < count) {
-#pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                const long long z = fx_round_div_pow2(fx_wmul(s[e], p.s_factor), p.s_shift);
-                scores[(size_t)e * p.chunk + at] = z;
-                top[e] = z > top[e] ? z : top[e];
             }
+            step();
+        }
+        if (b * kKvBlock + lane < cached) {
+#pragma unroll
+            for (int e = 0; e < EACH; e++) keep(e, b * kKvBlock + lane, s[e]);
+        }
+    }
+    if (own && warp == kAttWarps - 1) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            long long s = 0;
+            for (uint32_t d = lane; d < dk; d += 32) s += (long long)qs[e * dk + d] * fresh[d];
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            keep(e, cached, s);  // every lane the same
         }
     }
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-        for (int o = 16; o; o >>= 1) {
-            const long long other = __shfl_xor_sync(0xFFFFFFFFu, top[e], o);
-            top[e] = other > top[e] ? other : top[e];
-        }
+        for (int o = 16; o; o >>= 1) top[e] = max(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], o));
         if (lane == 0) s_red[warp][e] = top[e];
     }
     __syncthreads();
@@ -515,6 +580,8 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         *cluster.map_shared_rank(&s_max[rank][e], r) = v;
     }
     cluster.sync();
+
+    // ---- weights
     long long part[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
@@ -526,12 +593,12 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
             int64_t v = fx_to_i64(
-                table_at(p.table, p.table_len, fx_wsub(scores[(size_t)e * p.chunk + j], top[e]), p.offset));
+                table_at(p.table, p.table_len, fx_wsub(scores[j * EACH + e], top[e]), p.offset));
             if (v < 0 || v > INT32_MAX) {
                 bad = true;
                 v = 0;
             }
-            scores[(size_t)e * p.chunk + j] = v;
+            scores[j * EACH + e] = v;
             part[e] += v;
         }
     }
@@ -556,78 +623,111 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         if (part[e] == 0 && e < heads && rank == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDivide);
         inv[e] = part[e] ? 1.0 / (double)part[e] : 0.0;
     }
+    struct alignas(4 * EACH) Weights {
+        int w[EACH];
+    };
+    const auto weights_of = [&](uint32_t j) { return reinterpret_cast<Weights*>(scores + j * EACH); };
     for (uint32_t j = threadIdx.x; j < count; j += kAttThreads) {
+        Weights w;
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            const long long v = scores[(size_t)e * p.chunk + j];
-            scores[(size_t)e * p.chunk + j] = part[e] ? round_div_near(v << 16, part[e], inv[e]) : 0;
-        }
+        for (int e = 0; e < EACH; e++)
+            w.w[e] = part[e] ? (int)round_div_near(scores[j * EACH + e] << 16, part[e], inv[e]) : 0;
+        *weights_of(j) = w;
     }
     __syncthreads();
 
-    // A thread keeps four dimensions and takes every step-th token
-    const uint32_t wide = dv / 4, step = kAttThreads / wide, phase = threadIdx.x / wide, d4 = threadIdx.x % wide;
-    if (phase < step) {
-        long long y[EACH][4];
+    // ---- values: a lane keeps four dimensions (WIDE = 2: eight) and takes every step-th token
+    const uint32_t wide = (dv / 4 + WIDE - 1) / WIDE, step_t = 32 / wide, mine = lane / wide, d4 = lane % wide;
+    const bool on = mine < step_t, second = WIDE == 2 && d4 + wide < dv / 4;
+    long long y[EACH][4 * WIDE];
 #pragma unroll
-        for (int e = 0; e < EACH; e++) y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0;
-        const int32_t* vb = values + d4 * 4;
-        constexpr int kAhead = 8;
-        for (uint32_t j0 = phase; j0 < count; j0 += kAhead * step) {
-            int4 vv[kAhead];
+    for (int e = 0; e < EACH; e++)
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (j0 + i * step < count) vv[i] = __ldcg(reinterpret_cast<const int4*>(vb + (size_t)(j0 + i * step) * dv));
+        for (int i = 0; i < 4 * WIDE; i++) y[e][i] = 0;
+    auto take = [&](const int4& x, int w0, const Weights& w) {
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (j0 + i * step < count) {
-#pragma unroll
-                    for (int e = 0; e < EACH; e++) {
-                        const int w = (int)scores[(size_t)e * p.chunk + j0 + i * step];
-                        y[e][0] += (long long)w * vv[i].x;
-                        y[e][1] += (long long)w * vv[i].y;
-                        y[e][2] += (long long)w * vv[i].z;
-                        y[e][3] += (long long)w * vv[i].w;
-                    }
-                }
+        for (int e = 0; e < EACH; e++) {
+            y[e][w0] += (long long)w.w[e] * x.x;
+            y[e][w0 + 1] += (long long)w.w[e] * x.y;
+            y[e][w0 + 2] += (long long)w.w[e] * x.z;
+            y[e][w0 + 3] += (long long)w.w[e] * x.w;
         }
+    };
+    for (uint32_t b = warp; b < b1 - b0; b += kAttWarps) {
+        for (uint32_t i = 0; i < vpieces; i++) {
+            const uint32_t tokens = piece_tokens(b, i);
+            if (tokens == 0) break;
+            barrier_wait(bar + 8 * slot, phase, patience);
+            const int4* vv = reinterpret_cast<const int4*>(ring + slot * kAttPiece) + d4;
+            const uint32_t first = b * kKvBlock + i * vtokens;
+            if (on) {
+#pragma unroll 4
+                for (uint32_t j = mine; j < tokens; j += step_t) {
+                    const Weights w = *weights_of(first + j);
+                    take(vv[j * (dv / 4)], 0, w);
+                    if (second) take(vv[j * (dv / 4) + wide], 4 * (WIDE - 1), w);
+                }
+            }
+            step();
+        }
+    }
+    if (bad) atomicOr(p.err, kErrRange);
+    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
+    __syncthreads();  // the rings are done with
+    if (on) {
+        long long* to = sums + ((size_t)(warp * step_t + mine) * EACH) * dv;
 #pragma unroll
         for (int e = 0; e < EACH; e++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sums[((size_t)e * step + phase) * dv + d4 * 4 + i] = y[e][i];
+            for (int i = 0; i < 4; i++) {
+                to[e * dv + d4 * 4 + i] = y[e][i];
+                if (second) to[e * dv + (d4 + wide) * 4 + i] = y[e][4 * (WIDE - 1) + i];
+            }
     }
-    if (bad) atomicOr(p.err, kErrRange);
     __syncthreads();
     // output i belongs to block i / slice: its part goes there
     for (uint32_t i = threadIdx.x; i < heads * dv; i += kAttThreads) {
         const uint32_t e = i / dv, d = i % dv;
         unsigned long long v = 0;
-        for (uint32_t s = 0; s < step; s++) v += (unsigned long long)sums[((size_t)e * step + s) * dv + d];
+        for (uint32_t s = 0; s < kAttWarps * step_t; s++) v += (unsigned long long)sums[(size_t)s * EACH * dv + i];
+        if (own) v += (unsigned long long)((long long)weights_of(cached)->w[e] * fresh[dk + d]);
         *cluster.map_shared_rank(&acc[(size_t)rank * p.slice + i % p.slice], i / p.slice) = v;
     }
     cluster.sync();
     for (uint32_t i = threadIdx.x; i < p.slice && rank * p.slice + i < heads * dv; i += kAttThreads) {
         unsigned long long v = 0;
         for (uint32_t r = 0; r < ranks; r++) v += acc[(size_t)r * p.slice + i];
-        out[rank * p.slice + i] = fx_from_i64(fx_round_div_pow2((int64_t)v, p.out_shift));
+        out[rank * p.slice + i] = fx_from_i64(round_shift((int64_t)v, p.out_shift));
     }
 }
 
-size_t attend_shared(uint32_t each, uint32_t ranks, uint32_t blocks, uint32_t dk, uint32_t dv) {
-    const uint64_t chunk = ceil_div(blocks, ranks) * kKvBlock, slice = ceil_div(each * dv, ranks);
-    return each * (8 * chunk + 32ull * kAttThreads + 4ull * dk) + 8 * ((ranks * slice + 1) & ~1ull);
+// Shared memory of a block: rings (64 kB at least; in their place later the value sums, at most
+// 32 kB), scores, the others' sums, queries, the new token
+struct AttendPlan {
+    uint32_t each, ranks, depth, chunk, slice;
+    size_t shared;
+};
+
+AttendPlan attend_plan(uint32_t each, uint32_t ranks, uint32_t depth, uint32_t blocks, uint32_t dk, uint32_t dv) {
+    AttendPlan a{each, ranks, depth, 0, 0, 0};
+    a.chunk = (uint32_t)ceil_div(blocks, ranks) * kKvBlock + 1;
+    a.chunk += a.chunk % 2;
+    a.slice = (uint32_t)ceil_div(each * dv, ranks);
+    a.shared = (size_t)kAttWarps * depth * kAttPiece + 8ull * each * a.chunk + 8 * ((ranks * a.slice + 1) & ~1ull) +
+               4ull * (each * dk + dk + dv);
+    return a;
 }
 
-template <int EACH>
-int attend_launch(AttendArgs p, uint32_t ranks, cudaStream_t stream) {
+template <int EACH, int WIDE>
+int attend_launch(AttendArgs p, const AttendPlan& a, cudaStream_t stream) {
     p.groups = (uint32_t)ceil_div(p.each, EACH);
-    p.chunk = (uint32_t)ceil_div(p.c.cap / kKvBlock, ranks) * kKvBlock;
-    p.slice = (uint32_t)ceil_div(EACH * p.c.dv, ranks);
-    const size_t shared = attend_shared(EACH, ranks, p.c.cap / kKvBlock, p.c.dk, p.c.dv);
-    auto* kernel = k_kv_attend<EACH>;
+    p.chunk = a.chunk;
+    p.slice = a.slice;
+    p.depth = a.depth;
+    auto* kernel = k_kv_attend<EACH, WIDE>;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kAttShared, &set, true));
-    return launch(kernel, dim3(ranks, p.c.heads * p.groups, p.c.batch), kAttThreads, shared, ranks, stream, p);
+    return launch(kernel, dim3(a.ranks, p.c.heads * p.groups, p.c.batch), kAttThreads, a.shared, a.ranks, stream, p);
 }
 
 // ---- the next token ---------------------------------------------------------------------------
@@ -652,96 +752,97 @@ struct ChooseArgs {
 };
 
 constexpr int kChooseEach = 8;  // logits of a thread at a time
+constexpr uint32_t kChooseStep = kChooseThreads * kChooseEach;
 
-// One cluster per row, a block to an equal slice of the vocabulary, a step of
-// 4096 at a time: the logits start for registers, the history's tokens are
-// counted in shared memory, then the logits are finished; the blocks' maxima
-// meet in the first block.
-__global__ void __launch_bounds__(kChooseThreads) k_choose_token(const __grid_constant__ ChooseArgs p) {
-    constexpr uint32_t kStep = kChooseThreads * kChooseEach;
-    __shared__ uint32_t counts[kStep];
+// One cluster per row, a block to an equal run of the vocabulary in whole
+// words of the mask, a step of 4096 at a time: logits, biases and mask words
+// start for registers, the history's tokens are counted in shared memory, then
+// the logits are finished; the blocks' maxima meet in the first block.  A warp
+// takes 32 neighbours, so a mask word is one load.
+__global__ void __launch_bounds__(kChooseThreads, 2) k_choose_token(const __grid_constant__ ChooseArgs p) {
+    __shared__ uint32_t counts[kChooseStep];
     __shared__ long long s_v[kChooseWarps];
-    __shared__ unsigned long long s_j[kChooseWarps];
+    __shared__ uint32_t s_j[kChooseWarps];
     __shared__ long long best_v[kMaxRanks];
-    __shared__ unsigned long long best_j[kMaxRanks];
+    __shared__ uint32_t best_j[kMaxRanks];
+    constexpr uint32_t kNone = 0xFFFFFFFFu;
     cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
-    const uint64_t row = blockIdx.y, lo = p.v * rank / ranks, hi = p.v * (rank + 1) / ranks;
+    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t row = blockIdx.y;
+    const uint32_t words = (uint32_t)((p.v + 31) / 32);
+    const uint32_t lo = (uint32_t)((uint64_t)words * rank / ranks) * 32;
+    const uint32_t hi = min((uint32_t)((uint64_t)words * (rank + 1) / ranks) * 32, (uint32_t)p.v);
     cluster_arrive();  // every block has started before another writes into its shared memory
     let_next_start();
     wait_for_previous();
-    uint64_t past = 0;
+    uint32_t past = 0;
     if (p.history) {
-        past = p.history_len;
-        if (p.history_lens) {
-            const int64_t l = p.history_lens[row];
-            past = l < 0 ? 0 : (l < (int64_t)past ? l : past);
-        }
+        past = (uint32_t)p.history_len;
+        if (p.history_lens) past = (uint32_t)max(0, min(p.history_lens[row], (int32_t)past));
     }
+    const uint64_t* logits = p.logits + row * p.v;
+    const uint64_t* bias = p.bias ? p.bias + row * p.bias_stride : nullptr;
+    const uint32_t* allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
+    const int32_t* hist = p.history + row * p.history_len;
+    uint64_t* out = p.out + row * p.v;
     long long bv = INT64_MIN;
-    unsigned long long bj = UINT64_MAX;
+    uint32_t bj = kNone;
     bool bad = false;
-    for (uint64_t s0 = lo; s0 < hi; s0 += kStep) {
-        const uint64_t s1 = s0 + kStep < hi ? s0 + kStep : hi;
-        int64_t y[kChooseEach];
+    for (uint32_t s0 = lo; s0 < hi; s0 += kChooseStep) {
+        const uint32_t n = min(kChooseStep, hi - s0), first = s0 + threadIdx.x;
+        uint64_t x[kChooseEach], b[kChooseEach];
+        uint32_t mask[kChooseEach];
 #pragma unroll
         for (int i = 0; i < kChooseEach; i++) {
-            const uint64_t j = s0 + i * kChooseThreads + threadIdx.x;
-            if (j < s1) y[i] = fx_to_i64(__ldg(p.logits + row * p.v + j));
+            const bool on = i * kChooseThreads + threadIdx.x < n;
+            x[i] = on ? __ldg(logits + first + i * kChooseThreads) : 0;
+            b[i] = on && bias ? __ldg(bias + first + i * kChooseThreads) : 0;
+            mask[i] = on && allowed ? __ldg(allowed + first / 32 + i * kChooseWarps) : kNone;
         }
         if (past) {
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < kStep; i += kChooseThreads) counts[i] = 0;
+            for (uint32_t i = threadIdx.x; i < kChooseStep; i += kChooseThreads) counts[i] = 0;
             __syncthreads();
-            const int32_t* hist = p.history + row * p.history_len;
-            for (uint64_t i0 = threadIdx.x; i0 < past; i0 += kChooseThreads * 8) {
-                int32_t tok[8];
+            for (uint32_t i0 = threadIdx.x; i0 < past; i0 += kChooseThreads * 8) {
+                uint32_t tok[8];
 #pragma unroll
                 for (int q = 0; q < 8; q++)
-                    if (i0 + q * kChooseThreads < past) tok[q] = __ldg(hist + i0 + q * kChooseThreads);
+                    tok[q] = i0 + q * kChooseThreads < past ? (uint32_t)__ldg(hist + i0 + q * kChooseThreads) : s0;
 #pragma unroll
-                for (int q = 0; q < 8; q++)
-                    if (i0 + q * kChooseThreads < past) {
-                        bad |= tok[q] < 0 || (uint64_t)tok[q] >= p.v;
-                        const uint64_t at = (uint64_t)tok[q] - s0;  // huge for a token before the step
-                        if (tok[q] >= 0 && at < s1 - s0) atomicAdd(&counts[at], 1u);
-                    }
+                for (int q = 0; q < 8; q++) {
+                    bad |= tok[q] >= (uint32_t)p.v;
+                    if (tok[q] - s0 < n && i0 + q * kChooseThreads < past) atomicAdd(&counts[tok[q] - s0], 1u);
+                }
             }
             __syncthreads();
         }
 #pragma unroll
         for (int i = 0; i < kChooseEach; i++) {
-            const uint64_t j = s0 + i * kChooseThreads + threadIdx.x;
-            if (j >= s1) continue;
-            int64_t z = y[i];
-            const uint32_t c = past ? counts[j - s0] : 0;
+            const uint32_t at = i * kChooseThreads + threadIdx.x;
+            if (at >= n) continue;
+            int64_t z = fx_to_i64(x[i]);
+            const uint32_t c = past ? counts[at] : 0;
             if (c) {
-                z = fx_round_div_pow2(fx_wmul(z, z > 0 ? p.repeat_pos : p.repeat_neg), 16);
+                z = round_shift(fx_wmul(z, z > 0 ? p.repeat_pos : p.repeat_neg), 16);
                 z = fx_wsub(fx_wsub(z, p.presence), fx_wmul(p.frequency, c));
             }
-            if (p.bias) z = fx_wadd(z, fx_to_i64(__ldg(p.bias + row * p.bias_stride + j)));
-            if (p.allowed && !((__ldg(p.allowed + row * p.allowed_stride + j / 32) >> (j % 32)) & 1))
-                z = fx_wadd(z, p.mask_value);
-            p.out[row * p.v + j] = fx_from_i64(z);
-            if (z > bv || bj == UINT64_MAX) {
+            z = fx_wadd(z, fx_to_i64(b[i]));
+            if (!((mask[i] >> lane) & 1)) z = fx_wadd(z, p.mask_value);
+            out[first + i * kChooseThreads] = fx_from_i64(z);
+            if (z > bv || bj == kNone) {
                 bv = z;
-                bj = j;
+                bj = s0 + at;
             }
         }
     }
     if (bad && rank == 0) atomicOr(p.err, kErrIndex);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto take = [&](long long ov, unsigned long long oj) {
-        if (oj != UINT64_MAX && (bj == UINT64_MAX || ov > bv || (ov == bv && oj < bj))) {
+    auto take = [&](long long ov, uint32_t oj) {
+        if (oj != kNone && (bj == kNone || ov > bv || (ov == bv && oj < bj))) {
             bv = ov;
             bj = oj;
         }
     };
-    for (int o = 16; o; o >>= 1) {
-        const long long ov = __shfl_xor_sync(0xFFFFFFFFu, bv, o);
-        const unsigned long long oj = __shfl_xor_sync(0xFFFFFFFFu, bj, o);
-        take(ov, oj);
-    }
+    for (int o = 16; o; o >>= 1) take(__shfl_xor_sync(0xFFFFFFFFu, bv, o), __shfl_xor_sync(0xFFFFFFFFu, bj, o));
     if (lane == 0) {
         s_v[warp] = bv;
         s_j[warp] = bj;
@@ -756,7 +857,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_choose_token(const __grid_co
     cluster.sync();
     if (rank == 0 && threadIdx.x == 0) {
         for (uint32_t r = 0; r < ranks; r++) take(best_v[r], best_j[r]);
-        p.token[row] = (uint32_t)bj;
+        p.token[row] = bj;
     }
 }
 
@@ -865,18 +966,28 @@ int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t
     p.offset = offset;
     p.out = d_out;
     p.err = d_err;
-    // Query heads to a block: those that share a key head, up to four (their
-    // sums stay in registers); fewer where their scores do not fit.  Blocks to
-    // a cluster: enough to fill the device, more where the scores need it.
+    // Query heads to a block: those that share a key head, up to four (two where a value row is
+    // wider than 128: their sums stay in registers), fewer where their scores do not fit.  Blocks
+    // to a cluster: enough to fill the device with two to an SM, of four token blocks at least, up
+    // to eight (of clusters of sixteen not enough find room at once: 36 us instead of 25 for 16
+    // heads of 4096 tokens); sixteen only where the scores need it.
     const uint32_t blocks = (uint32_t)(capacity / kKvBlock);
-    for (uint32_t each = p.each >= 3 ? 4 : p.each;; each /= 2) {
+    const bool wide = dv > 128;
+    for (uint32_t each = p.each >= 3 && !wide ? 4 : p.each >= 2 ? 2 : 1;; each /= 2) {
         const uint64_t rows = batch * heads * ceil_div(p.each, each);
         uint32_t ranks = 1;
-        while (ranks < kMaxRanks && rows * ranks * 2 <= 2 * kSms && ranks < blocks) ranks *= 2;
-        while (ranks < kMaxRanks && attend_shared(each, ranks, blocks, p.c.dk, p.c.dv) > kAttShared) ranks *= 2;
-        if (attend_shared(each, ranks, blocks, p.c.dk, p.c.dv) > kAttShared && each > 1) continue;
-        return each == 4 ? attend_launch<4>(p, ranks, stream) : each == 2 ? attend_launch<2>(p, ranks, stream)
-                                                                          : attend_launch<1>(p, ranks, stream);
+        while (ranks < 8 && rows * ranks * 2 <= 2 * kSms && ranks * 8 <= blocks) ranks *= 2;
+        AttendPlan a = attend_plan(each, ranks, 2, blocks, p.c.dk, p.c.dv);
+        for (; a.shared > (a.ranks < 8 ? kAttShared / 2 : kAttShared) && a.ranks < kMaxRanks && a.ranks < blocks;)
+            a = attend_plan(each, a.ranks * 2, 2, blocks, p.c.dk, p.c.dv);
+        if (attend_plan(each, a.ranks, 3, blocks, p.c.dk, p.c.dv).shared <= kAttShared / 2)
+            a = attend_plan(each, a.ranks, 3, blocks, p.c.dk, p.c.dv);
+        if (a.shared > kAttShared && each > 1) continue;
+        if (a.shared > kAttShared) return (int)cudaErrorInvalidValue;
+        if (wide) return each == 2 ? attend_launch<2, 2>(p, a, stream) : attend_launch<1, 2>(p, a, stream);
+        return each == 4   ? attend_launch<4, 1>(p, a, stream)
+               : each == 2 ? attend_launch<2, 1>(p, a, stream)
+                           : attend_launch<1, 1>(p, a, stream);
     }
 }
 
@@ -894,7 +1005,7 @@ int zkie2_choose_token(const uint64_t* d_logits, uint64_t batch, uint64_t vocab,
                        frequency, d_bias, bias_stride, d_allowed, allowed_stride, mask_value, d_out, d_token, d_err};
     // Blocks to a row: one step of the vocabulary each, fewer once the rows fill the device
     uint32_t ranks = 1;
-    while (ranks < kMaxRanks && vocab > (uint64_t)ranks * kChooseThreads * kChooseEach && batch * ranks < 2 * kSms)
+    while (ranks < kMaxRanks && vocab > (uint64_t)ranks * kChooseStep && batch * ranks < 2 * kSms)
         ranks *= 2;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_choose_token), 0, &set, true));
