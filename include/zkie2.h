@@ -650,6 +650,10 @@ int zkie2_eq_combine(const uint64_t *h_points, const uint64_t *h_coeffs, uint32_
 uint64_t zkie2_q4_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group, uint64_t segment);
 int zkie2_q4_pack(const int8_t *d_codes, const int32_t *d_scales, uint64_t experts, uint64_t k, uint64_t n,
                   uint32_t group, uint64_t segment, uint32_t *d_packed, uint32_t *d_err, zkie_stream_t stream);
+/* Two packed weights of one shape, block by block side by side (twice as many
+ * words): a gate and an up weight for zkie2_moe_rows. */
+int zkie2_q4_pair(const uint32_t *d_a, const uint32_t *d_b, uint64_t experts, uint64_t k, uint64_t n, uint32_t group,
+                  uint32_t *d_out, zkie_stream_t stream);
 /* Op::Projection's out (Op::MatMul for shift = 0 and no bias) of m rows by one
  * packed weight: y = sum over segments of round_div(x w, 2^shift), + bias (n
  * values); with a table then table[clamp(y + offset, 0, table_len - 1)]
@@ -689,8 +693,8 @@ int zkie2_kv_attend(const uint64_t *d_q, uint64_t ldq, uint64_t q_heads, int64_t
 /* build_moe (models/deepseek-v2-lite/src/lib.rs:252-470) of m rows, two
  * launches to 16 rows: h wide, `experts` routed (top_k of them, hidden f) and
  * the shared experts (hidden shared_f) with weights of one group;
- * h_weights: a host array of 6 device pointers (packed gate, up, down, shared
- * gate, up, down); the router packed from h x experts field elements of at
+ * h_weights: a host array of 4 device pointers (the gate and up pair, down, the
+ * shared experts' pair, their down); the router packed from h x experts field elements of at
  * most 32639 in size.  Every Scale divides by 2^shift; the silu table is
  * indexed from its middle.  experts <= 256, top_k <= 16, |x| and |silu(gate)
  * up| <= 0x7F7F7F7F.  out: m x h (+ residual); gate (may be null): m x

@@ -173,6 +173,7 @@ SIGNATURES = {
     "zkie2_eq_combine": (i64, [pu64, pu64, u32, u32, vp, vp, vp]),
     "zkie2_q4_words": (u64, [u64, u64, u64, u32, u64]),
     "zkie2_q4_pack": (i64, [vp, vp, u64, u64, u64, u32, u64, vp, vp, vp]),
+    "zkie2_q4_pair": (i64, [vp, vp, u64, u64, u64, u32, vp, vp]),
     "zkie2_q4_project": (i64, [vp, u64, u64, vp, u64, u64, u32, u64, u32, vp, vp, u64, s64, vp, u64, vp, vp, vp]),
     "zkie2_kv_append": (i64, [vp, u64, vp, u64, u64, s64, u32, vp, vp, vp, u64, u64, u64, u64, u64, vp, vp]),
     "zkie2_kv_attend": (i64, [vp, u64, u64, s64, u32, vp, u64, vp, u64, s64, u32, vp, vp, vp, u64, u64, u64, u64, u64,

@@ -83,6 +83,14 @@ __global__ void k_q4_pack(const int8_t* __restrict__ codes, const int32_t* __res
     if (bad) atomicOr(err, kErrRange);
 }
 
+// two weights of one shape, block by block side by side
+__global__ void k_q4_pair(const uint4* __restrict__ a, const uint4* __restrict__ b, uint64_t blocks, uint32_t words,
+                          uint4* __restrict__ out) {
+    for (uint64_t i = blockIdx.x; i < blocks; i += gridDim.x)
+        for (uint32_t j = threadIdx.x; j < 2 * words; j += blockDim.x)
+            out[i * 2 * words + j] = j < words ? a[i * words + j] : b[i * words + j - words];
+}
+
 // ---- the product ----------------------------------------------------------------------------
 constexpr int kProjThreads = 512;
 constexpr int kProjWarps = kProjThreads / 32;
@@ -169,8 +177,8 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     // ---- the rows' digits
     for (uint32_t i = threadIdx.x; i < 3 * kCells; i += kProjThreads) acc.w[i] = 0;
     wait_for_previous();
-    if (!q4_digitise<kProjThreads>(p.x + (uint64_t)row0 * p.ldx, p.ldx, rows, p.s.segs, p.s.k_seg, p.s.kp_seg, digits,
-                                   p.stride))
+    if (!q4_digitise<kProjThreads, 4>(p.x + (uint64_t)row0 * p.ldx, p.ldx, p.s.segs, p.s.k_seg, p.s.kp_seg, 0,
+                                   rows * blocks * 16, digits, p.stride))
         atomicOr(p.err, kErrRange);
     __syncthreads();
 
@@ -568,7 +576,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     }
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-        for (int o = 16; o; o >>= 1) top[e] = max(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], o));
+        top[e] = warp_max(top[e]);
         if (lane == 0) s_red[warp][e] = top[e];
     }
     __syncthreads();
@@ -604,7 +612,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     }
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-        for (int o = 16; o; o >>= 1) part[e] += __shfl_xor_sync(0xFFFFFFFFu, part[e], o);
+        part[e] = warp_sum(part[e]);
         if (lane == 0) s_red[warp][e] = part[e];
     }
     __syncthreads();
@@ -615,13 +623,13 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         *cluster.map_shared_rank(&s_sum[rank][e], r) = v;
     }
     cluster.sync();
-    double inv[EACH];
+    float inv[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         part[e] = 0;
         for (uint32_t r = 0; r < ranks; r++) part[e] += s_sum[r][e];
         if (part[e] == 0 && e < heads && rank == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDivide);
-        inv[e] = part[e] ? 1.0 / (double)part[e] : 0.0;
+        inv[e] = 1.0f / (float)part[e];
     }
     struct alignas(4 * EACH) Weights {
         int w[EACH];
@@ -631,7 +639,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         Weights w;
 #pragma unroll
         for (int e = 0; e < EACH; e++)
-            w.w[e] = part[e] ? (int)round_div_near(scores[j * EACH + e] << 16, part[e], inv[e]) : 0;
+            w.w[e] = part[e] ? softmax_weight((uint32_t)scores[j * EACH + e], part[e], inv[e]) : 0;
         *weights_of(j) = w;
     }
     __syncthreads();
@@ -884,6 +892,20 @@ int zkie2_q4_pack(const int8_t* d_codes, const int32_t* d_scales, uint64_t exper
     const uint64_t blocks = ceil_div(experts * s.tiles * s.blocks * (s.bytes / 4), 256);
     k_q4_pack<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), 256, 0, stream>>>(
         d_codes, d_scales, (uint32_t)experts, s, d_packed, d_err);
+    ZK_LAUNCH_CHECK();
+    return 0;
+}
+
+int zkie2_q4_pair(const uint32_t* d_a, const uint32_t* d_b, uint64_t experts, uint64_t k, uint64_t n, uint32_t group,
+                  uint32_t* d_out, cudaStream_t stream) {
+    Q4Shape s;
+    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, 0, &s) || !d_a || !d_b || !d_out ||
+        (((uintptr_t)d_a | (uintptr_t)d_b | (uintptr_t)d_out) & 15))
+        return (int)cudaErrorInvalidValue;
+    const uint64_t blocks = experts * s.tiles * s.blocks;
+    k_q4_pair<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), 64, 0, stream>>>(
+        reinterpret_cast<const uint4*>(d_a), reinterpret_cast<const uint4*>(d_b), blocks, s.bytes / 16,
+        reinterpret_cast<uint4*>(d_out));
     ZK_LAUNCH_CHECK();
     return 0;
 }

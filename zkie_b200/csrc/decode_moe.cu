@@ -70,7 +70,7 @@ struct MoeArgs {
     uint64_t ldx;
     uint32_t m, h, experts, top_k, etiles;
     const uint4* router;
-    Q4Weight gate, up, down, sgate, sup, sdown;
+    Q4Weight up, down, sup, sdown;  // up: gate and up, block by block side by side
     const uint64_t* exp_table;
     uint64_t exp_len;
     const uint64_t* silu;
@@ -115,55 +115,80 @@ __global__ void k_moe_router_pack(const uint64_t* __restrict__ w, uint32_t h, ui
     if (bad) atomicOr(err, kErrRange);
 }
 
-// Logits of the 16 experts of tile 2 i + rank for 2 NT tokens, this warp's
-// part of K, added to sums (tokens x this block's experts)
+// Logits of the 16 experts of tile 2 own + rank, this warp's blocks [b0, b1),
+// added to sums (tokens x this block's experts); 2 NT tokens at a time, for
+// which two blocks of the router at a time are held in registers.
 template <int NT>
-__device__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t own, uint32_t rank, uint32_t tok0,
-                            uint32_t b0, uint32_t b1, const Limbs& sums, uint32_t pitch) {
+__device__ __forceinline__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t own, uint32_t rank,
+                                         uint32_t b0, uint32_t b1, const Limbs& sums, uint32_t pitch) {
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    int c[2][NT][4];
+    constexpr int kHeld = 2;
+    for (uint32_t tok0 = 0; tok0 < p.m; tok0 += 2 * NT) {
+        int c[2][NT][4];
 #pragma unroll
-    for (int w = 0; w < 2; w++)
+        for (int q = 0; q < 2; q++)
 #pragma unroll
-        for (int i = 0; i < NT; i++) c[w][i][0] = c[w][i][1] = c[w][i][2] = c[w][i][3] = 0;
-#pragma unroll 2
-    for (uint32_t b = b0; b < b1; b++) {
-        const uint4* r = p.router + ((uint64_t)(2 * own + rank) * p.gate.s.blocks + b) * 128 + lane;
-        const uint4 w00 = __ldg(r), w01 = __ldg(r + 32), w10 = __ldg(r + 64), w11 = __ldg(r + 96);
+            for (int i = 0; i < NT; i++) c[q][i][0] = c[q][i][1] = c[q][i][2] = c[q][i][3] = 0;
+        const uint8_t* from[NT];
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+            from[i] = digits + (size_t)(min(tok0 + 2 * i + (g >> 2), p.m - 1) * 4 + (g & 3)) * p.stride + 16 * t;
+        for (uint32_t b = b0; b < b1; b += kHeld) {
+            uint4 w[kHeld][4];  // half and byte: 00, 01, 10, 11
+#pragma unroll
+            for (int k = 0; k < kHeld; k++) {  // (a block past the end repeats the last, and is not used)
+                const uint4* r = p.router + ((uint64_t)(2 * own + rank) * p.up.s.blocks + min(b + k, b1 - 1)) * 128 + lane;
+#pragma unroll
+                for (int q = 0; q < 4; q++) w[k][q] = __ldg(r + 32 * q);
+            }
+#pragma unroll
+            for (int k = 0; k < kHeld; k++)
+                if (b + k < b1) {
+#pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(from[i] + (b + k) * 64);
+                        mma_s8(c[0][i], w[k][0].x, w[k][0].y, w[k][0].z, w[k][0].w, x.x, x.y);
+                        mma_s8(c[1][i], w[k][1].x, w[k][1].y, w[k][1].z, w[k][1].w, x.x, x.y);
+                        mma_s8(c[0][i], w[k][2].x, w[k][2].y, w[k][2].z, w[k][2].w, x.z, x.w);
+                        mma_s8(c[1][i], w[k][3].x, w[k][3].y, w[k][3].z, w[k][3].w, x.z, x.w);
+                    }
+                }
+        }
 #pragma unroll
         for (int i = 0; i < NT; i++) {
-            const uint32_t tok = min(tok0 + 2 * i + (g >> 2), p.m - 1);
-            const uint4 x = *reinterpret_cast<const uint4*>(digits + (size_t)(tok * 4 + (g & 3)) * p.stride + b * 64 + 16 * t);
-            mma_s8(c[0][i], w00.x, w00.y, w00.z, w00.w, x.x, x.y);
-            mma_s8(c[1][i], w01.x, w01.y, w01.z, w01.w, x.x, x.y);
-            mma_s8(c[0][i], w10.x, w10.y, w10.z, w10.w, x.z, x.w);
-            mma_s8(c[1][i], w11.x, w11.y, w11.z, w11.w, x.z, x.w);
-        }
-    }
+            const uint32_t tok = tok0 + 2 * i + (t >> 1);
+            if (tok < p.m) {
 #pragma unroll
-    for (int i = 0; i < NT; i++) {
-        const uint32_t tok = tok0 + 2 * i + (t >> 1);
-        if (tok < p.m) {
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const long long v = ((long long)c[0][i][2 * q] + ((long long)c[0][i][2 * q + 1] << 8)) +
-                                    (((long long)c[1][i][2 * q] << 8) + ((long long)c[1][i][2 * q + 1] << 16));
-                sums.add(tok * pitch + own * 16 + g + 8 * q, (long long)((unsigned long long)v << (16 * (t & 1))));
+                for (int q = 0; q < 2; q++) {
+                    const long long v = ((long long)c[0][i][2 * q] + ((long long)c[0][i][2 * q + 1] << 8)) +
+                                        (((long long)c[1][i][2 * q] << 8) + ((long long)c[1][i][2 * q + 1] << 16));
+                    sums.add(tok * pitch + own * 16 + g + 8 * q, (long long)((unsigned long long)v << (16 * (t & 1))));
+                }
             }
         }
     }
 }
 
+// The last warps of a block route the tokens while the others take the shared
+// experts' first batch.
+// Four of them, six for more than four tokens: a token is 3 us of a warp's time, the shared
+// experts' batch for sixteen tokens 90 us of it.
+__device__ __forceinline__ uint32_t route_warps(uint32_t m) { return m <= 4 ? 4 : 6; }
+__device__ __forceinline__ void route_sync(uint32_t m) {
+    asm volatile("bar.sync 1, %0;" ::"r"(route_warps(m) * 32) : "memory");
+}
+
 // One token's softmax over the experts and its top_k, by a warp: raw logits
 // of the pair's two blocks (tiles of experts alternate between them).  A key
 // holds an expert's value above its complement, so that the maximum is the
-// first in TopKSelect's order.
-__device__ void route_token(const MoeArgs& p, uint32_t r, const long long* even, const long long* odd, uint32_t pitch,
+// first in TopKSelect's order.  EACH: experts of a lane.
+template <int EACH>
+__device__ __forceinline__ void route_token(const MoeArgs& p, uint32_t r, const long long* even, const long long* odd, uint32_t pitch,
                             uint32_t* s_sel, int32_t* s_score, uint32_t* s_mask) {
     const uint32_t lane = threadIdx.x & 31;
-    long long z[kMaxExperts / 32], top = INT64_MIN;
+    long long z[EACH], top = INT64_MIN;
 #pragma unroll
-    for (int i = 0; i < (int)kMaxExperts / 32; i++) {
+    for (int i = 0; i < EACH; i++) {
         const uint32_t e = i * 32 + lane;
         z[i] = INT64_MIN;
         if (e < p.experts) {
@@ -171,40 +196,41 @@ __device__ void route_token(const MoeArgs& p, uint32_t r, const long long* even,
             top = max(top, z[i]);
         }
     }
-    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    long long sum = 0;
+    top = warp_max(top);
+    int64_t sum = 0;
     bool bad = false;
+    uint32_t v[EACH];
 #pragma unroll
-    for (int i = 0; i < (int)kMaxExperts / 32; i++)
+    for (int i = 0; i < EACH; i++) {
+        v[i] = 0;
         if (i * 32 + lane < p.experts) {
-            int64_t v = fx_to_i64(table_at(p.exp_table, p.exp_len, fx_wsub(z[i], top), (int64_t)p.exp_len));
-            if (v < 0 || v > INT32_MAX) {
-                bad = true;
-                v = 0;
-            }
-            z[i] = v;
-            sum += v;
+            const int64_t x = fx_to_i64(table_at(p.exp_table, p.exp_len, fx_wsub(z[i], top), (int64_t)p.exp_len));
+            bad |= x < 0 || x > INT32_MAX;
+            v[i] = x < 0 || x > INT32_MAX ? 0u : (uint32_t)x;
         }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        sum += v[i];
+    }
+    sum = warp_sum(sum);
     if (bad) atomicOr(p.err, kErrRange);
     if (sum == 0 && lane == 0) atomicOr(p.err, kErrDivide);
-    const double inv = sum ? 1.0 / (double)sum : 0.0;
-    uint32_t key[kMaxExperts / 32];  // values are at most 2^16
+    const float inv = 1.0f / (float)sum;
+    uint32_t key[EACH], gate[EACH];  // values are at most 2^16
 #pragma unroll
-    for (int i = 0; i < (int)kMaxExperts / 32; i++) {
+    for (int i = 0; i < EACH; i++) {
         const uint32_t e = i * 32 + lane;
-        key[i] = e < p.experts ? ((sum ? (uint32_t)round_div_near(z[i] << 16, sum, inv) : 0u) << 8 | (255 - e)) + 1 : 0;
+        key[i] = e < p.experts ? ((sum ? (uint32_t)softmax_weight(v[i], sum, inv) : 0u) << 8 | (255 - e)) + 1 : 0;
+        gate[i] = 0;
     }
-    uint32_t chosen = 0;
     for (uint32_t j = 0; j < p.top_k; j++) {
         uint32_t best = 0;
 #pragma unroll
-        for (int i = 0; i < (int)kMaxExperts / 32; i++) best = max(best, (chosen >> i) & 1 ? 0u : key[i]);
+        for (int i = 0; i < EACH; i++) best = max(best, key[i]);
         best = __reduce_max_sync(0xFFFFFFFFu, best);
 #pragma unroll
-        for (int i = 0; i < (int)kMaxExperts / 32; i++)
-            if (key[i] == best && !((chosen >> i) & 1)) {  // one lane's, the keys being different
-                chosen |= 1u << i;
+        for (int i = 0; i < EACH; i++)
+            if (key[i] == best) {  // one lane's, the keys being different
+                key[i] = 0;
+                gate[i] = (best - 1) >> 8;
                 s_sel[r * p.top_k + j] = i * 32 + lane;
                 s_score[r * p.top_k + j] = (int32_t)((best - 1) >> 8);
                 atomicOr(&s_mask[i * 32 + lane], 1u << r);
@@ -212,47 +238,45 @@ __device__ void route_token(const MoeArgs& p, uint32_t r, const long long* even,
     }
     if (p.gate_out && blockIdx.x == 0)
 #pragma unroll
-        for (int i = 0; i < (int)kMaxExperts / 32; i++)
+        for (int i = 0; i < EACH; i++)
             if (i * 32 + lane < p.experts)
-                p.gate_out[(uint64_t)r * p.experts + i * 32 + lane] = (chosen >> i) & 1 ? (key[i] - 1) >> 8 : 0;
+                p.gate_out[(uint64_t)r * p.experts + i * 32 + lane] = gate[i];
 }
 
-// The items of all experts, by one warp: running sums over the experts give
-// the places of their slots and items
-__device__ void list_items(const MoeArgs& p, const uint32_t* s_sel, const uint32_t* s_mask, Items* it) {
+// The items of all experts: running sums over the experts by one warp give the
+// places of their slots and items, then a thread per slot fills in its own.
+// The routing warps; `thread`: a thread's number among theirs.
+__device__ __forceinline__ void list_items(const MoeArgs& p, uint32_t thread, const uint32_t* s_sel, const uint32_t* s_mask,
+                           uint32_t* s_start, Items* it) {
     const uint32_t lane = threadIdx.x & 31;
-    uint32_t slot = 0, item = 0;
-    for (uint32_t e0 = 0; e0 < p.experts; e0 += 32) {
-        const uint32_t e = e0 + lane;
-        uint32_t mask = e < p.experts ? s_mask[e] : 0;
-        const uint32_t c = __popc(mask), i = (c + kTile - 1) / kTile;
-        uint32_t sc = c, si = i;
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, sc, o), b = __shfl_up_sync(0xFFFFFFFFu, si, o);
-            if ((int)lane >= o) {
-                sc += a;
-                si += b;
+    if (thread < 32) {
+        uint32_t slot = 0, item = 0;
+        for (uint32_t e0 = 0; e0 < p.experts; e0 += 32) {
+            const uint32_t e = e0 + lane, c = e < p.experts ? __popc(s_mask[e]) : 0, i = (c + kTile - 1) / kTile;
+            uint32_t both = c << 16 | i;  // two running sums in one
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, both, o);
+                if ((int)lane >= o) both += a;
             }
+            const uint32_t at = slot + (both >> 16) - c, first = item + (both & 0xFFFF) - i;
+            if (e < p.experts) s_start[e] = at;
+            for (uint32_t j = 0; j < i; j++) {
+                it->expert[first + j] = (uint8_t)e;
+                it->count[first + j] = (uint8_t)min(kTile, c - j * kTile);
+                it->first[first + j] = (uint16_t)(at + j * kTile);
+            }
+            both = __shfl_sync(0xFFFFFFFFu, both, 31);
+            slot += both >> 16;
+            item += both & 0xFFFF;
         }
-        const uint32_t at = slot + sc - c;
-        for (uint32_t j = 0; j < i; j++) {
-            const uint32_t k = item + si - i + j;
-            it->expert[k] = (uint8_t)e;
-            it->count[k] = (uint8_t)min(kTile, c - j * kTile);
-            it->first[k] = (uint16_t)(at + j * kTile);
-        }
-        for (uint32_t j = 0; j < c; j++) {
-            const uint32_t tok = __ffs(mask) - 1;
-            mask &= mask - 1;
-            uint32_t place = 0;
-            while (s_sel[tok * p.top_k + place] != e) place++;
-            it->slot[at + j] = (uint16_t)(tok * p.top_k + place);
-            it->token[at + j] = (uint8_t)tok;
-        }
-        slot += __shfl_sync(0xFFFFFFFFu, sc, 31);
-        item += __shfl_sync(0xFFFFFFFFu, si, 31);
+        if (lane == 0) it->n = item;
     }
-    if (lane == 0) it->n = item;
+    route_sync(p.m);
+    for (uint32_t i = thread; i < p.m * p.top_k; i += route_warps(p.m) * 32) {
+        const uint32_t e = s_sel[i], tok = i / p.top_k, at = s_start[e] + __popc(s_mask[e] & ((1u << tok) - 1));
+        it->slot[at] = (uint16_t)i;
+        it->token[at] = (uint8_t)tok;
+    }
 }
 
 constexpr uint32_t kUpBatch = 16;                                       // tiles whose sums are held at a time
@@ -262,13 +286,13 @@ constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile
 // gridDim.x for i = 0, 1, ..: first those of the shared experts (four tokens
 // to each), then those of the chosen experts' items; in batches, of which
 // every warp takes an equal run of blocks of 64 k (gate and up together).
-template <bool TWO, int DEPTH>
+template <bool TWO, int DEPTH, int RUN>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Items items;
-    __shared__ uint32_t s_mask[kMaxExperts], s_sel[kMaxSlots];
+    __shared__ uint32_t s_mask[kMaxExperts], s_start[kMaxExperts], s_sel[kMaxSlots];
     __shared__ __align__(8) uint64_t s_bar[kWarps * DEPTH];
-    constexpr uint32_t kBytes = TWO ? 576 : 544, kSlot = 2 * kBytes;
+    constexpr uint32_t kBytes = TWO ? 576 : 544, kPair = 2 * kBytes, kSlot = RUN * kPair;  // gate and up
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t pitch = (p.etiles + 1) / 2 * 16, rank = cluster.block_rank();
@@ -289,40 +313,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
 
     // ---- the block's tiles and the warp's stream of blocks; until the routing is known, the
     // shared experts' first batch
-    const uint32_t ft = p.gate.s.tiles, st = p.sgate.s.tiles, stiles = st * ((p.m + kTile - 1) / kTile);
-    const uint32_t blocks = p.gate.s.blocks;
+    const uint32_t ft = p.up.s.tiles, st = p.sup.s.tiles, stiles = st * ((p.m + kTile - 1) / kTile);
+    const uint32_t blocks = p.up.s.blocks;
     auto tiles_below = [&](uint32_t u) { return u > blockIdx.x ? (u - blockIdx.x + gridDim.x - 1) / gridDim.x : 0u; };
     const uint32_t early = min(tiles_below(stiles), kUpBatch);  // tiles of the batch before the routing
+    const uint32_t early_warps = kWarps - route_warps(p.m);
     uint32_t known = early;                                     // tiles of this block that may be asked for
-    uint32_t next_first = 0, next_n = early, next_at = warp * (early * blocks) / kWarps, next_end = (warp + 1) * (early * blocks) / kWarps;
+    // of n tiles' blocks, the first that warp w takes if `warps` share them (all past the last)
+    auto first_block = [&](uint32_t n, uint32_t w, uint32_t warps) { return min(w, warps) * (n * blocks) / warps; };
+    uint32_t next_first = 0, next_n = early, next_at = first_block(early, warp, early_warps);
+    uint32_t next_end = first_block(early, warp + 1, early_warps);
     uint32_t next_slot = 0, asked = 0, taken = 0;
-    const uint8_t *next_g = nullptr, *next_u = nullptr;
-    auto point = [&]() {  // at block next_at of the batch
-        const uint32_t i = next_first + next_at / blocks, u = blockIdx.x + i * gridDim.x;
+    uint32_t next_left = 0;  // blocks of the present tile still to be asked for
+    const uint8_t* next_w = nullptr;
+    auto next_tile = [&]() {  // lane 0 only: on to the tile at next_at, false at the end of what is known
+        while (next_at == next_end) {
+            if (next_first + next_n >= known) return false;
+            next_first += next_n;
+            next_n = min(kUpBatch, known - next_first);
+            next_at = first_block(next_n, warp, kWarps);
+            next_end = first_block(next_n, warp + 1, kWarps);
+        }
+        const uint32_t i = next_at / blocks, b = next_at - i * blocks, u = blockIdx.x + (next_first + i) * gridDim.x;
         const bool shared = u < stiles;
-        const uint64_t tile = shared ? u % st : (uint64_t)items.expert[(u - stiles) / ft] * ft + (u - stiles) % ft;
-        const uint64_t at = (tile * blocks + next_at % blocks) * kBytes;
-        next_g = (shared ? p.sgate.w : p.gate.w) + at;
-        next_u = (shared ? p.sup.w : p.up.w) + at;
+        const uint32_t v = shared ? u : u - stiles, item = v / (shared ? st : ft), tile = v - item * (shared ? st : ft);
+        next_w = shared ? p.sup.w + ((uint64_t)tile * blocks + b) * kPair
+                        : p.up.w + (((uint64_t)items.expert[item] * ft + tile) * blocks + b) * kPair;
+        next_left = min(next_end - next_at, blocks - b);
+        next_at += next_left;
+        return true;
     };
-    auto ask = [&]() {  // lane 0 only: fill the ring
+    auto ask = [&]() {  // lane 0 only: fill the ring, up to RUN blocks of one tile to a slot
         while (asked < taken + DEPTH) {
-            while (next_at == next_end) {
-                if (next_first + next_n >= known) return;  // at the end, or of what is known
-                next_first += next_n;
-                next_n = min(kUpBatch, known - next_first);
-                next_at = warp * (next_n * blocks) / kWarps;
-                next_end = (warp + 1) * (next_n * blocks) / kWarps;
-                next_g = nullptr;
-            }
-            if (next_g == nullptr || next_at % blocks == 0) point();
-            const uint32_t b = bar + 8 * next_slot, to = shared_addr(ring + next_slot * kSlot);
-            barrier_expect(b, kSlot);
-            bulk_copy(to, next_g, kBytes, b);
-            bulk_copy(to + kBytes, next_u, kBytes, b);
-            next_g += kBytes;
-            next_u += kBytes;
-            next_at++;
+            if (next_left == 0 && !next_tile()) return;
+            const uint32_t run = min((uint32_t)RUN, next_left), b = bar + 8 * next_slot;
+            barrier_expect(b, run * kPair);
+            bulk_copy(shared_addr(ring) + next_slot * kSlot, next_w, run * kPair, b);
+            next_left -= run;
+            next_w += run * kPair;
             asked++;
             next_slot = next_slot + 1 == DEPTH ? 0 : next_slot + 1;
         }
@@ -334,21 +362,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     for (uint32_t i = threadIdx.x; i < p.experts; i += kThreads) s_mask[i] = 0;
     wait_for_previous();
     bool bad = false;
-    bad |= !q4_digitise<kThreads>(p.x, p.ldx, p.m, 1, p.h, blocks * 64, digits, p.stride);
-    __syncthreads();
+    const uint32_t fours = p.m * blocks * 16;
+    if (p.m < 4) {
+        bad |= !q4_digitise<kThreads, 2>(p.x, p.ldx, 1, p.h, blocks * 64, 0, fours, digits, p.stride);
+        __syncthreads();
+        cluster_wait();
+    } else {  // half of them each, stored to both
+        cluster_wait();
+        bad |= !q4_digitise<kThreads, 8>(p.x, p.ldx, 1, p.h, blocks * 64, rank * (fours / 2), rank ? fours : fours / 2, digits,
+                                      p.stride, cluster.map_shared_rank(digits, rank ^ 1));
+        cluster.sync();
+    }
     {
         // tiles of 16 experts, every other one this block's; eight (or sixteen) warps to a tile
         const uint32_t own = (p.etiles - rank + 1) / 2, wide = own > 1 ? kWarps / 2 : kWarps;
         for (uint32_t i = warp / wide; i < own; i += kWarps / wide) {
             const uint32_t w = warp % wide, r0 = w * blocks / wide, r1 = (w + 1) * blocks / wide;
             if (p.m <= 2)
-                router_part<1>(p, digits, i, rank, 0, r0, r1, sums, pitch);
+                router_part<1>(p, digits, i, rank, r0, r1, sums, pitch);
             else
-                for (uint32_t tok = 0; tok < p.m; tok += 8) router_part<4>(p, digits, i, rank, tok, r0, r1, sums, pitch);
+                router_part<4>(p, digits, i, rank, r0, r1, sums, pitch);
         }
     }
     __syncthreads();
-    cluster_wait();
     {
         long long* mine = logits + rank * p.m * pitch;
         long long* there = cluster.map_shared_rank(mine, rank ^ 1);
@@ -362,11 +398,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
 
     Patience patience;
     uint32_t slot = 0, phase = 0;
+    bool routed = false;
     auto token_of = [&](bool shared, uint32_t first, uint32_t j) { return shared ? first + j : items.token[first + j]; };
-    // one batch of the block's tiles, from number `first` on: sums into acc, then the activations
-    auto run = [&](uint32_t first, uint32_t n) {
-        uint32_t at = warp * (n * blocks) / kWarps;
-        const uint32_t end = (warp + 1) * (n * blocks) / kWarps;
+    // a batch of the block's tiles, n from number `first` on, shared by `warps`: sums into acc
+    auto add_up = [&](uint32_t first, uint32_t n, uint32_t warps) {
+        uint32_t at = first_block(n, warp, warps);
+        const uint32_t end = first_block(n, warp + 1, warps);
         while (at < end) {
             const uint32_t i = at / blocks, u = blockIdx.x + (first + i) * gridDim.x;
             const bool shared = u < stiles;
@@ -383,18 +420,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
             uint32_t b = at % blocks;
             const uint32_t stop = min(blocks, b + end - at);
             at += stop - b;
-            for (; b < stop; b++) {
+            while (b < stop) {
                 barrier_wait(bar + 8 * slot, phase, patience);
                 const uint8_t* w = ring + slot * kSlot;
-                uint4 x[2];
-                x[0] = *reinterpret_cast<const uint4*>(from[0] + b * 64);
-                if (count > 2) {
-                    x[1] = *reinterpret_cast<const uint4*>(from[1] + b * 64);
-                    q4_block<TWO, 2>(sum[0], w, x);
-                    q4_block<TWO, 2>(sum[1], w + kBytes, x);
-                } else {
-                    q4_block<TWO, 1>(sum[0], w, x);
-                    q4_block<TWO, 1>(sum[1], w + kBytes, x);
+#pragma unroll
+                for (int r = 0; r < RUN; r++) {
+                    if (RUN > 1 && b == stop) break;
+                    uint4 x[2];
+                    x[0] = *reinterpret_cast<const uint4*>(from[0] + b * 64);
+                    if (count > 2) {
+                        x[1] = *reinterpret_cast<const uint4*>(from[1] + b * 64);
+                        q4_block<TWO, 2>(sum[0], w, x);
+                        q4_block<TWO, 2>(sum[1], w + kBytes, x);
+                    } else {
+                        q4_block<TWO, 1>(sum[0], w, x);
+                        q4_block<TWO, 1>(sum[1], w + kBytes, x);
+                    }
+                    b++;
+                    w += kPair;
                 }
                 taken++;
                 __syncwarp();  // every lane has read the slot
@@ -415,7 +458,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
                     }
                 }
         }
-        __syncthreads();
+    };
+    // and from them the activations
+    auto finish = [&](uint32_t first, uint32_t n) {
         for (uint32_t o = threadIdx.x; o < n * kTile * 16; o += kThreads) {
             const uint32_t i = o / (kTile * 16), j = o / 16 % kTile, c = o % 16, u = blockIdx.x + (first + i) * gridDim.x;
             const bool shared = u < stiles;
@@ -427,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
             const int64_t gi = round_shift(acc.get(cell), p.shift), ui = round_shift(acc.get(cell + kTile * 16), p.shift);
             acc.clear(cell);
             acc.clear(cell + kTile * 16);
-            if (f >= (shared ? p.sgate.s.n : p.gate.s.n)) continue;
+            if (f >= (shared ? p.sup.s.n : p.up.s.n)) continue;
             const int64_t s = fx_to_i64(table_at(p.silu, p.silu_len, gi, (int64_t)(p.silu_len / 2)));
             uint32_t d;
             bad |= !q4_digits(round_shift(fx_wmul(s, ui), p.shift), &d);
@@ -437,28 +482,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
 #pragma unroll
             for (int q = 0; q < 4; q++) to[64 * q] = (uint8_t)(d >> (8 * q));
         }
-        __syncthreads();
     };
-    run(0, early);
 
-    // ---- routing
-    cluster_wait();
-    for (uint32_t r = warp; r < p.m; r += kWarps)
-        route_token(p, r, logits, logits + p.m * pitch, pitch, s_sel, items.score, s_mask);
-    __syncthreads();
-    if (warp == 0) list_items(p, s_sel, s_mask, &items);
-    __syncthreads();
-    known = tiles_below(stiles + ft * items.n);
-    if (lane == 0) ask();
-    if (blockIdx.x == 0)
-        for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
-            reinterpret_cast<uint32_t*>(p.items)[i] = reinterpret_cast<const uint32_t*>(&items)[i];
-    for (uint32_t first = early; first < known; first += kUpBatch) run(first, min(kUpBatch, known - first));
+    // ---- the batches; routing beside the first, of the shared experts
+    for (uint32_t first = 0, n = early;; n = min(kUpBatch, known - first)) {
+        const bool routing = first == 0 && !routed;
+        add_up(first, n, routing ? early_warps : kWarps);
+        if (routing) {
+            __syncwarp();
+            cluster_wait();
+            if (warp >= early_warps) {
+                for (uint32_t r = warp - early_warps; r < p.m; r += kWarps - early_warps) {
+                    if (p.experts <= 64)
+                        route_token<2>(p, r, logits, logits + p.m * pitch, pitch, s_sel, items.score, s_mask);
+                    else
+                        route_token<kMaxExperts / 32>(p, r, logits, logits + p.m * pitch, pitch, s_sel, items.score, s_mask);
+                }
+                route_sync(p.m);
+                list_items(p, threadIdx.x - early_warps * 32, s_sel, s_mask, s_start, &items);
+            }
+        }
+        __syncthreads();
+        if (routing) {
+            routed = true;
+            known = tiles_below(stiles + ft * items.n);
+            if (lane == 0) ask();
+            if (blockIdx.x == 0)
+                for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
+                    reinterpret_cast<uint32_t*>(p.items)[i] = reinterpret_cast<const uint32_t*>(&items)[i];
+        }
+        finish(first, n);
+        first += n;
+        if (first >= known) break;
+        __syncthreads();
+    }
     if (bad) atomicOr(p.err, kErrRange);
     if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
 }
 
-constexpr int kDownDepth = 4;
+constexpr int kDownDepth = 3;
+constexpr uint32_t kDownRun = 2;  // blocks to a slot
 
 // Blocks of the stream that a warp of k_moe_down takes: the chosen experts'
 // items one after another, then the shared experts' runs of tokens
@@ -473,7 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Items items;
     __shared__ __align__(8) uint64_t s_bar[kWarps * kDownDepth];
-    constexpr uint32_t kBytes = TWO ? 576 : 544, kSlot = 2 * kBytes + 256 * kTile;
+    constexpr uint32_t kBytes = TWO ? 576 : 544, kSlot = kDownRun * (2 * kBytes + 256 * kTile);
+    constexpr uint32_t kDigits = 2 * kDownRun * kBytes;  // after both tiles' blocks: those of each token
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t rank = cluster.block_rank(), slots = p.m * p.top_k, cells = (slots + p.m) * 32;
@@ -521,18 +585,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
     }
     auto ask = [&]() {  // lane 0 only
         const uint32_t b = bar + 8 * next_slot, to = shared_addr(ring + next_slot * kSlot);
-        barrier_expect(b, 2 * kBytes + 256 * next.count);
-        bulk_copy(to, next.w0, kBytes, b);
-        bulk_copy(to + kBytes, next.w1, kBytes, b);
+        const uint32_t run = min(kDownRun, min(end - next_at, next.len - next.b));
+        barrier_expect(b, run * (2 * kBytes + 256 * next.count));
+        bulk_copy(to, next.w0, run * kBytes, b);
+        bulk_copy(to + kDownRun * kBytes, next.w1, run * kBytes, b);
         for (uint32_t j = 0; j < next.count; j++)
-            bulk_copy(to + 2 * kBytes + 256 * j,
+            bulk_copy(to + kDigits + kDownRun * 256 * j,
                       (next.shared ? p.sact + (uint64_t)(next.first + j) * ns * 256
-                                   : p.act + (uint64_t)items.slot[next.first + j] * nf * 256) + next.b * 256, 256, b);
+                                   : p.act + (uint64_t)items.slot[next.first + j] * nf * 256) + next.b * 256,
+                      run * 256, b);
         next_slot = next_slot + 1 == p.depth ? 0 : next_slot + 1;
-        next_at++;
-        next.w0 += kBytes;
-        next.w1 += kBytes;
-        if (++next.b == next.len && next_at < end) locate(next, next_at);
+        next_at += run;
+        next.b += run;
+        next.w0 += run * kBytes;
+        next.w1 += run * kBytes;
+        if (next.b == next.len && next_at < end) locate(next, next_at);
     };
     if (lane == 0)
         for (uint32_t i = 0; i < p.depth; i++)
@@ -545,20 +612,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         sum[0].clear();
         sum[1].clear();
         // digits of columns g: digit row g % 4 of token g / 4 (and 2 + g / 4) of the item
-        const uint32_t x0 = 2 * kBytes + min(g >> 2, now.count - 1) * 256 + (g & 3) * 64 + 16 * t;
-        const uint32_t x1 = 2 * kBytes + min(2 + (g >> 2), now.count - 1) * 256 + (g & 3) * 64 + 16 * t;
-        for (; at < stop; at++) {
+        const uint32_t x0 = kDigits + min(g >> 2, now.count - 1) * kDownRun * 256 + (g & 3) * 64 + 16 * t;
+        const uint32_t x1 = kDigits + min(2 + (g >> 2), now.count - 1) * kDownRun * 256 + (g & 3) * 64 + 16 * t;
+        while (at < stop) {
             barrier_wait(bar + 8 * slot, phase, patience);
             const uint8_t* s = ring + slot * kSlot;
-            uint4 x[2];
-            x[0] = *reinterpret_cast<const uint4*>(s + x0);
-            if (now.count > 2) {
-                x[1] = *reinterpret_cast<const uint4*>(s + x1);
-                q4_block<TWO, 2>(sum[0], s, x);
-                q4_block<TWO, 2>(sum[1], s + kBytes, x);
-            } else {
-                q4_block<TWO, 1>(sum[0], s, x);
-                q4_block<TWO, 1>(sum[1], s + kBytes, x);
+#pragma unroll
+            for (uint32_t r = 0; r < kDownRun; r++) {
+                if (at == stop) break;
+                uint4 x[2];
+                x[0] = *reinterpret_cast<const uint4*>(s + x0 + r * 256);
+                if (now.count > 2) {
+                    x[1] = *reinterpret_cast<const uint4*>(s + x1 + r * 256);
+                    q4_block<TWO, 2>(sum[0], s + r * kBytes, x);
+                    q4_block<TWO, 2>(sum[1], s + (kDownRun + r) * kBytes, x);
+                } else {
+                    q4_block<TWO, 1>(sum[0], s + r * kBytes, x);
+                    q4_block<TWO, 1>(sum[1], s + (kDownRun + r) * kBytes, x);
+                }
+                at++;
             }
             __syncwarp();  // every lane has read the slot
             if (lane == 0 && next_at < end) ask();
@@ -604,11 +676,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
 }
 
 // Dynamic shared memory of k_moe_up
-size_t up_shared(uint32_t m, uint32_t stride, uint32_t etiles, uint32_t bytes, uint32_t depth) {
-    return (size_t)kWarps * depth * 2 * bytes + 12 * kUpCells + (size_t)m * (4 * stride + 2 * 16 * 8 * ((etiles + 1) / 2));
+size_t up_shared(uint32_t m, uint32_t stride, uint32_t etiles, uint32_t bytes, uint32_t blocks) {
+    return (size_t)kWarps * blocks * 2 * bytes + 12 * kUpCells + (size_t)m * (4 * stride + 2 * 16 * 8 * ((etiles + 1) / 2));
 }
 
-constexpr uint32_t kUpShallow = 3, kUpDeep = 6;
+constexpr uint32_t kUpShallow = 3, kUpDeep = 6;  // blocks in a warp's ring: three slots of one or of two
 
 uint32_t tokens_at_once(uint32_t stride, uint32_t etiles, uint32_t bytes) {
     uint32_t m = kMaxTokens;
@@ -627,24 +699,24 @@ bool moe_shapes(uint64_t h, uint64_t experts, uint64_t top_k, uint64_t f, uint64
            q4_shape(h, shared_f, group, 0, &s->sup) && q4_shape(shared_f, h, group, 0, &s->sdown);
 }
 
-template <bool TWO, int DEPTH>
+template <bool TWO, int DEPTH, int RUN>
 int up_launch(const MoeArgs& p, cudaStream_t stream) {
     static std::atomic<uint64_t> set{0};
-    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_up<TWO, DEPTH>), kMaxShared, &set));
-    return launch(k_moe_up<TWO, DEPTH>, dim3(kSms), kThreads, up_shared(p.m, p.stride, p.etiles, p.gate.s.bytes, DEPTH),
-                  2, stream, p);
+    auto* kernel = k_moe_up<TWO, DEPTH, RUN>;
+    ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kMaxShared, &set));
+    return launch(kernel, dim3(kSms), kThreads, up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, DEPTH * RUN), 2, stream, p);
 }
 
 template <bool TWO>
 int moe_launch(MoeArgs p, cudaStream_t stream) {
-    const bool deep = up_shared(p.m, p.stride, p.etiles, p.gate.s.bytes, kUpDeep) <= kMaxShared;
-    const int rc = deep ? up_launch<TWO, kUpDeep>(p, stream) : up_launch<TWO, kUpShallow>(p, stream);
+    const bool deep = up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, kUpDeep) <= kMaxShared;
+    const int rc = deep ? up_launch<TWO, 3, 2>(p, stream) : up_launch<TWO, 3, 1>(p, stream);
     if (rc) return rc;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_down<TWO>), kMaxShared, &set));
-    const size_t sums = 12ull * (p.m * p.top_k + p.m) * 32, slot = (size_t)kWarps * (2 * p.down.s.bytes + 256 * kTile);
+    const size_t sums = 12ull * (p.m * p.top_k + p.m) * 32, slot = (size_t)kWarps * kDownRun * (2 * p.down.s.bytes + 256 * kTile);
     p.depth = kDownDepth;
-    while (p.depth * slot + sums > kMaxShared) p.depth--;  // three at least: 104 and 105 kB
+    while (p.depth > 1 && p.depth * slot + sums > kMaxShared) p.depth--;  // one of 70 kB fits beside 104 kB
     return launch(k_moe_down<TWO>, dim3((p.down.s.tiles + 1) / 2 * 2), kThreads, p.depth * slot + sums, 2, stream, p);
 }
 
@@ -693,15 +765,14 @@ int zkie2_moe_rows(const uint64_t* d_x, uint64_t ldx, uint64_t m, uint64_t h, ui
         !d_exp_table || exp_len == 0 || !d_silu_table || silu_len == 0 || !d_err || (m > 1 && ldx < h) ||
         (d_residual && m > 1 && ldr < h) || ((uintptr_t)d_router & 15) || ((uintptr_t)d_scratch & 15))
         return (int)cudaErrorInvalidValue;
-    for (int i = 0; i < 6; i++)
+    for (int i = 0; i < 4; i++)
         if (!h_weights[i] || ((uintptr_t)h_weights[i] & 15)) return (int)cudaErrorInvalidValue;
     if (m == 0) return 0;
     if (!d_x || !d_out || !d_scratch) return (int)cudaErrorInvalidValue;
     MoeArgs p{};
-    const Q4Shape* shape[6] = {&s.up, &s.up, &s.down, &s.sup, &s.sup, &s.sdown};
-    Q4Weight* weight[6] = {&p.gate, &p.up, &p.down, &p.sgate, &p.sup, &p.sdown};
-    for (int i = 0; i < 6; i++)
-        *weight[i] = Q4Weight{reinterpret_cast<const uint8_t*>(h_weights[i]), *shape[i]};
+    const Q4Shape* shape[4] = {&s.up, &s.down, &s.sup, &s.sdown};
+    Q4Weight* weight[4] = {&p.up, &p.down, &p.sup, &p.sdown};
+    for (int i = 0; i < 4; i++) *weight[i] = Q4Weight{reinterpret_cast<const uint8_t*>(h_weights[i]), *shape[i]};
     p.ldx = ldx;
     p.h = (uint32_t)h;
     p.experts = (uint32_t)experts;

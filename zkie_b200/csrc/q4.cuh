@@ -93,24 +93,26 @@ __device__ __forceinline__ void q4_store_digits(uint8_t* to, size_t stride, cons
     }
 }
 
-// The digits of `rows` rows of x (k_seg numbers to each of `segs` segments,
-// padded to kp_seg) into digit rows of `stride` bytes, four to a row; false in
-// a thread that met a number out of range.  A thread takes four numbers at a
-// time and has four such loads under way, whatever rows they belong to: one
+// The digits of rows of x (k_seg numbers to each of `segs` segments, padded to
+// kp_seg) into digit rows of `stride` bytes, four to a row: fours of numbers
+// [begin, end) counted over all rows, and to `also` (another block's shared
+// memory) where given; false in a thread that met a number out of range.  A thread takes four numbers at a
+// time and has AHEAD such loads under way, whatever rows they belong to: one
 // after the other, eight rows would cost eight times the memory's latency.
-template <int THREADS>
-__device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint64_t ldx, uint32_t rows, uint32_t segs,
-                                            uint32_t k_seg, uint32_t kp_seg, uint8_t* digits, uint32_t stride) {
-    const uint32_t quads = segs * kp_seg / 4, total = rows * quads;
+template <int THREADS, int AHEAD>
+__device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint64_t ldx, uint32_t segs, uint32_t k_seg,
+                                            uint32_t kp_seg, uint32_t begin, uint32_t end, uint8_t* digits,
+                                            uint32_t stride, uint8_t* also = nullptr) {
+    const uint32_t quads = segs * kp_seg / 4;
     const bool wide = (((uintptr_t)x | (ldx * 8)) & 15) == 0 && k_seg % 4 == 0;  // 16-byte loads
     bool ok = true;
-    for (uint32_t i0 = threadIdx.x; i0 < total; i0 += THREADS * 4) {
-        int64_t v[4][4];
-        uint32_t to[4];
+    for (uint32_t i0 = begin + threadIdx.x; i0 < end; i0 += THREADS * AHEAD) {
+        int64_t v[AHEAD][4];
+        uint32_t to[AHEAD];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
+        for (int u = 0; u < AHEAD; u++) {
             const uint32_t i = i0 + u * THREADS;
-            const bool on = i < total;
+            const bool on = i < end;
             const uint32_t r = on ? i / quads : 0, k0 = on ? (i % quads) * 4 : 0;
             const uint32_t seg = segs > 1 ? k0 / kp_seg : 0, in = k0 - seg * kp_seg;
             const uint64_t* from = x + r * ldx + seg * k_seg + in;
@@ -128,12 +130,13 @@ __device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint
             }
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+        for (int u = 0; u < AHEAD; u++)
             if (to[u] != ~0u) {
                 uint32_t d[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) ok &= q4_digits(fx_to_i64((uint64_t)v[u][j]), &d[j]);
                 q4_store_digits(digits + to[u], stride, d);
+                if (also) q4_store_digits(also + to[u], stride, d);
             }
     }
     return ok;
@@ -303,18 +306,34 @@ __device__ __forceinline__ uint64_t table_at(const uint64_t* __restrict__ table,
     return __ldg(table + (i < 0 ? 0 : (i > hi ? hi : i)));
 }
 
-// q = round_div(a, b) for a >= 0 below 2^52 and 0 < b below 2^52, with inv =
-// 1 / b to double precision: the estimate is off by one at most
-__device__ __forceinline__ int64_t round_div_near(int64_t a, int64_t b, double inv) {
-    int64_t q = (int64_t)((double)a * inv), r = a - q * b;
+// A softmax's weight, round_div(e 2^16, sum) for 0 <= e < 2^31 and e <= sum <
+// 2^52: estimated in single precision from inv = 1 / sum -- each of the five
+// roundings is off by 2^-23 at most, so the estimate of at most 2^16 by less
+// than 1/16 -- and set right by the remainder, which is exact.
+__device__ __forceinline__ int softmax_weight(uint32_t e, int64_t sum, float inv) {
+    const int64_t a = (int64_t)e << 16;
+    int q = (int)((float)e * 65536.0f * inv);
+    int64_t r = a - q * sum;
     if (r < 0) {
         q--;
-        r += b;
-    } else if (r >= b) {
+        r += sum;
+    } else if (r >= sum) {
         q++;
-        r -= b;
+        r -= sum;
     }
-    return 2 * r >= b ? q + 1 : q;
+    return 2 * r >= sum ? q + 1 : q;
+}
+
+// the maximum and the sum over a warp's lanes, in whole-warp reductions of 32 bits
+__device__ __forceinline__ int64_t warp_max(int64_t v) {
+    const int hi = __reduce_max_sync(0xFFFFFFFFu, (int)(v >> 32));
+    const uint32_t lo = __reduce_max_sync(0xFFFFFFFFu, (int)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (int64_t)((uint64_t)(uint32_t)hi << 32 | lo);
+}
+// of numbers in [0, 2^42)
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+    const uint32_t lo = __reduce_add_sync(0xFFFFFFFFu, (uint32_t)v & 0xFFFFu);
+    return ((int64_t)__reduce_add_sync(0xFFFFFFFFu, (uint32_t)(v >> 16)) << 16) + lo;
 }
 
 }  // namespace zk

@@ -378,7 +378,7 @@ class MoeBlock:
     and down (experts x f x h) and the shared experts' gate, up (h x shared f)
     and down weights, all of one group without segments, the exp and silu
     tables (field elements; silu's middle is zero) and how many experts a token
-    takes."""
+    takes.  The block keeps a copy of its own of the gate and up weights."""
 
     def __init__(self, router: torch.Tensor, gate: QuantWeight, up: QuantWeight, down: QuantWeight,
                  shared_gate: QuantWeight, shared_up: QuantWeight, shared_down: QuantWeight, exp_table: torch.Tensor,
@@ -386,14 +386,14 @@ class MoeBlock:
         self.h, self.f, self.shared_f = gate.k, gate.n, shared_gate.n
         self.experts, self.group, self.top_k, self.shift = gate.experts, gate.group, top_k, shift
         h, f, s, e = self.h, self.f, self.shared_f, self.experts
-        self.weights = (gate, up, down, shared_gate, shared_up, shared_down)
+        weights = (gate, up, down, shared_gate, shared_up, shared_down)
         want = ((e, h, f), (e, h, f), (e, f, h), (1, h, s), (1, h, s), (1, s, h))
-        for w, shape in zip(self.weights, want):
+        for w, shape in zip(weights, want):
             if (w.experts, w.k, w.n) != shape or w.group != self.group or w.segment:
                 raise ValueError(f"MoeBlock: weight {w.experts} x {w.k} x {w.n}, group {w.group}, segment {w.segment}: "
                                  f"{shape} with group {self.group} and no segments is wanted")
         self.device = dev = _device_of(router, "router")
-        if any(w.device != dev for w in self.weights):
+        if any(w.device != dev for w in weights):
             raise ValueError("MoeBlock: weights on the current device are wanted")
         router = _flat(router, "router", _U64, dev, (h, e))
         self.exp_table, self.silu_table = _flat(exp_table, "exp_table", _U64, dev), \
@@ -407,11 +407,20 @@ class MoeBlock:
         err = _err_word()
         check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self.router.data_ptr(), err.data_ptr(), _stream()), "zkie2_moe_router_pack")
         _check_err(err, "MoeBlock: router")
-        self._packed = (_lib.vp * 6)(*[w.pointer for w in self.weights])
+        self.packed = (self._pair(gate, up), down.packed, self._pair(shared_gate, shared_up), shared_down.packed)
+        self._packed = (_lib.vp * 4)(*[w.data_ptr() for w in self.packed])
         self._shape = (h, e, top_k, f, s, self.group)
         self._args = (self.router.data_ptr(), self._packed, exp_table.data_ptr(), exp_table.numel(),
                       silu_table.data_ptr(), silu_table.numel(), shift)
         self._scratch = {}  # elements by rows
+
+    @staticmethod
+    def _pair(a: QuantWeight, b: QuantWeight) -> torch.Tensor:
+        """Gate and up, block by block side by side: one copy brings both."""
+        out = torch.empty(2 * a.packed.numel(), dtype=torch.int32, device=a.packed.device)
+        check(lib.zkie2_q4_pair(a.pointer, b.pointer, a.experts, a.k, a.n, a.group, out.data_ptr(), _stream()),
+              "zkie2_q4_pair")
+        return out
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                 err: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
