@@ -111,7 +111,8 @@ struct ProjectArgs {
     uint64_t* out;
     uint32_t* err;
     uint32_t stride;  // bytes of a digit row in shared memory
-    uint32_t run;     // blocks to a slot of a ring
+    uint32_t run;     // blocks to a slot of a ring, at most
+    uint32_t unit;    // blocks that stay with one warp: a segment, or a slot where a tile has whole ones
 };
 
 constexpr int kProjDepth = 3;           // slots of a warp's ring
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     const uint32_t row0 = blockIdx.y * kRows, rows = min(kRows, p.m - row0);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t slot_bytes = p.run * kBytes;
-    uint8_t* ring = smem + (size_t)warp * kProjDepth * slot_bytes;
+    const uint32_t ring = shared_addr(smem) + warp * kProjDepth * slot_bytes;
     constexpr uint32_t kCells = kProjBatch * kRows * 16;  // (tile, row, column)
     const Limbs acc{reinterpret_cast<uint32_t*>(smem + (size_t)kProjWarps * kProjDepth * slot_bytes), kCells};
     uint8_t* digits = reinterpret_cast<uint8_t*>(acc.w + 3 * kCells);
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     // ---- this warp's stream of blocks, and the first of them on their way
     const uint32_t tile0 = (uint32_t)((uint64_t)blockIdx.x * p.s.tiles / gridDim.x);
     const uint32_t tile1 = (uint32_t)((uint64_t)(blockIdx.x + 1) * p.s.tiles / gridDim.x);
-    const uint32_t blocks = p.s.blocks, unit = SEG ? p.s.kp_seg / 64 : 1;
+    const uint32_t blocks = p.s.blocks, unit = p.unit;
     // blocks of a batch, counted from its first tile, that the warp takes
     auto first_of = [&](uint32_t batch, uint32_t w) {
         const uint32_t units = min(kProjBatch, tile1 - batch) * blocks / unit;
@@ -163,11 +164,11 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             next_at = first_of(next_batch, warp);
             next_end = first_of(next_batch, warp + 1);
         }
-        const uint32_t bytes = min(p.run, next_end - next_at) * kBytes;
-        barrier_expect(bar + 8 * next_slot, bytes);
-        bulk_copy(shared_addr(ring + next_slot * slot_bytes), p.w + ((uint64_t)next_batch * blocks + next_at) * kBytes, bytes,
+        const uint32_t run = min(min(p.run, next_end - next_at), blocks - next_at % blocks);  // within a tile
+        barrier_expect(bar + 8 * next_slot, run * kBytes);
+        bulk_copy(ring + next_slot * slot_bytes, p.w + ((uint64_t)next_batch * blocks + next_at) * kBytes, run * kBytes,
                   bar + 8 * next_slot);
-        next_at = min(next_at + p.run, next_end);
+        next_at += run;
         next_slot = next_slot + 1 == kProjDepth ? 0 : next_slot + 1;
     };
     if (lane == 0)
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
         atomicOr(p.err, kErrRange);
     __syncthreads();
 
-    const uint8_t* from = digits + (size_t)g * p.stride + 16 * t;  // column g: digit g % 4 of row g / 4
+    const uint32_t from = shared_addr(digits) + g * p.stride + 16 * t;  // column g: digit g % 4 of row g / 4
     Patience patience;
     uint32_t slot = 0, phase = 0;
     for (uint32_t batch = tile0; batch < tile1; batch += kProjBatch) {
@@ -204,36 +205,42 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             }
             if (!SEG) sum.clear();
         };
+        uint32_t x_at[NT];  // the digits of each pair of rows, at block b
+#pragma unroll
+        for (int i = 0; i < NT; i++) x_at[i] = from + i * 8 * p.stride + b * 64;
         while (at < end) {
-            const uint32_t run = min(p.run, end - at);
+            const uint32_t run = min(min(p.run, end - at), blocks - b);
             barrier_wait(bar + 8 * slot, phase, patience);
-            const uint8_t* block = ring + slot * slot_bytes;
-            for (uint32_t j = 0; j < run;) {
-                // blocks up to the end of the tile (or segment)
-                const uint32_t n = min(run - j, (SEG ? unit - b % unit : blocks - b));
-#pragma unroll 2
-                for (uint32_t q = 0; q < n; q++) {
-                    uint4 x[NT];
+            const Q4Lane lane_at(ring + slot * slot_bytes);
+            auto block = [&](uint32_t q) {
+                uint4 x[NT];
 #pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        x[i] = *reinterpret_cast<const uint4*>(from + (size_t)i * 8 * p.stride + (b + q) * 64);
-                    q4_block<TWO, NT, NT>(sum, block + q * kBytes, x);
-                }
-                j += n;
-                b += n;
-                block += n * kBytes;
-                if (SEG && b % unit == 0) {
+                for (int i = 0; i < NT; i++) x[i] = load16(x_at[i] + q * 64);
+                q4_block<TWO, NT, NT>(sum, lane_at, q * kBytes, x);
+            };
+            if (!SEG && run == 4) {
 #pragma unroll
-                    for (int i = 0; i < NT; i++) total[i] += round_shift(sum.finish(i), p.shift);
-                    sum.clear();
+                for (uint32_t q = 0; q < 4; q++) block(q);
+                b += 4;
+            } else {
+                for (uint32_t q = 0; q < run; q++) {
+                    block(q);
+                    if (SEG && ++b % unit == 0) {
+#pragma unroll
+                        for (int i = 0; i < NT; i++) total[i] += round_shift(sum.finish(i), p.shift);
+                        sum.clear();
+                    }
                 }
-                if (b == blocks) {
-                    flush();
-                    b = 0;
-                    tile++;
-                }
+                if (!SEG) b += run;
             }
             at += run;
+            if (b == blocks) {
+                flush();
+                b = 0;
+                tile++;
+            }
+#pragma unroll
+            for (int i = 0; i < NT; i++) x_at[i] = from + i * 8 * p.stride + b * 64;
             __syncwarp();  // every lane has read the slot
             if (lane == 0 && next_batch < tile1) ask();
             if (++slot == kProjDepth) {
@@ -305,7 +312,8 @@ int project_rows(ProjectArgs p, cudaStream_t stream) {
     // (2 kB a copy) where there is room, else of two or one
     for (uint32_t rows = p.m > 4 ? 8 : p.m > 2 ? 4 : 2;; rows /= 2)
         for (p.run = 4; p.run; p.run /= 2)
-            if (project_shared(p.s, rows, p.run) <= kMaxShared)
+            if (p.unit = p.s.segs > 1 ? p.s.kp_seg / 64 : p.s.blocks % p.run ? 1 : p.run;
+                project_shared(p.s, rows, p.run) <= kMaxShared)
                 return rows == 8   ? project_seg<TWO, 4>(p, stream)
                        : rows == 4 ? project_seg<TWO, 2>(p, stream)
                                    : project_seg<TWO, 1>(p, stream);

@@ -410,10 +410,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
             const uint32_t item = shared ? u / st : (u - stiles) / ft;
             const uint32_t tok0 = shared ? item * kTile : items.first[item];
             const uint32_t count = shared ? min(kTile, p.m - tok0) : items.count[item];
-            const uint8_t* from[2];
+            uint32_t from[2];
 #pragma unroll
             for (int q = 0; q < 2; q++)
-                from[q] = digits + (size_t)(token_of(shared, tok0, min(2 * q + (g >> 2), count - 1)) * 4 + (g & 3)) * p.stride + 16 * t;
+                from[q] = shared_addr(digits) + (token_of(shared, tok0, min(2 * q + (g >> 2), count - 1)) * 4 + (g & 3)) * p.stride + 16 * t;
             Q4Sum<2> sum[2];
             sum[0].clear();
             sum[1].clear();
@@ -422,22 +422,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
             at += stop - b;
             while (b < stop) {
                 barrier_wait(bar + 8 * slot, phase, patience);
-                const uint8_t* w = ring + slot * kSlot;
+                const Q4Lane lane_at(shared_addr(ring) + slot * kSlot);
 #pragma unroll
                 for (int r = 0; r < RUN; r++) {
                     if (RUN > 1 && b == stop) break;
                     uint4 x[2];
-                    x[0] = *reinterpret_cast<const uint4*>(from[0] + b * 64);
+                    x[0] = load16(from[0] + b * 64);
                     if (count > 2) {
-                        x[1] = *reinterpret_cast<const uint4*>(from[1] + b * 64);
-                        q4_block<TWO, 2>(sum[0], w, x);
-                        q4_block<TWO, 2>(sum[1], w + kBytes, x);
+                        x[1] = load16(from[1] + b * 64);
+                        q4_block<TWO, 2>(sum[0], lane_at, r * kPair, x);
+                        q4_block<TWO, 2>(sum[1], lane_at, r * kPair + kBytes, x);
                     } else {
-                        q4_block<TWO, 1>(sum[0], w, x);
-                        q4_block<TWO, 1>(sum[1], w + kBytes, x);
+                        q4_block<TWO, 1>(sum[0], lane_at, r * kPair, x);
+                        q4_block<TWO, 1>(sum[1], lane_at, r * kPair + kBytes, x);
                     }
                     b++;
-                    w += kPair;
                 }
                 taken++;
                 __syncwarp();  // every lane has read the slot
@@ -616,19 +615,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         const uint32_t x1 = kDigits + min(2 + (g >> 2), now.count - 1) * kDownRun * 256 + (g & 3) * 64 + 16 * t;
         while (at < stop) {
             barrier_wait(bar + 8 * slot, phase, patience);
-            const uint8_t* s = ring + slot * kSlot;
+            const uint32_t base = shared_addr(ring) + slot * kSlot;
+            const Q4Lane lane_at(base);
 #pragma unroll
             for (uint32_t r = 0; r < kDownRun; r++) {
                 if (at == stop) break;
                 uint4 x[2];
-                x[0] = *reinterpret_cast<const uint4*>(s + x0 + r * 256);
+                x[0] = load16(base + x0 + r * 256);
                 if (now.count > 2) {
-                    x[1] = *reinterpret_cast<const uint4*>(s + x1 + r * 256);
-                    q4_block<TWO, 2>(sum[0], s + r * kBytes, x);
-                    q4_block<TWO, 2>(sum[1], s + (kDownRun + r) * kBytes, x);
+                    x[1] = load16(base + x1 + r * 256);
+                    q4_block<TWO, 2>(sum[0], lane_at, r * kBytes, x);
+                    q4_block<TWO, 2>(sum[1], lane_at, (kDownRun + r) * kBytes, x);
                 } else {
-                    q4_block<TWO, 1>(sum[0], s + r * kBytes, x);
-                    q4_block<TWO, 1>(sum[1], s + (kDownRun + r) * kBytes, x);
+                    q4_block<TWO, 1>(sum[0], lane_at, r * kBytes, x);
+                    q4_block<TWO, 1>(sum[1], lane_at, (kDownRun + r) * kBytes, x);
                 }
                 at++;
             }

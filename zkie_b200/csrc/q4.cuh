@@ -167,7 +167,19 @@ struct Patience {
     bool failed = false;
 };
 
+// Shared memory by its own 32-bit addresses: a load is one instruction with its
+// offset in it, where a generic pointer costs 64-bit sums.
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint4 load16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t load4(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
 
 __device__ __forceinline__ void barrier_init(uint32_t bar) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
@@ -264,15 +276,20 @@ struct Limbs {
     __device__ __forceinline__ void clear(uint32_t at) const { w[at] = w[n + at] = w[2 * n + at] = 0; }
 };
 
-// One block of 64 k at `block` in shared memory against NT of the MAX pairs of
+// A lane's place in a block in shared memory: its codes, and its scales
+struct Q4Lane {
+    uint32_t codes, scales;
+    __device__ __forceinline__ explicit Q4Lane(uint32_t block)
+        : codes(block + (threadIdx.x & 31) * 16), scales(block + 512 + (threadIdx.x & 31) / 4 * 4) {}
+};
+
+// One block of 64 k, `off` bytes on from `at`, against NT of the MAX pairs of
 // rows, their digits in b.  TWO: two groups of 32 rows, else one.
 template <bool TWO, int NT, int MAX>
-__device__ __forceinline__ void q4_block(Q4Sum<MAX>& sum, const uint8_t* block, const uint4 (&b)[MAX]) {
+__device__ __forceinline__ void q4_block(Q4Sum<MAX>& sum, const Q4Lane& at, uint32_t off, const uint4 (&b)[MAX]) {
     constexpr uint32_t kHigh = 0xF0F0F0F0u;  // a code in a byte's high half is sixteen times itself
-    const uint32_t lane = threadIdx.x & 31;
-    const uint4 w = *reinterpret_cast<const uint4*>(block + lane * 16);
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(block + 512) + (lane >> 2);
-    const uint32_t s0 = scales[0], s1 = TWO ? scales[8] : 0;
+    const uint4 w = load16(at.codes + off);
+    const uint32_t s0 = load4(at.scales + off), s1 = TWO ? load4(at.scales + off + 32) : 0;
     int c[NT][4];
     {
         const uint32_t a0 = (w.x << 4) & kHigh, a1 = (w.y << 4) & kHigh, a2 = (w.z << 4) & kHigh,

@@ -30,7 +30,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .compose import _check_err, _err_word
+from .compose import _INDEX_WRITERS, _check_err, _err_word
 from .device import P, device
 
 _q4_project, _kv_attend, _moe_rows = lib.zkie2_q4_project, lib.zkie2_kv_attend, lib.zkie2_moe_rows
@@ -151,6 +151,26 @@ def quantise(w: torch.Tensor, group: int = 64, segment: int = 0) -> Tuple[torch.
     s = scales[..., row, :]
     codes = torch.div(2 * w + s, 2 * s, rounding_mode="floor").clamp(-8, 7)
     return codes.to(torch.int8), scales.to(torch.int32)
+
+
+def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: int = 64) -> dict:
+    """Quantise the weights that the ops of these kinds read (Projection w,
+    GatherMatMul w, MatMul b where no op writes it), in place: the Store gets
+    the dense tensor that the codes stand for, so the model that is run and
+    proven is the quantised one.  Returns {tensor id: (codes, scales, group)},
+    what QuantWeight takes."""
+    written = {t for op in ops if op.kind not in _INDEX_WRITERS for t in op.writes()}
+    done = {}
+    for op in ops:
+        t = op.b if op.kind == "MatMul" else getattr(op, "w", None)
+        if op.kind not in kinds or t is None or t in done or t in written:
+            continue
+        shape = (op.n_experts, op.k, op.n) if op.kind == "GatherMatMul" else (op.k, op.n)
+        codes, scales = quantise(store.get(t).reshape(shape), group)
+        row = _group_of(op.k, group, 0, codes.device)
+        store.v[t] = _field(codes.to(torch.int64) * scales.to(torch.int64)[..., row, :]).reshape(-1)
+        done[t] = (codes, scales, group)
+    return done
 
 
 class QuantWeight:
@@ -320,6 +340,12 @@ class KvCache:
                                   *self._args, word.data_ptr(), _raw_stream(dev)), "zkie2_kv_append")
         if err is None:
             _check_err(word, "append")
+
+    def room(self, limit: int, err: torch.Tensor):
+        """Set the error word's bit for a full cache where a sequence has
+        reached ``limit`` tokens: for a limit within the last block."""
+        if limit < self.capacity:
+            err.bitwise_or_((self.lens >= limit).any().to(torch.int32) * 16)
 
     def advance(self, tokens: int = 1):
         """Count ``tokens`` more in every active sequence."""

@@ -13,14 +13,22 @@ values gathered back by (token, expert), and Gather (scatter-add) into token
 order.  The tables are the reference's kinds: exp (2^21), the piecewise rsqrt,
 the 2^16 limb range, SiLU at scale 2^16 over 2^24 points, the causal mask and
 RoPE's cos / sin at scale 2^16.
+
+``moe_block`` and ``MoeLayerDecoder`` compute the experts and the whole layer
+for a few rows, one token at a time, with the weights of such a graph in 4
+bits (``decode.quantise_weights``), bit for bit the graph's rows.
 """
 from dataclasses import dataclass
 
 import numpy as np
+import torch
 
+from . import decode
 from .compose import (Add, BroadcastScale, CombineIdx, Gather, GatherMatMul, GeluIndex, IdxBroadcast, Lookup,
                       MatMul, PadIdx, Projection, RmsNorm, RoPE, Scale, ScaleVec, Scatter, Softmax, StableSoftmaxIndex,
-                      TopKSelect, Transpose)
+                      TopKSelect, Transpose, rms_norm_columns)
+from ._lib import check, lib
+from .device import device, ptr, stream_handle
 from .gkr import XorShift64
 from .gpt2 import RSQRT_TABLE_LEN, SCALE, _pad2, causal_mask, exp_table, from_i64, rsqrt_table, xorshift_fill
 
@@ -249,3 +257,98 @@ def moe_layer(store, s: MoeShape = DSV2_LITE, seed: int = 0xD5E):
     ops.append(Add(x2, ff, x3))
     return ops, x, x3
 
+
+
+# ---- token by token ---------------------------------------------------------------------------
+def moe_block(store, ops, weights: dict, exp_table: int, silu_table: int, shift: int = 16) -> decode.MoeBlock:
+    """The experts of a graph that ``build_moe`` built, for a few rows: the
+    router as it is, the routed and the shared experts' weights from what
+    ``decode.quantise_weights(store, ops)`` returned."""
+    at = next(i for i, op in enumerate(ops) if op.kind == "TopKSelect")
+    route, router = ops[at], ops[at - 4]  # MatMul, Scale, StableSoftmaxIndex, Softmax, TopKSelect
+    experts = [op for op in ops[at:] if op.kind == "GatherMatMul"]
+    shared = [op for op in ops[at:] if op.kind == "Projection"]
+    if router.kind != "MatMul" or len(experts) != 3 or len(shared) != 3:
+        raise ValueError("moe_block: not a graph of build_moe")
+    quant = lambda op: decode.QuantWeight(*weights[op.w])  # noqa: E731
+    return decode.MoeBlock(store.get(router.b).reshape(router.k, router.n), *[quant(op) for op in experts + shared],
+                           store.get(exp_table), store.get(silu_table), route.k, shift)
+
+
+class MoeLayerDecoder:
+    """One layer of ``moe_layer`` one token at a time, for ``batch`` sequences
+    side by side: RmsNorm, the kv latent with its norm and the rotated key that
+    all heads share, the heads' q, k and v as wide projections, RoPE, attention
+    over the cache (keys of nope + rope dimensions), the output projection
+    summed over the heads onto the residual, RmsNorm and ``moe_block``."""
+
+    def __init__(self, store, ops, s: MoeShape, weights: dict, batch: int = 1):
+        self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
+        wide = lambda t, n: store.get(t).view(torch.int64).reshape(-1, n)[0].repeat(batch).view(torch.uint64)  # noqa: E731
+        norms = [op for op in ops if op.kind == "RmsNorm"]
+        proj = [op for op in ops if op.kind == "Projection"]
+        ropes = [op for op in ops if op.kind == "RoPE"]
+        soft = next(op for op in ops if op.kind == "Softmax")
+        silu = next(op for op in ops if op.kind == "Lookup" and op.table != norms[0].rsqrt_table and
+                    any(o.kind == "GeluIndex" and o.out == op.idx for o in ops))
+        if len(proj) != 2 + 5 * s.heads + 3 or len(norms) != 3:
+            raise ValueError("MoeLayerDecoder: not a graph of moe_layer with this shape")
+
+        def quant(ids, dim, segment=0):
+            parts = [weights[o.w] for o in ids]
+            return decode.QuantWeight(torch.cat([p[0] for p in parts], dim), torch.cat([p[1] for p in parts], dim),
+                                      parts[0][2], segment)
+
+        kinds = [[proj[2 + 5 * h + j] for h in range(s.heads)] for j in range(5)]  # q nope, q rope, k nope, v, o
+        self.latent = quant([proj[0], proj[1]], 1)          # kv latent | shared rope key
+        self.q, self.kv = quant(kinds[0] + kinds[1], 1), quant(kinds[2] + kinds[3], 1)
+        self.o = quant(kinds[4], 0, s.v_head)
+        self.norms = [(wide(op.w, op.d), op.d) for op in norms]  # input, latent, after attention
+        self.rsqrt, self.exp = store.get(norms[0].rsqrt_table), store.get(soft.table)
+        half = s.qk_rope // 2
+        self.cos, self.sin = (store.get(t).view(torch.int64).reshape(s.m, half) for t in (ropes[0].cos, ropes[0].sin))
+        self.block = moe_block(store, ops, weights, soft.table, silu.table, s.shift)
+        self.cache = decode.KvCache.zeros(batch, s.heads, s.qk_nope + s.qk_rope, s.v_head, s.m)
+
+    def _norm(self, x, i):
+        w, d = self.norms[i]
+        return rms_norm_columns(x.reshape(-1), w, self.rsqrt, self.batch, d, d, self.err)["out"].reshape(self.batch, d)
+
+    def _rotate(self, x, heads):
+        """RoPE of batch x (heads rope) at each sequence's position."""
+        s = self.s
+        at = self.cache.lens.clamp(0, s.m - 1).to(torch.int64)
+        cos, sin = (t[at].reshape(-1).view(torch.uint64) for t in (self.cos, self.sin))
+        x = x.contiguous().reshape(-1)
+        out = torch.empty_like(x)
+        check(lib.zkie2_op_rope(ptr(x), x.numel(), ptr(cos), ptr(sin), self.batch, s.qk_rope, s.shift, ptr(out),
+                                stream_handle()), "zkie2_op_rope")
+        return out.reshape(self.batch, heads * s.qk_rope)
+
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        """The layer's output rows (batch x hidden) for the next token of every
+        sequence; its key and value go into the cache, the position is counted."""
+        s, b = self.s, self.batch
+        i64 = lambda t: t.view(torch.int64)  # noqa: E731
+        self.cache.room(s.m, self.err)  # the graph's positions, not the cache's whole blocks
+        h = self._norm(x, 0)
+        lat = decode.project(h, self.latent, s.shift, err=self.err)
+        kv = decode.project(self._norm(lat[:, :s.kv_lora].contiguous(), 1), self.kv, s.shift, err=self.err)
+        q = decode.project(h, self.q, s.shift, err=self.err)
+        nope, rope, n = s.heads * s.qk_nope, s.qk_rope, s.heads
+        side = lambda a, r: torch.cat([i64(a).reshape(b, n, -1), r], 2).reshape(b, -1).view(torch.uint64)  # noqa: E731
+        key = i64(self._rotate(lat[:, s.kv_lora:], 1)).reshape(b, 1, rope).expand(b, n, rope)
+        query = i64(self._rotate(q[:, nope:], n)).reshape(b, n, rope)
+        a = decode.attend(side(q[:, :nope], query), self.cache, self.exp, k=side(kv[:, :nope], key), v=kv[:, nope:],
+                          score_scale=(7519, 32), offset=1 << s.exp_bits, err=self.err)
+        x = decode.project(a, self.o, s.shift, residual=x, err=self.err)
+        out, _ = self.block.forward(self._norm(x, 2), residual=x, err=self.err)
+        self.cache.advance()
+        return out
+
+    def check(self):
+        """Raise if a step since the last check met data its kernels do not take."""
+        try:
+            decode.check_err(self.err, "MoeLayerDecoder")
+        finally:
+            self.err.zero_()

@@ -22,17 +22,24 @@
 
 Builders take any store with ``push`` / ``push_idx`` taking numpy arrays (the
 device Store, or a host store for the CPU checker).
+
+``Gpt2Decoder`` answers one token at a time with the weights of such a graph
+in 4 bits (``decode.quantise_weights``): its logits are the graph's rows, bit
+for bit.
 """
 import ctypes as C
 from dataclasses import dataclass
+from typing import Optional
 
 import numpy as np
+import torch
 
-from . import _lib
-from ._lib import lib
+from . import _lib, decode
+from ._lib import check, lib
+from .device import device, ptr, stream_handle
 from .gkr import XorShift64
 from .compose import (Add, Argmax, GeluIndex, Layernorm, LayerNormCentered, Lookup, MatMul, Projection, Scale, Softmax,
-                      SoftmaxIndex, StableSoftmaxIndex, Transpose)
+                      SoftmaxIndex, StableSoftmaxIndex, Transpose, layer_norm_centered_columns)
 
 P = 0xFFFFFFFF00000001
 SCALE = 65536.0
@@ -343,3 +350,164 @@ def gpt2_model(store, s: LayerShape, layers: int = 12, seed: int = 0x6B2):
     out = store.push_idx(None)
     ops.append(Argmax(logits_masked, sel, thr, gate, d1, d2, out, m, V))
     return ops, tok_t, out
+
+
+# ---- token by token ---------------------------------------------------------------------------
+class Gpt2Decoder:
+    """The graph of ``gpt2_model`` one token at a time, for ``batch`` sequences
+    side by side: the tied embedding and its position row, per layer
+    LayerNormCentered, the heads' q, k and v as one projection, attention over
+    the layer's cache, the output projection summed over the heads onto the
+    residual, LayerNormCentered, the feed-forward with the gelu table; the
+    final norm, the lm_head and the choice of the token.
+
+    ``weights`` is what ``decode.quantise_weights(store, ops, ("Projection",
+    "MatMul"))`` returned for the graph: the Store then holds the same numbers,
+    and a step's adjusted logits (without penalties) are the row that
+    ``forward_ops`` leaves in the Argmax arm's input, so the tokens generated
+    are the ones the graph proves.  Sequences hold at most the graph's m
+    tokens.  ``tokens`` (uint32, batch) is each sequence's next token to take;
+    a step replaces it by its choice."""
+
+    def __init__(self, store, ops, s: LayerShape, weights: dict, batch: int = 1):
+        self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
+        rows = lambda t, n: store.get(t).reshape(-1, n)[0]  # noqa: E731  a row vector broadcast over m rows
+        wide = lambda t, n: rows(t, n).view(torch.int64).repeat(batch).view(torch.uint64)  # noqa: E731
+
+        def quant(ids, dim, segment=0):
+            parts = [weights[t] for t in ids]
+            return decode.QuantWeight(torch.cat([p[0] for p in parts], dim), torch.cat([p[1] for p in parts], dim),
+                                      parts[0][2], segment)
+
+        norms = [op for op in ops if op.kind == "LayerNormCentered"]
+        projections = [op for op in ops if op.kind == "Projection"]
+        per = 4 * s.heads + 2  # a layer's projections: q, k, v, o per head, then fc and proj
+        if len(projections) % per or len(norms) != 2 * (len(projections) // per) + 1:
+            raise ValueError("Gpt2Decoder: not a graph of gpt2_model with this shape")
+        if s.d * s.vocab > 0x7FFFFFFF:
+            raise ValueError("Gpt2Decoder: an embedding table of at most 2^31 - 1 entries is wanted")
+        tables = {op.kind: op for op in ops}
+        self.exp = store.get(tables["Softmax"].table)
+        lookups = [op for op in ops if op.kind == "Lookup"]
+        self.gelu, self.rsqrt = store.get(lookups[1].table), store.get(norms[0].rsqrt_table)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device())
+        self.layers, self.witness = [], []
+        for i in range(0, len(projections), per):
+            layer = projections[i:i + per]
+            heads, fc, proj = layer[:4 * s.heads], layer[-2], layer[-1]
+            kinds = [[heads[4 * h + j] for h in range(s.heads)] for j in range(4)]
+            n = 2 * (i // per)
+            cat = lambda ids: torch.cat([rows(t, s.dh).view(torch.int64) for t in ids]).view(torch.uint64)  # noqa: E731
+            # the output bias is added after the heads' sum: Add(acc, o_b)
+            o_b = next(op.b for op in ops if op.kind == "Add" and op.a == self._sum_of(ops, [o.out for o in kinds[3]]))
+            self.layers.append(dict(
+                ln1=(wide(norms[n].w, s.d), wide(norms[n].b, s.d)), ln2=(wide(norms[n + 1].w, s.d), wide(norms[n + 1].b, s.d)),
+                qkv=quant([o.w for j in range(3) for o in kinds[j]], 1), qkv_b=cat([o.bias for j in range(3) for o in kinds[j]]),
+                o=quant([o.w for o in kinds[3]], 0, s.dh), o_b=rows(o_b, s.d).clone(),
+                fc=quant([fc.w], 1), fc_b=rows(fc.bias, s.ffn).clone(),
+                proj=quant([proj.w], 1), proj_b=rows(proj.bias, s.d).clone(),
+                cache=decode.KvCache.zeros(batch, s.heads, s.dh, s.dh, s.m, self.lens)))
+            scaled = {op.x: op.out for op in ops if op.kind == "Scale"}
+            self.witness.append(([scaled[o.out] for o in kinds[1]], [o.out for o in kinds[2]]))
+        self.lnf = (wide(norms[-1].w, s.d), wide(norms[-1].b, s.d))
+        lm = next(op for op in ops if op.kind == "MatMul" and op.a == norms[-1].out)
+        self.lm = quant([lm.b], 1)
+        self.wte, self.pos = store.get(lookups[0].table), store.get(ops[1].b).reshape(s.m, s.d)
+        self.columns = torch.arange(s.d, dtype=torch.int32, device=device()) * s.vocab
+        bits = np.arange(-(-s.vocab // 32) * 32) < s.vocab_real
+        self.allowed = torch.from_numpy(np.packbits(bits, bitorder="little").view(np.int32).copy()).to(device())
+        self.tokens = torch.zeros(batch, dtype=torch.uint32, device=device())
+
+    @staticmethod
+    def _sum_of(ops, heads):
+        """The tensor that adds up the heads' outputs."""
+        acc = heads[0]
+        for h in heads[1:]:
+            acc = next(op.c for op in ops if op.kind == "Add" and op.a == acc and op.b == h)
+        return acc
+
+    def load(self, store, sequence: int, tokens: int):
+        """Take the first ``tokens`` positions of a forward pass of the graph as
+        the past of one sequence: its scaled keys and values, from the Store."""
+        s = self.s
+        if not 0 <= sequence < self.batch or not 0 <= tokens <= s.m:
+            raise ValueError("load: a sequence of the batch and at most the graph's positions are wanted")
+        self.lens[sequence] = 0
+        for layer, (ks, vs) in zip(self.layers, self.witness):
+            c = layer["cache"]
+            one = decode.KvCache(c.k[sequence:sequence + 1], c.v[sequence:sequence + 1], self.lens[sequence:sequence + 1])
+            side = lambda ids: torch.stack([store.get(t).view(torch.int64).reshape(s.m, s.dh)[:tokens] for t in ids],  # noqa: E731
+                                           dim=1).reshape(1, tokens, -1).contiguous().view(torch.uint64)
+            if tokens:
+                one.append(side(ks), side(vs), err=self.err)
+        self.lens[sequence] = tokens
+
+    def _norm(self, x, w):
+        return layer_norm_centered_columns(x.reshape(-1), w[0], w[1], self.rsqrt, self.batch, self.s.d, self.s.d_real,
+                                           self.err)["out"].reshape(self.batch, self.s.d)
+
+    def _embed(self):
+        s, n = self.s, self.batch * self.s.d
+        idx = (self.columns + self.tokens.view(torch.int32)[:, None]).contiguous()
+        rows, x = torch.empty(n, dtype=torch.uint64, device=idx.device), torch.empty(n, dtype=torch.uint64, device=idx.device)
+        sh = stream_handle()
+        check(lib.zkie2_op_lookup(idx.data_ptr(), n, ptr(self.wte), self.wte.numel(), ptr(rows), self.err.data_ptr(), sh),
+              "zkie2_op_lookup")
+        at = self.lens.clamp(0, s.m - 1).to(torch.int64)
+        pos = self.pos.view(torch.int64)[at].reshape(-1).view(torch.uint64)
+        check(lib.zkie2_op_add(ptr(rows), ptr(pos), n, ptr(x), sh), "zkie2_op_add")
+        return x.reshape(self.batch, s.d)
+
+    def logits(self) -> torch.Tensor:
+        """One step up to the lm_head: the logits (batch x vocab) after the
+        present tokens, whose keys and values go into the caches at position
+        lens (``lens`` stays)."""
+        s = self.s
+        self.layers[0]["cache"].room(s.m, self.err)  # the graph's positions, not the cache's whole blocks
+        x = self._embed()
+        hd = s.heads * s.dh
+        for w in self.layers:
+            r = decode.project(self._norm(x, w["ln1"]), w["qkv"], s.shift, bias=w["qkv_b"], err=self.err)
+            a = decode.attend(r[:, :hd], w["cache"], self.exp, k=r[:, hd:2 * hd], v=r[:, 2 * hd:], q_scale=(23170, 16),
+                              k_scale=(23170, 16), score_scale=(1, 16), offset=1 << s.exp_bits, err=self.err)
+            x = decode.project(a, w["o"], s.shift, bias=w["o_b"], residual=x, err=self.err)
+            f = decode.project(self._norm(x, w["ln2"]), w["fc"], s.shift, bias=w["fc_b"], table=self.gelu,
+                               offset=1 << (s.gelu_bits - 1), err=self.err)
+            x = decode.project(f, w["proj"], s.shift, bias=w["proj_b"], residual=x, err=self.err)
+        return decode.project(self._norm(x, self.lnf), self.lm, 0, err=self.err)
+
+    def step(self, **choice):
+        """Take ``tokens``, choose the next ones (``choice``: what
+        ``decode.choose_token`` takes; the vocabulary's padding is masked as in
+        the graph unless ``allowed`` is given) and count the position.  Returns
+        (tokens, adjusted logits).  Nothing is read back: ``check`` does."""
+        choice.setdefault("allowed", self.allowed)
+        tokens, logits = decode.choose_token(self.logits(), err=self.err, **choice)
+        layer = self.layers[0]["cache"]
+        layer.advance()
+        self.tokens.copy_(tokens)
+        return self.tokens, logits
+
+    def capture(self, **choice) -> Optional[torch.cuda.CUDAGraph]:
+        """A step recorded as a CUDA graph, to be replayed once per token; the
+        position and the tokens it ran on for warm-up are put back."""
+        lens, tokens = self.lens.clone(), self.tokens.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            self.step(**choice)
+            self.lens.copy_(lens)
+            self.tokens.copy_(tokens)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self.step(**choice)
+        return graph
+
+    def check(self):
+        """Raise if a step since the last check met data its kernels do not take."""
+        try:
+            decode.check_err(self.err, "Gpt2Decoder")
+        finally:
+            self.err.zero_()
