@@ -123,10 +123,11 @@ constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 // is rounded by itself), whatever tiles they belong to, against the digits of
 // 2 NT rows in shared memory.  The 64-bit sums meet in shared memory; a thread
 // per output then rounds and finishes it.
-template <bool TWO, int NT, bool SEG>
+template <int G, int NT, bool SEG>
 __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_constant__ ProjectArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_bar[kProjWarps * kProjDepth];
+    constexpr bool TWO = G == 32;
     constexpr uint32_t kRows = 2 * NT, kBytes = TWO ? 576 : 544;
     const uint32_t row0 = blockIdx.y * kRows, rows = min(kRows, p.m - row0);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -218,9 +219,19 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
                 for (int i = 0; i < NT; i++) x[i] = load16(x_at[i] + q * 64);
                 q4_block<TWO, NT, NT>(sum, lane_at, q * kBytes, x);
             };
-            if (!SEG && run == 4) {
+            if (!SEG && run == 4 && (G != 128 || unit == 4)) {
 #pragma unroll
-                for (uint32_t q = 0; q < 4; q++) block(q);
+                for (uint32_t q = 0; q < 4; q += 2) {
+                    if (G == 128) {  // four blocks from a multiple of four on: two whole groups
+                        uint4 x[2][NT];
+#pragma unroll
+                        for (int i = 0; i < 2 * NT; i++) x[i / NT][i % NT] = load16(x_at[i % NT] + (q + i / NT) * 64);
+                        q4_group<NT>(sum, lane_at, q * kBytes, kBytes, x);
+                    } else {
+                        block(q);
+                        block(q + 1);
+                    }
+                }
                 b += 4;
             } else {
                 for (uint32_t q = 0; q < run; q++) {
@@ -292,21 +303,21 @@ size_t project_shared(const Q4Shape& s, uint32_t rows, uint32_t run) {
     return (size_t)kProjWarps * kProjDepth * run * s.bytes + (size_t)rows * (kProjBatch * 16 * 12 + 4 * q4_digit_stride(s.blocks));
 }
 
-template <bool TWO, int NT, bool SEG>
+template <int G, int NT, bool SEG>
 int project_launch(const ProjectArgs& p, cudaStream_t stream) {
-    auto* kernel = k_q4_project<TWO, NT, SEG>;
+    auto* kernel = k_q4_project<G, NT, SEG>;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kMaxShared, &set));
     const dim3 grid(p.s.tiles < (uint32_t)kSms ? p.s.tiles : kSms, (unsigned)ceil_div(p.m, 2 * NT));
     return launch(kernel, grid, kProjThreads, project_shared(p.s, 2 * NT, p.run), 1, stream, p);
 }
 
-template <bool TWO, int NT>
+template <int G, int NT>
 int project_seg(const ProjectArgs& p, cudaStream_t stream) {
-    return p.s.segs > 1 ? project_launch<TWO, NT, true>(p, stream) : project_launch<TWO, NT, false>(p, stream);
+    return p.s.segs > 1 ? project_launch<G, NT, true>(p, stream) : project_launch<G, NT, false>(p, stream);
 }
 
-template <bool TWO>
+template <int G>
 int project_rows(ProjectArgs p, cudaStream_t stream) {
     // Rows to a block: up to eight, as many as their digits leave room for; slots of four blocks
     // (2 kB a copy) where there is room, else of two or one
@@ -314,9 +325,9 @@ int project_rows(ProjectArgs p, cudaStream_t stream) {
         for (p.run = 4; p.run; p.run /= 2)
             if (p.unit = p.s.segs > 1 ? p.s.kp_seg / 64 : p.s.blocks % p.run ? 1 : p.run;
                 project_shared(p.s, rows, p.run) <= kMaxShared)
-                return rows == 8   ? project_seg<TWO, 4>(p, stream)
-                       : rows == 4 ? project_seg<TWO, 2>(p, stream)
-                                   : project_seg<TWO, 1>(p, stream);
+                return rows == 8   ? project_seg<G, 4>(p, stream)
+                       : rows == 4 ? project_seg<G, 2>(p, stream)
+                                   : project_seg<G, 1>(p, stream);
 }
 
 // ---- the cache ------------------------------------------------------------------------------
@@ -943,7 +954,9 @@ int zkie2_q4_project(const uint64_t* d_x, uint64_t ldx, uint64_t m, const uint32
     p.out = d_out;
     p.err = d_err;
     p.stride = q4_digit_stride(p.s.blocks);
-    return group == 32 ? project_rows<true>(p, stream) : project_rows<false>(p, stream);
+    return group == 32   ? project_rows<32>(p, stream)
+           : group == 64 ? project_rows<64>(p, stream)
+                         : project_rows<128>(p, stream);
 }
 
 int zkie2_kv_append(const uint64_t* d_k, uint64_t ldk, const uint64_t* d_v, uint64_t ldv, uint64_t tokens,

@@ -283,32 +283,47 @@ struct Q4Lane {
         : codes(block + (threadIdx.x & 31) * 16), scales(block + 512 + (threadIdx.x & 31) / 4 * 4) {}
 };
 
+// The products of one block's codes with NT pairs of rows, added to c: first
+// the rows whose codes lie in the low halves, then those in the high ones.
+template <int NT, int MAX, bool LOW>
+__device__ __forceinline__ void q4_half(int (&c)[NT][4], const uint4& w, const uint4 (&b)[MAX], bool fresh) {
+    constexpr uint32_t kHigh = 0xF0F0F0F0u;  // a code in a byte's high half is sixteen times itself
+    const uint32_t a0 = (LOW ? w.x << 4 : w.x) & kHigh, a1 = (LOW ? w.y << 4 : w.y) & kHigh,
+                   a2 = (LOW ? w.z << 4 : w.z) & kHigh, a3 = (LOW ? w.w << 4 : w.w) & kHigh;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        const uint32_t b0 = LOW ? b[i].x : b[i].z, b1 = LOW ? b[i].y : b[i].w;
+        if (fresh)
+            mma_s8_new(c[i], a0, a1, a2, a3, b0, b1);
+        else
+            mma_s8(c[i], a0, a1, a2, a3, b0, b1);
+    }
+}
+
 // One block of 64 k, `off` bytes on from `at`, against NT of the MAX pairs of
 // rows, their digits in b.  TWO: two groups of 32 rows, else one.
 template <bool TWO, int NT, int MAX>
 __device__ __forceinline__ void q4_block(Q4Sum<MAX>& sum, const Q4Lane& at, uint32_t off, const uint4 (&b)[MAX]) {
-    constexpr uint32_t kHigh = 0xF0F0F0F0u;  // a code in a byte's high half is sixteen times itself
     const uint4 w = load16(at.codes + off);
     const uint32_t s0 = load4(at.scales + off), s1 = TWO ? load4(at.scales + off + 32) : 0;
     int c[NT][4];
-    {
-        const uint32_t a0 = (w.x << 4) & kHigh, a1 = (w.y << 4) & kHigh, a2 = (w.z << 4) & kHigh,
-                       a3 = (w.w << 4) & kHigh;
-#pragma unroll
-        for (int i = 0; i < NT; i++) mma_s8_new(c[i], a0, a1, a2, a3, b[i].x, b[i].y);
-    }
+    q4_half<NT, MAX, true>(c, w, b, true);
     if (TWO) sum.template add_group<NT>(c, s0);
-    {
-        const uint32_t a0 = w.x & kHigh, a1 = w.y & kHigh, a2 = w.z & kHigh, a3 = w.w & kHigh;
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-            if (TWO)
-                mma_s8_new(c[i], a0, a1, a2, a3, b[i].z, b[i].w);
-            else
-                mma_s8(c[i], a0, a1, a2, a3, b[i].z, b[i].w);
-        }
-    }
+    q4_half<NT, MAX, false>(c, w, b, TWO);
     sum.template add_group<NT>(c, TWO ? s1 : s0);
+}
+
+// Two blocks that share a group of 128 rows: scaled once
+template <int NT>
+__device__ __forceinline__ void q4_group(Q4Sum<NT>& sum, const Q4Lane& at, uint32_t off, uint32_t bytes,
+                                         const uint4 (&b)[2][NT]) {
+    int c[NT][4];
+    const uint4 w = load16(at.codes + off), v = load16(at.codes + off + bytes);
+    q4_half<NT, NT, true>(c, w, b[0], true);
+    q4_half<NT, NT, false>(c, w, b[0], false);
+    q4_half<NT, NT, true>(c, v, b[1], false);
+    q4_half<NT, NT, false>(c, v, b[1], false);
+    sum.template add_group<NT>(c, load4(at.scales + off));
 }
 
 // round_div(a, 2^s): the quotient rounded down, plus the highest bit shifted out
