@@ -182,11 +182,12 @@ def test_choose_refusals(zk):
 def test_python_refuses_host_tensors(zk):
     import torch
     d = zk.decode
-    x = torch.zeros((2, 64), dtype=torch.uint64)
+    x, err = torch.zeros((2, 64), dtype=torch.uint64), torch.zeros(1, dtype=torch.int32)
 
     class Weight:  # stands for a QuantWeight: never reached
-        n, k, experts, device = 16, 64, 1, 0
-    for call in (lambda: d.project(x, Weight(), 16), lambda: d.choose_token(x), lambda: d.project([1], Weight(), 16),
+        call = (0, A, 64, 16, 64, 0, 1)
+    for call in (lambda: d.project(x, Weight(), 16, err=err), lambda: d.choose_token(x, err=err),
+                 lambda: d.project([1], Weight(), 16, err=err),
                  lambda: d.KvCache(torch.zeros((1, 1, 1, 1, 32, 4), dtype=torch.int32),
                                    torch.zeros((1, 1, 32, 4), dtype=torch.int32), torch.zeros(1, dtype=torch.int32))):
         with pytest.raises(ValueError, match="CUDA device is wanted"):

@@ -1,0 +1,303 @@
+// calls.cpp -- the per-token calls of zkie_b200/decode.py as a CPython
+// extension (zkie_b200/_calls.so): argument checks, output allocation and the
+// call of the C entry point.  A step of generation makes some eighty of these
+// calls, each of a few microseconds on the device; in Python with ctypes the
+// checks and the conversion of 18 to 28 arguments took 5 to 9 us of a call.
+// The C functions are libzkie_b200.so's own (include/zkie2.h).
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <Python.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstdint>
+#include <sstream>
+#include <string>
+
+#include "../../include/zkie2.h"
+
+namespace {
+
+// thrown where a Python error has been set
+struct Refused {};
+
+[[noreturn]] void refuse(const std::string& what) {
+    PyErr_SetString(PyExc_ValueError, what.c_str());
+    throw Refused{};
+}
+
+std::string said(const at::Tensor& t) {
+    std::ostringstream s;
+    s << t.scalar_type() << " " << t.sizes() << " with strides " << t.strides() << " on " << t.device();
+    return s.str();
+}
+
+const at::Tensor& tensor(PyObject* o, const char* name) {
+    if (!THPVariable_Check(o)) refuse(std::string(name) + ": a tensor on the current CUDA device is wanted, not " +
+                                      Py_TYPE(o)->tp_name);
+    return THPVariable_Unpack(o);
+}
+
+// the tensor that the call's device is taken from
+int device_of(const at::Tensor& t, const char* name) {
+    if (!t.is_cuda() || t.get_device() != c10::cuda::current_device())
+        refuse(std::string(name) + ": a tensor on the current CUDA device is wanted, not " + said(t));
+    return t.get_device();
+}
+
+// a matrix of field elements with rows of `cols` numbers of unit stride that do not overlap
+struct Rows {
+    const uint64_t* data = nullptr;
+    int64_t n = 0, stride = 0;
+};
+Rows rows(const at::Tensor& t, const char* name, int64_t cols, int dev) {
+    if (t.scalar_type() != at::kUInt64 || !t.is_cuda() || t.get_device() != dev || t.dim() != 2 || t.size(1) != cols ||
+        (cols > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < cols))
+        refuse(std::string(name) + ": a uint64 matrix of " + std::to_string(cols) +
+               " columns on the call's device, unit stride within its rows, is wanted, not " + said(t));
+    return {static_cast<const uint64_t*>(t.data_ptr()), t.size(0), t.stride(0)};
+}
+
+// a contiguous tensor of a type (and a shape)
+template <typename T>
+T* flat(const at::Tensor& t, const char* name, at::ScalarType type, int dev, at::IntArrayRef shape) {
+    if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != dev || !t.is_contiguous() || t.sizes() != shape) {
+        std::ostringstream s;
+        s << name << ": a contiguous " << type << " tensor " << shape << " on the call's device is wanted, not " << said(t);
+        refuse(s.str());
+    }
+    return static_cast<T*>(t.data_ptr());
+}
+// a table of field elements: its length is what it is
+const uint64_t* table_of(const at::Tensor& t, const char* name, int dev) {
+    if (t.numel() == 0) refuse(std::string(name) + ": an empty table");
+    return flat<uint64_t>(t, name, at::kUInt64, dev, {t.numel()});
+}
+
+int64_t number(PyObject* o) {
+    const int64_t v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw Refused{};
+    return v;
+}
+void* address(PyObject* o) {
+    void* p = PyLong_AsVoidPtr(o);
+    if (!p && PyErr_Occurred()) throw Refused{};
+    return p;
+}
+// a shift of a rounding division
+uint32_t shift_of(PyObject* o, const char* name) {
+    const int64_t v = number(o);
+    if (v < 0 || v > 62) refuse(std::string(name) + ": a shift 0 .. 62 is wanted");
+    return (uint32_t)v;
+}
+struct Scale {
+    int64_t factor;
+    uint32_t shift;
+};
+Scale scale(PyObject* o, const char* name) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 2) refuse(std::string(name) + ": (factor, shift) is wanted");
+    return {number(PyTuple_GET_ITEM(o, 0)), shift_of(PyTuple_GET_ITEM(o, 1), name)};
+}
+
+at::Tensor make(at::IntArrayRef shape, at::ScalarType type, int dev) {
+    return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, dev));
+}
+at::Tensor output(PyObject* o, at::IntArrayRef shape, int dev) {
+    if (o == Py_None) return make(shape, at::kUInt64, dev);
+    const at::Tensor& t = tensor(o, "out");
+    flat<uint64_t>(t, "out", at::kUInt64, dev, shape);
+    return t;
+}
+uint32_t* word(PyObject* o, int dev) {
+    const at::Tensor& t = tensor(o, "err");
+    if (t.numel() != 1) refuse("err: one int32 word is wanted, not " + said(t));
+    return reinterpret_cast<uint32_t*>(flat<int32_t>(t, "err", at::kInt, dev, t.sizes()));
+}
+zkie_stream_t stream(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
+
+void done(int rc, const char* what) {
+    if (rc) {
+        PyErr_Format(PyExc_RuntimeError, "%s failed with CUDA error %d", what, rc);
+        throw Refused{};
+    }
+}
+
+template <typename F>
+PyObject* guarded(F f) {
+    try {
+        return f();
+    } catch (const Refused&) {
+    } catch (const std::exception& e) {  // an allocation that failed
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
+// project(x, (device, pointer, k, n, group, segment, experts), shift, bias, table, offset, residual, out, err)
+PyObject* project(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 9) refuse("project: 9 arguments");
+        const at::Tensor& x = tensor(a[0], "x");
+        const int dev = device_of(x, "x");
+        int64_t w[7];
+        for (int i = 0; i < 7; i++) w[i] = i == 1 ? 0 : number(PyTuple_GET_ITEM(a[1], i));
+        const auto* packed = static_cast<const uint32_t*>(address(PyTuple_GET_ITEM(a[1], 1)));
+        const int64_t k = w[2], n = w[3];
+        const Rows in = rows(x, "x", k, dev);
+        if (w[6] != 1 || w[0] != dev) refuse("project: one weight (no stack of experts) on the call's device is wanted");
+        if (in.n > 65535) refuse("project: at most 65535 rows are wanted");
+        const uint32_t shift = shift_of(a[2], "project");
+        const uint64_t* bias = a[3] == Py_None ? nullptr : flat<uint64_t>(tensor(a[3], "bias"), "bias", at::kUInt64, dev, {n});
+        const uint64_t* table = nullptr;
+        int64_t table_len = 0, offset = 0;
+        if (a[4] != Py_None) {
+            const at::Tensor& t = tensor(a[4], "table");
+            table = table_of(t, "table", dev);
+            table_len = t.numel();
+            offset = a[5] == Py_None ? table_len / 2 : number(a[5]);
+        }
+        Rows residual;
+        if (a[6] != Py_None) {
+            residual = rows(tensor(a[6], "residual"), "residual", n, dev);
+            if (residual.n != in.n)
+                refuse("residual: " + std::to_string(residual.n) + " rows, " + std::to_string(in.n) + " are wanted");
+        }
+        const at::Tensor out = output(a[7], {in.n, n}, dev);
+        done(zkie2_q4_project(in.data, in.stride, in.n, packed, k, n, (uint32_t)w[4], w[5], shift, bias, table, table_len,
+                              offset, residual.data, residual.stride, static_cast<uint64_t*>(out.data_ptr()),
+                              word(a[8], dev), stream(dev)), "zkie2_q4_project");
+        return THPVariable_Wrap(out);
+    });
+}
+
+// attend(q, (device, k, v, lens, batch, heads, dk, dv, capacity), table, k, v, q_scale, k_scale, score_scale, offset,
+//        out_shift, out, err)
+PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 12) refuse("attend: 12 arguments");
+        const at::Tensor& q = tensor(a[0], "q");
+        const int dev = device_of(q, "q");
+        PyObject* c = a[1];
+        auto* ck = static_cast<int32_t*>(address(PyTuple_GET_ITEM(c, 1)));
+        auto* cv = static_cast<int32_t*>(address(PyTuple_GET_ITEM(c, 2)));
+        const auto* lens = static_cast<const int32_t*>(address(PyTuple_GET_ITEM(c, 3)));
+        const int64_t batch = number(PyTuple_GET_ITEM(c, 4)), heads = number(PyTuple_GET_ITEM(c, 5)),
+                      dk = number(PyTuple_GET_ITEM(c, 6)), dv = number(PyTuple_GET_ITEM(c, 7)),
+                      cap = number(PyTuple_GET_ITEM(c, 8));
+        const int64_t cols = q.dim() == 2 ? q.size(1) : 0;
+        if (cols == 0 || cols % (heads * dk) || cols / dk > 65535)
+            refuse("q: a row per sequence of a multiple of " + std::to_string(heads * dk) + " columns is wanted, not " + said(q));
+        const Rows in = rows(q, "q", cols, dev);
+        if (in.n != batch || (a[3] == Py_None) != (a[4] == Py_None) || number(PyTuple_GET_ITEM(c, 0)) != dev)
+            refuse("attend: a row per sequence, k and v together, and the cache's device are wanted");
+        Rows k, v;
+        if (a[3] != Py_None) {
+            k = rows(tensor(a[3], "k"), "k", heads * dk, dev);
+            v = rows(tensor(a[4], "v"), "v", heads * dv, dev);
+            if (k.n != batch || v.n != batch) refuse("attend: a row of k and v per sequence is wanted");
+        }
+        const at::Tensor& t = tensor(a[2], "table");
+        const uint64_t* table = table_of(t, "table", dev);
+        const Scale qs = scale(a[5], "q_scale"), ks = scale(a[6], "k_scale"), ss = scale(a[7], "score_scale");
+        const int64_t offset = a[8] == Py_None ? t.numel() : number(a[8]);
+        const uint32_t out_shift = shift_of(a[9], "out_shift");
+        const at::Tensor out = output(a[10], {batch, cols / dk * dv}, dev);
+        done(zkie2_kv_attend(in.data, in.stride, cols / dk, qs.factor, qs.shift, k.data, k.stride, v.data, v.stride, ks.factor,
+                             ks.shift, ck, cv, lens, batch, heads, dk, dv, cap, ss.factor, ss.shift, table, t.numel(), offset,
+                             out_shift, static_cast<uint64_t*>(out.data_ptr()), word(a[11], dev), stream(dev)),
+             "zkie2_kv_attend");
+        return THPVariable_Wrap(out);
+    });
+}
+
+// moe(x, (device, h, experts, top_k, f, shared_f, group, router, weights, exp, exp_len, silu, silu_len, shift), residual,
+//     out, err) -> (out, gate)
+PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 5) refuse("moe: 5 arguments");
+        const at::Tensor& x = tensor(a[0], "x");
+        const int dev = device_of(x, "x");
+        auto item = [&](int i) { return PyTuple_GET_ITEM(a[1], i); };
+        const int64_t h = number(item(1)), experts = number(item(2)), top_k = number(item(3)), f = number(item(4)),
+                      shared_f = number(item(5)), group = number(item(6));
+        const Rows in = rows(x, "x", h, dev);
+        if (in.n > 65535 || number(item(0)) != dev) refuse("MoeBlock: at most 65535 rows, on the weights' device, are wanted");
+        Rows residual;
+        if (a[2] != Py_None) {
+            residual = rows(tensor(a[2], "residual"), "residual", h, dev);
+            if (residual.n != in.n)
+                refuse("residual: " + std::to_string(residual.n) + " rows, " + std::to_string(in.n) + " are wanted");
+        }
+        const at::Tensor out = output(a[3], {in.n, h}, dev), gate = make({in.n, experts}, at::kUInt64, dev);
+        // this call's own: calls on other streams may run beside it
+        const uint64_t elems = zkie2_moe_rows_scratch_elems(in.n, h, experts, top_k, f, shared_f, (uint32_t)group);
+        const at::Tensor scratch = make({(int64_t)elems + 1}, at::kLong, dev);
+        done(zkie2_moe_rows(in.data, in.stride, in.n, h, experts, top_k, f, shared_f, (uint32_t)group,
+                            static_cast<const uint32_t*>(address(item(7))),
+                            static_cast<const uint32_t* const*>(address(item(8))), static_cast<const uint64_t*>(address(item(9))),
+                            number(item(10)), static_cast<const uint64_t*>(address(item(11))), number(item(12)),
+                            (uint32_t)number(item(13)), residual.data, residual.stride, static_cast<uint64_t*>(out.data_ptr()),
+                            static_cast<uint64_t*>(gate.data_ptr()), word(a[4], dev), static_cast<uint64_t*>(scratch.data_ptr()),
+                            stream(dev)), "zkie2_moe_rows");
+        return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(gate));
+    });
+}
+
+// choose(logits, history, history_lens, (pos, neg), presence, frequency, bias, allowed, mask_value, out, err) -> (token, out)
+PyObject* choose(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 11) refuse("choose: 11 arguments");
+        const at::Tensor& x = tensor(a[0], "logits");
+        const int dev = device_of(x, "logits");
+        if (x.dim() != 2 || x.size(1) == 0 || x.size(0) > 65535 || x.size(1) > 0x7FFFFFFF)
+            refuse("logits: at most 65535 rows of a vocabulary are wanted, not " + said(x));
+        const int64_t b = x.size(0), v = x.size(1), words = (v + 31) / 32;
+        const auto* logits = flat<uint64_t>(x, "logits", at::kUInt64, dev, {b, v});
+        const int32_t *history = nullptr, *lens = nullptr;
+        int64_t tokens = 0;
+        if (a[1] != Py_None) {
+            const at::Tensor& t = tensor(a[1], "history");
+            if (t.dim() != 2 || t.size(0) != b) refuse("history: " + std::to_string(b) + " rows of tokens are wanted, not " + said(t));
+            tokens = t.size(1);
+            history = flat<int32_t>(t, "history", at::kInt, dev, {b, tokens});
+            if (a[2] != Py_None) lens = flat<int32_t>(tensor(a[2], "history_lens"), "history_lens", at::kInt, dev, {b});
+        } else if (a[2] != Py_None) {
+            refuse("choose_token: history_lens without a history");
+        }
+        if (!PyTuple_Check(a[3]) || PyTuple_GET_SIZE(a[3]) != 2) refuse("repeat: two factors are wanted");
+        const uint64_t* bias = nullptr;
+        int64_t bias_stride = 0, allowed_stride = 0;
+        if (a[6] != Py_None) {
+            const at::Tensor& t = tensor(a[6], "bias");
+            bias_stride = t.dim() == 1 ? 0 : v;
+            bias = bias_stride ? flat<uint64_t>(t, "bias", at::kUInt64, dev, {b, v}) : flat<uint64_t>(t, "bias", at::kUInt64, dev, {v});
+        }
+        const uint32_t* allowed = nullptr;
+        if (a[7] != Py_None) {
+            const at::Tensor& t = tensor(a[7], "allowed");
+            allowed_stride = t.dim() == 1 ? 0 : words;
+            allowed = reinterpret_cast<const uint32_t*>(allowed_stride ? flat<int32_t>(t, "allowed", at::kInt, dev, {b, words})
+                                                                       : flat<int32_t>(t, "allowed", at::kInt, dev, {words}));
+        }
+        const at::Tensor out = output(a[9], {b, v}, dev), token = make({b}, at::kUInt32, dev);
+        if (b && out.data_ptr() == x.data_ptr()) refuse("choose_token: out may not be the logits");
+        done(zkie2_choose_token(logits, b, v, history, tokens, lens, number(PyTuple_GET_ITEM(a[3], 0)),
+                                number(PyTuple_GET_ITEM(a[3], 1)), number(a[4]), number(a[5]), bias, bias_stride, allowed,
+                                allowed_stride, number(a[8]), static_cast<uint64_t*>(out.data_ptr()),
+                                static_cast<uint32_t*>(token.data_ptr()), word(a[10], dev), stream(dev)), "zkie2_choose_token");
+        return Py_BuildValue("(NN)", THPVariable_Wrap(token), THPVariable_Wrap(out));
+    });
+}
+
+PyMethodDef methods[] = {
+    {"project", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(project)), METH_FASTCALL, nullptr},
+    {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
+    {"moe", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(moe)), METH_FASTCALL, nullptr},
+    {"choose", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(choose)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }

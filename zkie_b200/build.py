@@ -3,7 +3,9 @@
 Every .cu / .cpp under zkie_b200/csrc is compiled to an object under
 zkie_b200/_build (incrementally, in parallel) and linked with the static CUDA
 runtime into zkie_b200/libzkie_b200.so.  The shared object travels with the
-source tree; nothing is JIT-compiled at import time.
+source tree; nothing is JIT-compiled at import time.  zkie_b200/_calls.so, the Python
+binding of the per-token calls (binding/calls.cpp, over torch's headers), is
+built beside it and finds the library by its own place.
 """
 import concurrent.futures as cf
 import os
@@ -16,6 +18,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libzkie_b200.so")
+BINDING = os.path.join(HERE, "binding", "calls.cpp")
+CALLS = os.path.join(HERE, "_calls.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -69,6 +73,26 @@ def _compile(src: str, obj: str, verbose_ptxas: bool) -> str:
     return res.stderr
 
 
+def build_calls(force: bool = False):
+    """The Python extension zkie_b200._calls (after the library it links)."""
+    newest = max(os.path.getmtime(f) for f in (BINDING, os.path.join(INCLUDE, "zkie2.h")))
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
+        return
+    import sysconfig
+    import torch
+    base = os.path.dirname(torch.__file__)
+    inc = [sysconfig.get_paths()["include"], os.path.join(base, "include"),
+           os.path.join(base, "include", "torch", "csrc", "api", "include"), os.path.join(os.path.dirname(nvcc()), "..", "include")]
+    tmp = CALLS + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *["-I" + d for d in inc], BINDING, "-o", tmp, "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda", "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING}:\n{res.stderr}")
+    os.replace(tmp, CALLS)
+
+
 def build(force: bool = False, verbose_ptxas: bool = False, jobs: int = 8) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cpp")))
@@ -92,6 +116,7 @@ def build(force: bool = False, verbose_ptxas: bool = False, jobs: int = 8) -> st
         cmd = [nvcc()] + ARCH + ["-shared", "--cudart", "static", "-o", tmp] + objs + ["-ldl"]
         subprocess.check_call(cmd)
         os.replace(tmp, LIB)
+    build_calls(force)
     if verbose_ptxas:
         for s, log in logs:
             sys.stderr.write(f"== {os.path.basename(s)}\n{log}")

@@ -24,17 +24,16 @@ likes (``check_err``); not given, the call reads its own, which synchronises,
 and raises ValueError.  Besides the op layer's bits, 8 is a value outside the
 32-bit range the kernels take (computed on as zero) and 16 a full cache.
 """
+import ctypes as C
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
+from . import _calls  # after the library it links
 from .compose import _INDEX_WRITERS, _check_err, _err_word
 from .device import P, device
-
-_q4_project, _kv_attend, _moe_rows = lib.zkie2_q4_project, lib.zkie2_kv_attend, lib.zkie2_moe_rows
-_choose = lib.zkie2_choose_token
 
 GROUPS = (32, 64, 128)
 KV_BLOCK = 32
@@ -46,10 +45,7 @@ def check_err(err: torch.Tensor, what: str = "decode"):
     _check_err(err, what)
 
 
-# A step makes a call per operator and layer, each of a few microseconds on the
-# device, so the checks below are written to cost less than that.
 _U64, _I32 = torch.uint64, torch.int32
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _stream() -> int:
@@ -58,53 +54,19 @@ def _stream() -> int:
 
 def _device_of(t, name: str) -> int:
     """The index of the device that ``t`` and the call are on."""
-    if isinstance(t, torch.Tensor):
-        dev = t.get_device()
-        if dev >= 0 and dev == _current_device():
-            return dev
-    _refuse(t, name, None, "a tensor on the current CUDA device")
-
-
-def _refuse(t, name: str, dtype, what: str):
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name}: {what} is wanted, not {type(t).__name__}")
-    if not t.is_cuda or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{name}: {what} is wanted{'' if dtype is None else f' ({dtype}, CUDA)'}, not {t.dtype} on "
-                         f"{t.device}")
-    if t.get_device() != _current_device():
-        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{_current_device()}")
-    raise ValueError(f"{name}: {what} is wanted, not shape {tuple(t.shape)} with strides {t.stride()}")
-
-
-def _rows(t, name: str, cols: int, dev: int) -> Tuple[int, int]:
-    """(rows, row stride) of a matrix of field elements with rows of ``cols``
-    numbers of unit stride that do not overlap."""
-    if isinstance(t, torch.Tensor) and t.dtype is _U64 and t.get_device() == dev:
-        shape = t.shape
-        if len(shape) == 2 and shape[1] == cols:
-            s0, s1 = t.stride()
-            if (s1 == 1 or cols == 1) and (s0 >= cols or shape[0] < 2):
-                return shape[0], s0
-    _refuse(t, name, _U64, f"a matrix of {cols} columns, unit stride within its rows,")
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == torch.cuda.current_device():
+        return t.get_device()
+    what = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise ValueError(f"{name}: a tensor on the current CUDA device is wanted, not {what}")
 
 
 def _flat(t, name: str, dtype, dev: int, shape=None) -> torch.Tensor:
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and \
-            (shape is None or t.shape == shape):
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == dev and t.is_contiguous() and \
+            (shape is None or tuple(t.shape) == tuple(shape)):
         return t
-    _refuse(t, name, dtype, "a contiguous tensor" + ("" if shape is None else f" of shape {tuple(shape)}"))
-
-
-def _word(err: Optional[torch.Tensor], dev: int) -> torch.Tensor:
-    if err is None:
-        return _err_word()
-    if err.dtype is _I32 and err.get_device() == dev and err.numel() == 1:
-        return err
-    _refuse(err, "err", _I32, "an int32 word")
-
-
-def _out(out, like: torch.Tensor, shape, dev: int) -> torch.Tensor:
-    return like.new_empty(shape) if out is None else _flat(out, "out", _U64, dev, shape)
+    what = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise ValueError(f"{name}: a contiguous {dtype} tensor{'' if shape is None else f' of shape {tuple(shape)}'} on the "
+                     f"call's device is wanted, not {what}")
 
 
 def _signed(t: torch.Tensor) -> torch.Tensor:
@@ -207,6 +169,7 @@ class QuantWeight:
         dev = codes.device
         self.packed = torch.empty(words, dtype=torch.int32, device=dev)
         self.device, self.pointer = self.packed.get_device(), self.packed.data_ptr()
+        self.call = (self.device, self.pointer, self.k, self.n, group, segment, self.experts)
         err = _err_word()
         check(lib.zkie2_q4_pack(codes.data_ptr(), scales.data_ptr(), self.experts, self.k, self.n, group, segment,
                                 self.packed.data_ptr(), err.data_ptr(), _stream()), "zkie2_q4_pack")
@@ -249,30 +212,8 @@ def project(x: torch.Tensor, weight: QuantWeight, shift: int, *, bias: Optional[
     then ``table[clamp(y + offset, 0, len - 1)]`` (GeluIndex and Lookup; offset
     defaults to the table's middle) and ``+ residual`` (m x n; Add) where
     given.  shift 0 without a bias is the MatMul arm.  |x| <= 0x7F7F7F7F."""
-    dev = _device_of(x, "x")
-    n = weight.n
-    m, ldx = _rows(x, "x", weight.k, dev)
-    if weight.experts != 1 or weight.device != dev:
-        raise ValueError("project: one weight (no stack of experts) on the current device is wanted")
-    if not 0 <= shift <= 62 or m > 65535:
-        raise ValueError("project: shift 0 .. 62 and at most 65535 rows are wanted")
-    p_bias = p_table = p_residual = None
-    table_len = ldr = 0
-    if bias is not None:
-        p_bias = _flat(bias, "bias", _U64, dev, (n,)).data_ptr()
-    if table is not None:
-        p_table, table_len = _flat(table, "table", _U64, dev).data_ptr(), table.numel()
-        if table_len == 0:
-            raise ValueError("project: an empty table")
-    if residual is not None:
-        rows, ldr = _rows(residual, "residual", n, dev)
-        if rows != m:
-            raise ValueError(f"residual: {rows} rows, {m} are wanted")
-        p_residual = residual.data_ptr()
-    out, word = _out(out, x, (m, n), dev), _word(err, dev)
-    check(_q4_project(x.data_ptr(), ldx, m, weight.pointer, weight.k, n, weight.group, weight.segment, shift, p_bias,
-                      p_table, table_len, table_len // 2 if offset is None else offset, p_residual, ldr, out.data_ptr(),
-                      word.data_ptr(), _raw_stream(dev)), "zkie2_q4_project")
+    word = _err_word() if err is None else err
+    out = _calls.project(x, weight.call, shift, bias, table, offset, residual, out, word)
     if err is None:
         _check_err(word, "project")
     return out
@@ -308,8 +249,8 @@ class KvCache:
         if (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("KvCache: 16-byte aligned buffers are wanted")
         self.k, self.v, self.lens = k, v, lens
-        self._args = (k.data_ptr(), v.data_ptr(), lens.data_ptr(), self.batch, self.heads, self.dk, self.dv,
-                      self.capacity)
+        self.call = (dev, k.data_ptr(), v.data_ptr(), lens.data_ptr(), self.batch, self.heads, self.dk, self.dv,
+                     self.capacity)
 
     @classmethod
     def zeros(cls, batch: int, heads: int, dk: int, dv: int, capacity: int,
@@ -330,14 +271,14 @@ class KvCache:
         shift).  |key| <= 2^27, values in 32 bits."""
         dev = _device_of(k, "k")
         for name, t, cols in (("k", k, self.heads * self.dk), ("v", v, self.heads * self.dv)):
-            if t.dtype is not _U64 or t.get_device() != dev or t.dim() != 3 or t.shape[0] != self.batch or \
-                    t.shape[1] != k.shape[1] or t.shape[2] != cols:
-                _refuse(t, name, _U64, f"a tensor of {self.batch} sequences, as many tokens each and {cols} columns,")
+            if not isinstance(t, torch.Tensor) or t.dtype != _U64 or t.get_device() != dev or t.dim() != 3 or \
+                    tuple(t.shape) != (self.batch, k.shape[1], cols):
+                raise ValueError(f"{name}: uint64 ({self.batch}, tokens, {cols}), as many tokens of k and v, is wanted")
         if self.device != dev or k.shape[1] > 1 << 17 or not 0 <= k_scale[1] <= 62:
             raise ValueError("append: the cache's device, at most 131072 tokens and a shift 0 .. 62 are wanted")
-        k, v, word = k.contiguous(), v.contiguous(), _word(err, dev)
+        k, v, word = k.contiguous(), v.contiguous(), _err_word() if err is None else _flat(err, "err", _I32, dev)
         check(lib.zkie2_kv_append(k.data_ptr(), k.shape[2], v.data_ptr(), v.shape[2], k.shape[1], *k_scale,
-                                  *self._args, word.data_ptr(), _raw_stream(dev)), "zkie2_kv_append")
+                                  *self.call[1:], word.data_ptr(), _stream()), "zkie2_kv_append")
         if err is None:
             _check_err(word, "append")
 
@@ -367,31 +308,8 @@ def attend(q: torch.Tensor, cache: KvCache, table: torch.Tensor, *, k: Optional[
     table[0] each in its softmax's sum: the rows agree where that is zero, as
     in the models' tables.  A sequence without tokens answers zeros.  Scaled
     queries and keys |q|, |k| <= 2^27; table values in [0, 2^31)."""
-    dev = _device_of(q, "q")
-    batch, one, dk, dv = cache.batch, cache.heads, cache.dk, cache.dv
-    cols = q.shape[-1]
-    heads = cols // dk
-    if cols == 0 or cols % (one * dk) or heads > 65535:
-        raise ValueError(f"q: {cols} columns, a multiple of {one * dk} is wanted")
-    rows, ldq = _rows(q, "q", cols, dev)
-    if rows != batch or (k is None) != (v is None) or cache.device != dev:
-        raise ValueError("attend: a row per sequence, k and v together, and the cache's device are wanted")
-    p_k = p_v = None
-    ldk = ldv = 0
-    if k is not None:
-        rk, ldk = _rows(k, "k", one * dk, dev)
-        rv, ldv = _rows(v, "v", one * dv, dev)
-        if rk != batch or rv != batch:
-            raise ValueError("attend: a row of k and v per sequence is wanted")
-        p_k, p_v = k.data_ptr(), v.data_ptr()
-    table_len = _flat(table, "table", _U64, dev).numel()
-    if table_len == 0 or not (0 <= q_scale[1] <= 62 and 0 <= k_scale[1] <= 62 and 0 <= score_scale[1] <= 62 and
-                              0 <= out_shift <= 62):
-        raise ValueError("attend: a table and shifts 0 .. 62 are wanted")
-    out, word = _out(out, q, (batch, heads * dv), dev), _word(err, dev)
-    check(_kv_attend(q.data_ptr(), ldq, heads, *q_scale, p_k, ldk, p_v, ldv, *k_scale, *cache._args, *score_scale,
-                     table.data_ptr(), table_len, table_len if offset is None else offset, out_shift, out.data_ptr(),
-                     word.data_ptr(), _raw_stream(dev)), "zkie2_kv_attend")
+    word = _err_word() if err is None else err
+    out = _calls.attend(q, cache.call, table, k, v, q_scale, k_scale, score_scale, offset, out_shift, out, word)
     if err is None:
         _check_err(word, "attend")
     return out
@@ -435,10 +353,8 @@ class MoeBlock:
         _check_err(err, "MoeBlock: router")
         self.packed = (self._pair(gate, up), down.packed, self._pair(shared_gate, shared_up), shared_down.packed)
         self._packed = (_lib.vp * 4)(*[w.data_ptr() for w in self.packed])
-        self._shape = (h, e, top_k, f, s, self.group)
-        self._args = (self.router.data_ptr(), self._packed, exp_table.data_ptr(), exp_table.numel(),
-                      silu_table.data_ptr(), silu_table.numel(), shift)
-        self._scratch = {}  # elements by rows
+        self.call = (dev, h, e, top_k, f, s, self.group, self.router.data_ptr(), C.addressof(self._packed),
+                     exp_table.data_ptr(), exp_table.numel(), silu_table.data_ptr(), silu_table.numel(), shift)
 
     @staticmethod
     def _pair(a: QuantWeight, b: QuantWeight) -> torch.Tensor:
@@ -453,27 +369,11 @@ class MoeBlock:
         """(out, gate) of the rows of x (m x h, m <= 65535; two launches to 16
         rows): the layer's output (+ residual where given) and TopKSelect's
         gate (m x experts).  |x| and |silu(gate) up| <= 0x7F7F7F7F."""
-        dev = _device_of(x, "x")
-        m, ldx = _rows(x, "x", self.h, dev)
-        if m > 65535 or self.device != dev:
-            raise ValueError("MoeBlock: at most 65535 rows, on the weights' device, are wanted")
-        p_residual, ldr = None, 0
-        if residual is not None:
-            rows, ldr = _rows(residual, "residual", self.h, dev)
-            if rows != m:
-                raise ValueError(f"residual: {rows} rows, {m} are wanted")
-            p_residual = residual.data_ptr()
-        out, word = _out(out, x, (m, self.h), dev), _word(err, dev)
-        gate = x.new_empty((m, self.experts))
-        elems = self._scratch.get(m)
-        if elems is None:
-            elems = self._scratch[m] = max(lib.zkie2_moe_rows_scratch_elems(m, *self._shape), 1)
-        scratch = x.new_empty(elems)  # this call's own: calls on other streams may run beside it
-        check(_moe_rows(x.data_ptr(), ldx, m, *self._shape, *self._args, p_residual, ldr, out.data_ptr(),
-                        gate.data_ptr(), word.data_ptr(), scratch.data_ptr(), _raw_stream(dev)), "zkie2_moe_rows")
+        word = _err_word() if err is None else err
+        both = _calls.moe(x, self.call, residual, out, word)
         if err is None:
             _check_err(word, "MoeBlock")
-        return out, gate
+        return both
 
 
 # ---- the next token -----------------------------------------------------------------------------------
@@ -495,35 +395,8 @@ def choose_token(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     - ``+ mask_value`` where bit v % 32 of word v / 32 of ``allowed`` (int32
       words, ceil(vocab / 32), or batch x that) is clear.  With the graph's
       mask value a row that allows nothing still has a maximum."""
-    dev = _device_of(logits, "logits")
-    if logits.dim() != 2 or logits.shape[1] == 0 or logits.shape[0] > 65535 or logits.shape[1] > 0x7FFFFFFF:
-        raise ValueError(f"logits: shape {tuple(logits.shape)}, at most 65535 rows of a vocabulary are wanted")
-    b, v = logits.shape
-    _flat(logits, "logits", _U64, dev)
-    p_bias = p_allowed = p_history = p_lens = None
-    bias_stride = allowed_stride = tokens = 0
-    if bias is not None:
-        bias_stride = 0 if bias.dim() == 1 else v
-        p_bias = _flat(bias, "bias", _U64, dev, (b, v) if bias_stride else (v,)).data_ptr()
-    if allowed is not None:
-        words = (v + 31) // 32
-        allowed_stride = 0 if allowed.dim() == 1 else words
-        p_allowed = _flat(allowed, "allowed", _I32, dev, (b, words) if allowed_stride else (words,)).data_ptr()
-    if history is not None:
-        if history.dim() != 2 or history.shape[0] != b:
-            raise ValueError(f"history: shape {tuple(history.shape)}, {b} rows of tokens are wanted")
-        p_history, tokens = _flat(history, "history", _I32, dev).data_ptr(), history.shape[1]
-        if history_lens is not None:
-            p_lens = _flat(history_lens, "history_lens", _I32, dev, (b,)).data_ptr()
-    elif history_lens is not None:
-        raise ValueError("choose_token: history_lens without a history")
-    out, word = _out(out, logits, (b, v), dev), _word(err, dev)
-    if out is logits or (b and out.data_ptr() == logits.data_ptr()):
-        raise ValueError("choose_token: out may not be the logits")
-    token = logits.new_empty(b, dtype=torch.uint32)
-    check(_choose(logits.data_ptr(), b, v, p_history, tokens, p_lens, *repeat, presence, frequency, p_bias, bias_stride,
-                  p_allowed, allowed_stride, mask_value, out.data_ptr(), token.data_ptr(), word.data_ptr(),
-                  _raw_stream(dev)), "zkie2_choose_token")
+    word = _err_word() if err is None else err
+    both = _calls.choose(logits, history, history_lens, repeat, presence, frequency, bias, allowed, mask_value, out, word)
     if err is None:
         _check_err(word, "choose_token")
-    return token, out
+    return both
