@@ -70,7 +70,8 @@ def test_quantise_is_nearest(zk):
 @pytest.mark.parametrize("m,k,n,group,segment,shift", [
     (1, 1, 1, 32, 0, 0), (1, 64, 16, 64, 0, 16), (2, 100, 17, 32, 0, 8), (3, 130, 300, 128, 0, 16),
     (4, 768, 64, 64, 64, 16), (5, 60, 33, 64, 20, 7), (8, 1024, 192, 128, 128, 16), (9, 200, 40, 32, 0, 1),
-    (17, 96, 50, 64, 32, 16), (8, 4100, 20, 64, 0, 16), (3, 8192, 31, 128, 0, 0), (1, 2048, 5000, 32, 0, 16)])
+    (17, 96, 50, 64, 32, 16), (8, 4100, 20, 64, 0, 16), (3, 8192, 31, 128, 0, 0), (1, 2048, 5000, 32, 0, 16),
+    (2, 40, 45000, 64, 0, 3), (5, 260, 4000, 128, 0, 16), (3, 512, 2400, 128, 256, 9)])
 def test_project(zk, m, k, n, group, segment, shift):
     rng = np.random.default_rng(m * k + n)
     w = ref.weight(rng, k, n, group, segment)
@@ -99,6 +100,24 @@ def test_project_epilogue_and_strides(zk, offset):
     assert got is out
     want = ref.project(x, *w, 32, 0, 20, table=table, offset=500 if offset is None else offset, residual=res)
     assert np.array_equal(_s(got), want)
+
+
+def test_project_odd_rows(zk):
+    """Rows that start at odd places (8-byte aligned only) and none at all."""
+    import torch
+    rng = np.random.default_rng(12)
+    w, wide = ref.weight(rng, 130, 40, 64), rng.integers(-(1 << 20), 1 << 20, (6, 133))
+    q, u = _quant(zk, w, 64), _u(wide)
+    for off in (0, 1, 2, 3):
+        got = zk.decode.project(u[:, off:off + 130], q, 12)
+        assert np.array_equal(_s(got), ref.project(wide[:, off:off + 130], *w, 64, 0, 12))
+    got = zk.decode.project(u[1::2, 1:131], q, 12)
+    assert np.array_equal(_s(got), ref.project(wide[1::2, 1:131], *w, 64, 0, 12))
+    assert zk.decode.project(u[:0, :130], q, 12).shape == (0, 40)
+    with pytest.raises(ValueError, match="unit stride"):
+        zk.decode.project(torch.as_strided(u, (3, 130), (133, 2)), q, 12)
+    with pytest.raises(ValueError, match="unit stride"):
+        zk.decode.project(torch.as_strided(u, (3, 130), (7, 1)), q, 12)
 
 
 def test_project_extremes(zk):
@@ -138,6 +157,8 @@ def _cache(zk, rng, b, hk, dk, dv, cap, lens, big=False):
     (1, 1, 1, 4, 4, 32, [0]), (1, 2, 1, 64, 64, 64, [31]), (3, 2, 1, 64, 64, 96, [32, 0, 95]),
     (2, 3, 2, 40, 24, 320, [33, 300]), (2, 1, 3, 16, 100, 64, [5, 63]), (1, 2, 4, 128, 128, 2048, [2000]),
     (1, 1, 9, 8, 12, 160, [129]), (2, 2, 1, 192, 128, 512, [511, 256]), (1, 1, 1, 256, 256, 992, [700]),
+    (1, 1, 2, 36, 132, 128, [70]), (1, 2, 5, 4, 200, 96, [65]), (1, 1, 4, 8, 8, 131072, [131071]),
+    (1, 1, 1, 16, 4, 131072, [100003]),
     (40, 5, 1, 16, 16, 64, list(range(40)))])
 def test_attend(zk, b, hk, each, dk, dv, cap, lens):
     rng = np.random.default_rng(dk + cap + b)
@@ -161,6 +182,30 @@ def test_attend(zk, b, hk, each, dk, dv, cap, lens):
     cache.advance()
     again = zk.decode.attend(rows[:, :heads * dk], cache, _u(table), q_scale=(23170, 16), score_scale=scale)
     assert np.array_equal(_s(again), want)  # the same tokens, now from the cache alone
+
+
+def test_attend_far_into_a_large_cache(zk):
+    """A cache of more than 2^32 numbers: the last heads' keys and values."""
+    import torch
+    rng = np.random.default_rng(14)
+    hk, dk, dv, cap, n = 130, 256, 4, 131072, 40
+    cache = zk.decode.KvCache.zeros(1, hk, dk, dv, cap)
+    assert cache.k.numel() > 1 << 32
+    keys, values = rng.integers(-(1 << 19), 1 << 19, (hk, 64, dk)), rng.integers(-(1 << 19), 1 << 19, (hk, 64, dv))
+    cache.k[0, :, cap // 32 - 2:] = _i32(ref.blocks_of(keys))
+    cache.v[0, :, cap - 64:] = _i32(values)
+    cache.lens.fill_(cap - 1)
+    q, nk, nv = (rng.integers(-(1 << 18), 1 << 18, (1, hk * d)) for d in (dk, dk, dv))
+    table = _exp_table()
+    got = _s(zk.decode.attend(_u(q), cache, _u(table), k=_u(nk), v=_u(nv), score_scale=(4096, 32))).reshape(hk, dv)
+    for h in (0, 63, hk - 1):
+        full_k, full_v = np.zeros((cap, dk), dtype=np.int64), np.zeros((cap, dv), dtype=np.int64)
+        full_k[-64:], full_v[-64:] = keys[h], values[h]
+        full_k[-1], full_v[-1] = nk.reshape(hk, dk)[h], nv.reshape(hk, dv)[h]
+        z = ref.round_shift((full_k @ q.reshape(hk, dk)[h]) * 4096, 32)
+        want = ref.round_shift(ref.softmax(z, table) @ full_v, 16)
+        assert np.array_equal(got[h], want), h
+    assert torch.equal(cache.v[0, :, cap - 1].cpu(), torch.from_numpy(nv.reshape(hk, dv).astype(np.int32)))
 
 
 def test_attend_inactive_empty_and_full(zk):
@@ -249,7 +294,8 @@ def _moe_block(zk, router, w, group, top_k, exp_table, silu):
 
 @pytest.mark.parametrize("m,h,experts,top_k,f,shared,group", [
     (1, 16, 1, 1, 8, 8, 32), (1, 64, 8, 2, 48, 96, 64), (3, 100, 17, 3, 40, 33, 32), (8, 256, 33, 6, 64, 128, 128),
-    (16, 130, 64, 6, 70, 50, 64), (17, 64, 4, 4, 32, 16, 32), (40, 48, 20, 5, 20, 24, 64), (5, 1000, 200, 16, 24, 40, 128)])
+    (16, 130, 64, 6, 70, 50, 64), (17, 64, 4, 4, 32, 16, 32), (40, 48, 20, 5, 20, 24, 64), (5, 1000, 200, 16, 24, 40, 128),
+    (16, 70, 40, 16, 24, 20, 32), (3, 8192, 5, 2, 16, 20, 64), (2, 64, 4, 2, 8192, 8190, 128), (7, 40, 256, 9, 600, 5, 64)])
 def test_moe_block(zk, m, h, experts, top_k, f, shared, group):
     rng = np.random.default_rng(m + h)
     router, w = _moe_case(rng, h, experts, f, shared, group)
@@ -330,6 +376,10 @@ def test_choose_token_ties_empty_masks_and_bad_history(zk):
     assert int(err.item()) == 1 and np.array_equal(_s(out), want) and tok.tolist() == want_tok.tolist() == [0, 4999]
     with pytest.raises(ValueError, match="index"):
         zk.decode.choose_token(_u(logits), _i32(hist))
+    # no history, and rows that are none
+    empty = zk.decode.choose_token(_u(logits), _i32(np.zeros((2, 0))), _i32([0, 0]), presence=5)[1]
+    assert np.array_equal(_s(empty), logits)
+    assert zk.decode.choose_token(_u(logits)[:0])[0].shape == (0,)
     # a length past the row is the whole row, a negative one none of it
     got = zk.decode.choose_token(_u(logits), _i32(hist), _i32([-4, 9]), presence=1, err=err)[1]
     assert np.array_equal(_s(got), ref.choose(logits, hist, [0, 3], presence=1)[1])

@@ -262,6 +262,7 @@ PyObject* choose(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             tokens = t.size(1);
             history = flat<int32_t>(t, "history", at::kInt, dev, {b, tokens});
             if (a[2] != Py_None) lens = flat<int32_t>(tensor(a[2], "history_lens"), "history_lens", at::kInt, dev, {b});
+            if (tokens == 0) history = lens = nullptr;  // an empty tensor has no address
         } else if (a[2] != Py_None) {
             refuse("choose_token: history_lens without a history");
         }

@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
         }
         __syncthreads();
     }
-    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
+    patience_end(patience, p.err);
 }
 
 // dynamic shared memory for blocks of `rows` rows and a ring of `run` blocks to a slot
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         }
     }
     if (bad) atomicOr(p.err, kErrRange);
-    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
+    patience_end(patience, p.err);
     __syncthreads();  // the rings are done with
     if (on) {
         long long* to = sums + ((size_t)(warp * step_t + mine) * EACH) * dv;

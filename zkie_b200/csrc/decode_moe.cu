@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
         __syncthreads();
     }
     if (bad) atomicOr(p.err, kErrRange);
-    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
+    patience_end(patience, p.err);
 }
 
 constexpr int kDownDepth = 3;
@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         if (p.residual) f = gl_canon(gl_add(f, gl_canon(__ldg(p.residual + r * p.ldr + n))));
         p.out[r * (uint64_t)p.h + n] = f;
     }
-    if (patience.failed && lane == 0) atomicOr(p.err, kErrWait);
+    patience_end(patience, p.err);
     cluster.sync();  // no block leaves while its sums may still be read
 }
 

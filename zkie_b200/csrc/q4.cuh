@@ -210,6 +210,13 @@ __device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, Pati
     patience.failed = true;
     patience.tries = 64;
 }
+// At a kernel's end: a wait that gave up is told, and the copies that it was
+// for get another ten milliseconds before their shared memory is given away.
+__device__ __forceinline__ void patience_end(const Patience& patience, uint32_t* err) {
+    if (!patience.failed) return;
+    atomicOr(err, kErrWait);
+    for (int i = 0; i < 100; i++) __nanosleep(100000);
+}
 
 // ---- overlap with the kernel before (programmatic dependent launch) --------------------------
 // Every kernel here lets its successor start early and waits, before it reads

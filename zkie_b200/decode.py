@@ -353,6 +353,7 @@ class MoeBlock:
         _check_err(err, "MoeBlock: router")
         self.packed = (self._pair(gate, up), down.packed, self._pair(shared_gate, shared_up), shared_down.packed)
         self._packed = (_lib.vp * 4)(*[w.data_ptr() for w in self.packed])
+        torch.cuda.current_stream().synchronize()  # weights are complete before a call: it reads them at once
         self.call = (dev, h, e, top_k, f, s, self.group, self.router.data_ptr(), C.addressof(self._packed),
                      exp_table.data_ptr(), exp_table.numel(), silu_table.data_ptr(), silu_table.numel(), shift)
 
