@@ -1012,14 +1012,15 @@ int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t
     // Query heads to a block: those that share a key head, up to four (two where a value row is
     // wider than 128: their sums stay in registers), fewer where their scores do not fit.  Blocks
     // to a cluster: enough to fill the device with two to an SM, of four token blocks at least, up
-    // to eight (of clusters of sixteen not enough find room at once: 36 us instead of 25 for 16
-    // heads of 4096 tokens); sixteen only where the scores need it.
+    // to eight, as many as find room at once (264 blocks in clusters of eight, 284 in smaller ones,
+    // but 224 in clusters of sixteen: 36 us instead of 27 for 16 heads of 4096 tokens); sixteen only
+    // where the scores need it.
     const uint32_t blocks = (uint32_t)(capacity / kKvBlock);
     const bool wide = dv > 128;
     for (uint32_t each = p.each >= 3 && !wide ? 4 : p.each >= 2 ? 2 : 1;; each /= 2) {
         const uint64_t rows = batch * heads * ceil_div(p.each, each);
         uint32_t ranks = 1;
-        while (ranks < 8 && rows * ranks * 2 <= 2 * kSms && ranks * 8 <= blocks) ranks *= 2;
+        while (ranks < 8 && rows * ranks * 2 <= (ranks == 4 ? 264 : 284) && ranks * 8 <= blocks) ranks *= 2;
         AttendPlan a = attend_plan(each, ranks, 2, blocks, p.c.dk, p.c.dv);
         for (; a.shared > (a.ranks < 8 ? kAttShared / 2 : kAttShared) && a.ranks < kMaxRanks && a.ranks < blocks;)
             a = attend_plan(each, a.ranks * 2, 2, blocks, p.c.dk, p.c.dv);
