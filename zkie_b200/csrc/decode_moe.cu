@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
         while (next_at == next_end) {
             if (next_first + next_n >= known) return false;
             next_first += next_n;
-            next_n = min(kUpBatch, known - next_first);
+            next_n = min(next_first == early && early < kUpBatch ? kUpBatch - early : kUpBatch, known - next_first);
             next_at = first_block(next_n, warp, kWarps);
             next_end = first_block(next_n, warp + 1, kWarps);
         }
@@ -400,8 +400,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     uint32_t slot = 0, phase = 0;
     bool routed = false;
     auto token_of = [&](bool shared, uint32_t first, uint32_t j) { return shared ? first + j : items.token[first + j]; };
-    // a batch of the block's tiles, n from number `first` on, shared by `warps`: sums into acc
-    auto add_up = [&](uint32_t first, uint32_t n, uint32_t warps) {
+    // a batch of the block's tiles, n from number `first` on, shared by `warps`: sums into acc, from
+    // place `base` on
+    auto add_up = [&](uint32_t first, uint32_t n, uint32_t warps, uint32_t base) {
         uint32_t at = first_block(n, warp, warps);
         const uint32_t end = first_block(n, warp + 1, warps);
         while (at < end) {
@@ -453,40 +454,57 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
 #pragma unroll
                     for (int mat = 0; mat < 2; mat++) {
                         const long long v = sum[mat].finish(q);
-                        if (j < count) acc.add(((i * 2 + mat) * kTile + j) * 16 + g + 8 * (t & 1), v);
+                        if (j < count) acc.add((((base + i) * 2 + mat) * kTile + j) * 16 + g + 8 * (t & 1), v);
                     }
                 }
         }
     };
-    // and from them the activations
+    // and from them the activations, two of a thread at a time: their SiLU entries come together
     auto finish = [&](uint32_t first, uint32_t n) {
-        for (uint32_t o = threadIdx.x; o < n * kTile * 16; o += kThreads) {
-            const uint32_t i = o / (kTile * 16), j = o / 16 % kTile, c = o % 16, u = blockIdx.x + (first + i) * gridDim.x;
-            const bool shared = u < stiles;
-            const uint32_t item = shared ? u / st : (u - stiles) / ft, f = (shared ? u % st : (u - stiles) % ft) * 16 + c;
-            const uint32_t tok0 = shared ? item * kTile : items.first[item];
-            const uint32_t count = shared ? min(kTile, p.m - tok0) : items.count[item];
-            if (j >= count) continue;  // its sums are zero
-            const uint32_t cell = (i * 2 * kTile + j) * 16 + c;
-            const int64_t gi = round_shift(acc.get(cell), p.shift), ui = round_shift(acc.get(cell + kTile * 16), p.shift);
-            acc.clear(cell);
-            acc.clear(cell + kTile * 16);
-            if (f >= (shared ? p.sup.s.n : p.up.s.n)) continue;
-            const int64_t s = fx_to_i64(table_at(p.silu, p.silu_len, gi, (int64_t)(p.silu_len / 2)));
-            uint32_t d;
-            bad |= !q4_digits(round_shift(fx_wmul(s, ui), p.shift), &d);
-            uint8_t* to = (shared ? p.sact + (uint64_t)(tok0 + j) * p.sdown.s.blocks * 256
-                                  : p.act + (uint64_t)items.slot[tok0 + j] * p.down.s.blocks * 256) +
-                          f / 64 * 256 + q4_pos(f % 64);
+        constexpr int kOuts = 2;
+        for (uint32_t o0 = threadIdx.x; o0 < n * kTile * 16; o0 += kThreads * kOuts) {
+            uint8_t* to[kOuts];
+            int64_t up[kOuts];
+            uint64_t silu[kOuts];
 #pragma unroll
-            for (int q = 0; q < 4; q++) to[64 * q] = (uint8_t)(d >> (8 * q));
+            for (int q = 0; q < kOuts; q++) {
+                to[q] = nullptr;
+                const uint32_t o = o0 + q * kThreads;
+                if (o >= n * kTile * 16) continue;
+                const uint32_t i = o / (kTile * 16), j = o / 16 % kTile, c = o % 16, u = blockIdx.x + (first + i) * gridDim.x;
+                const bool shared = u < stiles;
+                const uint32_t v = shared ? u : u - stiles, per = shared ? st : ft, item = v / per, f = (v - item * per) * 16 + c;
+                const uint32_t tok0 = shared ? item * kTile : items.first[item];
+                const uint32_t count = shared ? min(kTile, p.m - tok0) : items.count[item];
+                if (j >= count) continue;  // its sums are zero
+                const uint32_t cell = (i * 2 * kTile + j) * 16 + c;
+                const int64_t gi = round_shift(acc.get(cell), p.shift);
+                up[q] = round_shift(acc.get(cell + kTile * 16), p.shift);
+                acc.clear(cell);
+                acc.clear(cell + kTile * 16);
+                if (f >= (shared ? p.sup.s.n : p.up.s.n)) continue;
+                silu[q] = table_at(p.silu, p.silu_len, gi, (int64_t)(p.silu_len / 2));
+                to[q] = (shared ? p.sact + (uint64_t)(tok0 + j) * p.sdown.s.blocks * 256
+                                : p.act + (uint64_t)items.slot[tok0 + j] * p.down.s.blocks * 256) +
+                        f / 64 * 256 + q4_pos(f % 64);
+            }
+#pragma unroll
+            for (int q = 0; q < kOuts; q++)
+                if (to[q]) {
+                    uint32_t d;
+                    bad |= !q4_digits(round_shift(fx_wmul(fx_to_i64(silu[q]), up[q]), p.shift), &d);
+#pragma unroll
+                    for (int b = 0; b < 4; b++) to[q][64 * b] = (uint8_t)(d >> (8 * b));
+                }
         }
     };
 
-    // ---- the batches; routing beside the first, of the shared experts
-    for (uint32_t first = 0, n = early;; n = min(kUpBatch, known - first)) {
-        const bool routing = first == 0 && !routed;
-        add_up(first, n, routing ? early_warps : kWarps);
+    // ---- the batches; routing beside the first, of the shared experts, whose sums are held to be
+    // finished with the next batch's
+    uint32_t base = 0;
+    for (uint32_t first = 0, n = early;; n = min(kUpBatch - base, known - first)) {
+        const bool routing = !routed;
+        add_up(first, n, routing ? early_warps : kWarps, base);
         if (routing) {
             __syncwarp();
             cluster_wait();
@@ -510,8 +528,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
                 for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
                     reinterpret_cast<uint32_t*>(p.items)[i] = reinterpret_cast<const uint32_t*>(&items)[i];
         }
-        finish(first, n);
         first += n;
+        if (routing && early < kUpBatch && first < known) {
+            base = early;
+            continue;
+        }
+        finish(first - n - base, base + n);
+        base = 0;
         if (first >= known) break;
         __syncthreads();
     }
