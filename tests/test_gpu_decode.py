@@ -383,3 +383,51 @@ def test_choose_token_ties_empty_masks_and_bad_history(zk):
     # a length past the row is the whole row, a negative one none of it
     got = zk.decode.choose_token(_u(logits), _i32(hist), _i32([-4, 9]), presence=1, err=err)[1]
     assert np.array_equal(_s(got), ref.choose(logits, hist, [0, 3], presence=1)[1])
+
+
+# ---- outputs that are given --------------------------------------------------------------------------
+def test_outputs_apart_from_inputs(zk):
+    """An output may be the residual, and shares memory with nothing else that a call reads."""
+    import torch
+    rng = np.random.default_rng(77)
+    m, k = 3, 64
+    w = ref.weight(rng, k, k, 32)
+    q = _quant(zk, w, 32)
+    x, r = rng.integers(-1 << 18, 1 << 18, (m, k)), rng.integers(-1 << 18, 1 << 18, (m, k))
+    want = ref.project(x, *w, 32, 0, 16, residual=r)
+    both = torch.cat([_u(x), _u(r)])
+    out = zk.decode.project(both[:m], q, 16, residual=both[m:], out=both[m:])
+    assert out.data_ptr() == both[m:].data_ptr() and np.array_equal(_s(both[m:]), want)
+    for to in (both[:m], both[1:m + 1]):
+        with pytest.raises(ValueError, match="shares memory"):
+            zk.decode.project(both[:m], q, 16, out=to)
+    with pytest.raises(ValueError, match="shares memory"):
+        zk.decode.project(_u(x), q, 16, residual=both[:m], out=both[1:m + 1])
+    table = _u(_exp_table(10))
+    cache = zk.decode.KvCache.zeros(m, 1, k, k, 32)
+    with pytest.raises(ValueError, match="shares memory"):
+        zk.decode.attend(both[:m], cache, table, out=both[:m])
+    with pytest.raises(ValueError, match="shares memory"):
+        zk.decode.attend(_u(x), cache, table, k=_u(x), v=both[m:], out=both[m:])
+    logits, bias = both[:m], both[m]
+    with pytest.raises(ValueError, match="shares memory"):
+        zk.decode.choose_token(logits, out=logits)
+    with pytest.raises(ValueError, match="shares memory"):
+        zk.decode.choose_token(_u(x), bias=bias, out=both[m:])
+    with pytest.raises(AttributeError):
+        cache.lens = cache.lens + 1
+
+
+def test_moe_output_apart_from_input(zk):
+    rng = np.random.default_rng(78)
+    m, h = 2, 64
+    router, w = _moe_case(rng, h, 4, 32, 32, 32)
+    block = _moe_block(zk, router, w, 32, 2, _exp_table(), _silu_table())
+    x, r = rng.integers(-1 << 17, 1 << 17, (m, h)), rng.integers(-1 << 17, 1 << 17, (m, h))
+    to = _u(r)
+    plain, gate = block.forward(_u(x), residual=_u(r))
+    got, gate2 = block.forward(_u(x), residual=to, out=to)
+    assert np.array_equal(_s(got), _s(plain)) and np.array_equal(_s(gate), _s(gate2))
+    xs = _u(x)
+    with pytest.raises(ValueError, match="shares memory"):
+        block.forward(xs, out=xs)

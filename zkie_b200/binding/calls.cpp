@@ -5,7 +5,7 @@
 // checks and the conversion of 18 to 28 arguments took 5 to 9 us of a call.
 // The C functions are libzkie_b200.so's own (include/zkie2.h).
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <Python.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -101,13 +101,22 @@ Scale scale(PyObject* o, const char* name) {
 }
 
 at::Tensor make(at::IntArrayRef shape, at::ScalarType type, int dev) {
-    return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, dev));
+    return at::Tensor(at::detail::empty_cuda(shape, type, at::Device(at::kCUDA, (at::DeviceIndex)dev), std::nullopt));
 }
 at::Tensor output(PyObject* o, at::IntArrayRef shape, int dev) {
     if (o == Py_None) return make(shape, at::kUInt64, dev);
     const at::Tensor& t = tensor(o, "out");
     flat<uint64_t>(t, "out", at::kUInt64, dev, shape);
     return t;
+}
+// A given output shares no memory with what the blocks of a call read at different times; the
+// residual may be the output itself, each number being read by the thread that writes it.
+void apart(PyObject* given, const at::Tensor& out, const Rows& in, int64_t cols, const char* name, bool same = false) {
+    if (given == Py_None || in.n == 0 || !in.data) return;
+    const auto* a = static_cast<const uint64_t*>(out.data_ptr());
+    const uint64_t *a_end = a + out.numel(), *b_end = in.data + (in.n - 1) * in.stride + cols;
+    if (same && in.data == a && (in.n == 1 || in.stride == cols)) return;
+    if (a < b_end && in.data < a_end) refuse(std::string("out shares memory with ") + name);
 }
 uint32_t* word(PyObject* o, int dev) {
     const at::Tensor& t = tensor(o, "err");
@@ -164,6 +173,8 @@ PyObject* project(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 refuse("residual: " + std::to_string(residual.n) + " rows, " + std::to_string(in.n) + " are wanted");
         }
         const at::Tensor out = output(a[7], {in.n, n}, dev);
+        apart(a[7], out, in, k, "x");
+        apart(a[7], out, residual, n, "the residual (and is not it)", true);
         done(zkie2_q4_project(in.data, in.stride, in.n, packed, k, n, (uint32_t)w[4], w[5], shift, bias, table, table_len,
                               offset, residual.data, residual.stride, static_cast<uint64_t*>(out.data_ptr()),
                               word(a[8], dev), stream(dev)), "zkie2_q4_project");
@@ -203,6 +214,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const int64_t offset = a[8] == Py_None ? t.numel() : number(a[8]);
         const uint32_t out_shift = shift_of(a[9], "out_shift");
         const at::Tensor out = output(a[10], {batch, cols / dk * dv}, dev);
+        apart(a[10], out, in, cols, "q");
+        apart(a[10], out, k, heads * dk, "k");
+        apart(a[10], out, v, heads * dv, "v");
         done(zkie2_kv_attend(in.data, in.stride, cols / dk, qs.factor, qs.shift, k.data, k.stride, v.data, v.stride, ks.factor,
                              ks.shift, ck, cv, lens, batch, heads, dk, dv, cap, ss.factor, ss.shift, table, t.numel(), offset,
                              out_shift, static_cast<uint64_t*>(out.data_ptr()), word(a[11], dev), stream(dev)),
@@ -230,6 +244,8 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 refuse("residual: " + std::to_string(residual.n) + " rows, " + std::to_string(in.n) + " are wanted");
         }
         const at::Tensor out = output(a[3], {in.n, h}, dev), gate = make({in.n, experts}, at::kUInt64, dev);
+        apart(a[3], out, in, h, "x");
+        apart(a[3], out, residual, h, "the residual (and is not it)", true);
         // this call's own: calls on other streams may run beside it
         const uint64_t elems = zkie2_moe_rows_scratch_elems(in.n, h, experts, top_k, f, shared_f, (uint32_t)group);
         const at::Tensor scratch = make({(int64_t)elems + 1}, at::kLong, dev);
@@ -282,7 +298,8 @@ PyObject* choose(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                                                                        : flat<int32_t>(t, "allowed", at::kInt, dev, {words}));
         }
         const at::Tensor out = output(a[9], {b, v}, dev), token = make({b}, at::kUInt32, dev);
-        if (b && out.data_ptr() == x.data_ptr()) refuse("choose_token: out may not be the logits");
+        apart(a[9], out, {logits, b, v}, v, "the logits");
+        apart(a[9], out, {bias, bias_stride ? b : 1, v}, v, "the bias");
         done(zkie2_choose_token(logits, b, v, history, tokens, lens, number(PyTuple_GET_ITEM(a[3], 0)),
                                 number(PyTuple_GET_ITEM(a[3], 1)), number(a[4]), number(a[5]), bias, bias_stride, allowed,
                                 allowed_stride, number(a[8]), static_cast<uint64_t*>(out.data_ptr()),

@@ -86,7 +86,7 @@ def build_calls(force: bool = False):
     tmp = CALLS + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *["-I" + d for d in inc], BINDING, "-o", tmp, "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu",
-           "-lc10", "-lc10_cuda", "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING}:\n{res.stderr}")

@@ -248,9 +248,14 @@ class KvCache:
                              "131072 are wanted")
         if (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("KvCache: 16-byte aligned buffers are wanted")
-        self.k, self.v, self.lens = k, v, lens
+        self._k, self._v, self._lens = k, v, lens
         self.call = (dev, k.data_ptr(), v.data_ptr(), lens.data_ptr(), self.batch, self.heads, self.dk, self.dv,
                      self.capacity)
+
+    # read, and written in place, but not replaced: calls hold their addresses
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    lens = property(lambda self: self._lens)
 
     @classmethod
     def zeros(cls, batch: int, heads: int, dk: int, dv: int, capacity: int,
