@@ -1047,12 +1047,24 @@ int zkie2_choose_token(const uint64_t* d_logits, uint64_t batch, uint64_t vocab,
     if (!d_logits || !d_out || !d_token) return (int)cudaErrorInvalidValue;
     const ChooseArgs p{d_logits, vocab, d_history, history_len, d_history_lens, repeat_pos, repeat_neg, presence,
                        frequency, d_bias, bias_stride, d_allowed, allowed_stride, mask_value, d_out, d_token, d_err};
-    // Blocks to a row: one step of the vocabulary each, fewer once the rows fill the device
-    uint32_t ranks = 1;
-    while (ranks < kMaxRanks && vocab > (uint64_t)ranks * kChooseStep && batch * ranks < 2 * kSms)
-        ranks *= 2;
+    // Blocks to a row: the fewest steps of the vocabulary at which the rows' clusters find room at
+    // once, with up to half as many blocks again where those do too.  A second wave of clusters
+    // costs more than a second step (sixteen rows of 50257 logits: 9.3 us as clusters of thirteen,
+    // 12.8 of sixteen; 32 rows 12.8 us as clusters of nine, 18.7 of sixteen), and clusters that
+    // fill an SM's share of threads evenly more than the steps alone (24 rows: 11.2 and 12.8 us).
     static std::atomic<uint64_t> set{0};
-    ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_choose_token), 0, &set, true));
+    static std::atomic<uint32_t> known[kMaxRanks + 1];
+    const void* kernel = reinterpret_cast<const void*>(k_choose_token);
+    ZK_TRY(allow_shared(kernel, 0, &set, true));
+    auto fits = [&](uint32_t r) { return clusters_at_once(kernel, kChooseThreads, 0, r, known) >= batch; };
+    const uint64_t all = ceil_div(vocab, kChooseStep);
+    uint32_t need = all < kMaxRanks ? (uint32_t)all : kMaxRanks;
+    for (; need > 1; need--) {
+        need = (uint32_t)ceil_div(all, ceil_div(all, need));  // as few blocks at the same number of steps
+        if (fits(need)) break;
+    }
+    uint32_t ranks = need + need / 2 < kMaxRanks ? need + need / 2 : kMaxRanks;
+    while (ranks > need && !fits(ranks)) ranks--;
     return launch(k_choose_token, dim3(ranks, (unsigned)batch), kChooseThreads, 0, ranks, stream, p);
 }
 

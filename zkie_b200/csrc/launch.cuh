@@ -28,6 +28,27 @@ inline cudaError_t allow_shared(const void* kernel, size_t bytes, std::atomic<ui
     return e;
 }
 
+// Clusters of `cluster` blocks of a kernel that the present device holds at once: asked for once
+// per size and remembered in `known`, a word to a size (devices of one kind in one program).
+inline uint32_t clusters_at_once(const void* kernel, int threads, size_t shared, uint32_t cluster,
+                                 std::atomic<uint32_t>* known) {
+    if (const uint32_t n = known[cluster].load(std::memory_order_relaxed)) return n;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+    known[cluster].store((uint32_t)n, std::memory_order_relaxed);
+    return (uint32_t)n;
+}
+
 template <typename Args>
 int launch(void (*kernel)(const Args), dim3 grid, int threads, size_t shared, uint32_t cluster, cudaStream_t stream,
            const Args& args) {
