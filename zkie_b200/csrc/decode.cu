@@ -113,6 +113,8 @@ struct ProjectArgs {
     uint32_t stride;  // bytes of a digit row in shared memory
     uint32_t run;     // blocks to a slot of a ring, at most
     uint32_t unit;    // blocks that stay with one warp: a segment, or a slot where a tile has whole ones
+    uint32_t units;   // of a tile
+    uint32_t some, more;  // tiles of a grid's block: some, and one more in the first `more` of them
 };
 
 constexpr int kProjDepth = 3;           // slots of a warp's ring
@@ -146,15 +148,14 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     __syncwarp();
 
     // ---- this warp's stream of blocks, and the first of them on their way
-    const uint32_t tile0 = (uint32_t)((uint64_t)blockIdx.x * p.s.tiles / gridDim.x);
-    const uint32_t tile1 = (uint32_t)((uint64_t)(blockIdx.x + 1) * p.s.tiles / gridDim.x);
+    const uint32_t tile0 = blockIdx.x * p.some + min(blockIdx.x, p.more), tile1 = tile0 + p.some + (blockIdx.x < p.more);
     const uint32_t blocks = p.s.blocks, unit = p.unit;
     // blocks of a batch, counted from its first tile, that the warp takes
     auto first_of = [&](uint32_t batch, uint32_t w) {
-        const uint32_t units = min(kProjBatch, tile1 - batch) * blocks / unit;
-        return (uint32_t)((uint64_t)w * units / kProjWarps) * unit;
+        return w * (min(kProjBatch, tile1 - batch) * p.units) / kProjWarps * unit;
     };
     uint32_t next_batch = tile0, next_at = first_of(tile0, warp), next_end = first_of(tile0, warp + 1), next_slot = 0;
+    uint32_t next_b = next_at % blocks;  // within its tile
     auto ask = [&]() {  // lane 0 only
         while (next_at == next_end) {
             next_batch += kProjBatch;
@@ -164,12 +165,14 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             }
             next_at = first_of(next_batch, warp);
             next_end = first_of(next_batch, warp + 1);
+            next_b = next_at % blocks;
         }
-        const uint32_t run = min(min(p.run, next_end - next_at), blocks - next_at % blocks);  // within a tile
+        const uint32_t run = min(min(p.run, next_end - next_at), blocks - next_b);  // within a tile
         barrier_expect(bar + 8 * next_slot, run * kBytes);
         bulk_copy(ring + next_slot * slot_bytes, p.w + ((uint64_t)next_batch * blocks + next_at) * kBytes, run * kBytes,
                   bar + 8 * next_slot);
         next_at += run;
+        next_b = next_b + run == blocks ? 0 : next_b + run;
         next_slot = next_slot + 1 == kProjDepth ? 0 : next_slot + 1;
     };
     if (lane == 0)
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     for (uint32_t batch = tile0; batch < tile1; batch += kProjBatch) {
         uint32_t at = first_of(batch, warp);
         const uint32_t end = first_of(batch, warp + 1);
-        uint32_t tile = at / blocks, b = at % blocks;
+        uint32_t tile = at / blocks, b = at % blocks, in_seg = 0;
         Q4Sum<NT> sum;
         sum.clear();
         long long total[NT];  // of the tile's segments, each rounded
@@ -236,7 +239,8 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             } else {
                 for (uint32_t q = 0; q < run; q++) {
                     block(q);
-                    if (SEG && ++b % unit == 0) {
+                    if (SEG && (b++, ++in_seg == unit)) {
+                        in_seg = 0;
 #pragma unroll
                         for (int i = 0; i < NT; i++) total[i] += round_shift(sum.finish(i), p.shift);
                         sum.clear();
@@ -304,11 +308,14 @@ size_t project_shared(const Q4Shape& s, uint32_t rows, uint32_t run) {
 }
 
 template <int G, int NT, bool SEG>
-int project_launch(const ProjectArgs& p, cudaStream_t stream) {
+int project_launch(ProjectArgs p, cudaStream_t stream) {
     auto* kernel = k_q4_project<G, NT, SEG>;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kMaxShared, &set));
     const dim3 grid(p.s.tiles < (uint32_t)kSms ? p.s.tiles : kSms, (unsigned)ceil_div(p.m, 2 * NT));
+    p.units = p.s.blocks / p.unit;
+    p.some = p.s.tiles / grid.x;
+    p.more = p.s.tiles % grid.x;
     return launch(kernel, grid, kProjThreads, project_shared(p.s, 2 * NT, p.run), 1, stream, p);
 }
 

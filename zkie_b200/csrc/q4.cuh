@@ -83,6 +83,15 @@ __device__ __forceinline__ void mma_s8_new(int (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
+// q4_digits of a field element's number: v, less p = 2^64 - 0xFFFFFFFF from 2^63 on, in the few
+// instructions of which a block spends one set on every number of its rows
+__device__ __forceinline__ bool q4_digits_of(uint64_t v, uint32_t* d) {
+    const uint64_t x = v + (uint32_t)((int32_t)(v >> 32) >> 31), t = x + 0x7F7F7F7Fu;
+    const bool ok = t <= 0xFEFEFEFEull;
+    *d = ok ? ((uint32_t)t + 0x01010101u) ^ 0x80808080u : 0u;
+    return ok;
+}
+
 // the digits of four consecutive k, one word to each of the four digit rows
 __device__ __forceinline__ void q4_store_digits(uint8_t* to, size_t stride, const uint32_t (&d)[4]) {
 #pragma unroll
@@ -104,18 +113,20 @@ __device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint
                                             uint32_t kp_seg, uint32_t begin, uint32_t end, uint8_t* digits,
                                             uint32_t stride, uint8_t* also = nullptr) {
     const uint32_t quads = segs * kp_seg / 4;
+    const uint32_t per_row = 0xFFFFFFFFu / quads + 1, per_seg = 0xFFFFFFFFu / kp_seg + 1;  // reciprocals for __umulhi:
+    // exact, a quotient's numerator and divisor being below 2^16 (and the divisor no less than 16)
     const bool wide = (((uintptr_t)x | (ldx * 8)) & 15) == 0 && k_seg % 4 == 0;  // 16-byte loads
     bool ok = true;
     for (uint32_t i0 = begin + threadIdx.x; i0 < end; i0 += THREADS * AHEAD) {
-        int64_t v[AHEAD][4];
+        uint64_t v[AHEAD][4];
         uint32_t to[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const uint32_t i = i0 + u * THREADS;
             const bool on = i < end;
-            const uint32_t r = on ? i / quads : 0, k0 = on ? (i % quads) * 4 : 0;
-            const uint32_t seg = segs > 1 ? k0 / kp_seg : 0, in = k0 - seg * kp_seg;
-            const uint64_t* from = x + r * ldx + seg * k_seg + in;
+            const uint32_t r = on ? __umulhi(i, per_row) : 0, k0 = on ? (i - r * quads) * 4 : 0;
+            const uint32_t seg = segs > 1 ? __umulhi(k0, per_seg) : 0, in = k0 - seg * kp_seg;
+            const uint64_t* from = x + r * ldx + (seg * k_seg + in);
             to[u] = on ? r * 4 * stride + q4_pos(k0) : ~0u;
             if (wide) {
                 ulonglong2 lo = make_ulonglong2(0, 0), hi = lo;
@@ -123,10 +134,10 @@ __device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint
                     lo = __ldg(reinterpret_cast<const ulonglong2*>(from));
                     hi = __ldg(reinterpret_cast<const ulonglong2*>(from) + 1);
                 }
-                v[u][0] = (int64_t)lo.x, v[u][1] = (int64_t)lo.y, v[u][2] = (int64_t)hi.x, v[u][3] = (int64_t)hi.y;
+                v[u][0] = lo.x, v[u][1] = lo.y, v[u][2] = hi.x, v[u][3] = hi.y;
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[u][j] = on && in + j < k_seg ? (int64_t)__ldg(from + j) : 0;
+                for (int j = 0; j < 4; j++) v[u][j] = on && in + j < k_seg ? __ldg(from + j) : 0;
             }
         }
 #pragma unroll
@@ -134,7 +145,7 @@ __device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint
             if (to[u] != ~0u) {
                 uint32_t d[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) ok &= q4_digits(fx_to_i64((uint64_t)v[u][j]), &d[j]);
+                for (int j = 0; j < 4; j++) ok &= q4_digits_of(v[u][j], &d[j]);
                 q4_store_digits(digits + to[u], stride, d);
                 if (also) q4_store_digits(also + to[u], stride, d);
             }
