@@ -125,6 +125,15 @@ constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 // is rounded by itself), whatever tiles they belong to, against the digits of
 // 2 NT rows in shared memory.  The 64-bit sums meet in shared memory; a thread
 // per output then rounds and finishes it.
+//
+// Bound by: for few rows and a wide weight the weight's bytes (1024 x 65536 in
+// groups of 128, one row: 36 MB in 10.6 us, of which 3 us are the launch, the
+// row's digits and the last sums: 4.8 TB/s in between); for eight rows what a
+// warp does per block and pair of rows, about ten cycles of the SM (18.3 us:
+// 2.0 TB/s); for a small weight the launch and three trips to memory (1024 x
+// 192: 3.0 us).  A ring's slots are of four blocks because copies of 2176
+// bytes reach 5.8 TB/s and single blocks 3.7; 24 warps of 80 registers instead
+// of 16 of 127 take 20.8 us for the eight rows, 20 warps 19.9.
 template <int G, int NT, bool SEG>
 __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_constant__ ProjectArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -225,7 +234,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             if (!SEG && run == 4 && (G != 128 || unit == 4)) {
 #pragma unroll
                 for (uint32_t q = 0; q < 4; q += 2) {
-                    if (G == 128) {  // four blocks from a multiple of four on: two whole groups
+                    if (G == 128) {  // two whole groups (block by block: 20.2 us instead of 18.3)
                         uint4 x[2][NT];
 #pragma unroll
                         for (int i = 0; i < 2 * NT; i++) x[i / NT][i % NT] = load16(x_at[i % NT] + (q + i / NT) * 64);
@@ -326,8 +335,10 @@ int project_seg(const ProjectArgs& p, cudaStream_t stream) {
 
 template <int G>
 int project_rows(ProjectArgs p, cudaStream_t stream) {
-    // Rows to a block: up to eight, as many as their digits leave room for; slots of four blocks
-    // (2 kB a copy) where there is room, else of two or one
+    // Rows to a block: as many as there are, up to eight, so that a weight is read once for them, and
+    // as their digits leave room for (1024 x 65536: eight rows 18.3 us, four 13.9, two 11.3, one row
+    // with eight's kernel 16.9 instead of 10.6).  Slots of four blocks where there is room, else of
+    // two or one (one row 10.6, 13.2, 18.0 us; a weight of 1024 x 192 in 3.0, 2.9, 2.8).
     for (uint32_t rows = p.m > 4 ? 8 : p.m > 2 ? 4 : 2;; rows /= 2)
         for (p.run = 4; p.run; p.run /= 2)
             if (p.unit = p.s.segs > 1 ? p.s.kp_seg / 64 : p.s.blocks % p.run ? 1 : p.run;
@@ -410,6 +421,7 @@ constexpr uint32_t kMaxRanks = 16;   // blocks of a cluster
 constexpr size_t kAttShared = 220 * 1024;
 constexpr uint32_t kAttPiece = 4096;  // bytes of a ring's slot
 constexpr uint32_t kKeyDims = 32;     // dimensions of 32 keys to a slot
+constexpr uint32_t kAttDepth = 2;     // slots of a warp's ring (three: the same times)
 
 struct AttendArgs {
     KvCache c;
@@ -427,7 +439,6 @@ struct AttendArgs {
     uint32_t* err;
     uint32_t chunk;  // scores that a block has room for
     uint32_t slice;  // outputs that a block of the cluster finishes
-    uint32_t depth;  // slots of a warp's ring
 };
 
 // One cluster per sequence, key head and EACH of its query heads; a block
@@ -440,12 +451,21 @@ struct AttendArgs {
 // exchange.  A block writes what the others need into their shared memory
 // before each meeting, so that nothing is fetched from a neighbour after it.
 // The new token is taken from its rows, not from the cache it is stored to.
-// A product is one 32 x 32 + 64 bit multiply-add, 32 a clock on an SM, which
-// for four query heads to a key head costs about what the memory does.
+// A product is one 32 x 32 + 64 bit multiply-add, 32 a clock on an SM.
+//
+// Bound by: for one long sequence the two streams (16 heads of 192 + 128, 4096
+// tokens: 82 MB in 26.8 us, keys 8.5 us and values 6 at 4.5 to 5 TB/s, between
+// them 7 us of meetings and table entries, the first bytes 4); for a ragged
+// batch the longest sequence's blocks, whose cluster is as large as any other
+// (eight sequences of up to 8192 tokens, four query heads to a key head: 71
+// us, of which multiply-adds cost 12, table entries 10, the streams the
+// rest); for a short one the chain of latencies (512 tokens: 8.5 us).  Half
+// the heads' products in double precision: 69 us instead of 71, not kept; an
+// L2 prefetch of the values during the softmax: 29 to 32 us instead of 27.
 template <int EACH, int WIDE>
 __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_constant__ AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(8) uint64_t s_bar[kAttWarps * 4];
+    __shared__ __align__(8) uint64_t s_bar[kAttWarps * kAttDepth];
     __shared__ long long s_red[kAttWarps][EACH];
     __shared__ long long s_max[kMaxRanks][EACH], s_sum[kMaxRanks][EACH];
     cg::cluster_group cluster = cg::this_cluster();
@@ -454,10 +474,10 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     const uint32_t heads = min((uint32_t)EACH, p.each - e0), dk = p.c.dk, dv = p.c.dv;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t* out = p.out + ((uint64_t)seq * p.c.heads * p.each + (uint64_t)h * p.each + e0) * dv;
-    const uint32_t bar = shared_addr(&s_bar[warp * 4]);
+    const uint32_t bar = shared_addr(&s_bar[warp * kAttDepth]);
     let_next_start();
     if (lane == 0) {
-        for (uint32_t i = 0; i < p.depth; i++) barrier_init(bar + 8 * i);
+        for (uint32_t i = 0; i < kAttDepth; i++) barrier_init(bar + 8 * i);
         barrier_init_done();
     }
     __syncwarp();
@@ -481,10 +501,10 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     const int32_t* keys = p.c.k + key_at(head, p.c.cap / kKvBlock, dk, t0, 0);
     const int32_t* values = p.c.v + (head * p.c.cap + t0) * dv;
 
-    uint8_t* ring = smem + (size_t)warp * p.depth * kAttPiece;
+    uint8_t* ring = smem + (size_t)warp * kAttDepth * kAttPiece;
     long long* sums = reinterpret_cast<long long*>(smem);  // in the rings' place, once they are done
     // chunk x EACH; a token's weights later take the first half of its scores' place, as 32-bit numbers
-    long long* scores = reinterpret_cast<long long*>(smem + (size_t)kAttWarps * p.depth * kAttPiece);
+    long long* scores = reinterpret_cast<long long*>(smem + (size_t)kAttWarps * kAttDepth * kAttPiece);
     unsigned long long* acc = reinterpret_cast<unsigned long long*>(scores + (size_t)EACH * p.chunk);  // ranks x slice
     int* qs = reinterpret_cast<int*>(acc + (((size_t)ranks * p.slice + 1) & ~(size_t)1));              // EACH x dk
     int* fresh = qs + EACH * dk;                                                                       // dk + dv
@@ -516,7 +536,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         }
         barrier_expect(bar + 8 * next_slot, bytes);
         bulk_copy(shared_addr(ring + next_slot * kAttPiece), from, bytes, bar + 8 * next_slot);
-        next_slot = next_slot + 1 == p.depth ? 0 : next_slot + 1;
+        next_slot = next_slot + 1 == kAttDepth ? 0 : next_slot + 1;
         next_i++;
         if (next_v ? next_i == vpieces || piece_tokens(next_b, next_i) == 0 : next_i == kpieces) {
             next_i = 0;
@@ -524,13 +544,13 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         }
     };
     if (lane == 0)
-        for (uint32_t i = 0; i < p.depth; i++) ask();
+        for (uint32_t i = 0; i < kAttDepth; i++) ask();
     Patience patience;
     uint32_t slot = 0, phase = 0;
     auto step = [&]() {  // on to the next slot, this one being filled again
         __syncwarp();
         if (lane == 0) ask();
-        if (++slot == p.depth) {
+        if (++slot == kAttDepth) {
             slot = 0;
             phase ^= 1;
         }
@@ -735,19 +755,19 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     }
 }
 
-// Shared memory of a block: rings (64 kB at least; in their place later the value sums, at most
+// Shared memory of a block: rings (64 kB; in their place later the value sums, at most
 // 32 kB), scores, the others' sums, queries, the new token
 struct AttendPlan {
-    uint32_t each, ranks, depth, chunk, slice;
+    uint32_t each, ranks, chunk, slice;
     size_t shared;
 };
 
-AttendPlan attend_plan(uint32_t each, uint32_t ranks, uint32_t depth, uint32_t blocks, uint32_t dk, uint32_t dv) {
-    AttendPlan a{each, ranks, depth, 0, 0, 0};
+AttendPlan attend_plan(uint32_t each, uint32_t ranks, uint32_t blocks, uint32_t dk, uint32_t dv) {
+    AttendPlan a{each, ranks, 0, 0, 0};
     a.chunk = (uint32_t)ceil_div(blocks, ranks) * kKvBlock + 1;
     a.chunk += a.chunk % 2;
     a.slice = (uint32_t)ceil_div(each * dv, ranks);
-    a.shared = (size_t)kAttWarps * depth * kAttPiece + 8ull * each * a.chunk + 8 * ((ranks * a.slice + 1) & ~1ull) +
+    a.shared = (size_t)kAttWarps * kAttDepth * kAttPiece + 8ull * each * a.chunk + 8 * ((ranks * a.slice + 1) & ~1ull) +
                4ull * (each * dk + dk + dv);
     return a;
 }
@@ -757,7 +777,6 @@ int attend_launch(AttendArgs p, const AttendPlan& a, cudaStream_t stream) {
     p.groups = (uint32_t)ceil_div(p.each, EACH);
     p.chunk = a.chunk;
     p.slice = a.slice;
-    p.depth = a.depth;
     auto* kernel = k_kv_attend<EACH, WIDE>;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kAttShared, &set, true));
@@ -793,6 +812,12 @@ constexpr uint32_t kChooseStep = kChooseThreads * kChooseEach;
 // start for registers, the history's tokens are counted in shared memory, then
 // the logits are finished; the blocks' maxima meet in the first block.  A warp
 // takes 32 neighbours, so a mask word is one load.
+//
+// Bound by the chain launch - lengths - history - logits - cluster: one row of
+// 65536 takes 5.8 us, sixteen of 50257 with histories of 4096 9.3 us (19.7 MB:
+// 2.1 TB/s, every block reading its row's whole history).  Histories loaded
+// before their lengths are known: 13.7 us instead of 12.8 at the time; four
+// logits to a thread, three blocks to an SM: 13.0; 1024 threads: 16.7.
 __global__ void __launch_bounds__(kChooseThreads, 2) k_choose_token(const __grid_constant__ ChooseArgs p) {
     __shared__ uint32_t counts[kChooseStep];
     __shared__ long long s_v[kChooseWarps];
@@ -1016,8 +1041,9 @@ int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t
     p.offset = offset;
     p.out = d_out;
     p.err = d_err;
-    // Query heads to a block: those that share a key head, up to four (two where a value row is
-    // wider than 128: their sums stay in registers), fewer where their scores do not fit.  Blocks
+    // Query heads to a block: those that share a key head, up to four (a ragged batch of eight with four
+    // heads to a key head: 71 us, two at a time 77; two at most where a value row is wider than 128:
+    // their sums stay in registers), fewer where their scores do not fit.  Blocks
     // to a cluster: enough to fill the device with two to an SM, of four token blocks at least, up
     // to eight, as many as find room at once (264 blocks in clusters of eight, 284 in smaller ones,
     // but 224 in clusters of sixteen: 36 us instead of 27 for 16 heads of 4096 tokens); sixteen only
@@ -1028,11 +1054,9 @@ int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t
         const uint64_t rows = batch * heads * ceil_div(p.each, each);
         uint32_t ranks = 1;
         while (ranks < 8 && rows * ranks * 2 <= (ranks == 4 ? 264 : 284) && ranks * 8 <= blocks) ranks *= 2;
-        AttendPlan a = attend_plan(each, ranks, 2, blocks, p.c.dk, p.c.dv);
+        AttendPlan a = attend_plan(each, ranks, blocks, p.c.dk, p.c.dv);
         for (; a.shared > (a.ranks < 8 ? kAttShared / 2 : kAttShared) && a.ranks < kMaxRanks && a.ranks < blocks;)
-            a = attend_plan(each, a.ranks * 2, 2, blocks, p.c.dk, p.c.dv);
-        if (attend_plan(each, a.ranks, 3, blocks, p.c.dk, p.c.dv).shared <= kAttShared / 2)
-            a = attend_plan(each, a.ranks, 3, blocks, p.c.dk, p.c.dv);
+            a = attend_plan(each, a.ranks * 2, blocks, p.c.dk, p.c.dv);
         if (a.shared > kAttShared && each > 1) continue;
         if (a.shared > kAttShared) return (int)cudaErrorInvalidValue;
         if (wide) return each == 2 ? attend_launch<2, 2>(p, a, stream) : attend_launch<1, 2>(p, a, stream);

@@ -116,13 +116,14 @@ __global__ void k_moe_router_pack(const uint64_t* __restrict__ w, uint32_t h, ui
 }
 
 // Logits of the 16 experts of tile 2 own + rank, this warp's blocks [b0, b1),
-// added to sums (tokens x this block's experts); 2 NT tokens at a time, for
-// which two blocks of the router at a time are held in registers.
-template <int NT>
+// added to sums (tokens x this block's experts); eight tokens at a time, for
+// which two blocks of the router at a time are held in registers (a second
+// form for two tokens: 0.4 us less for one token, 0.2 to 1.3 more for three
+// to eight, whose registers it changes).
 __device__ __forceinline__ void router_part(const MoeArgs& p, const uint8_t* digits, uint32_t own, uint32_t rank,
                                          uint32_t b0, uint32_t b1, const Limbs& sums, uint32_t pitch) {
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr int kHeld = 2;
+    constexpr int kHeld = 2, NT = 4;
     for (uint32_t tok0 = 0; tok0 < p.m; tok0 += 2 * NT) {
         int c[2][NT][4];
 #pragma unroll
@@ -279,6 +280,10 @@ __device__ __forceinline__ void list_items(const MoeArgs& p, uint32_t thread, co
     }
 }
 
+// Fours of numbers from which on the blocks of a pair work out half of the digits each: 16 x 2048
+// numbers 102.4 us for the layer instead of 105.3 (8 x 2048 66.5 and 67.2, 4 x 2048 42.9 and 42.3,
+// 8 x 512 18.3 and 17.1)
+constexpr uint32_t kShareDigits = 4096;
 constexpr uint32_t kUpBatch = 16;                                       // tiles whose sums are held at a time
 constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile, gate or up, token, column)
 
@@ -286,6 +291,14 @@ constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile
 // gridDim.x for i = 0, 1, ..: first those of the shared experts (four tokens
 // to each), then those of the chosen experts' items; in batches, of which
 // every warp takes an equal run of blocks of 64 k (gate and up together).
+//
+// Bound by (2048 wide, 64 experts of 1408, six to a token, the shared ones
+// 2816): for one token a chain -- digits 2.3 us, logits 2.1, routing 3.4 beside
+// the shared experts' first tiles, the chosen experts' tiles 5 (20 MB: 4 TB/s);
+// for sixteen the same chain (6.3, 6.5 and 10.5 us) and 31 us of streaming the
+// 51 or so chosen experts' gate and up at about 5 TB/s.  Two blocks to a
+// cluster share the digits and the router: clusters of four or eight would
+// share more, but only 132 or 120 of their blocks run at once.
 template <bool TWO, int DEPTH, int RUN>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -363,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     wait_for_previous();
     bool bad = false;
     const uint32_t fours = p.m * blocks * 16;
-    if (p.m < 4) {
+    if (fours < kShareDigits) {
         bad |= !q4_digitise<kThreads, 2>(p.x, p.ldx, 1, p.h, blocks * 64, 0, fours, digits, p.stride);
         __syncthreads();
         cluster_wait();
@@ -378,10 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
         const uint32_t own = (p.etiles - rank + 1) / 2, wide = own > 1 ? kWarps / 2 : kWarps;
         for (uint32_t i = warp / wide; i < own; i += kWarps / wide) {
             const uint32_t w = warp % wide, r0 = w * blocks / wide, r1 = (w + 1) * blocks / wide;
-            if (p.m <= 2)
-                router_part<1>(p, digits, i, rank, r0, r1, sums, pitch);
-            else
-                router_part<4>(p, digits, i, rank, r0, r1, sums, pitch);
+            router_part(p, digits, i, rank, r0, r1, sums, pitch);
         }
     }
     __syncthreads();
@@ -510,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
             cluster_wait();
             if (warp >= early_warps) {
                 for (uint32_t r = warp - early_warps; r < p.m; r += kWarps - early_warps) {
-                    if (p.experts <= 64)
+                    if (p.experts <= 64)  // (the general form: 25.6 us instead of 23.1 for one token)
                         route_token<2>(p, r, logits, logits + p.m * pitch, pitch, s_sel, items.score, s_mask);
                     else
                         route_token<kMaxExperts / 32>(p, r, logits, logits + p.m * pitch, pitch, s_sel, items.score, s_mask);
@@ -553,6 +563,13 @@ struct DownAt {
     const uint8_t *w0, *w1;  // block b of the two tiles
 };
 
+// A pair of blocks to 32 output columns, half of the stream each; digits come
+// with the codes, a slot's copies under one barrier.
+//
+// Bound by (sizes as above): one token 7 us, of which 1.5 pass before the items
+// are there and 4 stream 10 MB; sixteen tokens 25 us, 18 of them streaming 81 MB
+// of codes and half as much again of digits from the second-level cache, in
+// copies of 1088 and 512 bytes (4.4 TB/s of codes).
 template <bool TWO>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -732,6 +749,8 @@ int up_launch(const MoeArgs& p, cudaStream_t stream) {
 
 template <bool TWO>
 int moe_launch(MoeArgs p, cudaStream_t stream) {
+    // two blocks to a slot where there is room: 66.5 us instead of 69.1 for eight tokens of 2048, the
+    // same for one (22.8 to 23.1)
     const bool deep = up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, kUpDeep) <= kMaxShared;
     const int rc = deep ? up_launch<TWO, 3, 2>(p, stream) : up_launch<TWO, 3, 1>(p, stream);
     if (rc) return rc;

@@ -6,12 +6,14 @@
 // four signed byte digits, x = sum_p d_p 256^p, and the digits of two rows
 // are the eight columns of an m16n8k32 integer matrix instruction whose 16
 // rows are 16 columns n of the weight.  A warp thus streams the codes of 16
-// columns once, in 512-byte blocks of 64 k (16 bytes to a lane, contiguous),
-// and spends two instructions a block on two rows of x.  The instruction is
-// the warp-wide mma.sync: a product for at most a few rows is bound by the
-// bytes of the weight, at 4 bits a multiply, and its use of the matrix pipe
-// is a few per cent either way, so nothing is gained from accumulators in
-// tensor memory and a good deal of set-up is saved.
+// columns once, in blocks of 64 k (512 bytes of codes, 16 to a lane), and
+// spends two instructions a block on two rows of x.  The instruction is the
+// warp-wide mma.sync (two cycles of an SM, latency 20): with up to eight rows
+// a product is bound by the weight's bytes and by what each warp does around
+// the instruction -- taking codes apart, scaling groups -- and the matrix pipe
+// is busy 19 % of the time at eight rows, so accumulators in
+// tensor memory would save nothing and cost their set-up in a call of a few
+// microseconds.
 //
 // The sums are exact: within a block 16 c d stays below 2^29 even with two
 // digits joined, the scaled group sums are added in 64 bits, and a padded K
