@@ -293,12 +293,16 @@ constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile
 // every warp takes an equal run of blocks of 64 k (gate and up together).
 //
 // Bound by (2048 wide, 64 experts of 1408, six to a token, the shared ones
-// 2816): for one token a chain -- digits 2.3 us, logits 2.1, routing 3.4 beside
-// the shared experts' first tiles, the chosen experts' tiles 5 (20 MB: 4 TB/s);
-// for sixteen the same chain (6.3, 6.5 and 10.5 us) and 31 us of streaming the
-// 51 or so chosen experts' gate and up at about 5 TB/s.  Two blocks to a
-// cluster share the digits and the router: clusters of four or eight would
-// share more, but only 132 or 120 of their blocks run at once.
+// 2816): for one token a chain -- digits 2.1 us, logits 3.3, routing 3.4 beside
+// the shared experts' first tiles, then the chosen experts' tiles 5 (20 MB: 4
+// TB/s); for sixteen the same chain (6.2, 6.6 and 9.8 us) and 46 us over the
+// gate and up of the 51 or so chosen experts (162 MB: 3.5 TB/s), which is the
+// warps' own work: codes taken apart, scales, slots asked for (issue slots 53 %
+// used over the whole kernel, matrix pipe 12 %; the codes prefetched into the
+// second-level cache 4, 8 or 16 blocks ahead: 106 to 109 us for the layer
+// instead of 103).  Two blocks to a cluster share the digits and the router:
+// clusters of four or eight would share more, but only 132 or 120 of their
+// blocks run at once.
 template <bool TWO, int DEPTH, int RUN>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -567,9 +571,9 @@ struct DownAt {
 // with the codes, a slot's copies under one barrier.
 //
 // Bound by (sizes as above): one token 7 us, of which 1.5 pass before the items
-// are there and 4 stream 10 MB; sixteen tokens 25 us, 18 of them streaming 81 MB
-// of codes and half as much again of digits from the second-level cache, in
-// copies of 1088 and 512 bytes (4.4 TB/s of codes).
+// are there and 4 stream 10 MB; sixteen tokens 33 us, 3 before the items, 26 over
+// 81 MB of codes (3.2 TB/s) and as many bytes of digits from the second-level
+// cache, in copies of 1088 and 512 bytes.
 template <bool TWO>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
