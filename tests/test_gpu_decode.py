@@ -431,3 +431,34 @@ def test_moe_output_apart_from_input(zk):
     xs = _u(x)
     with pytest.raises(ValueError, match="shares memory"):
         block.forward(xs, out=xs)
+
+
+@pytest.mark.parametrize("b,v", [(15, 4097), (22, 20000), (40, 8193), (70, 33000), (300, 12345), (1000, 40)])
+def test_choose_token_many_rows(zk, b, v):
+    """More rows than find room as clusters of one step's blocks: fewer blocks
+    to a row, more steps, down to one block."""
+    rng = np.random.default_rng(b)
+    logits, history = rng.integers(-(1 << 35), 1 << 35, (b, v)), rng.integers(0, v, (b, 50)).astype(np.int32)
+    bias = rng.integers(-(1 << 33), 1 << 33, v)
+    tok, out = zk.decode.choose_token(_u(logits), _i32(history), presence=1 << 34, bias=_u(bias))
+    want_tok, want = ref.choose(logits, history, presence=1 << 34, bias=bias)
+    assert np.array_equal(_s(out), want) and np.array_equal(tok.cpu().numpy(), want_tok)
+
+
+def test_moe_no_rows(zk):
+    rng = np.random.default_rng(9)
+    router, w = _moe_case(rng, 32, 4, 16, 16, 32)
+    out, gate = _moe_block(zk, router, w, 32, 2, _exp_table(12), _silu_table(12)).forward(_u(np.zeros((0, 32), dtype=np.int64)))
+    assert out.shape == (0, 32) and gate.shape == (0, 4)
+
+
+def test_numbers_beyond_the_field(zk):
+    """Words from p on stand for what they are modulo p, as in the op layer."""
+    import torch
+    rng = np.random.default_rng(10)
+    k, n = 70, 33
+    w = ref.weight(rng, k, n, 64)
+    x = rng.integers(0, 1 << 30, (2, k))
+    q = _quant(zk, w, 64)
+    beyond = torch.from_numpy((x.astype(np.uint64) + np.uint64(0xFFFFFFFF00000001))).cuda()
+    assert np.array_equal(_s(zk.decode.project(beyond, q, 10)), ref.project(x, *w, 64, 0, 10))

@@ -53,7 +53,7 @@ struct Rows {
 };
 Rows rows(const at::Tensor& t, const char* name, int64_t cols, int dev) {
     if (t.scalar_type() != at::kUInt64 || !t.is_cuda() || t.get_device() != dev || t.dim() != 2 || t.size(1) != cols ||
-        (cols > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < cols))
+        (cols > 1 && t.size(0) > 0 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < cols))
         refuse(std::string(name) + ": a uint64 matrix of " + std::to_string(cols) +
                " columns on the call's device, unit stride within its rows, is wanted, not " + said(t));
     return {static_cast<const uint64_t*>(t.data_ptr()), t.size(0), t.stride(0)};
