@@ -656,7 +656,9 @@ uint64_t zkie2_q4_words(uint64_t experts, uint64_t k, uint64_t n, uint32_t group
 int zkie2_q4_pack(const int8_t *d_codes, const int32_t *d_scales, uint64_t experts, uint64_t k, uint64_t n,
                   uint32_t group, uint64_t segment, uint32_t *d_packed, uint32_t *d_err, zkie_stream_t stream);
 /* Two packed weights of one shape, block by block side by side (twice as many
- * words): a gate and an up weight for zkie2_moe_rows. */
+ * words): a gate and an up weight for zkie2_moe_rows.  d_b null: the tiles of 16
+ * columns of one weight two by two, an odd last one beside zeros (words: the
+ * weight's for n rounded up to 32): its down weights. */
 int zkie2_q4_pair(const uint32_t *d_a, const uint32_t *d_b, uint64_t experts, uint64_t k, uint64_t n, uint32_t group,
                   uint32_t *d_out, zkie_stream_t stream);
 /* Op::Projection's out (Op::MatMul for shift = 0 and no bias) of m rows by one

@@ -83,12 +83,20 @@ __global__ void k_q4_pack(const int8_t* __restrict__ codes, const int32_t* __res
     if (bad) atomicOr(err, kErrRange);
 }
 
-// two weights of one shape, block by block side by side
-__global__ void k_q4_pair(const uint4* __restrict__ a, const uint4* __restrict__ b, uint64_t blocks, uint32_t words,
+// two weights of one shape, block by block side by side; or (b null) the tiles of one two by two,
+// with zeros beside an odd one
+__global__ void k_q4_pair(const uint4* __restrict__ a, const uint4* __restrict__ b, Q4Shape s, uint64_t blocks,
                           uint4* __restrict__ out) {
-    for (uint64_t i = blockIdx.x; i < blocks; i += gridDim.x)
-        for (uint32_t j = threadIdx.x; j < 2 * words; j += blockDim.x)
-            out[i * 2 * words + j] = j < words ? a[i * words + j] : b[i * words + j - words];
+    const uint32_t words = s.bytes / 16, pairs = (s.tiles + 1) / 2;
+    for (uint64_t i = blockIdx.x; i < blocks; i += gridDim.x) {  // of a weight, or of its pairs
+        const uint64_t at = i % s.blocks, tile = i / s.blocks % pairs * 2, expert = i / s.blocks / pairs;
+        const uint4* from = b ? a + i * words : a + ((expert * s.tiles + tile) * s.blocks + at) * words;
+        const uint4* beside = b ? b + i * words : tile + 1 < s.tiles ? from + (uint64_t)s.blocks * words : nullptr;
+        for (uint32_t j = threadIdx.x; j < words; j += blockDim.x) {
+            out[i * 2 * words + j] = from[j];
+            out[(i * 2 + 1) * words + j] = beside ? beside[j] : make_uint4(0, 0, 0, 0);
+        }
+    }
 }
 
 // ---- the product ----------------------------------------------------------------------------
@@ -950,12 +958,12 @@ int zkie2_q4_pack(const int8_t* d_codes, const int32_t* d_scales, uint64_t exper
 int zkie2_q4_pair(const uint32_t* d_a, const uint32_t* d_b, uint64_t experts, uint64_t k, uint64_t n, uint32_t group,
                   uint32_t* d_out, cudaStream_t stream) {
     Q4Shape s;
-    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, 0, &s) || !d_a || !d_b || !d_out ||
+    if (experts == 0 || experts > 4096 || !q4_shape(k, n, group, 0, &s) || !d_a || !d_out ||
         (((uintptr_t)d_a | (uintptr_t)d_b | (uintptr_t)d_out) & 15))
         return (int)cudaErrorInvalidValue;
-    const uint64_t blocks = experts * s.tiles * s.blocks;
+    const uint64_t blocks = experts * (d_b ? s.tiles : (s.tiles + 1) / 2) * s.blocks;
     k_q4_pair<<<(unsigned)(blocks < kSms * 16 ? blocks : kSms * 16), 64, 0, stream>>>(
-        reinterpret_cast<const uint4*>(d_a), reinterpret_cast<const uint4*>(d_b), blocks, s.bytes / 16,
+        reinterpret_cast<const uint4*>(d_a), reinterpret_cast<const uint4*>(d_b), s, blocks,
         reinterpret_cast<uint4*>(d_out));
     ZK_LAUNCH_CHECK();
     return 0;

@@ -70,7 +70,7 @@ struct MoeArgs {
     uint64_t ldx;
     uint32_t m, h, experts, top_k, etiles;
     const uint4* router;
-    Q4Weight up, down, sup, sdown;  // up: gate and up, block by block side by side
+    Q4Weight up, down, sup, sdown;  // up: gate and up, block by block side by side; down: pairs of tiles
     const uint64_t* exp_table;
     uint64_t exp_len;
     const uint64_t* silu;
@@ -81,8 +81,8 @@ struct MoeArgs {
     uint64_t* out;
     uint64_t* gate_out;  // m x experts (or null)
     Items* items;
-    uint8_t* act;        // the activation's digits: a slot's blocks of 64, in each its four digit rows
-    uint8_t* sact;       // the same of the shared experts, a token's blocks
+    uint8_t* act;        // the activation's digits: an item's blocks of 64, in each its tokens' four digit rows
+    uint8_t* sact;       // the same of the shared experts, tokens four at a time
     uint32_t* err;
     uint32_t stride;     // bytes of a digit row of x
     uint32_t depth;      // slots of a ring of k_moe_down
@@ -498,9 +498,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
                 acc.clear(cell + kTile * 16);
                 if (f >= (shared ? p.sup.s.n : p.up.s.n)) continue;
                 silu[q] = table_at(p.silu, p.silu_len, gi, (int64_t)(p.silu_len / 2));
-                to[q] = (shared ? p.sact + (uint64_t)(tok0 + j) * p.sdown.s.blocks * 256
-                                : p.act + (uint64_t)items.slot[tok0 + j] * p.down.s.blocks * 256) +
-                        f / 64 * 256 + q4_pos(f % 64);
+                to[q] = (shared ? p.sact + (uint64_t)tok0 * p.sdown.s.blocks * 256
+                                : p.act + (uint64_t)tok0 * p.down.s.blocks * 256) +
+                        (f / 64 * count + j) * 256 + q4_pos(f % 64);
             }
 #pragma unroll
             for (int q = 0; q < kOuts; q++)
@@ -564,7 +564,7 @@ constexpr uint32_t kDownRun = 2;  // blocks to a slot
 struct DownAt {
     uint32_t b, len, count, first;
     bool shared;
-    const uint8_t *w0, *w1;  // block b of the two tiles
+    const uint8_t *w, *x;  // block b of the two tiles, and of the tokens' digits
 };
 
 // A pair of blocks to 32 output columns, half of the stream each; digits come
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
     __shared__ Items items;
     __shared__ __align__(8) uint64_t s_bar[kWarps * kDownDepth];
     constexpr uint32_t kBytes = TWO ? 576 : 544, kSlot = kDownRun * (2 * kBytes + 256 * kTile);
-    constexpr uint32_t kDigits = 2 * kDownRun * kBytes;  // after both tiles' blocks: those of each token
+    constexpr uint32_t kDigits = 2 * kDownRun * kBytes;  // after the tiles' blocks: those of the tokens
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t rank = cluster.block_rank(), slots = p.m * p.top_k, cells = (slots + p.m) * 32;
@@ -595,9 +595,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
     }
     __syncwarp();
     for (uint32_t i = threadIdx.x; i < 3 * cells; i += kThreads) acc.w[i] = 0;
-    const uint32_t tiles = p.down.s.tiles, t0 = (blockIdx.x / 2) * 2, t1 = min(t0 + 1, tiles - 1);
-    if (threadIdx.x < 2)  // the shared experts' codes of these columns start for the second-level cache
-        prefetch_l2(p.sdown.w + (uint64_t)(threadIdx.x ? t1 : t0) * p.sdown.s.blocks * kBytes, p.sdown.s.blocks * kBytes);
+    const uint32_t pairs = (p.down.s.tiles + 1) / 2, pair = blockIdx.x / 2;
+    if (threadIdx.x == 0)  // the shared experts' codes of these columns start for the second-level cache
+        prefetch_l2(p.sdown.w + (uint64_t)pair * p.sdown.s.blocks * 2 * kBytes, p.sdown.s.blocks * 2 * kBytes);
     wait_for_previous();
     for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
         reinterpret_cast<uint32_t*>(&items)[i] = __ldcg(reinterpret_cast<const uint32_t*>(p.items) + i);
@@ -616,9 +616,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         d.b = in % d.len;
         d.first = d.shared ? item * kTile : items.first[item];
         d.count = d.shared ? min(kTile, p.m - d.first) : items.count[item];
-        const uint8_t* w = d.shared ? p.sdown.w : p.down.w + (uint64_t)items.expert[item] * tiles * nf * kBytes;
-        d.w0 = w + ((uint64_t)t0 * d.len + d.b) * kBytes;
-        d.w1 = w + ((uint64_t)t1 * d.len + d.b) * kBytes;
+        const uint8_t* w = d.shared ? p.sdown.w : p.down.w + (uint64_t)items.expert[item] * pairs * nf * 2 * kBytes;
+        d.w = w + ((uint64_t)pair * d.len + d.b) * 2 * kBytes;
+        d.x = (d.shared ? p.sact : p.act) + ((uint64_t)d.first * d.len + d.b * d.count) * 256;
     };
     DownAt next, now;
     uint32_t next_at = at, next_slot = 0;
@@ -630,18 +630,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         const uint32_t b = bar + 8 * next_slot, to = shared_addr(ring + next_slot * kSlot);
         const uint32_t run = min(kDownRun, min(end - next_at, next.len - next.b));
         barrier_expect(b, run * (2 * kBytes + 256 * next.count));
-        bulk_copy(to, next.w0, run * kBytes, b);
-        bulk_copy(to + kDownRun * kBytes, next.w1, run * kBytes, b);
-        for (uint32_t j = 0; j < next.count; j++)
-            bulk_copy(to + kDigits + kDownRun * 256 * j,
-                      (next.shared ? p.sact + (uint64_t)(next.first + j) * ns * 256
-                                   : p.act + (uint64_t)items.slot[next.first + j] * nf * 256) + next.b * 256,
-                      run * 256, b);
+        bulk_copy(to, next.w, run * 2 * kBytes, b);
+        bulk_copy(to + kDigits, next.x, run * 256 * next.count, b);
         next_slot = next_slot + 1 == p.depth ? 0 : next_slot + 1;
         next_at += run;
         next.b += run;
-        next.w0 += run * kBytes;
-        next.w1 += run * kBytes;
+        next.w += run * 2 * kBytes;
+        next.x += run * 256 * next.count;
         if (next.b == next.len && next_at < end) locate(next, next_at);
     };
     if (lane == 0)
@@ -655,8 +650,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         sum[0].clear();
         sum[1].clear();
         // digits of columns g: digit row g % 4 of token g / 4 (and 2 + g / 4) of the item
-        const uint32_t x0 = kDigits + min(g >> 2, now.count - 1) * kDownRun * 256 + (g & 3) * 64 + 16 * t;
-        const uint32_t x1 = kDigits + min(2 + (g >> 2), now.count - 1) * kDownRun * 256 + (g & 3) * 64 + 16 * t;
+        const uint32_t x0 = kDigits + min(g >> 2, now.count - 1) * 256 + (g & 3) * 64 + 16 * t;
+        const uint32_t x1 = kDigits + min(2 + (g >> 2), now.count - 1) * 256 + (g & 3) * 64 + 16 * t;
         while (at < stop) {
             barrier_wait(bar + 8 * slot, phase, patience);
             const uint32_t base = shared_addr(ring) + slot * kSlot;
@@ -665,14 +660,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
             for (uint32_t r = 0; r < kDownRun; r++) {
                 if (at == stop) break;
                 uint4 x[2];
-                x[0] = load16(base + x0 + r * 256);
+                x[0] = load16(base + x0 + r * now.count * 256);
                 if (now.count > 2) {
-                    x[1] = load16(base + x1 + r * 256);
-                    q4_block<TWO, 2>(sum[0], lane_at, r * kBytes, x);
-                    q4_block<TWO, 2>(sum[1], lane_at, (kDownRun + r) * kBytes, x);
+                    x[1] = load16(base + x1 + r * now.count * 256);
+                    q4_block<TWO, 2>(sum[0], lane_at, 2 * r * kBytes, x);
+                    q4_block<TWO, 2>(sum[1], lane_at, (2 * r + 1) * kBytes, x);
                 } else {
-                    q4_block<TWO, 1>(sum[0], lane_at, r * kBytes, x);
-                    q4_block<TWO, 1>(sum[1], lane_at, (kDownRun + r) * kBytes, x);
+                    q4_block<TWO, 1>(sum[0], lane_at, 2 * r * kBytes, x);
+                    q4_block<TWO, 1>(sum[1], lane_at, (2 * r + 1) * kBytes, x);
                 }
                 at++;
             }
@@ -702,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
     const Limbs there{cluster.map_shared_rank(acc.w, rank ^ 1), cells};
     for (uint32_t o = threadIdx.x; o < p.m * 16; o += kThreads) {
         const uint32_t c = rank * 16 + (o & 15), r = o >> 4;
-        const uint64_t n = (uint64_t)t0 * 16 + c;
+        const uint64_t n = (uint64_t)pair * 32 + c;
         if (n >= p.h) continue;
         const uint32_t s = (slots + r) * 32 + c;
         int64_t y = round_shift(fx_wadd(acc.get(s), there.get(s)), p.shift);

@@ -327,7 +327,7 @@ class MoeBlock:
     and down (experts x f x h) and the shared experts' gate, up (h x shared f)
     and down weights, all of one group without segments, the exp and silu
     tables (field elements; silu's middle is zero) and how many experts a token
-    takes.  The block keeps a copy of its own of the gate and up weights."""
+    takes.  The block keeps copies of its own of the weights."""
 
     def __init__(self, router: torch.Tensor, gate: QuantWeight, up: QuantWeight, down: QuantWeight,
                  shared_gate: QuantWeight, shared_up: QuantWeight, shared_down: QuantWeight, exp_table: torch.Tensor,
@@ -356,18 +356,21 @@ class MoeBlock:
         err = _err_word()
         check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self.router.data_ptr(), err.data_ptr(), _stream()), "zkie2_moe_router_pack")
         _check_err(err, "MoeBlock: router")
-        self.packed = (self._pair(gate, up), down.packed, self._pair(shared_gate, shared_up), shared_down.packed)
+        self.packed = (self._pair(gate, up), self._pair(down), self._pair(shared_gate, shared_up), self._pair(shared_down))
         self._packed = (_lib.vp * 4)(*[w.data_ptr() for w in self.packed])
         torch.cuda.current_stream().synchronize()  # weights are complete before a call: it reads them at once
         self.call = (dev, h, e, top_k, f, s, self.group, self.router.data_ptr(), C.addressof(self._packed),
                      exp_table.data_ptr(), exp_table.numel(), silu_table.data_ptr(), silu_table.numel(), shift)
 
     @staticmethod
-    def _pair(a: QuantWeight, b: QuantWeight) -> torch.Tensor:
-        """Gate and up, block by block side by side: one copy brings both."""
-        out = torch.empty(2 * a.packed.numel(), dtype=torch.int32, device=a.packed.device)
-        check(lib.zkie2_q4_pair(a.pointer, b.pointer, a.experts, a.k, a.n, a.group, out.data_ptr(), _stream()),
-              "zkie2_q4_pair")
+    def _pair(a: QuantWeight, b: Optional[QuantWeight] = None) -> torch.Tensor:
+        """Gate and up, or the tiles of down two by two, block by block side by
+        side: one copy brings both."""
+        tiles = -(-a.n // 16)
+        words = a.packed.numel() // tiles * (2 * tiles if b is not None else tiles + tiles % 2)
+        out = torch.empty(words, dtype=torch.int32, device=a.packed.device)
+        check(lib.zkie2_q4_pair(a.pointer, b.pointer if b is not None else None, a.experts, a.k, a.n, a.group, out.data_ptr(),
+                                _stream()), "zkie2_q4_pair")
         return out
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
