@@ -284,8 +284,8 @@ __device__ __forceinline__ void list_items(const MoeArgs& p, uint32_t thread, co
 // numbers 102.4 us for the layer instead of 105.3 (8 x 2048 66.5 and 67.2, 4 x 2048 42.9 and 42.3,
 // 8 x 512 18.3 and 17.1)
 constexpr uint32_t kShareDigits = 4096;
-constexpr uint32_t kUpBatch = 16;                                       // tiles whose sums are held at a time
-constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile, gate or up, token, column)
+// Sums of a batch of tiles: (tile, gate or up, token, column)
+constexpr uint32_t up_cells(uint32_t batch) { return batch * 2 * kTile * 16; }
 
 // The tiles of 16 hidden columns that a block takes, u = blockIdx.x + i
 // gridDim.x for i = 0, 1, ..: first those of the shared experts (four tokens
@@ -303,20 +303,21 @@ constexpr uint32_t kUpCells = kUpBatch * 2 * kTile * 16;                // (tile
 // instead of 103).  Two blocks to a cluster share the digits and the router:
 // clusters of four or eight would share more, but only 132 or 120 of their
 // blocks run at once.
-template <bool TWO, int DEPTH, int RUN>
+template <bool TWO, int DEPTH, int RUN, uint32_t BATCH>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Items items;
     __shared__ uint32_t s_mask[kMaxExperts], s_start[kMaxExperts], s_sel[kMaxSlots];
     __shared__ __align__(8) uint64_t s_bar[kWarps * DEPTH];
     constexpr uint32_t kBytes = TWO ? 576 : 544, kPair = 2 * kBytes, kSlot = RUN * kPair;  // gate and up
+    constexpr uint32_t kCells = up_cells(BATCH);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t pitch = (p.etiles + 1) / 2 * 16, rank = cluster.block_rank();
     uint8_t* ring = smem + (size_t)warp * DEPTH * kSlot;
-    const Limbs acc{reinterpret_cast<uint32_t*>(smem + (size_t)kWarps * DEPTH * kSlot), kUpCells};
-    const Limbs sums{acc.w, p.m * pitch};  // of the logits, before the tiles': at most kUpCells
-    long long* logits = reinterpret_cast<long long*>(acc.w + 3 * kUpCells);  // of the pair's even tiles, then the odd ones
+    const Limbs acc{reinterpret_cast<uint32_t*>(smem + (size_t)kWarps * DEPTH * kSlot), kCells};
+    const Limbs sums{acc.w, p.m * pitch};  // of the logits, before the tiles': at most kCells
+    long long* logits = reinterpret_cast<long long*>(acc.w + 3 * kCells);  // of the pair's even tiles, then the odd ones
     uint8_t* digits = reinterpret_cast<uint8_t*>(logits + 2 * p.m * pitch);
     const uint32_t bar = shared_addr(&s_bar[warp * DEPTH]);
     cluster_arrive();  // both blocks have started before one writes into the other's shared memory
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     const uint32_t ft = p.up.s.tiles, st = p.sup.s.tiles, stiles = st * ((p.m + kTile - 1) / kTile);
     const uint32_t blocks = p.up.s.blocks;
     auto tiles_below = [&](uint32_t u) { return u > blockIdx.x ? (u - blockIdx.x + gridDim.x - 1) / gridDim.x : 0u; };
-    const uint32_t early = min(tiles_below(stiles), kUpBatch);  // tiles of the batch before the routing
+    const uint32_t early = min(tiles_below(stiles), BATCH);  // tiles of the batch before the routing
     const uint32_t early_warps = kWarps - route_warps(p.m);
     uint32_t known = early;                                     // tiles of this block that may be asked for
     // of n tiles' blocks, the first that warp w takes if `warps` share them (all past the last)
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
         while (next_at == next_end) {
             if (next_first + next_n >= known) return false;
             next_first += next_n;
-            next_n = min(next_first == early && early < kUpBatch ? kUpBatch - early : kUpBatch, known - next_first);
+            next_n = min(next_first == early && early < BATCH ? BATCH - early : BATCH, known - next_first);
             next_at = first_block(next_n, warp, kWarps);
             next_end = first_block(next_n, warp + 1, kWarps);
         }
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     if (lane == 0) ask();
 
     // ---- the rows' digits and the logits
-    for (uint32_t i = threadIdx.x; i < 3 * kUpCells; i += kThreads) acc.w[i] = 0;
+    for (uint32_t i = threadIdx.x; i < 3 * kCells; i += kThreads) acc.w[i] = 0;
     for (uint32_t i = threadIdx.x; i < p.experts; i += kThreads) s_mask[i] = 0;
     wait_for_previous();
     bool bad = false;
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     // ---- the batches; routing beside the first, of the shared experts, whose sums are held to be
     // finished with the next batch's
     uint32_t base = 0;
-    for (uint32_t first = 0, n = early;; n = min(kUpBatch - base, known - first)) {
+    for (uint32_t first = 0, n = early;; n = min(BATCH - base, known - first)) {
         const bool routing = !routed;
         add_up(first, n, routing ? early_warps : kWarps, base);
         if (routing) {
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
                     reinterpret_cast<uint32_t*>(p.items)[i] = reinterpret_cast<const uint32_t*>(&items)[i];
         }
         first += n;
-        if (routing && early < kUpBatch && first < known) {
+        if (routing && early < BATCH && first < known) {
             base = early;
             continue;
         }
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     patience_end(patience, p.err);
 }
 
-constexpr int kDownDepth = 3;
+constexpr int kDownDepth = 2;     // slots of a ring (three: the same times)
 constexpr uint32_t kDownRun = 2;  // blocks to a slot
 
 // Blocks of the stream that a warp of k_moe_down takes: the chosen experts'
@@ -715,15 +716,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
 }
 
 // Dynamic shared memory of k_moe_up
-size_t up_shared(uint32_t m, uint32_t stride, uint32_t etiles, uint32_t bytes, uint32_t blocks) {
-    return (size_t)kWarps * blocks * 2 * bytes + 12 * kUpCells + (size_t)m * (4 * stride + 2 * 16 * 8 * ((etiles + 1) / 2));
+size_t up_shared(uint32_t m, uint32_t stride, uint32_t etiles, uint32_t bytes, uint32_t blocks, uint32_t batch) {
+    return (size_t)kWarps * blocks * 2 * bytes + 12 * up_cells(batch) + (size_t)m * (4 * stride + 2 * 16 * 8 * ((etiles + 1) / 2));
 }
 
-constexpr uint32_t kUpShallow = 3, kUpDeep = 6;  // blocks in a warp's ring: three slots of one or of two
 
 uint32_t tokens_at_once(uint32_t stride, uint32_t etiles, uint32_t bytes) {
     uint32_t m = kMaxTokens;
-    while (m > 1 && up_shared(m, stride, etiles, bytes, kUpShallow) > kMaxShared) m--;
+    while (m > 1 && up_shared(m, stride, etiles, bytes, 3, 16) > kMaxShared) m--;
     return m;
 }
 
@@ -738,20 +738,27 @@ bool moe_shapes(uint64_t h, uint64_t experts, uint64_t top_k, uint64_t f, uint64
            q4_shape(h, shared_f, group, 0, &s->sup) && q4_shape(shared_f, h, group, 0, &s->sdown);
 }
 
-template <bool TWO, int DEPTH, int RUN>
+template <bool TWO, int DEPTH, int RUN, uint32_t BATCH>
 int up_launch(const MoeArgs& p, cudaStream_t stream) {
     static std::atomic<uint64_t> set{0};
-    auto* kernel = k_moe_up<TWO, DEPTH, RUN>;
+    auto* kernel = k_moe_up<TWO, DEPTH, RUN, BATCH>;
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(kernel), kMaxShared, &set));
-    return launch(kernel, dim3(kSms), kThreads, up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, DEPTH * RUN), 2, stream, p);
+    return launch(kernel, dim3(kSms), kThreads, up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, DEPTH * RUN, BATCH), 2, stream, p);
 }
 
 template <bool TWO>
 int moe_launch(MoeArgs p, cudaStream_t stream) {
-    // two blocks to a slot where there is room: 66.5 us instead of 69.1 for eight tokens of 2048, the
-    // same for one (22.8 to 23.1)
-    const bool deep = up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, kUpDeep) <= kMaxShared;
-    const int rc = deep ? up_launch<TWO, 3, 2>(p, stream) : up_launch<TWO, 3, 1>(p, stream);
+    auto fits = [&](uint32_t blocks, uint32_t batch) {
+        return p.m * ((p.etiles + 1) / 2 * 16) <= up_cells(batch) &&
+               up_shared(p.m, p.stride, p.etiles, p.up.s.bytes, blocks, batch) <= kMaxShared;
+    };
+    // A ring of two slots of two blocks, with batches of eight tiles where those of sixteen leave no
+    // room for it, else of three slots of one (twelve tokens of 2048: 76.5, 79.1 and 82.2 us, sixteen
+    // 91.4 and 94.4; three slots of two: 59.5 us for eight tokens instead of 58.6, 22.8 for one
+    // instead of 22.3).
+    const int rc = fits(4, 16)  ? up_launch<TWO, 2, 2, 16>(p, stream)
+                   : fits(4, 8) ? up_launch<TWO, 2, 2, 8>(p, stream)
+                                : up_launch<TWO, 3, 1, 16>(p, stream);
     if (rc) return rc;
     static std::atomic<uint64_t> set{0};
     ZK_TRY(allow_shared(reinterpret_cast<const void*>(k_moe_down<TWO>), kMaxShared, &set));
