@@ -125,7 +125,7 @@ struct ProjectArgs {
     uint32_t some, more;  // tiles of a grid's block: some, and one more in the first `more` of them
 };
 
-constexpr int kProjDepth = 3;           // slots of a warp's ring
+constexpr int kProjDepth = 2;           // slots of a warp's ring (three: one row of 1024 x 65536 10.6 us instead of 10.2)
 constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 
 // A block takes an equal run of the tiles of 16 columns, in batches; of a
@@ -135,13 +135,14 @@ constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 // per output then rounds and finishes it.
 //
 // Bound by: for few rows and a wide weight the weight's bytes (1024 x 65536 in
-// groups of 128, one row: 36 MB in 10.6 us, of which 3 us are the launch, the
-// row's digits and the last sums: 4.8 TB/s in between); for eight rows what a
-// warp does per block and pair of rows, about ten cycles of the SM (18.3 us:
+// groups of 128, one row: 36 MB in 10.2 us, of which 3 us are the launch, the
+// row's digits and the last sums: 5 TB/s in between); for eight rows what a
+// warp does per block and pair of rows, about ten cycles of the SM (17.9 us:
 // 2.0 TB/s); for a small weight the launch and three trips to memory (1024 x
 // 192: 3.0 us).  A ring's slots are of four blocks because copies of 2176
-// bytes reach 5.8 TB/s and single blocks 3.7; 24 warps of 80 registers instead
-// of 16 of 127 take 20.8 us for the eight rows, 20 warps 19.9.
+// bytes reach 5.8 TB/s and single blocks 3.7 (eight blocks to a slot: within 4
+// % either way); with three slots to a ring, 24 warps of 80 registers instead
+// of 16 of 127 take 20.8 us for the eight rows instead of 18.3, 20 warps 19.9.
 template <int G, int NT, bool SEG>
 __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_constant__ ProjectArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             if (!SEG && run == 4 && (G != 128 || unit == 4)) {
 #pragma unroll
                 for (uint32_t q = 0; q < 4; q += 2) {
-                    if (G == 128) {  // two whole groups (block by block: 20.2 us instead of 18.3)
+                    if (G == 128) {  // two whole groups (eight rows block by block: 10 % more)
                         uint4 x[2][NT];
 #pragma unroll
                         for (int i = 0; i < 2 * NT; i++) x[i / NT][i % NT] = load16(x_at[i % NT] + (q + i / NT) * 64);
@@ -344,9 +345,9 @@ int project_seg(const ProjectArgs& p, cudaStream_t stream) {
 template <int G>
 int project_rows(ProjectArgs p, cudaStream_t stream) {
     // Rows to a block: as many as there are, up to eight, so that a weight is read once for them, and
-    // as their digits leave room for (1024 x 65536: eight rows 18.3 us, four 13.9, two 11.3, one row
-    // with eight's kernel 16.9 instead of 10.6).  Slots of four blocks where there is room, else of
-    // two or one (one row 10.6, 13.2, 18.0 us; a weight of 1024 x 192 in 3.0, 2.9, 2.8).
+    // as their digits leave room for (1024 x 65536: eight rows 17.9 us, four 13.5, two 10.8, one 10.2,
+    // one row with eight's kernel 16.9).  Slots of four blocks where there is room, else of two or one
+    // (one row 10.6, 13.2, 18.0 us, of rings of three; a weight of 1024 x 192 in 3.0, 2.9, 2.8).
     for (uint32_t rows = p.m > 4 ? 8 : p.m > 2 ? 4 : 2;; rows /= 2)
         for (p.run = 4; p.run; p.run /= 2)
             if (p.unit = p.s.segs > 1 ? p.s.kp_seg / 64 : p.s.blocks % p.run ? 1 : p.run;
