@@ -295,14 +295,14 @@ constexpr uint32_t up_cells(uint32_t batch) { return batch * 2 * kTile * 16; }
 // Bound by (2048 wide, 64 experts of 1408, six to a token, the shared ones
 // 2816): for one token a chain -- digits 2.1 us, logits 3.3, routing 3.4 beside
 // the shared experts' first tiles, then the chosen experts' tiles 5 (20 MB: 4
-// TB/s); for sixteen the same chain (6.2, 6.6 and 9.8 us) and 46 us over the
-// gate and up of the 51 or so chosen experts (162 MB: 3.5 TB/s), which is the
-// warps' own work: codes taken apart, scales, slots asked for (issue slots 53 %
-// used over the whole kernel, matrix pipe 12 %; the codes prefetched into the
-// second-level cache 4, 8 or 16 blocks ahead: 106 to 109 us for the layer
-// instead of 103).  Two blocks to a cluster share the digits and the router:
-// clusters of four or eight would share more, but only 132 or 120 of their
-// blocks run at once.
+// TB/s); for sixteen the same chain (6.2, 6.6 and 9.8 us) and some 43 us over
+// the gate and up of the 51 or so chosen experts (162 MB: 3.8 TB/s), which is
+// the warps' own work: codes taken apart, scales, slots asked for (issue slots
+// 53 % used over the whole kernel, matrix pipe 12 %).  The codes prefetched into
+// the second-level cache 4, 8 or 16 blocks ahead: 3 to 6 % slower; the router's
+// blocks through the rings, ahead of the first codes: 4 %.  Two blocks to a
+// cluster share the digits and the router: clusters of four or eight would
+// share more, but only 132 or 120 of their blocks run at once.
 template <bool TWO, int DEPTH, int RUN, uint32_t BATCH>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -571,10 +571,13 @@ struct DownAt {
 // A pair of blocks to 32 output columns, half of the stream each; digits come
 // with the codes, a slot's copies under one barrier.
 //
-// Bound by (sizes as above): one token 7 us, of which 1.5 pass before the items
-// are there and 4 stream 10 MB; sixteen tokens 33 us, 3 before the items, 26 over
-// 81 MB of codes (3.2 TB/s) and as many bytes of digits from the second-level
-// cache, in copies of 1088 and 512 bytes.
+// Bound by (sizes as above): one token 6.5 us, of which 1.5 pass before the
+// items are there and 3.5 stream 10 MB; sixteen tokens some 25 us, 3 before the
+// items, 18 over 81 MB of codes (4.5 TB/s) and as many bytes of digits from the
+// second-level cache, by the number of copies: two to a slot, one of 2176 bytes
+// of codes and one of digits, where a copy to each tile and token took the layer
+// from 94 to 103 us.  Slots of more blocks but fewer tokens' digits, two or
+// three blocks by what fits: 97 to 104 us.
 template <bool TWO>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant__ MoeArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
