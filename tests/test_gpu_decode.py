@@ -462,3 +462,16 @@ def test_numbers_beyond_the_field(zk):
     q = _quant(zk, w, 64)
     beyond = torch.from_numpy((x.astype(np.uint64) + np.uint64(0xFFFFFFFF00000001))).cuda()
     assert np.array_equal(_s(zk.decode.project(beyond, q, 10)), ref.project(x, *w, 64, 0, 10))
+
+
+@pytest.mark.parametrize("m,h,experts,top_k,f,shared,group", [
+    (16, 2048, 20, 3, 32, 40, 64), (16, 2048, 20, 3, 33, 500, 32), (15, 2048, 256, 4, 20, 24, 128),
+    (12, 2048, 10, 4, 100, 300, 64)])
+def test_moe_block_of_many_wide_tokens(zk, m, h, experts, top_k, f, shared, group):
+    """Tokens whose digits leave less room for rings and sums."""
+    rng = np.random.default_rng(h + experts)
+    router, w = _moe_case(rng, h, experts, f, shared, group)
+    x, exp_table, silu = rng.integers(-(1 << 17), 1 << 17, (m, h)), _exp_table(), _silu_table()
+    out, gate = _moe_block(zk, router, w, group, top_k, exp_table, silu).forward(_u(x))
+    want, want_gate = ref.moe(x, router, w, group, exp_table, silu, top_k)
+    assert np.array_equal(_s(gate), want_gate) and np.array_equal(_s(out), want)
