@@ -44,7 +44,8 @@ inline uint32_t clusters_at_once(const void* kernel, int threads, size_t shared,
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) cudaGetLastError();  // not the launch's
+    if (n < 1) n = 1;
     known[cluster].store((uint32_t)n, std::memory_order_relaxed);
     return (uint32_t)n;
 }
