@@ -463,14 +463,16 @@ struct AttendArgs {
 // A product is one 32 x 32 + 64 bit multiply-add, 32 a clock on an SM.
 //
 // Bound by: for one long sequence the two streams (16 heads of 192 + 128, 4096
-// tokens: 82 MB in 26.8 us, keys 8.5 us and values 6 at 4.5 to 5 TB/s, between
-// them 7 us of meetings and table entries, the first bytes 4); for a ragged
+// tokens: 82 MB in 26.6 us, keys 10 us and values 7 at 4.5 to 5 TB/s, between
+// them 7 us of meetings and table entries, the first bytes 2); for a ragged
 // batch the longest sequence's blocks, whose cluster is as large as any other
-// (eight sequences of up to 8192 tokens, four query heads to a key head: 71
+// (eight sequences of up to 8192 tokens, four query heads to a key head: 69
 // us, of which multiply-adds cost 12, table entries 10, the streams the
 // rest); for a short one the chain of latencies (512 tokens: 8.5 us).  Half
 // the heads' products in double precision: 69 us instead of 71, not kept; an
-// L2 prefetch of the values during the softmax: 29 to 32 us instead of 27.
+// L2 prefetch of the values during the softmax: 29 to 32 us instead of 27; the
+// table's entries asked for sixteen at a time by a thread: the same 71, their
+// number is what costs.
 template <int EACH, int WIDE>
 __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_constant__ AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -492,6 +494,13 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     __syncwarp();
     wait_for_previous();
 
+    // The queries, asked for before the first keys: behind them they arrive 2 us later
+    uint64_t q_in[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; u++) {
+        const uint32_t i = threadIdx.x + u * kAttThreads;  // dk <= kAttThreads
+        q_in[u] = i < heads * dk ? __ldg(p.q + seq * p.ldq + (uint64_t)(h * p.each + e0) * dk + i) : 0;
+    }
     const int64_t len = p.c.lens[seq];
     const bool append = p.rows.k != nullptr && len >= 0 && len < p.c.cap;
     if (p.rows.k != nullptr && len >= p.c.cap && threadIdx.x == 0) atomicOr(p.err, kErrFull);
@@ -566,17 +575,15 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     };
 
     bool bad = false;
-    for (uint32_t i = threadIdx.x; i < EACH * dk; i += kAttThreads) {
-        int64_t y = 0;
-        if (i / dk < heads) {
-            const int64_t x = fx_to_i64(__ldg(p.q + seq * p.ldq + (uint64_t)(h * p.each + e0) * dk + i));
-            y = round_shift(fx_wmul(x, p.q_factor), p.q_shift);
-            if (y < -kKeyLimit || y > kKeyLimit) {
-                bad = true;
-                y = 0;
-            }
+#pragma unroll
+    for (int u = 0; u < EACH; u++) {
+        const uint32_t i = threadIdx.x + u * kAttThreads;
+        int64_t y = round_shift(fx_wmul(fx_to_i64(q_in[u]), p.q_factor), p.q_shift);
+        if (y < -kKeyLimit || y > kKeyLimit) {
+            bad = true;
+            y = 0;
         }
-        qs[i] = (int)y;
+        if (i < EACH * dk) qs[i] = (int)y;
     }
     if (own)  // store the new token (blocks of other query heads of this key head store the same numbers)
         for (uint32_t d = threadIdx.x; d < dk + dv; d += kAttThreads)
@@ -1051,7 +1058,7 @@ int zkie2_kv_attend(const uint64_t* d_q, uint64_t ldq, uint64_t q_heads, int64_t
     p.out = d_out;
     p.err = d_err;
     // Query heads to a block: those that share a key head, up to four (a ragged batch of eight with four
-    // heads to a key head: 71 us, two at a time 77; two at most where a value row is wider than 128:
+    // heads to a key head: two at a time 9 % more; two at most where a value row is wider than 128:
     // their sums stay in registers), fewer where their scores do not fit.  Blocks
     // to a cluster: enough to fill the device with two to an SM, of four token blocks at least, up
     // to eight, as many as find room at once (264 blocks in clusters of eight, 284 in smaller ones,
