@@ -137,9 +137,9 @@ constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 // Bound by: for few rows and a wide weight the weight's bytes (1024 x 65536 in
 // groups of 128, one row: 36 MB in 10.2 us, of which 3 us are the launch, the
 // row's digits and the last sums: 5 TB/s in between); for eight rows what a
-// warp does per block and pair of rows, about ten cycles of the SM (17.9 us:
-// 2.0 TB/s); for a small weight the launch and three trips to memory (1024 x
-// 192: 3.0 us).  A ring's slots are of four blocks because copies of 2176
+// warp does per block and pair of rows, about ten cycles of the SM (17.5 us:
+// 2.1 TB/s); for a small weight the launch and three trips to memory (1024 x
+// 192: 2.9 us).  A ring's slots are of four blocks because copies of 2176
 // bytes reach 5.8 TB/s and single blocks 3.7 (eight blocks to a slot: within 4
 // % either way); with three slots to a ring, 24 warps of 80 registers instead
 // of 16 of 127 take 20.8 us for the eight rows instead of 18.3, 20 warps 19.9.
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
             if (next_batch < tile1) ask();
 
     // ---- the rows' digits
-    for (uint32_t i = threadIdx.x; i < 3 * kCells; i += kProjThreads) acc.w[i] = 0;
+    acc.template clear<kProjThreads>();
     wait_for_previous();
     if (!q4_digitise<kProjThreads, 4>(p.x + (uint64_t)row0 * p.ldx, p.ldx, p.s.segs, p.s.k_seg, p.s.kp_seg, 0,
                                    rows * blocks * 16, digits, p.stride))
@@ -284,37 +284,38 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
         if (b) flush();
         __syncthreads();
         const uint32_t tiles = min(kProjBatch, tile1 - batch);
-        constexpr int kOuts = 4;  // outputs of a thread whose operands are under way together
-        for (uint32_t o0 = threadIdx.x; o0 < tiles * kRows * 16; o0 += kProjThreads * kOuts) {
-            uint64_t bias[kOuts], residual[kOuts];
+        // a thread's outputs, NT of a batch: one row and one column of 16 in every kStep-th tile, their
+        // operands under way together
+        constexpr uint32_t kStep = kProjBatch / NT;
+        const uint32_t r = threadIdx.x / 16 % kRows, tile1st = threadIdx.x / (16 * kRows);
+        const uint32_t n1st = (batch + tile1st) * 16 + threadIdx.x % 16;
+        bool on[NT];
+        uint64_t bias[NT], residual[NT];
 #pragma unroll
-            for (int u = 0; u < kOuts; u++) {
-                const uint32_t o = o0 + u * kProjThreads, r = o / 16 % kRows, n = (batch + o / (kRows * 16)) * 16 + o % 16;
-                const bool on = o < tiles * kRows * 16 && r < rows && n < p.s.n;
-                bias[u] = on && p.bias ? __ldg(p.bias + n) : 0;
-                residual[u] = on && p.residual ? __ldg(p.residual + (row0 + r) * p.ldr + n) : 0;
-            }
-            int64_t y[kOuts];
-#pragma unroll
-            for (int u = 0; u < kOuts; u++) {
-                const uint32_t o = o0 + u * kProjThreads;
-                if (o >= tiles * kRows * 16) continue;
-                y[u] = SEG ? acc.get(o) : round_shift(acc.get(o), p.shift);
-                acc.clear(o);
-                y[u] = fx_wadd(y[u], fx_to_i64(bias[u]));
-            }
-            uint64_t f[kOuts];
-#pragma unroll
-            for (int u = 0; u < kOuts; u++)
-                f[u] = o0 + u * kProjThreads >= tiles * kRows * 16 ? 0
-                       : p.table ? gl_canon(table_at(p.table, p.table_len, y[u], p.offset)) : fx_from_i64(y[u]);
-#pragma unroll
-            for (int u = 0; u < kOuts; u++) {
-                const uint32_t o = o0 + u * kProjThreads, r = o / 16 % kRows, n = (batch + o / (kRows * 16)) * 16 + o % 16;
-                if (o < tiles * kRows * 16 && r < rows && n < p.s.n)
-                    p.out[(row0 + r) * (uint64_t)p.s.n + n] = p.residual ? gl_canon(gl_add(f[u], gl_canon(residual[u]))) : f[u];
-            }
+        for (int u = 0; u < NT; u++) {
+            const uint32_t n = n1st + u * kStep * 16;
+            on[u] = r < rows && tile1st + u * kStep < tiles && n < p.s.n;
+            bias[u] = on[u] && p.bias ? __ldg(p.bias + n) : 0;
+            residual[u] = on[u] && p.residual ? __ldg(p.residual + (uint64_t)(row0 + r) * p.ldr + n) : 0;
         }
+        uint64_t f[NT];
+#pragma unroll
+        for (int u = 0; u < NT; u++) {
+            f[u] = 0;
+            if (!on[u]) continue;
+            const uint32_t o = threadIdx.x + u * kProjThreads;
+            int64_t y = SEG ? acc.get(o) : round_shift(acc.get(o), p.shift);
+            acc.clear(o);
+            y = fx_wadd(y, q4_number(bias[u]));
+            f[u] = p.table ? table_at(p.table, p.table_len, y, p.offset) : fx_from_i64(y);
+        }
+        uint64_t* out = p.out + (uint64_t)(row0 + r) * p.s.n + n1st;
+#pragma unroll
+        for (int u = 0; u < NT; u++)
+            if (on[u]) {
+                if (p.table) f[u] = gl_canon(f[u]);
+                out[u * kStep * 16] = p.residual ? gl_canon(gl_add(f[u], gl_canon(residual[u]))) : f[u];
+            }
         __syncthreads();
     }
     patience_end(patience, p.err);
@@ -345,7 +346,7 @@ int project_seg(const ProjectArgs& p, cudaStream_t stream) {
 template <int G>
 int project_rows(ProjectArgs p, cudaStream_t stream) {
     // Rows to a block: as many as there are, up to eight, so that a weight is read once for them, and
-    // as their digits leave room for (1024 x 65536: eight rows 17.9 us, four 13.5, two 10.8, one 10.2,
+    // as their digits leave room for (1024 x 65536: eight rows 17.5 us, four 13.7, two 10.7, one 10.2,
     // one row with eight's kernel 16.9).  Slots of four blocks where there is room, else of two or one
     // (one row 10.6, 13.2, 18.0 us, of rings of three; a weight of 1024 x 192 in 3.0, 2.9, 2.8).
     for (uint32_t rows = p.m > 4 ? 8 : p.m > 2 ? 4 : 2;; rows /= 2)

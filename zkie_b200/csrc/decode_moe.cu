@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     if (lane == 0) ask();
 
     // ---- the rows' digits and the logits
-    for (uint32_t i = threadIdx.x; i < 3 * kCells; i += kThreads) acc.w[i] = 0;
+    acc.template clear<kThreads>();
     for (uint32_t i = threadIdx.x; i < p.experts; i += kThreads) s_mask[i] = 0;
     wait_for_previous();
     bool bad = false;
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         barrier_init_done();
     }
     __syncwarp();
-    for (uint32_t i = threadIdx.x; i < 3 * cells; i += kThreads) acc.w[i] = 0;
+    acc.template clear<kThreads>();
     const uint32_t pairs = (p.down.s.tiles + 1) / 2, pair = blockIdx.x / 2;
     if (threadIdx.x == 0)  // the shared experts' codes of these columns start for the second-level cache
         prefetch_l2(p.sdown.w + (uint64_t)pair * p.sdown.s.blocks * 2 * kBytes, p.sdown.s.blocks * 2 * kBytes);

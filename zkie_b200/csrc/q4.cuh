@@ -85,10 +85,14 @@ __device__ __forceinline__ void mma_s8_new(int (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 
-// q4_digits of a field element's number: v, less p = 2^64 - 0xFFFFFFFF from 2^63 on, in the few
-// instructions of which a block spends one set on every number of its rows
+// fx_to_i64 in three instructions: v, less p = 2^64 - 0xFFFFFFFF from 2^63 on
+__device__ __forceinline__ int64_t q4_number(uint64_t v) {
+    return (int64_t)(v + (uint32_t)((int32_t)(v >> 32) >> 31));
+}
+
+// q4_digits of a field element, which every block does for every number of its rows
 __device__ __forceinline__ bool q4_digits_of(uint64_t v, uint32_t* d) {
-    const uint64_t x = v + (uint32_t)((int32_t)(v >> 32) >> 31), t = x + 0x7F7F7F7Fu;
+    const uint64_t t = (uint64_t)q4_number(v) + 0x7F7F7F7Fu;
     const bool ok = t <= 0xFEFEFEFEull;
     *d = ok ? ((uint32_t)t + 0x01010101u) ^ 0x80808080u : 0u;
     return ok;
@@ -294,6 +298,10 @@ struct Limbs {
                            ((unsigned long long)w[2 * n + at] << 44));
     }
     __device__ __forceinline__ void clear(uint32_t at) const { w[at] = w[n + at] = w[2 * n + at] = 0; }
+    template <int THREADS>  // all of them (four and a 16-byte boundary at least), by a whole block
+    __device__ __forceinline__ void clear() const {
+        for (uint32_t i = threadIdx.x; i < 3 * n / 4; i += THREADS) reinterpret_cast<uint4*>(w)[i] = make_uint4(0, 0, 0, 0);
+    }
 };
 
 // A lane's place in a block in shared memory: its codes, and its scales
