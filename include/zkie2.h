@@ -702,8 +702,9 @@ int zkie2_kv_attend(const uint64_t *d_q, uint64_t ldq, uint64_t q_heads, int64_t
  * the shared experts (hidden shared_f) with weights of one group;
  * h_weights: a host array of 4 device pointers, all from zkie2_q4_pair (gate
  * and up, down's tiles two by two, the same of the shared experts); the router
- * packed from h x experts field elements of at most 32639 in size.  Every Scale divides by 2^shift; the silu table is
- * indexed from its middle.  experts <= 256, top_k <= 16, |x| and |silu(gate)
+ * packed from h x experts field elements of at most 32639 in size.  The shared
+ * experts' Projections divide by 2^shift, every Scale and ScaleVec by 2^16 as
+ * in the graph; the silu table is indexed from its middle.  experts <= 256, top_k <= 16, |x| and |silu(gate)
  * up| <= 0x7F7F7F7F.  out: m x h (+ residual); gate (may be null): m x
  * experts, TopKSelect's gate.  d_scratch: 16-byte aligned. */
 uint64_t zkie2_moe_router_words(uint64_t h, uint64_t experts);

@@ -1,0 +1,45 @@
+"""The single-token decoders on the device at other shapes than the models'
+own: bit for bit the graph's rows, or a refusal."""
+import numpy as np
+import pytest
+
+from tests import decode_ref as ref, decode_shapes as ds_ref
+from tests.test_gpu_decode import _moe_case, _quant, _s, _u
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("shift", [0, 9, 14, 20])
+@pytest.mark.parametrize("m,h,experts,top_k,f,shared,group", [
+    (1, 64, 8, 2, 48, 96, 64), (3, 100, 17, 3, 40, 33, 32), (17, 64, 4, 4, 32, 16, 128)])
+def test_moe_block_shared_shift(zk, m, h, experts, top_k, f, shared, group, shift):
+    """The shift is the shared experts' Projections'; small numbers, so that a
+    shift of none keeps them in range."""
+    rng = np.random.default_rng(m + shift)
+    router, w = _moe_case(rng, h, experts, f, shared, group)
+    if shift < 12:  # |gate|, |up| of the shared experts below 2^22, silu(gate) up / 2^16 below 2^31
+        w[3:] = [(c, np.minimum(s, 1)) for c, s in w[3:]]
+    x = rng.integers(-(1 << (17 if shift >= 12 else 10)), 1 << (17 if shift >= 12 else 10), (m, h))
+    exp, silu = ds_ref.exp_table(), ds_ref.silu_table()
+    block = zk.decode.MoeBlock(_u(router), *[_quant(zk, t, group) for t in w], _u(exp), _u(silu), top_k, shift)
+    out, gate = block.forward(_u(x))
+    want, want_gate = ds_ref.moe(x, router, w, group, exp, silu, top_k, shift)
+    assert np.array_equal(_s(gate), want_gate)
+    assert np.array_equal(_s(out), want)
+
+
+@pytest.mark.parametrize("shift", [13, 14, 18])
+def test_moe_layer_steps_equal_the_graph_at_other_shifts(zk, shift):
+    import torch
+    from zkie_b200 import deepseek as ds
+    s = ds.MoeShape(**ds_ref.MOE, shift=shift)
+    store = zk.compose.Store()
+    ops, x, out = ds.moe_layer(store, s)
+    weights = zk.decode.quantise_weights(store, ops)
+    zk.compose.forward_ops(store, ops)
+    rows = lambda t: store.get(t).view(torch.int64).reshape(s.m, s.h)  # noqa: E731
+    dec = ds.MoeLayerDecoder(store, ops, s, weights, 2)
+    for i in range(s.m):
+        got = dec.step(rows(x)[i:i + 1].expand(2, s.h).contiguous().view(torch.uint64))
+        assert torch.equal(got.view(torch.int64), rows(out)[i:i + 1].expand(2, s.h)), i
+    dec.check()

@@ -46,6 +46,7 @@ constexpr uint32_t kTile = 4;        // tokens of an expert taken at a time
 constexpr uint32_t kMaxSlots = kMaxTokens * kMaxTop;
 constexpr size_t kMaxShared = 220 * 1024;
 constexpr int32_t kRouterLimit = 32639;  // two signed bytes
+constexpr uint32_t kScale = 16;  // build_moe divides by 2^16 (:252-470), except in the shared experts' Projections
 
 struct Q4Weight {
     const uint8_t* w;
@@ -75,7 +76,7 @@ struct MoeArgs {
     uint64_t exp_len;
     const uint64_t* silu;
     uint64_t silu_len;
-    uint32_t shift;
+    uint32_t shift;  // of the shared experts' Projections
     const uint64_t* residual;
     uint64_t ldr;
     uint64_t* out;
@@ -193,7 +194,7 @@ __device__ __forceinline__ void route_token(const MoeArgs& p, uint32_t r, const 
         const uint32_t e = i * 32 + lane;
         z[i] = INT64_MIN;
         if (e < p.experts) {
-            z[i] = round_shift((e / 16 % 2 ? odd : even)[r * pitch + e / 32 * 16 + e % 16], p.shift);
+            z[i] = round_shift((e / 16 % 2 ? odd : even)[r * pitch + e / 32 * 16 + e % 16], kScale);
             top = max(top, z[i]);
         }
     }
@@ -493,8 +494,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
                 const uint32_t count = shared ? min(kTile, p.m - tok0) : items.count[item];
                 if (j >= count) continue;  // its sums are zero
                 const uint32_t cell = (i * 2 * kTile + j) * 16 + c;
-                const int64_t gi = round_shift(acc.get(cell), p.shift);
-                up[q] = round_shift(acc.get(cell + kTile * 16), p.shift);
+                const uint32_t shift = shared ? p.shift : kScale;
+                const int64_t gi = round_shift(acc.get(cell), shift);
+                up[q] = round_shift(acc.get(cell + kTile * 16), shift);
                 acc.clear(cell);
                 acc.clear(cell + kTile * 16);
                 if (f >= (shared ? p.sup.s.n : p.up.s.n)) continue;
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
             for (int q = 0; q < kOuts; q++)
                 if (to[q]) {
                     uint32_t d;
-                    bad |= !q4_digits(round_shift(fx_wmul(fx_to_i64(silu[q]), up[q]), p.shift), &d);
+                    bad |= !q4_digits(round_shift(fx_wmul(fx_to_i64(silu[q]), up[q]), kScale), &d);
 #pragma unroll
                     for (int b = 0; b < 4; b++) to[q][64 * b] = (uint8_t)(d >> (8 * b));
                 }
@@ -707,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         int64_t y = round_shift(fx_wadd(acc.get(s), there.get(s)), p.shift);
         for (uint32_t j = 0; j < p.top_k; j++) {
             const uint32_t k = (r * p.top_k + j) * 32 + c;
-            const int64_t d = round_shift(fx_wadd(acc.get(k), there.get(k)), p.shift);
+            const int64_t d = round_shift(fx_wadd(acc.get(k), there.get(k)), kScale);
             y = fx_wadd(y, round_shift(fx_wmul(d, items.score[r * p.top_k + j]), 16));
         }
         uint64_t f = fx_from_i64(y);

@@ -327,7 +327,9 @@ class MoeBlock:
     and down (experts x f x h) and the shared experts' gate, up (h x shared f)
     and down weights, all of one group without segments, the exp and silu
     tables (field elements; silu's middle is zero) and how many experts a token
-    takes.  The block keeps copies of its own of the weights."""
+    takes.  ``shift`` is the shared experts' Projections', as in the graph,
+    whose other products are all divided by 2^16.  The block keeps copies of
+    its own of the weights."""
 
     def __init__(self, router: torch.Tensor, gate: QuantWeight, up: QuantWeight, down: QuantWeight,
                  shared_gate: QuantWeight, shared_up: QuantWeight, shared_down: QuantWeight, exp_table: torch.Tensor,

@@ -19,6 +19,7 @@ for a few rows, one token at a time, with the weights of such a graph in 4
 bits (``decode.quantise_weights``), bit for bit the graph's rows.
 """
 from dataclasses import dataclass
+from typing import Optional
 
 import numpy as np
 import torch
@@ -260,19 +261,26 @@ def moe_layer(store, s: MoeShape = DSV2_LITE, seed: int = 0xD5E):
 
 
 # ---- token by token ---------------------------------------------------------------------------
-def moe_block(store, ops, weights: dict, exp_table: int, silu_table: int, shift: int = 16) -> decode.MoeBlock:
+def moe_block(store, ops, weights: dict, exp_table: int, silu_table: int, shift: Optional[int] = None) -> decode.MoeBlock:
     """The experts of a graph that ``build_moe`` built, for a few rows: the
     router as it is, the routed and the shared experts' weights from what
-    ``decode.quantise_weights(store, ops)`` returned."""
+    ``decode.quantise_weights(store, ops)`` returned, the shift of the shared
+    experts' Projections from the graph (one that is given has to be it)."""
     at = next(i for i, op in enumerate(ops) if op.kind == "TopKSelect")
     route, router = ops[at], ops[at - 4]  # MatMul, Scale, StableSoftmaxIndex, Softmax, TopKSelect
     experts = [op for op in ops[at:] if op.kind == "GatherMatMul"]
     shared = [op for op in ops[at:] if op.kind == "Projection"]
+    scales = [op for op in ops[at - 3:] if op.kind in ("Scale", "ScaleVec")]
     if router.kind != "MatMul" or len(experts) != 3 or len(shared) != 3:
         raise ValueError("moe_block: not a graph of build_moe")
+    if any((op.factor, op.shift) != (1, 16) for op in scales if op.kind == "Scale") or \
+            any(op.shift != 16 for op in scales if op.kind == "ScaleVec") or len({op.shift for op in shared}) != 1:
+        raise ValueError("moe_block: not a graph of build_moe: Scales by 2^16 and one shift of the shared experts are wanted")
+    if shift not in (None, shared[0].shift):
+        raise ValueError(f"moe_block: shift {shift}, the graph's shared experts have {shared[0].shift}")
     quant = lambda op: decode.QuantWeight(*weights[op.w])  # noqa: E731
     return decode.MoeBlock(store.get(router.b).reshape(router.k, router.n), *[quant(op) for op in experts + shared],
-                           store.get(exp_table), store.get(silu_table), route.k, shift)
+                           store.get(exp_table), store.get(silu_table), route.k, shared[0].shift)
 
 
 class MoeLayerDecoder:
