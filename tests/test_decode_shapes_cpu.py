@@ -57,3 +57,45 @@ def test_moe_block_refuses_other_scales(zk, monkeypatch, kind, field, value):
             block()
         setattr(op, field, was)
     block()
+
+
+# ---- tables with which a causal graph's masked columns would count ------------------------------------
+def test_masked_columns_count_where_the_table_does_not_begin_with_zero(zk):
+    """Why the decoders want a table that does: the graph's row counts table[0]
+    for every later position, attention over a cache knows none of them."""
+    rng, c, m = np.random.default_rng(2), zk.compose, 8
+    rows = {}
+    for bits in (19, 20, 21):
+        table = ref.signed(zk.gpt2.exp_table(bits))
+        st = co.HostStore()
+        push = lambda a: st.push(ref.field(np.ascontiguousarray(a).reshape(-1)))  # noqa: E731
+        z, idx, e, p = rng.integers(-(1 << 18), 1 << 18, (m, m)), st.push_idx(None), st.push(None), st.push(None)
+        co.forward_ops(st, [c.StableSoftmaxIndex(push(z), st.push(zk.gpt2.causal_mask(m)), idx, table.size, table.size, m, m),
+                            c.Softmax(idx, e, p, push(table), m, m)])
+        got = ref.signed(st.get(p)).reshape(m, m)
+        rows[bits] = all(np.array_equal(got[i, :i + 1], ref.softmax(z[i, :i + 1], table)) for i in range(m))
+        assert (table[0] == 0) == rows[bits]
+    assert rows == {19: False, 20: True, 21: True}
+
+
+def _gpt2_ops(zk, **shape):
+    s = zk.gpt2.LayerShape(**{**ds_ref.GPT2, **shape})
+    st = co.HostStore()
+    return st, zk.gpt2.gpt2_model(st, s, layers=1)[0], s
+
+
+def _moe_ops(zk, **shape):
+    from zkie_b200 import deepseek as ds
+    s = ds.MoeShape(**{**ds_ref.MOE, **shape})
+    st = co.HostStore()
+    return st, ds.moe_layer(st, s)[0], s
+
+
+def test_decoders_refuse_a_table_that_does_not_begin_with_zero(zk):
+    """Before anything else: no device is needed."""
+    from zkie_b200 import deepseek as ds
+    for bits in (16, 19):
+        with pytest.raises(ValueError, match="begins with zero"):
+            zk.gpt2.Gpt2Decoder(*_gpt2_ops(zk, exp_bits=bits), {})
+        with pytest.raises(ValueError, match="begins with zero"):
+            ds.MoeLayerDecoder(*_moe_ops(zk, exp_bits=bits), {})

@@ -43,3 +43,19 @@ def test_moe_layer_steps_equal_the_graph_at_other_shifts(zk, shift):
         got = dec.step(rows(x)[i:i + 1].expand(2, s.h).contiguous().view(torch.uint64))
         assert torch.equal(got.view(torch.int64), rows(out)[i:i + 1].expand(2, s.h)), i
     dec.check()
+
+
+# ---- what the decoders refuse -----------------------------------------------------------------------
+def test_decoders_refuse_a_table_that_does_not_begin_with_zero(zk):
+    """A table of 2^19 entries begins with 22, which the graph counts for every masked column."""
+    from zkie_b200 import deepseek as ds
+    store = zk.compose.Store()
+    s = zk.gpt2.LayerShape(**ds_ref.GPT2, exp_bits=19)
+    ops, _, _ = zk.gpt2.gpt2_model(store, s, layers=1)
+    with pytest.raises(ValueError, match="begins with zero"):
+        zk.gpt2.Gpt2Decoder(store, ops, s, zk.decode.quantise_weights(store, ops, ("Projection", "MatMul")))
+    store = zk.compose.Store()
+    s = ds.MoeShape(**{**ds_ref.MOE, "exp_bits": 19})
+    ops, _, _ = ds.moe_layer(store, s)
+    with pytest.raises(ValueError, match="begins with zero"):
+        ds.MoeLayerDecoder(store, ops, s, zk.decode.quantise_weights(store, ops))

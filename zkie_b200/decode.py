@@ -311,13 +311,26 @@ def attend(q: torch.Tensor, cache: KvCache, table: torch.Tensor, *, k: Optional[
     key through Scale (k_scale), and attended to; ``cache.advance`` then counts
     it.  Rows may be columns of a wider matrix.  A graph's masked columns count
     table[0] each in its softmax's sum: the rows agree where that is zero, as
-    in the models' tables.  A sequence without tokens answers zeros.  Scaled
+    in the models' tables from 2^20 entries on, and where no masked score is
+    2^30 - len(table) above the row's largest (the graph's mask takes off 2^30).
+    A sequence without tokens answers zeros.  Scaled
     queries and keys |q|, |k| <= 2^27; table values in [0, 2^31)."""
     word = _err_word() if err is None else err
     out = _calls.attend(q, cache.call, table, k, v, q_scale, k_scale, score_scale, offset, out_shift, out, word)
     if err is None:
         _check_err(word, "attend")
     return out
+
+
+def masked_counts_nothing(table, what: str):
+    """Refuse a causal graph's exp table that does not begin with zero: the
+    graph counts the first entry for every masked column of a softmax row, and
+    attention over a cache, which has no such columns, would answer other rows
+    (exp at scale 2^16 rounds to zero from 2^20 entries on)."""
+    first = int(_signed(table[:1])[0]) if isinstance(table, torch.Tensor) else int(table[0]) % P
+    if first:
+        raise ValueError(f"{what}: an exp table that begins with zero is wanted, this one with {first}: the graph's masked "
+                         "columns would count")
 
 
 # ---- a mixture-of-experts layer -----------------------------------------------------------------------

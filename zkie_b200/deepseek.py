@@ -288,15 +288,17 @@ class MoeLayerDecoder:
     side by side: RmsNorm, the kv latent with its norm and the rotated key that
     all heads share, the heads' q, k and v as wide projections, RoPE, attention
     over the cache (keys of nope + rope dimensions), the output projection
-    summed over the heads onto the residual, RmsNorm and ``moe_block``."""
+    summed over the heads onto the residual, RmsNorm and ``moe_block``.  The
+    graph's exp table begins with zero (exp_bits from 20 on)."""
 
     def __init__(self, store, ops, s: MoeShape, weights: dict, batch: int = 1):
+        soft = next(op for op in ops if op.kind == "Softmax")
+        decode.masked_counts_nothing(store.get(soft.table), "MoeLayerDecoder")
         self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
         wide = lambda t, n: store.get(t).view(torch.int64).reshape(-1, n)[0].repeat(batch).view(torch.uint64)  # noqa: E731
         norms = [op for op in ops if op.kind == "RmsNorm"]
         proj = [op for op in ops if op.kind == "Projection"]
         ropes = [op for op in ops if op.kind == "RoPE"]
-        soft = next(op for op in ops if op.kind == "Softmax")
         silu = next(op for op in ops if op.kind == "Lookup" and op.table != norms[0].rsqrt_table and
                     any(o.kind == "GeluIndex" and o.out == op.idx for o in ops))
         if len(proj) != 2 + 5 * s.heads + 3 or len(norms) != 3:

@@ -365,11 +365,14 @@ class Gpt2Decoder:
     "MatMul"))`` returned for the graph: the Store then holds the same numbers,
     and a step's adjusted logits (without penalties) are the row that
     ``forward_ops`` leaves in the Argmax arm's input, so the tokens generated
-    are the ones the graph proves.  Sequences hold at most the graph's m
+    are the ones the graph proves.  The graph's exp table begins with zero
+    (exp_bits from 20 on).  Sequences hold at most the graph's m
     tokens.  ``tokens`` (uint32, batch) is each sequence's next token to take;
     a step replaces it by its choice."""
 
     def __init__(self, store, ops, s: LayerShape, weights: dict, batch: int = 1):
+        tables = {op.kind: op for op in ops}
+        decode.masked_counts_nothing(store.get(tables["Softmax"].table), "Gpt2Decoder")
         self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
         rows = lambda t, n: store.get(t).reshape(-1, n)[0]  # noqa: E731  a row vector broadcast over m rows
         wide = lambda t, n: rows(t, n).view(torch.int64).repeat(batch).view(torch.uint64)  # noqa: E731
@@ -386,7 +389,6 @@ class Gpt2Decoder:
             raise ValueError("Gpt2Decoder: not a graph of gpt2_model with this shape")
         if s.d * s.vocab > 0x7FFFFFFF:
             raise ValueError("Gpt2Decoder: an embedding table of at most 2^31 - 1 entries is wanted")
-        tables = {op.kind: op for op in ops}
         self.exp = store.get(tables["Softmax"].table)
         lookups = [op for op in ops if op.kind == "Lookup"]
         self.gelu, self.rsqrt = store.get(lookups[1].table), store.get(norms[0].rsqrt_table)
