@@ -56,3 +56,36 @@ def moe_graph(zk, store, rng, group=32, **shape):
         store.v[op.w] = ref.field(dense.reshape(-1))
         weights.append(w)
     return s, ops, weights, top
+
+
+def liven(store, ops):
+    """Numbers at which every part of a layer counts, in place of a builder's
+    (whose norms' scales of 1 to 5 in 2^16 leave little but the biases, and
+    whose weights are all positive): norms' scales about 1, weights of both
+    signs, embeddings about 1.  Zeros stay, the padding among them."""
+    def numbers(t):
+        v = store.get(t)
+        return ref.signed(v if isinstance(v, np.ndarray) else v.cpu().numpy())
+
+    def put(t, v):
+        if isinstance(store.get(t), np.ndarray):
+            store.v[t] = ref.field(v)
+        else:
+            import torch
+            store.v[t] = torch.from_numpy(ref.field(v)).to(store.get(t).device)
+
+    written, news = {t for op in ops for t in op.writes()}, {}
+    for i, op in enumerate(ops):
+        if op.kind == "LayerNormCentered":
+            news[op.w], news[op.b] = (lambda v: 60000 + 2000 * v), (lambda v: 3000 * v)
+        elif op.kind in ("Projection", "GatherMatMul") or (op.kind == "MatMul" and op.b not in written):
+            t = op.b if op.kind == "MatMul" else op.w
+            if numbers(t).min() >= 0:
+                news[t] = lambda v: (2 * v - v.max()) * 12000 // v.max()
+        elif i == 0 and op.kind == "Lookup":
+            news[op.table] = lambda v: (v - 25) * 3000
+        elif i == 1 and op.kind == "Add":
+            news[op.b] = lambda v: (v - 25) * 2000
+    for t, f in news.items():
+        v = numbers(t)
+        put(t, np.where(v != 0, f(v), 0))

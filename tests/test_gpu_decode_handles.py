@@ -1,0 +1,162 @@
+"""Weights, caches, expert blocks and decoders that are copied, restored or
+changed: each works on its own memory."""
+import copy
+import io
+
+import numpy as np
+import pytest
+
+from tests import decode_ref as ref, decode_shapes as ds_ref
+from tests.test_gpu_decode import _cache, _exp_table, _i32, _moe_block, _moe_case, _quant, _s, _silu_table, _u
+
+pytestmark = pytest.mark.gpu
+
+
+
+def _saved(handle):
+    import torch
+    file = io.BytesIO()
+    torch.save(handle, file)  # (plain pickle does not read torch's uint64 tensors back)
+    file.seek(0)
+    return torch.load(file, weights_only=False)
+
+
+COPIES = {"deepcopy": copy.deepcopy, "saved": _saved}
+
+
+@pytest.mark.parametrize("how", COPIES)
+def test_a_forked_cache_steps_apart(zk, how):
+    """Two continuations of one sequence: each sees the common past and its own
+    tokens, the other's cache stays as it was."""
+    rng = np.random.default_rng(1)
+    hk, dk, dv, cap, n = 2, 16, 12, 64, 20
+    keys, values, cache = _cache(zk, rng, 1, hk, dk, dv, cap, [n])
+    table, q = _exp_table(), rng.integers(-(1 << 18), 1 << 18, (1, hk * dk))
+    fork = COPIES[how](cache)
+    for a, b in ((fork.k, cache.k), (fork.v, cache.v), (fork.lens, cache.lens)):
+        assert a.data_ptr() != b.data_ptr()
+    before = [t.clone() for t in (cache.k, cache.v, cache.lens)]
+    sides = [(cache, keys, values), (fork, keys.copy(), values.copy())]
+    for step in range(3):
+        for c, ks, vs in reversed(sides):
+            nk, nv = rng.integers(-(1 << 18), 1 << 18, (1, hk * dk)), rng.integers(-(1 << 18), 1 << 18, (1, hk * dv))
+            ks[0, :, n + step], vs[0, :, n + step] = nk.reshape(hk, dk), nv.reshape(hk, dv)
+            got = zk.decode.attend(_u(q), c, _u(table), k=_u(nk), v=_u(nv))
+            c.advance()
+            want = np.concatenate([ref.attend(q[0, h * dk:(h + 1) * dk], ks[0, h, :n + step + 1], vs[0, h, :n + step + 1], table, (1, 16))
+                                   for h in range(hk)])
+            assert np.array_equal(_s(got)[0], want)
+            if c is fork and step == 0:
+                assert all(bool((a == b).all()) for a, b in zip(before, (cache.k, cache.v, cache.lens)))
+    for c, ks, vs in sides:
+        assert c.lens.tolist() == [n + 3]
+        assert np.array_equal(ref.keys_of(c.k.cpu().numpy()), ks) and np.array_equal(c.v.cpu().numpy(), vs)
+    # and a prompt's rows
+    tail = rng.integers(-99, 99, (1, 2, hk * dk)), rng.integers(-99, 99, (1, 2, hk * dv))
+    fork.append(_u(tail[0]), _u(tail[1]))
+    assert np.array_equal(fork.v[0, :, n + 3:n + 5].cpu().numpy(), np.moveaxis(tail[1].reshape(2, hk, dv), 0, 1))
+    assert np.array_equal(cache.v.cpu().numpy(), sides[0][2])
+
+
+@pytest.mark.parametrize("how", COPIES)
+def test_a_copied_weight_has_its_own_memory(zk, how):
+    rng = np.random.default_rng(2)
+    w, x = ref.weight(rng, 96, 40, 32), rng.integers(-(1 << 18), 1 << 18, (3, 96))
+    q = _quant(zk, w, 32)
+    other = COPIES[how](q)
+    q.packed.zero_()  # codes and scales of zero
+    assert not _s(zk.decode.project(_u(x), q, 9)).any()
+    del q
+    _i32(np.full(1 << 16, -1))  # whoever takes the memory that is free now
+    assert np.array_equal(_s(zk.decode.project(_u(x), other, 9)), ref.project(x, *w, 32, 0, 9))
+    assert np.array_equal(other.codes()[0].cpu().numpy(), w[0])
+
+
+@pytest.mark.parametrize("how", COPIES)
+def test_a_copied_block_has_its_own_memory(zk, how):
+    rng = np.random.default_rng(3)
+    router, w = _moe_case(rng, 64, 8, 48, 40, 32)
+    x, exp, silu = rng.integers(-(1 << 17), 1 << 17, (3, 64)), _exp_table(), _silu_table()
+    block = _moe_block(zk, router, w, 32, 3, exp, silu)
+    other = COPIES[how](block)
+    for t in (block.router, *block.packed, block.exp_table, block.silu_table):
+        t.zero_()
+    del block
+    out, gate = other.forward(_u(x))
+    want, want_gate = ref.moe(x, router, w, 32, exp, silu, 3)
+    assert np.array_equal(_s(out), want) and np.array_equal(_s(gate), want_gate)
+
+
+def test_tensors_of_handles_are_not_replaced(zk):
+    import torch
+    rng = np.random.default_rng(4)
+    q = _quant(zk, ref.weight(rng, 64, 16, 32), 32)
+    router, w = _moe_case(rng, 32, 4, 16, 16, 32)
+    block = _moe_block(zk, router, w, 32, 2, _exp_table(12), _silu_table(12))
+    cache = zk.decode.KvCache.zeros(1, 1, 4, 4, 32)
+    for handle, names in ((q, ("packed",)), (block, ("router", "packed", "exp_table", "silu_table")), (cache, ("k", "v", "lens"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(handle, name, getattr(handle, name))
+    # memory that has become less is refused, not read past its end
+    x = _u(np.ones((1, 64), dtype=np.int64))
+    q.packed.resize_(16)
+    with pytest.raises(ValueError, match="QuantWeight: packed"):
+        zk.decode.project(x, q, 4)
+    block.packed[1].resize_(16)
+    with pytest.raises(ValueError, match="MoeBlock: packed"):
+        block.forward(x[:, :32])
+    k = _u(np.ones((1, 4), dtype=np.int64))
+    cache.v.resize_(4)
+    with pytest.raises(ValueError, match="KvCache: v"):
+        zk.decode.attend(k, cache, _u(_exp_table(8)), k=k, v=k)
+    with pytest.raises(ValueError, match="sizes"):
+        cache.append(k[None], k[None])
+    with pytest.raises(ValueError, match="handle"):
+        zk.decode._calls.project(x, (1, 2), 4, None, None, None, None, None, torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+def test_a_forked_decoder_steps_apart(zk):
+    """A GPT-2 decoder copied in the middle of a text: both go on, each with
+    other tokens, as two decoders that had the same past from the start."""
+    import torch
+    s = zk.gpt2.LayerShape(**ds_ref.GPT2)
+    store = zk.compose.Store()
+    ops, tokens, _ = zk.gpt2.gpt2_model(store, s, layers=2)
+    ds_ref.liven(store, ops)
+    weights = zk.decode.quantise_weights(store, ops, ("Projection", "MatMul"))
+    text = store.get_idx(tokens).view(torch.int32)
+    new = lambda: zk.gpt2.Gpt2Decoder(store, ops, s, weights, batch=1)  # noqa: E731
+
+    def run(dec, ids):
+        out = []
+        for t in ids:
+            dec.tokens.copy_(t.reshape(1).view(torch.uint32))
+            out.append(dec.step()[1].view(torch.int64).clone())
+        return torch.cat(out)
+
+    past, left, right = text[:10], text[10:20], text.flip(0)[:10]
+    want, apart = [], []
+    for rest in (left, right):
+        dec = new()
+        run(dec, past)
+        want.append(run(dec, rest))
+        apart.append(dec)
+    dec = new()
+    run(dec, past)
+    fork = copy.deepcopy(dec)
+    assert all(layer["cache"].lens.data_ptr() == fork.lens.data_ptr() for layer in fork.layers)
+    got_right = run(fork, right[:5])
+    got_left = run(dec, left)
+    assert torch.equal(got_left, want[0])
+    assert torch.equal(torch.cat([got_right, run(fork, right[5:])]), want[1])
+    for one, other in zip((dec, fork), apart):
+        one.check()
+        for a, b in zip(one.layers, other.layers):
+            assert torch.equal(a["cache"].k, b["cache"].k) and torch.equal(a["cache"].v, b["cache"].v)
+        assert one.lens.tolist() == [20]
+    assert not torch.equal(dec.layers[0]["cache"].v, fork.layers[0]["cache"].v)
+    with pytest.raises(AttributeError):
+        dec.lens = dec.lens.clone()
+    with pytest.raises(AttributeError):
+        dec.tokens = dec.tokens.clone()

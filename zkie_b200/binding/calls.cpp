@@ -80,11 +80,32 @@ int64_t number(PyObject* o) {
     if (v == -1 && PyErr_Occurred()) throw Refused{};
     return v;
 }
-void* address(PyObject* o) {
-    void* p = PyLong_AsVoidPtr(o);
-    if (!p && PyErr_Occurred()) throw Refused{};
-    return p;
-}
+// What a handle holds: its tensors and sizes.  Addresses are taken from the tensors at the call,
+// so that a handle that was copied or restored works on its own memory and one whose tensors were
+// given other memory is not read past its end.
+struct Handle {
+    PyObject* items;
+    const char* name;
+    int dev;
+    Handle(PyObject* o, Py_ssize_t size, const char* what, int on) : items(o), name(what), dev(on) {
+        if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != size) refuse(std::string(what) + ": a handle of zkie_b200.decode is wanted");
+    }
+    PyObject* at(int i) const { return PyTuple_GET_ITEM(items, i); }
+    int64_t size(int i) const { return number(at(i)); }
+    template <typename T>
+    T* memory(PyObject* o, const char* what, at::ScalarType type, int64_t numel) const {
+        const std::string full = std::string(name) + ": " + what;
+        const at::Tensor& t = tensor(o, full.c_str());
+        if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != dev || !t.is_contiguous() || t.numel() != numel)
+            refuse(full + " is not the memory of " + std::to_string(numel) + " numbers on the call's device that it was, but " +
+                   said(t));
+        return static_cast<T*>(t.data_ptr());
+    }
+    template <typename T>
+    T* memory(int i, const char* what, at::ScalarType type, int64_t numel) const {
+        return memory<T>(at(i), what, type, numel);
+    }
+};
 // a shift of a rounding division
 uint32_t shift_of(PyObject* o, const char* name) {
     const int64_t v = number(o);
@@ -143,18 +164,19 @@ PyObject* guarded(F f) {
     return nullptr;
 }
 
-// project(x, (device, pointer, k, n, group, segment, experts), shift, bias, table, offset, residual, out, err)
+// project(x, (packed, k, n, group, segment, experts), shift, bias, table, offset, residual, out, err)
 PyObject* project(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 9) refuse("project: 9 arguments");
         const at::Tensor& x = tensor(a[0], "x");
         const int dev = device_of(x, "x");
-        int64_t w[7];
-        for (int i = 0; i < 7; i++) w[i] = i == 1 ? 0 : number(PyTuple_GET_ITEM(a[1], i));
-        const auto* packed = static_cast<const uint32_t*>(address(PyTuple_GET_ITEM(a[1], 1)));
-        const int64_t k = w[2], n = w[3];
+        const Handle w(a[1], 6, "QuantWeight", dev);
+        const int64_t k = w.size(1), n = w.size(2), segment = w.size(4), experts = w.size(5);
+        const uint32_t group = (uint32_t)w.size(3);
         const Rows in = rows(x, "x", k, dev);
-        if (w[6] != 1 || w[0] != dev) refuse("project: one weight (no stack of experts) on the call's device is wanted");
+        if (experts != 1) refuse("project: one weight (no stack of experts) is wanted");
+        const auto* packed = reinterpret_cast<const uint32_t*>(
+            w.memory<int32_t>(0, "packed", at::kInt, (int64_t)zkie2_q4_words(1, k, n, group, segment)));
         if (in.n > 65535) refuse("project: at most 65535 rows are wanted");
         const uint32_t shift = shift_of(a[2], "project");
         const uint64_t* bias = a[3] == Py_None ? nullptr : flat<uint64_t>(tensor(a[3], "bias"), "bias", at::kUInt64, dev, {n});
@@ -175,33 +197,31 @@ PyObject* project(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const at::Tensor out = output(a[7], {in.n, n}, dev);
         apart(a[7], out, in, k, "x");
         apart(a[7], out, residual, n, "the residual (and is not it)", true);
-        done(zkie2_q4_project(in.data, in.stride, in.n, packed, k, n, (uint32_t)w[4], w[5], shift, bias, table, table_len,
+        done(zkie2_q4_project(in.data, in.stride, in.n, packed, k, n, group, segment, shift, bias, table, table_len,
                               offset, residual.data, residual.stride, static_cast<uint64_t*>(out.data_ptr()),
                               word(a[8], dev), stream(dev)), "zkie2_q4_project");
         return THPVariable_Wrap(out);
     });
 }
 
-// attend(q, (device, k, v, lens, batch, heads, dk, dv, capacity), table, k, v, q_scale, k_scale, score_scale, offset,
+// attend(q, (k, v, lens, batch, heads, dk, dv, capacity), table, k, v, q_scale, k_scale, score_scale, offset,
 //        out_shift, out, err)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 12) refuse("attend: 12 arguments");
         const at::Tensor& q = tensor(a[0], "q");
         const int dev = device_of(q, "q");
-        PyObject* c = a[1];
-        auto* ck = static_cast<int32_t*>(address(PyTuple_GET_ITEM(c, 1)));
-        auto* cv = static_cast<int32_t*>(address(PyTuple_GET_ITEM(c, 2)));
-        const auto* lens = static_cast<const int32_t*>(address(PyTuple_GET_ITEM(c, 3)));
-        const int64_t batch = number(PyTuple_GET_ITEM(c, 4)), heads = number(PyTuple_GET_ITEM(c, 5)),
-                      dk = number(PyTuple_GET_ITEM(c, 6)), dv = number(PyTuple_GET_ITEM(c, 7)),
-                      cap = number(PyTuple_GET_ITEM(c, 8));
+        const Handle c(a[1], 8, "KvCache", dev);
+        const int64_t batch = c.size(3), heads = c.size(4), dk = c.size(5), dv = c.size(6), cap = c.size(7);
+        auto* ck = c.memory<int32_t>(0, "k", at::kInt, batch * heads * cap * dk);
+        auto* cv = c.memory<int32_t>(1, "v", at::kInt, batch * heads * cap * dv);
+        const auto* lens = c.memory<int32_t>(2, "lens", at::kInt, batch);
         const int64_t cols = q.dim() == 2 ? q.size(1) : 0;
         if (cols == 0 || cols % (heads * dk) || cols / dk > 65535)
             refuse("q: a row per sequence of a multiple of " + std::to_string(heads * dk) + " columns is wanted, not " + said(q));
         const Rows in = rows(q, "q", cols, dev);
-        if (in.n != batch || (a[3] == Py_None) != (a[4] == Py_None) || number(PyTuple_GET_ITEM(c, 0)) != dev)
-            refuse("attend: a row per sequence, k and v together, and the cache's device are wanted");
+        if (in.n != batch || (a[3] == Py_None) != (a[4] == Py_None))
+            refuse("attend: a row per sequence, and k and v together, are wanted");
         Rows k, v;
         if (a[3] != Py_None) {
             k = rows(tensor(a[3], "k"), "k", heads * dk, dev);
@@ -225,18 +245,28 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
-// moe(x, (device, h, experts, top_k, f, shared_f, group, router, weights, exp, exp_len, silu, silu_len, shift), residual,
-//     out, err) -> (out, gate)
+// moe(x, (h, experts, top_k, f, shared_f, group, shift, router, gate and up, down, the shared experts' same, exp, silu),
+//     residual, out, err) -> (out, gate)
 PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 5) refuse("moe: 5 arguments");
         const at::Tensor& x = tensor(a[0], "x");
         const int dev = device_of(x, "x");
-        auto item = [&](int i) { return PyTuple_GET_ITEM(a[1], i); };
-        const int64_t h = number(item(1)), experts = number(item(2)), top_k = number(item(3)), f = number(item(4)),
-                      shared_f = number(item(5)), group = number(item(6));
+        const Handle b(a[1], 14, "MoeBlock", dev);
+        const int64_t h = b.size(0), experts = b.size(1), top_k = b.size(2), f = b.size(3), shared_f = b.size(4);
+        const uint32_t group = (uint32_t)b.size(5);
         const Rows in = rows(x, "x", h, dev);
-        if (in.n > 65535 || number(item(0)) != dev) refuse("MoeBlock: at most 65535 rows, on the weights' device, are wanted");
+        if (in.n > 65535) refuse("MoeBlock: at most 65535 rows are wanted");
+        const auto* router = reinterpret_cast<const uint32_t*>(
+            b.memory<int32_t>(7, "router", at::kInt, (int64_t)zkie2_moe_router_words(h, experts)));
+        const int64_t pairs = (h + 31) / 32 * 32;  // columns of the down weights' pairs of tiles
+        const int64_t words[4] = {2 * (int64_t)zkie2_q4_words(experts, h, f, group, 0), (int64_t)zkie2_q4_words(experts, f, pairs, group, 0),
+                                  2 * (int64_t)zkie2_q4_words(1, h, shared_f, group, 0), (int64_t)zkie2_q4_words(1, shared_f, pairs, group, 0)};
+        const uint32_t* weights[4];
+        for (int i = 0; i < 4; i++)
+            weights[i] = reinterpret_cast<const uint32_t*>(b.memory<int32_t>(8 + i, "packed", at::kInt, words[i]));
+        const at::Tensor &exp = tensor(b.at(12), "exp_table"), &silu = tensor(b.at(13), "silu_table");
+        const uint64_t *exp_table = table_of(exp, "exp_table", dev), *silu_table = table_of(silu, "silu_table", dev);
         Rows residual;
         if (a[2] != Py_None) {
             residual = rows(tensor(a[2], "residual"), "residual", h, dev);
@@ -247,13 +277,11 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         apart(a[3], out, in, h, "x");
         apart(a[3], out, residual, h, "the residual (and is not it)", true);
         // this call's own: calls on other streams may run beside it
-        const uint64_t elems = zkie2_moe_rows_scratch_elems(in.n, h, experts, top_k, f, shared_f, (uint32_t)group);
+        const uint64_t elems = zkie2_moe_rows_scratch_elems(in.n, h, experts, top_k, f, shared_f, group);
         const at::Tensor scratch = make({(int64_t)elems + 1}, at::kLong, dev);
-        done(zkie2_moe_rows(in.data, in.stride, in.n, h, experts, top_k, f, shared_f, (uint32_t)group,
-                            static_cast<const uint32_t*>(address(item(7))),
-                            static_cast<const uint32_t* const*>(address(item(8))), static_cast<const uint64_t*>(address(item(9))),
-                            number(item(10)), static_cast<const uint64_t*>(address(item(11))), number(item(12)),
-                            (uint32_t)number(item(13)), residual.data, residual.stride, static_cast<uint64_t*>(out.data_ptr()),
+        done(zkie2_moe_rows(in.data, in.stride, in.n, h, experts, top_k, f, shared_f, group, router, weights, exp_table,
+                            exp.numel(), silu_table, silu.numel(), (uint32_t)b.size(6), residual.data, residual.stride,
+                            static_cast<uint64_t*>(out.data_ptr()),
                             static_cast<uint64_t*>(gate.data_ptr()), word(a[4], dev), static_cast<uint64_t*>(scratch.data_ptr()),
                             stream(dev)), "zkie2_moe_rows");
         return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(gate));

@@ -24,12 +24,10 @@ likes (``check_err``); not given, the call reads its own, which synchronises,
 and raises ValueError.  Besides the op layer's bits, 8 is a value outside the
 32-bit range the kernels take (computed on as zero) and 16 a full cache.
 """
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
 from ._lib import check, lib
 from . import _calls  # after the library it links
 from .compose import _INDEX_WRITERS, _check_err, _err_word
@@ -135,6 +133,12 @@ def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: in
     return done
 
 
+def _kept(name: str) -> property:
+    """A handle's tensor: read, and written in place, but not replaced -- calls
+    take it from ``call``, which a copy or a pickle of the handle has its own of."""
+    return property(lambda self: getattr(self, name))
+
+
 class QuantWeight:
     """A weight w[k][n] = codes[k][n] scales[row of k][n] in 4 bits, laid out
     once for the kernels (``packed``).
@@ -167,13 +171,15 @@ class QuantWeight:
             raise ValueError("QuantWeight: a code outside [-8, 7] or a scale outside [0, 65535]")
         codes, scales = codes.contiguous(), scales.to(torch.int32).contiguous()
         dev = codes.device
-        self.packed = torch.empty(words, dtype=torch.int32, device=dev)
-        self.device, self.pointer = self.packed.get_device(), self.packed.data_ptr()
-        self.call = (self.device, self.pointer, self.k, self.n, group, segment, self.experts)
+        self._packed = torch.empty(words, dtype=torch.int32, device=dev)
+        self.call = (self._packed, self.k, self.n, group, segment, self.experts)
         err = _err_word()
         check(lib.zkie2_q4_pack(codes.data_ptr(), scales.data_ptr(), self.experts, self.k, self.n, group, segment,
                                 self.packed.data_ptr(), err.data_ptr(), _stream()), "zkie2_q4_pack")
         _check_err(err, "QuantWeight")
+
+    packed = _kept("_packed")
+    device = property(lambda self: self._packed.get_device())
 
     def _blocks(self) -> torch.Tensor:
         return self.packed.reshape(self.experts, -(-self.n // 16), -1, 144 if self.group == 32 else 136)
@@ -230,7 +236,7 @@ class KvCache:
     multiples of 4 up to 256, the capacity a multiple of 32 up to 131072."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor):
-        self.device = dev = _device_of(k, "k")
+        dev = _device_of(k, "k")
         _flat(k, "k", _I32, dev)
         _flat(v, "v", _I32, dev)
         _flat(lens, "lens", _I32, dev)
@@ -249,13 +255,11 @@ class KvCache:
         if (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("KvCache: 16-byte aligned buffers are wanted")
         self._k, self._v, self._lens = k, v, lens
-        self.call = (dev, k.data_ptr(), v.data_ptr(), lens.data_ptr(), self.batch, self.heads, self.dk, self.dv,
-                     self.capacity)
+        self._numels = (k.numel(), v.numel(), lens.numel())
+        self.call = (k, v, lens, self.batch, self.heads, self.dk, self.dv, self.capacity)
 
-    # read, and written in place, but not replaced: calls hold their addresses
-    k = property(lambda self: self._k)
-    v = property(lambda self: self._v)
-    lens = property(lambda self: self._lens)
+    k, v, lens = _kept("_k"), _kept("_v"), _kept("_lens")
+    device = property(lambda self: self._k.get_device())
 
     @classmethod
     def zeros(cls, batch: int, heads: int, dk: int, dv: int, capacity: int,
@@ -282,8 +286,11 @@ class KvCache:
         if self.device != dev or k.shape[1] > 1 << 17 or not 0 <= k_scale[1] <= 62:
             raise ValueError("append: the cache's device, at most 131072 tokens and a shift 0 .. 62 are wanted")
         k, v, word = k.contiguous(), v.contiguous(), _err_word() if err is None else _flat(err, "err", _I32, dev)
+        mine, sizes = self.call[:3], self.call[3:]
+        if any(t.numel() != n for t, n in zip(mine, self._numels)):
+            raise ValueError("append: the cache's tensors have other sizes than they had")
         check(lib.zkie2_kv_append(k.data_ptr(), k.shape[2], v.data_ptr(), v.shape[2], k.shape[1], *k_scale,
-                                  *self.call[1:], word.data_ptr(), _stream()), "zkie2_kv_append")
+                                  *[t.data_ptr() for t in mine], *sizes, word.data_ptr(), _stream()), "zkie2_kv_append")
         if err is None:
             _check_err(word, "append")
 
@@ -356,26 +363,26 @@ class MoeBlock:
             if (w.experts, w.k, w.n) != shape or w.group != self.group or w.segment:
                 raise ValueError(f"MoeBlock: weight {w.experts} x {w.k} x {w.n}, group {w.group}, segment {w.segment}: "
                                  f"{shape} with group {self.group} and no segments is wanted")
-        self.device = dev = _device_of(router, "router")
+        dev = _device_of(router, "router")
         if any(w.device != dev for w in weights):
             raise ValueError("MoeBlock: weights on the current device are wanted")
         router = _flat(router, "router", _U64, dev, (h, e))
-        self.exp_table, self.silu_table = _flat(exp_table, "exp_table", _U64, dev), \
-            _flat(silu_table, "silu_table", _U64, dev)
+        self._exp, self._silu = _flat(exp_table, "exp_table", _U64, dev), _flat(silu_table, "silu_table", _U64, dev)
         if exp_table.numel() == 0 or silu_table.numel() == 0:
             raise ValueError("MoeBlock: an empty table")
         if not 1 <= top_k <= min(e, 16) or e > 256 or not 0 <= shift <= 62:
             raise ValueError("MoeBlock: at most 256 experts, 1 .. 16 of them to a token, and a shift 0 .. 62 are wanted")
-        self.router = torch.empty(lib.zkie2_moe_router_words(h, e), dtype=torch.int32,
-                                  device=router.device)
+        self._router = torch.empty(lib.zkie2_moe_router_words(h, e), dtype=torch.int32,
+                                   device=router.device)
         err = _err_word()
-        check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self.router.data_ptr(), err.data_ptr(), _stream()), "zkie2_moe_router_pack")
+        check(lib.zkie2_moe_router_pack(router.data_ptr(), h, e, self._router.data_ptr(), err.data_ptr(), _stream()), "zkie2_moe_router_pack")
         _check_err(err, "MoeBlock: router")
-        self.packed = (self._pair(gate, up), self._pair(down), self._pair(shared_gate, shared_up), self._pair(shared_down))
-        self._packed = (_lib.vp * 4)(*[w.data_ptr() for w in self.packed])
+        self._packed = (self._pair(gate, up), self._pair(down), self._pair(shared_gate, shared_up), self._pair(shared_down))
         torch.cuda.current_stream().synchronize()  # weights are complete before a call: it reads them at once
-        self.call = (dev, h, e, top_k, f, s, self.group, self.router.data_ptr(), C.addressof(self._packed),
-                     exp_table.data_ptr(), exp_table.numel(), silu_table.data_ptr(), silu_table.numel(), shift)
+        self.call = (h, e, top_k, f, s, self.group, shift, self._router, *self._packed, self._exp, self._silu)
+
+    router, packed, exp_table, silu_table = _kept("_router"), _kept("_packed"), _kept("_exp"), _kept("_silu")
+    device = property(lambda self: self._router.get_device())
 
     @staticmethod
     def _pair(a: QuantWeight, b: Optional[QuantWeight] = None) -> torch.Tensor:
@@ -384,7 +391,7 @@ class MoeBlock:
         tiles = -(-a.n // 16)
         words = a.packed.numel() // tiles * (2 * tiles if b is not None else tiles + tiles % 2)
         out = torch.empty(words, dtype=torch.int32, device=a.packed.device)
-        check(lib.zkie2_q4_pair(a.pointer, b.pointer if b is not None else None, a.experts, a.k, a.n, a.group, out.data_ptr(),
+        check(lib.zkie2_q4_pair(a.packed.data_ptr(), b.packed.data_ptr() if b is not None else None, a.experts, a.k, a.n, a.group, out.data_ptr(),
                                 _stream()), "zkie2_q4_pair")
         return out
 

@@ -392,7 +392,7 @@ class Gpt2Decoder:
         self.exp = store.get(tables["Softmax"].table)
         lookups = [op for op in ops if op.kind == "Lookup"]
         self.gelu, self.rsqrt = store.get(lookups[1].table), store.get(norms[0].rsqrt_table)
-        self.lens = torch.zeros(batch, dtype=torch.int32, device=device())
+        self._lens = torch.zeros(batch, dtype=torch.int32, device=device())
         self.layers, self.witness = [], []
         for i in range(0, len(projections), per):
             layer = projections[i:i + per]
@@ -418,7 +418,10 @@ class Gpt2Decoder:
         self.columns = torch.arange(s.d, dtype=torch.int32, device=device()) * s.vocab
         bits = np.arange(-(-s.vocab // 32) * 32) < s.vocab_real
         self.allowed = torch.from_numpy(np.packbits(bits, bitorder="little").view(np.int32).copy()).to(device())
-        self.tokens = torch.zeros(batch, dtype=torch.uint32, device=device())
+        self._tokens = torch.zeros(batch, dtype=torch.uint32, device=device())
+
+    # read, and written in place, but not replaced: the caches count in lens
+    lens, tokens = decode._kept("_lens"), decode._kept("_tokens")
 
     @staticmethod
     def _sum_of(ops, heads):
