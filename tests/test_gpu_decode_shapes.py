@@ -45,6 +45,53 @@ def test_moe_layer_steps_equal_the_graph_at_other_shifts(zk, shift):
     dec.check()
 
 
+# ---- numbers at which attention, norms and experts count ------------------------------------------
+@pytest.mark.parametrize("shift,group", [(16, 32), (16, 128), (14, 64), (17, 64)])
+def test_gpt2_steps_equal_the_graph_where_attention_counts(zk, shift, group):
+    """Every position's logits and choice, two sequences at different places."""
+    import torch
+    s = zk.gpt2.LayerShape(**ds_ref.GPT2, shift=shift)
+    store = zk.compose.Store()
+    ops, tok, out = zk.gpt2.gpt2_model(store, s, layers=2)
+    ds_ref.liven(store, ops)
+    weights = zk.decode.quantise_weights(store, ops, ("Projection", "MatMul"), group)
+    zk.compose.forward_ops(store, ops)
+    logits = store.get(next(op for op in ops if op.kind == "Argmax").x).view(torch.int64).reshape(s.m, s.vocab)
+    tokens, argmax = store.get_idx(tok).view(torch.int32), store.get_idx(out).view(torch.int32)
+    assert len(set(argmax.tolist())) > 20
+    dec = zk.gpt2.Gpt2Decoder(store, ops, s, weights, batch=2)
+    dec.load(store, 1, 13)
+    for i in range(s.m - 13):
+        at = [i, 13 + i]
+        dec.tokens.copy_(tokens[at].view(torch.uint32))
+        token, got = dec.step()
+        assert torch.equal(got.view(torch.int64), logits[at]), i
+        assert torch.equal(token.view(torch.int32), argmax[at]), i
+    dec.check()
+
+
+@pytest.mark.parametrize("shift", [14, 16])
+def test_moe_layer_steps_equal_the_graph_where_attention_counts(zk, shift):
+    """Three sequences over one text, begun at different steps."""
+    import torch
+    from zkie_b200 import deepseek as ds
+    s = ds.MoeShape(**ds_ref.MOE, shift=shift)
+    store = zk.compose.Store()
+    ops, x, out = ds.moe_layer(store, s)
+    ds_ref.liven(store, ops)
+    weights = zk.decode.quantise_weights(store, ops)
+    zk.compose.forward_ops(store, ops)
+    rows = lambda t: store.get(t).view(torch.int64).reshape(s.m, s.h)  # noqa: E731
+    dec = ds.MoeLayerDecoder(store, ops, s, weights, 3)
+    first = [0, 3, 4]
+    for i in range(s.m):
+        at = [max(i - f, 0) for f in first]
+        dec.cache.lens.copy_(torch.tensor(at))
+        got = dec.step(rows(x)[at].view(torch.uint64))
+        assert torch.equal(got.view(torch.int64), rows(out)[at]), i
+    dec.check()
+
+
 # ---- what the decoders refuse -----------------------------------------------------------------------
 def test_decoders_refuse_a_table_that_does_not_begin_with_zero(zk):
     """A table of 2^19 entries begins with 22, which the graph counts for every masked column."""
