@@ -99,3 +99,32 @@ def test_decoders_refuse_a_table_that_does_not_begin_with_zero(zk):
             zk.gpt2.Gpt2Decoder(*_gpt2_ops(zk, exp_bits=bits), {})
         with pytest.raises(ValueError, match="begins with zero"):
             ds.MoeLayerDecoder(*_moe_ops(zk, exp_bits=bits), {})
+
+
+@pytest.mark.parametrize("change", [dict(shift=14), dict(exp_bits=21), dict(gelu_bits=20), dict(d_real=40), dict(vocab_real=499),
+                                    dict(m=32), dict(d=32), dict(dh=8), dict(heads=2), dict(ffn=64), dict(vocab=256)])
+def test_gpt2_decoder_refuses_another_shape(zk, change):
+    """A shape that is not the graph's would compute other rows."""
+    import dataclasses
+    st, ops, s = _gpt2_ops(zk, exp_bits=20, gelu_bits=18)
+    with pytest.raises(ValueError, match="shape"):
+        zk.gpt2.Gpt2Decoder(st, ops, dataclasses.replace(s, **change), {})
+
+
+@pytest.mark.parametrize("change", [dict(shift=14), dict(exp_bits=21), dict(m=16), dict(h=64), dict(heads=1), dict(qk_nope=8),
+                                    dict(qk_rope=4), dict(v_head=8), dict(kv_lora=16)])
+def test_moe_decoder_refuses_another_shape(zk, change):
+    import dataclasses
+    from zkie_b200 import deepseek as ds
+    st, ops, s = _moe_ops(zk)
+    with pytest.raises(ValueError, match="shape"):
+        ds.MoeLayerDecoder(st, ops, dataclasses.replace(s, **change), {})
+
+
+def test_decoders_know_their_shapes(zk):
+    from zkie_b200 import deepseek as ds
+    for change in (dict(), dict(vocab_real=512), dict(heads=1, dh=48), dict(shift=9, gelu_bits=12, exp_bits=20)):
+        assert zk.gpt2.Gpt2Decoder._shaped(*_gpt2_ops(zk, **change))
+    for change in (dict(), dict(heads=1), dict(shift=12, moe=48, top_k=1)):
+        _, ops, s = _moe_ops(zk, **change)
+        assert ds.MoeLayerDecoder._shaped(ops, s)

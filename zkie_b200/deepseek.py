@@ -292,6 +292,8 @@ class MoeLayerDecoder:
     graph's exp table begins with zero (exp_bits from 20 on)."""
 
     def __init__(self, store, ops, s: MoeShape, weights: dict, batch: int = 1):
+        if not self._shaped(ops, s):
+            raise ValueError("MoeLayerDecoder: not a graph of moe_layer with this shape")
         soft = next(op for op in ops if op.kind == "Softmax")
         decode.masked_counts_nothing(store.get(soft.table), "MoeLayerDecoder")
         self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
@@ -301,8 +303,6 @@ class MoeLayerDecoder:
         ropes = [op for op in ops if op.kind == "RoPE"]
         silu = next(op for op in ops if op.kind == "Lookup" and op.table != norms[0].rsqrt_table and
                     any(o.kind == "GeluIndex" and o.out == op.idx for o in ops))
-        if len(proj) != 2 + 5 * s.heads + 3 or len(norms) != 3:
-            raise ValueError("MoeLayerDecoder: not a graph of moe_layer with this shape")
 
         def quant(ids, dim, segment=0):
             parts = [weights[o.w] for o in ids]
@@ -319,6 +319,24 @@ class MoeLayerDecoder:
         self.cos, self.sin = (store.get(t).view(torch.int64).reshape(s.m, half) for t in (ropes[0].cos, ropes[0].sin))
         self.block = moe_block(store, ops, weights, soft.table, silu.table, s.shift)
         self.cache = decode.KvCache.zeros(batch, s.heads, s.qk_nope + s.qk_rope, s.v_head, s.m)
+
+    @staticmethod
+    def _shaped(ops, s: MoeShape) -> bool:
+        """Whether the graph is moe_layer's of this shape: the attention's sizes,
+        shifts, Scales and tables (the experts are read from the graph)."""
+        of = {}
+        for op in ops:
+            of.setdefault(op.kind, []).append(op)
+        proj, norms = of.get("Projection", []), of.get("RmsNorm", [])
+        if len(proj) != 2 + 5 * s.heads + 3 or len(norms) != 3:
+            return False
+        sizes = [(s.h, s.kv_lora), (s.h, s.qk_rope)] + [
+            (s.h, s.qk_nope), (s.h, s.qk_rope), (s.kv_lora, s.qk_nope), (s.kv_lora, s.v_head), (s.v_head, s.h)] * s.heads
+        return [(op.m, op.k, op.n, op.shift) for op in proj[:-3]] == [(s.m, k, n, s.shift) for k, n in sizes] and \
+            [(op.m, op.d, op.n_real) for op in norms] == [(s.m, d, d) for d in (s.h, s.kv_lora, s.h)] and \
+            [(op.m, op.d, op.shift) for op in of["RoPE"]] == [(s.m, s.qk_rope, s.shift)] * (1 + s.heads) and \
+            [(op.factor, op.shift) for op in of["Scale"][:2 * s.heads]] == [(7519, 32), (1, 16)] * s.heads and \
+            all((op.offset, op.table_len) == (1 << s.exp_bits,) * 2 for op in of["StableSoftmaxIndex"])
 
     def _norm(self, x, i):
         w, d = self.norms[i]

@@ -371,6 +371,8 @@ class Gpt2Decoder:
     a step replaces it by its choice."""
 
     def __init__(self, store, ops, s: LayerShape, weights: dict, batch: int = 1):
+        if not self._shaped(store, ops, s):
+            raise ValueError("Gpt2Decoder: not a graph of gpt2_model with this shape")
         tables = {op.kind: op for op in ops}
         decode.masked_counts_nothing(store.get(tables["Softmax"].table), "Gpt2Decoder")
         self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
@@ -385,8 +387,6 @@ class Gpt2Decoder:
         norms = [op for op in ops if op.kind == "LayerNormCentered"]
         projections = [op for op in ops if op.kind == "Projection"]
         per = 4 * s.heads + 2  # a layer's projections: q, k, v, o per head, then fc and proj
-        if len(projections) % per or len(norms) != 2 * (len(projections) // per) + 1:
-            raise ValueError("Gpt2Decoder: not a graph of gpt2_model with this shape")
         if s.d * s.vocab > 0x7FFFFFFF:
             raise ValueError("Gpt2Decoder: an embedding table of at most 2^31 - 1 entries is wanted")
         self.exp = store.get(tables["Softmax"].table)
@@ -422,6 +422,34 @@ class Gpt2Decoder:
 
     # read, and written in place, but not replaced: the caches count in lens
     lens, tokens = decode._kept("_lens"), decode._kept("_tokens")
+
+    @staticmethod
+    def _shaped(store, ops, s: LayerShape) -> bool:
+        """Whether the graph is gpt2_model's of this shape: sizes, shifts, the
+        Scales' factors, the tables' offsets and the vocabulary's mask."""
+        of = {}
+        for op in ops:
+            of.setdefault(op.kind, []).append(op)
+        proj, norms, per = of.get("Projection", []), of.get("LayerNormCentered", []), 4 * s.heads + 2
+        layers = len(proj) // per
+        if not layers or len(proj) % per or len(norms) != 2 * layers + 1 or "Argmax" not in of:
+            return False
+        sizes = [(s.d, s.dh)] * 3 + [(s.dh, s.d)]
+        sizes = sizes * s.heads + [(s.d, s.ffn), (s.ffn, s.d)]
+        if any((op.m, op.k, op.n, op.shift) != (s.m, *sizes[i % per], s.shift) for i, op in enumerate(proj)) or \
+                any((op.m, op.d, op.n_real) != (s.m, s.d, s.d_real) for op in norms):
+            return False
+        scales = [(23170, 16)] * 2 + [(1, 16)] * 2  # queries, keys, scores, outputs
+        if [(op.factor, op.shift) for op in of["Scale"]] != scales * (layers * s.heads) or \
+                any((op.offset, op.table_len) != (1 << s.exp_bits,) * 2 for op in of["StableSoftmaxIndex"]) or \
+                any((op.offset, op.table_len) != (1 << s.gelu_bits >> 1, 1 << s.gelu_bits) for op in of["GeluIndex"]):
+            return False
+        last = of["Argmax"][-1]
+        mask = next((store.get(op.b)[:s.vocab] for op in of["Add"] if op.c == last.x), None)
+        if mask is None or (last.m, last.n) != (s.m, s.vocab):
+            return False
+        mask = mask.cpu().numpy() if isinstance(mask, torch.Tensor) else mask
+        return np.array_equal(mask, from_i64(np.where(np.arange(s.vocab) < s.vocab_real, 0, decode.MASKED)))
 
     @staticmethod
     def _sum_of(ops, heads):
