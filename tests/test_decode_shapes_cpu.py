@@ -128,3 +128,17 @@ def test_decoders_know_their_shapes(zk):
     for change in (dict(), dict(heads=1), dict(shift=12, moe=48, top_k=1)):
         _, ops, s = _moe_ops(zk, **change)
         assert ds.MoeLayerDecoder._shaped(ops, s)
+
+
+# ---- rows of a step -----------------------------------------------------------------------------------
+def test_moe_decoder_refuses_other_rows(zk):
+    """Fewer rows than sequences would be read past their end: refused before
+    anything is enqueued (no device is needed)."""
+    import torch
+    from zkie_b200 import deepseek as ds
+    dec = object.__new__(ds.MoeLayerDecoder)
+    dec.s, dec.batch = ds.MoeShape(**ds_ref.MOE), 3
+    for x in (torch.zeros((3, 128), dtype=torch.uint64), torch.zeros((2, 128), dtype=torch.uint64), torch.zeros(384, dtype=torch.uint64),
+              torch.zeros((3, 128), dtype=torch.int64), torch.zeros((3, 64), dtype=torch.uint64), [0]):
+        with pytest.raises(ValueError, match="MoeLayerDecoder: x"):
+            dec.step(x)

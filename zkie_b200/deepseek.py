@@ -355,8 +355,15 @@ class MoeLayerDecoder:
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """The layer's output rows (batch x hidden) for the next token of every
-        sequence; its key and value go into the cache, the position is counted."""
+        sequence (x: batch x hidden on the current device); its key and value go
+        into the cache, the position is counted."""
         s, b = self.s, self.batch
+        if not isinstance(x, torch.Tensor) or x.dtype != torch.uint64 or tuple(x.shape) != (b, s.h) or not x.is_cuda or \
+                x.get_device() != torch.cuda.current_device():
+            raise ValueError(f"MoeLayerDecoder: x of uint64 ({b}, {s.h}) on the current device is wanted")
+        if self.cache.batch != b:
+            raise ValueError("MoeLayerDecoder: a cache of as many sequences is wanted")
+        x = x.contiguous()
         i64 = lambda t: t.view(torch.int64)  # noqa: E731
         self.cache.room(s.m, self.err)  # the graph's positions, not the cache's whole blocks
         h = self._norm(x, 0)
