@@ -160,3 +160,63 @@ def test_a_forked_decoder_steps_apart(zk):
         dec.lens = dec.lens.clone()
     with pytest.raises(AttributeError):
         dec.tokens = dec.tokens.clone()
+
+
+# ---- captured steps -----------------------------------------------------------------------------------
+def _lively(zk, batch, prompt):
+    import torch
+    s = zk.gpt2.LayerShape(**ds_ref.GPT2)
+    store = zk.compose.Store()
+    ops, tokens, _ = zk.gpt2.gpt2_model(store, s, layers=2)
+    ds_ref.liven(store, ops)
+    weights = zk.decode.quantise_weights(store, ops, ("Projection", "MatMul"))
+    zk.compose.forward_ops(store, ops)
+    text = store.get_idx(tokens).view(torch.int32)
+
+    def new():
+        dec = zk.gpt2.Gpt2Decoder(store, ops, s, weights, batch)
+        for b in range(batch):
+            dec.load(store, b, prompt + b)
+        dec.tokens.copy_(text[[prompt + b for b in range(batch)]].view(torch.uint32))
+        return dec
+    return s, new
+
+
+def test_a_captured_step_keeps_what_it_reads(zk):
+    """The penalties' history, a bias and a mask that nobody else holds, and a
+    decoder that is dropped: a replay reads them as they were, and its logits
+    can be read."""
+    import gc
+
+    import torch
+    s, new = _lively(zk, 2, 9)
+    rng = np.random.default_rng(5)
+    history, bias = rng.integers(0, s.vocab_real, (2, 30)), rng.integers(-(1 << 33), 1 << 33, (2, s.vocab))
+    allowed = rng.integers(-(1 << 31), 1 << 31, (2, s.vocab // 32))
+    choice = lambda: dict(history=_i32(history), history_lens=_i32([30, 17]), bias=_u(bias), allowed=_i32(allowed),  # noqa: E731
+                          repeat=(52429, 81920), presence=1 << 30, frequency=1 << 29)
+    dec, kept, want = new(), choice(), []
+    for _ in range(12):
+        tokens, logits = dec.step(**kept)
+        want.append((tokens.view(torch.int32).clone(), logits.view(torch.int64).clone()))
+    graph = new().capture(**choice())
+    gc.collect()
+    rubbish = [torch.full((n,), 0x5A5A5A5A, dtype=torch.int32, device="cuda") for n in (2, 17, 32, 60, 64, 1024, 2048, 2048) for _ in range(20)]
+    for tokens, logits in want:
+        graph.replay()
+        assert torch.equal(graph.tokens.view(torch.int32), tokens) and torch.equal(graph.logits.view(torch.int64), logits)
+    assert graph.decoder.lens.tolist() == [21, 22] and graph.tokens.data_ptr() == graph.decoder.tokens.data_ptr()
+    graph.decoder.check()
+    assert len(rubbish) == 160
+
+
+def test_capture_leaves_no_error_of_its_own(zk):
+    """A full sequence: recording a step says nothing, replaying it does."""
+    s, new = _lively(zk, 1, 5)
+    dec = new()
+    dec.lens.fill_(s.m)
+    graph = dec.capture()
+    dec.check()
+    graph.replay()
+    with pytest.raises(ValueError, match="full"):
+        dec.check()

@@ -29,7 +29,6 @@ for bit.
 """
 import ctypes as C
 from dataclasses import dataclass
-from typing import Optional
 
 import numpy as np
 import torch
@@ -353,6 +352,16 @@ def gpt2_model(store, s: LayerShape, layers: int = 12, seed: int = 0x6B2):
 
 
 # ---- token by token ---------------------------------------------------------------------------
+class CapturedStep(torch.cuda.CUDAGraph):
+    """A step of a Gpt2Decoder as a CUDA graph: ``replay()`` takes the
+    decoder's next tokens and leaves the choice in ``tokens`` (the decoder's
+    own) and the adjusted logits in ``logits`` (batch x vocab), until the next
+    replay.  The graph keeps the decoder and the tensors of ``choice``, whose
+    addresses it has recorded."""
+
+    decoder = choice = tokens = logits = None
+
+
 class Gpt2Decoder:
     """The graph of ``gpt2_model`` one token at a time, for ``batch`` sequences
     side by side: the tied embedding and its position row, per layer
@@ -521,21 +530,25 @@ class Gpt2Decoder:
         self.tokens.copy_(tokens)
         return self.tokens, logits
 
-    def capture(self, **choice) -> Optional[torch.cuda.CUDAGraph]:
+    def capture(self, **choice) -> "CapturedStep":
         """A step recorded as a CUDA graph, to be replayed once per token; the
-        position and the tokens it ran on for warm-up are put back."""
-        lens, tokens = self.lens.clone(), self.tokens.clone()
+        position, the tokens and the error word of the step that it ran for
+        warm-up are put back.  What ``choice`` gives is read from the same
+        memory at every replay."""
+        lens, tokens, err = self.lens.clone(), self.tokens.clone(), self.err.clone()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             self.step(**choice)
             self.lens.copy_(lens)
             self.tokens.copy_(tokens)
+            self.err.copy_(err)
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
-        graph = torch.cuda.CUDAGraph()
+        graph = CapturedStep()
+        graph.decoder, graph.choice = self, choice
         with torch.cuda.graph(graph):
-            self.step(**choice)
+            graph.tokens, graph.logits = self.step(**choice)
         return graph
 
     def check(self):
