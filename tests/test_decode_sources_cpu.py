@@ -1,0 +1,46 @@
+"""What can be told of the single-token kernels from their source."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "zkie_b200", "csrc")
+FILES = ("q4.cuh", "decode.cu", "decode_moe.cu")
+
+
+def _code(name):
+    """The file without its comments."""
+    with open(os.path.join(CSRC, name)) as f:
+        return re.sub(r"//[^\n]*|/\*.*?\*/", "", f.read(), flags=re.S)
+
+
+def _body(code, start):
+    """From `start` on, the text up to the brace that closes the first one."""
+    depth, i = 0, code.index("{", start)
+    for j in range(i, len(code)):
+        depth += {"{": 1, "}": -1}.get(code[j], 0)
+        if depth == 0:
+            return code[start:j + 1]
+    raise AssertionError("no end")
+
+
+def test_no_read_only_loads():
+    """A kernel that starts while the one before it runs reads what that one
+    wrote: not through __ldg, whose data has to stay the same while the kernel
+    runs, nor with intrinsics that the compiler may move to before the wait."""
+    for name in FILES:
+        assert not re.findall(r"__ldg|__ldc[gasv]|__ldlu|ld\.global\.nc|ld\.global", _code(name)), name
+
+
+def test_kernels_that_start_early_wait_and_restrict_nothing():
+    """Every kernel that is launched to overlap the one before it waits for it,
+    and none promises that its pointers are read-only (__restrict__)."""
+    early = 0
+    for name in FILES:
+        code = _code(name)
+        for m in re.finditer(r"__global__", code):
+            text = _body(code, m.start())
+            if "let_next_start()" in text or "__grid_constant__" in text:
+                early += 1
+                assert text.count("wait_for_previous();") == 1 and "__restrict__" not in text, text[:200]
+        for m in re.finditer(r"__device__ __forceinline__ [^;{]*\{", code):
+            assert "__restrict__" not in m.group(), m.group()
+    assert early == 5

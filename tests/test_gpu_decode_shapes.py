@@ -106,3 +106,58 @@ def test_decoders_refuse_a_table_that_does_not_begin_with_zero(zk):
     ops, _, _ = ds.moe_layer(store, s)
     with pytest.raises(ValueError, match="begins with zero"):
         ds.MoeLayerDecoder(store, ops, s, zk.decode.quantise_weights(store, ops))
+
+
+# ---- one call after another over the same memory ---------------------------------------------------
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_chain_over_reused_memory(zk, captured):
+    """Projection -> attention -> projection onto the residual in place -> choice,
+    every result written over memory that the call before last read: the same
+    numbers as with memory of their own."""
+    import torch
+    d = zk.decode
+    rng = np.random.default_rng(8)
+    b, heads, dh, width, vocab, cap = 3, 4, 32, 128, 600, 96
+    qkv, o, up, lm = (_quant(zk, ref.weight(rng, k, n, 32, seg, most=60), 32, seg) for k, n, seg in
+                      ((width, 3 * heads * dh, 0), (heads * dh, width, dh), (width, width, 0), (width, vocab, 0)))
+    table, bias = _u(ds_ref.exp_table()), _u(rng.integers(-9000, 9000, vocab))
+    gelu, start = _u(rng.integers(-60000, 60000, 1 << 12)), _u(rng.integers(-(1 << 17), 1 << 17, (b, width)))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    steps, hd = 24, heads * dh
+    pool = torch.zeros(4 * b * vocab, dtype=torch.int64, device="cuda").view(torch.uint64)
+    at = lambda off, n: pool[off:off + b * n].reshape(b, n)  # noqa: E731
+
+    def run(x, cache, reuse):
+        place = (lambda off, n: at(off, n)) if reuse else (lambda off, n: None)
+        said, x = [], x.clone()
+        for i in range(steps):
+            r = d.project(x, qkv, 12, out=place(0, 3 * hd), err=err)
+            a = d.attend(r[:, :hd], cache, table, k=r[:, hd:2 * hd], v=r[:, 2 * hd:], score_scale=(11585, 32),
+                         out=place(b * 3 * hd, hd), err=err)
+            x = d.project(a, o, 12, residual=x, out=x if reuse else None, err=err)
+            u = d.project(x, up, 12, table=gelu, out=place(0, width), err=err)  # over the queries
+            x = d.project(u, up, 12, residual=x, out=x if reuse else None, err=err)
+            l = d.project(x, lm, 0, out=place(b * width, vocab), err=err)       # over keys and attention
+            token, y = d.choose_token(l, bias=bias, out=place(b * (width + vocab), vocab), err=err)
+            cache.advance()
+            said += [t.view(torch.int32 if t.dtype == torch.uint32 else torch.int64).clone() for t in (token, y, x)]
+        return said
+
+    new = lambda: d.KvCache.zeros(b, heads, dh, dh, cap)  # noqa: E731
+    want = run(start, new(), False)
+    if captured:
+        cache = new()
+        run(start, cache, True)
+        cache.lens.zero_()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(start, cache, True)
+        for _ in range(3):
+            cache.lens.zero_()
+            graph.replay()
+            assert all(torch.equal(p, q) for p, q in zip(want, got))
+    else:
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(want, run(start, new(), True)))
+    assert int(err.item()) == 0 and len({int(t[0]) for t in want[::3]}) > 3

@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
         for (int u = 0; u < NT; u++) {
             const uint32_t n = n1st + u * kStep * 16;
             on[u] = r < rows && tile1st + u * kStep < tiles && n < p.s.n;
-            bias[u] = on[u] && p.bias ? __ldg(p.bias + n) : 0;
-            residual[u] = on[u] && p.residual ? __ldg(p.residual + (uint64_t)(row0 + r) * p.ldr + n) : 0;
+            bias[u] = on[u] && p.bias ? p.bias[n] : 0;
+            residual[u] = on[u] && p.residual ? p.residual[(uint64_t)(row0 + r) * p.ldr + n] : 0;
         }
         uint64_t f[NT];
 #pragma unroll
@@ -391,7 +391,7 @@ __device__ __forceinline__ bool kv_store(const KvCache& c, const KvRows& rows, u
                                          uint64_t tok, uint32_t d, int* copy = nullptr) {
     const uint64_t head = (uint64_t)seq * c.heads + h;
     if (d < c.dk) {
-        const int64_t x = fx_to_i64(__ldg(rows.k + row * rows.ldk + (uint64_t)h * c.dk + d));
+        const int64_t x = fx_to_i64(rows.k[row * rows.ldk + (uint64_t)h * c.dk + d]);
         const int64_t y = fx_round_div_pow2(fx_wmul(x, rows.factor), rows.shift);
         const bool ok = y >= -kKeyLimit && y <= kKeyLimit;
         if (copy) *copy = ok ? (int32_t)y : 0;
@@ -399,7 +399,7 @@ __device__ __forceinline__ bool kv_store(const KvCache& c, const KvRows& rows, u
         return ok;
     }
     d -= c.dk;
-    const int64_t y = fx_to_i64(__ldg(rows.v + row * rows.ldv + (uint64_t)h * c.dv + d));
+    const int64_t y = fx_to_i64(rows.v[row * rows.ldv + (uint64_t)h * c.dv + d]);
     const bool ok = y >= INT32_MIN && y <= INT32_MAX;
     if (copy) *copy = ok ? (int32_t)y : 0;
     c.v[(head * c.cap + tok) * c.dv + d] = ok ? (int32_t)y : 0;
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
 #pragma unroll
     for (int u = 0; u < EACH; u++) {
         const uint32_t i = threadIdx.x + u * kAttThreads;  // dk <= kAttThreads
-        q_in[u] = i < heads * dk ? __ldg(p.q + seq * p.ldq + (uint64_t)(h * p.each + e0) * dk + i) : 0;
+        q_in[u] = i < heads * dk ? p.q[seq * p.ldq + (uint64_t)(h * p.each + e0) * dk + i] : 0;
     }
     const int64_t len = p.c.lens[seq];
     const bool append = p.rows.k != nullptr && len >= 0 && len < p.c.cap;
@@ -871,9 +871,9 @@ __global__ void __launch_bounds__(kChooseThreads, 2) k_choose_token(const __grid
 #pragma unroll
         for (int i = 0; i < kChooseEach; i++) {
             const bool on = i * kChooseThreads + threadIdx.x < n;
-            x[i] = on ? __ldg(logits + first + i * kChooseThreads) : 0;
-            b[i] = on && bias ? __ldg(bias + first + i * kChooseThreads) : 0;
-            mask[i] = on && allowed ? __ldg(allowed + first / 32 + i * kChooseWarps) : kNone;
+            x[i] = on ? logits[first + i * kChooseThreads] : 0;
+            b[i] = on && bias ? bias[first + i * kChooseThreads] : 0;
+            mask[i] = on && allowed ? allowed[first / 32 + i * kChooseWarps] : kNone;
         }
         if (past) {
             __syncthreads();
@@ -883,7 +883,7 @@ __global__ void __launch_bounds__(kChooseThreads, 2) k_choose_token(const __grid
                 uint32_t tok[8];
 #pragma unroll
                 for (int q = 0; q < 8; q++)
-                    tok[q] = i0 + q * kChooseThreads < past ? (uint32_t)__ldg(hist + i0 + q * kChooseThreads) : s0;
+                    tok[q] = i0 + q * kChooseThreads < past ? (uint32_t)hist[i0 + q * kChooseThreads] : s0;
 #pragma unroll
                 for (int q = 0; q < 8; q++) {
                     bad |= tok[q] >= (uint32_t)p.v;

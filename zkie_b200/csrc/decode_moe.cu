@@ -141,7 +141,7 @@ __device__ __forceinline__ void router_part(const MoeArgs& p, const uint8_t* dig
             for (int k = 0; k < kHeld; k++) {  // (a block past the end repeats the last, and is not used)
                 const uint4* r = p.router + ((uint64_t)(2 * own + rank) * p.up.s.blocks + min(b + k, b1 - 1)) * 128 + lane;
 #pragma unroll
-                for (int q = 0; q < 4; q++) w[k][q] = __ldg(r + 32 * q);
+                for (int q = 0; q < 4; q++) w[k][q] = r[32 * q];
             }
 #pragma unroll
             for (int k = 0; k < kHeld; k++)
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         prefetch_l2(p.sdown.w + (uint64_t)pair * p.sdown.s.blocks * 2 * kBytes, p.sdown.s.blocks * 2 * kBytes);
     wait_for_previous();
     for (uint32_t i = threadIdx.x; i < sizeof(Items) / 4; i += kThreads)
-        reinterpret_cast<uint32_t*>(&items)[i] = __ldcg(reinterpret_cast<const uint32_t*>(p.items) + i);
+        reinterpret_cast<uint32_t*>(&items)[i] = reinterpret_cast<const uint32_t*>(p.items)[i];
     __syncthreads();
 
     const uint32_t nf = p.down.s.blocks, ns = p.sdown.s.blocks;
@@ -713,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
             y = fx_wadd(y, round_shift(fx_wmul(d, items.score[r * p.top_k + j]), 16));
         }
         uint64_t f = fx_from_i64(y);
-        if (p.residual) f = gl_canon(gl_add(f, gl_canon(__ldg(p.residual + r * p.ldr + n))));
+        if (p.residual) f = gl_canon(gl_add(f, gl_canon(p.residual[r * p.ldr + n])));
         p.out[r * (uint64_t)p.h + n] = f;
     }
     patience_end(patience, p.err);

@@ -115,7 +115,7 @@ __device__ __forceinline__ void q4_store_digits(uint8_t* to, size_t stride, cons
 // time and has AHEAD such loads under way, whatever rows they belong to: one
 // after the other, eight rows would cost eight times the memory's latency.
 template <int THREADS, int AHEAD>
-__device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint64_t ldx, uint32_t segs, uint32_t k_seg,
+__device__ __forceinline__ bool q4_digitise(const uint64_t* x, uint64_t ldx, uint32_t segs, uint32_t k_seg,
                                             uint32_t kp_seg, uint32_t begin, uint32_t end, uint8_t* digits,
                                             uint32_t stride, uint8_t* also = nullptr) {
     const uint32_t quads = segs * kp_seg / 4;
@@ -137,13 +137,13 @@ __device__ __forceinline__ bool q4_digitise(const uint64_t* __restrict__ x, uint
             if (wide) {
                 ulonglong2 lo = make_ulonglong2(0, 0), hi = lo;
                 if (on && in < k_seg) {
-                    lo = __ldg(reinterpret_cast<const ulonglong2*>(from));
-                    hi = __ldg(reinterpret_cast<const ulonglong2*>(from) + 1);
+                    lo = reinterpret_cast<const ulonglong2*>(from)[0];
+                    hi = reinterpret_cast<const ulonglong2*>(from)[1];
                 }
                 v[u][0] = lo.x, v[u][1] = lo.y, v[u][2] = hi.x, v[u][3] = hi.y;
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[u][j] = on && in + j < k_seg ? __ldg(from + j) : 0;
+                for (int j = 0; j < 4; j++) v[u][j] = on && in + j < k_seg ? from[j] : 0;
             }
         }
 #pragma unroll
@@ -238,7 +238,10 @@ __device__ __forceinline__ void patience_end(const Patience& patience, uint32_t*
 // ---- overlap with the kernel before (programmatic dependent launch) --------------------------
 // Every kernel here lets its successor start early and waits, before it reads
 // or writes anything that an earlier kernel may have written or may still
-// read, until all earlier kernels are done.
+// read, until all earlier kernels are done.  What they may have written is then
+// read with plain loads: __ldg wants data that stays the same while the kernel
+// runs, its time before the wait included, and the compiler may move it (and
+// __ldcg) to before the wait.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -360,10 +363,10 @@ __device__ __forceinline__ int64_t round_shift(int64_t a, uint32_t s) {
 }
 
 // from_i64(to_i64(v)'s table entry): Op::GeluIndex and Op::Lookup on one value
-__device__ __forceinline__ uint64_t table_at(const uint64_t* __restrict__ table, uint64_t len, int64_t v,
+__device__ __forceinline__ uint64_t table_at(const uint64_t* table, uint64_t len, int64_t v,
                                              int64_t offset) {
     const int64_t i = fx_wadd(v, offset), hi = (int64_t)len - 1;
-    return __ldg(table + (i < 0 ? 0 : (i > hi ? hi : i)));
+    return table[i < 0 ? 0 : (i > hi ? hi : i)];
 }
 
 // A softmax's weight, round_div(e 2^16, sum) for 0 <= e < 2^31 and e <= sum <
