@@ -220,3 +220,52 @@ def test_capture_leaves_no_error_of_its_own(zk):
     graph.replay()
     with pytest.raises(ValueError, match="full"):
         dec.check()
+
+
+# ---- outputs that are given ----------------------------------------------------------------------------
+def test_outputs_apart_from_everything_else(zk):
+    """Biases, tables, masks, histories, weights, caches and the error word:
+    an output over one of them is refused before anything is enqueued."""
+    import torch
+    d, rng = zk.decode, np.random.default_rng(6)
+    m, k, v = 4, 64, 96
+    u64 = lambda t: t.reshape(-1)[:t.numel() // 2 * 2].view(torch.uint64)  # noqa: E731  any tensor's memory
+    err = torch.zeros(2 * m * v, dtype=torch.int32, device="cuda")
+    cells = lambda t, n, off=0: u64(t)[off:off + m * n].reshape(m, n)  # noqa: E731
+    q, x = _quant(zk, ref.weight(rng, k, k, 32), 32), _u(rng.integers(-99, 99, (m, k)))
+    out, table = torch.zeros((m, k), dtype=torch.uint64, device="cuda"), torch.zeros(2 * m * k, dtype=torch.uint64, device="cuda")
+    assert q.packed.numel() >= 2 * m * k
+
+    def refused(call):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    for row in range(m):
+        refused(lambda: d.project(x, q, 16, bias=out[row], out=out))
+    refused(lambda: d.project(x, q, 16, table=table, out=cells(table, k, 5)))
+    refused(lambda: d.project(x, q, 16, table=table[m * k - 1:], out=cells(table, k)))
+    refused(lambda: d.project(x, q, 16, out=cells(q.packed, k)))
+    refused(lambda: d.project(x, q, 16, out=cells(err, k), err=err[8:9]))
+    d.project(x, q, 16, bias=table[:k], table=table[k:], out=out, err=err[:1])
+
+    cache = d.KvCache.zeros(m, 1, k, k, 32)
+    big = d.KvCache(cache.k, cache.v, err[:m])
+    refused(lambda: d.attend(x, cache, table, out=cells(table, k, 7)))
+    refused(lambda: d.attend(x, cache, table, out=cells(cache.k, k)))
+    refused(lambda: d.attend(x, cache, table, out=cells(cache.v, k, 3)))
+    refused(lambda: d.attend(x, big, table, out=cells(err, k), err=err[-1:]))
+    refused(lambda: d.attend(x, cache, table, out=cells(err, k), err=err[3:4]))
+
+    router, w = _moe_case(rng, k, 4, 32, 32, 32)
+    block = _moe_block(zk, router, w, 32, 2, _exp_table(), _silu_table())
+    for t in (block.packed[0], block.packed[2], block.exp_table, block.silu_table):
+        refused(lambda: block.forward(x, out=cells(t, k, 1)))
+    refused(lambda: block.forward(x, out=cells(err, k), err=err[1:2]))
+
+    logits = _u(rng.integers(-99, 99, (m, v)))
+    words = torch.zeros(2 * m * v + 16, dtype=torch.int32, device="cuda")
+    refused(lambda: d.choose_token(logits, allowed=words[:3], out=cells(words, v)))
+    refused(lambda: d.choose_token(logits, allowed=words[:3 * m].reshape(m, 3), out=cells(words, v, 1)))
+    refused(lambda: d.choose_token(logits, words[-5 * m:].reshape(m, 5), out=cells(words, v)))
+    refused(lambda: d.choose_token(logits, _i32(np.zeros((m, 2))), words[40:40 + m], out=cells(words, v)))
+    refused(lambda: d.choose_token(logits, out=cells(words, v), err=words[9:10]))
+    assert not err[1:].any()

@@ -130,15 +130,26 @@ at::Tensor output(PyObject* o, at::IntArrayRef shape, int dev) {
     flat<uint64_t>(t, "out", at::kUInt64, dev, shape);
     return t;
 }
-// A given output shares no memory with what the blocks of a call read at different times; the
-// residual may be the output itself, each number being read by the thread that writes it.
-void apart(PyObject* given, const at::Tensor& out, const Rows& in, int64_t cols, const char* name, bool same = false) {
-    if (given == Py_None || in.n == 0 || !in.data) return;
-    const auto* a = static_cast<const uint64_t*>(out.data_ptr());
-    const uint64_t *a_end = a + out.numel(), *b_end = in.data + (in.n - 1) * in.stride + cols;
-    if (same && in.data == a && (in.n == 1 || in.stride == cols)) return;
-    if (a < b_end && in.data < a_end) refuse(std::string("out shares memory with ") + name);
-}
+// A given output shares no memory with anything that the blocks of a call read (or write) at
+// different times; the residual may be the output itself, each number being read by the thread that
+// writes it.
+struct Apart {
+    const char *begin = nullptr, *end = nullptr;  // none where the call makes its output
+    Apart(PyObject* given, const at::Tensor& out) {
+        if (given == Py_None || out.numel() == 0) return;
+        begin = static_cast<const char*>(out.data_ptr());
+        end = begin + out.nbytes();
+    }
+    void from(const void* data, int64_t bytes, const char* name) const {
+        const char* b = static_cast<const char*>(data);
+        if (begin && b && bytes > 0 && begin < b + bytes && b < end) refuse(std::string("out shares memory with ") + name);
+    }
+    void from(const at::Tensor& t, const char* name) const { from(t.numel() ? t.data_ptr() : nullptr, (int64_t)t.nbytes(), name); }
+    void from(const Rows& in, int64_t cols, const char* name, bool same = false) const {
+        if (in.n == 0 || (same && reinterpret_cast<const char*>(in.data) == begin && (in.n == 1 || in.stride == cols))) return;
+        from(in.data, 8 * ((in.n - 1) * in.stride + cols), name);
+    }
+};
 uint32_t* word(PyObject* o, int dev) {
     const at::Tensor& t = tensor(o, "err");
     if (t.numel() != 1) refuse("err: one int32 word is wanted, not " + said(t));
@@ -195,8 +206,13 @@ PyObject* project(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 refuse("residual: " + std::to_string(residual.n) + " rows, " + std::to_string(in.n) + " are wanted");
         }
         const at::Tensor out = output(a[7], {in.n, n}, dev);
-        apart(a[7], out, in, k, "x");
-        apart(a[7], out, residual, n, "the residual (and is not it)", true);
+        const Apart apart(a[7], out);
+        apart.from(in, k, "x");
+        apart.from(residual, n, "the residual (and is not it)", true);
+        apart.from(bias, 8 * n, "the bias");
+        apart.from(table, 8 * table_len, "the table");
+        apart.from(tensor(w.at(0), "packed"), "the weight");
+        apart.from(tensor(a[8], "err"), "the error word");
         done(zkie2_q4_project(in.data, in.stride, in.n, packed, k, n, group, segment, shift, bias, table, table_len,
                               offset, residual.data, residual.stride, static_cast<uint64_t*>(out.data_ptr()),
                               word(a[8], dev), stream(dev)), "zkie2_q4_project");
@@ -234,9 +250,13 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const int64_t offset = a[8] == Py_None ? t.numel() : number(a[8]);
         const uint32_t out_shift = shift_of(a[9], "out_shift");
         const at::Tensor out = output(a[10], {batch, cols / dk * dv}, dev);
-        apart(a[10], out, in, cols, "q");
-        apart(a[10], out, k, heads * dk, "k");
-        apart(a[10], out, v, heads * dv, "v");
+        const Apart apart(a[10], out);
+        apart.from(in, cols, "q");
+        apart.from(k, heads * dk, "k");
+        apart.from(v, heads * dv, "v");
+        apart.from(t, "the table");
+        for (int i = 0; i < 3; i++) apart.from(tensor(c.at(i), "cache"), "the cache");
+        apart.from(tensor(a[11], "err"), "the error word");
         done(zkie2_kv_attend(in.data, in.stride, cols / dk, qs.factor, qs.shift, k.data, k.stride, v.data, v.stride, ks.factor,
                              ks.shift, ck, cv, lens, batch, heads, dk, dv, cap, ss.factor, ss.shift, table, t.numel(), offset,
                              out_shift, static_cast<uint64_t*>(out.data_ptr()), word(a[11], dev), stream(dev)),
@@ -274,8 +294,11 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                 refuse("residual: " + std::to_string(residual.n) + " rows, " + std::to_string(in.n) + " are wanted");
         }
         const at::Tensor out = output(a[3], {in.n, h}, dev), gate = make({in.n, experts}, at::kUInt64, dev);
-        apart(a[3], out, in, h, "x");
-        apart(a[3], out, residual, h, "the residual (and is not it)", true);
+        const Apart apart(a[3], out);
+        apart.from(in, h, "x");
+        apart.from(residual, h, "the residual (and is not it)", true);
+        for (int i = 7; i < 14; i++) apart.from(tensor(b.at(i), "MoeBlock"), "the block's weights and tables");
+        apart.from(tensor(a[4], "err"), "the error word");
         // this call's own: calls on other streams may run beside it
         const uint64_t elems = zkie2_moe_rows_scratch_elems(in.n, h, experts, top_k, f, shared_f, group);
         const at::Tensor scratch = make({(int64_t)elems + 1}, at::kLong, dev);
@@ -326,8 +349,13 @@ PyObject* choose(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                                                                        : flat<int32_t>(t, "allowed", at::kInt, dev, {words}));
         }
         const at::Tensor out = output(a[9], {b, v}, dev), token = make({b}, at::kUInt32, dev);
-        apart(a[9], out, {logits, b, v}, v, "the logits");
-        apart(a[9], out, {bias, bias_stride ? b : 1, v}, v, "the bias");
+        const Apart apart(a[9], out);
+        apart.from(x, "the logits");
+        apart.from(bias, 8 * v * (bias_stride ? b : 1), "the bias");
+        apart.from(allowed, 4 * words * (allowed_stride ? b : 1), "the mask");
+        apart.from(history, 4 * b * tokens, "the history");
+        apart.from(lens, 4 * b, "the history's lengths");
+        apart.from(tensor(a[10], "err"), "the error word");
         done(zkie2_choose_token(logits, b, v, history, tokens, lens, number(PyTuple_GET_ITEM(a[3], 0)),
                                 number(PyTuple_GET_ITEM(a[3], 1)), number(a[4]), number(a[5]), bias, bias_stride, allowed,
                                 allowed_stride, number(a[8]), static_cast<uint64_t*>(out.data_ptr()),
