@@ -269,3 +269,27 @@ def test_outputs_apart_from_everything_else(zk):
     refused(lambda: d.choose_token(logits, _i32(np.zeros((m, 2))), words[40:40 + m], out=cells(words, v)))
     refused(lambda: d.choose_token(logits, out=cells(words, v), err=words[9:10]))
     assert not err[1:].any()
+
+
+def test_caches_apart_from_their_rows(zk):
+    """A cache is written while its rows are read: they share no memory, nor do
+    its own tensors."""
+    import torch
+    d = zk.decode
+    mem = torch.zeros(32 * 8 * 4, dtype=torch.int32, device="cuda")
+    k, v, lens = mem[:256].reshape(1, 1, 1, 2, 32, 4), mem[256:512].reshape(1, 1, 32, 8), mem[512:513]
+    cache, table = d.KvCache(k, v, lens), _u(_exp_table(8))
+    u64 = lambda a: mem[a:a + 16].view(torch.uint64).reshape(1, 8)  # noqa: E731
+    free = u64(600)
+    for args in ((u64(0), free, free), (free, u64(100), free), (free, free, u64(248)), (free, u64(500), free)):
+        with pytest.raises(ValueError, match="shares memory"):
+            d.attend(args[0], cache, table, k=args[1], v=args[2])
+    for args in ((u64(100), free), (free, u64(240)), (free, u64(512))):
+        with pytest.raises(ValueError, match="share memory"):
+            cache.append(args[0][None], args[1][None])
+    for bad in ((k, mem[252:508].reshape(1, 1, 32, 8), lens), (k, v, mem[3:4]), (k, v, mem[511:512])):
+        with pytest.raises(ValueError, match="share memory"):
+            d.KvCache(*bad)
+    assert not mem.any()
+    d.attend(free, cache, table, k=free, v=free)  # side by side they may lie
+    d.attend(u64(0), cache, table)  # and what is only read may be read twice

@@ -130,19 +130,21 @@ at::Tensor output(PyObject* o, at::IntArrayRef shape, int dev) {
     flat<uint64_t>(t, "out", at::kUInt64, dev, shape);
     return t;
 }
-// A given output shares no memory with anything that the blocks of a call read (or write) at
-// different times; the residual may be the output itself, each number being read by the thread that
-// writes it.
+// What a call writes -- an output that is given, a cache -- shares no memory with anything that its
+// blocks read (or write) at different times; the residual may be the output itself, each number being
+// read by the thread that writes it.
 struct Apart {
     const char *begin = nullptr, *end = nullptr;  // none where the call makes its output
-    Apart(PyObject* given, const at::Tensor& out) {
-        if (given == Py_None || out.numel() == 0) return;
+    const char* what;
+    explicit Apart(const at::Tensor& out, const char* name) : what(name) {
+        if (out.numel() == 0) return;
         begin = static_cast<const char*>(out.data_ptr());
         end = begin + out.nbytes();
     }
+    Apart(PyObject* given, const at::Tensor& out) : Apart(given == Py_None ? at::Tensor() : out, "out") {}
     void from(const void* data, int64_t bytes, const char* name) const {
         const char* b = static_cast<const char*>(data);
-        if (begin && b && bytes > 0 && begin < b + bytes && b < end) refuse(std::string("out shares memory with ") + name);
+        if (begin && b && bytes > 0 && begin < b + bytes && b < end) refuse(std::string(what) + " shares memory with " + name);
     }
     void from(const at::Tensor& t, const char* name) const { from(t.numel() ? t.data_ptr() : nullptr, (int64_t)t.nbytes(), name); }
     void from(const Rows& in, int64_t cols, const char* name, bool same = false) const {
@@ -257,6 +259,13 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         apart.from(t, "the table");
         for (int i = 0; i < 3; i++) apart.from(tensor(c.at(i), "cache"), "the cache");
         apart.from(tensor(a[11], "err"), "the error word");
+        for (int i = 0; i < 2 && k.data; i++) {  // the new token is stored while other blocks read
+            const Apart cache(tensor(c.at(i), "cache"), "the cache");
+            cache.from(in, cols, "q");
+            cache.from(k, heads * dk, "k");
+            cache.from(v, heads * dv, "v");
+            cache.from(t, "the table");
+        }
         done(zkie2_kv_attend(in.data, in.stride, cols / dk, qs.factor, qs.shift, k.data, k.stride, v.data, v.stride, ks.factor,
                              ks.shift, ck, cv, lens, batch, heads, dk, dv, cap, ss.factor, ss.shift, table, t.numel(), offset,
                              out_shift, static_cast<uint64_t*>(out.data_ptr()), word(a[11], dev), stream(dev)),

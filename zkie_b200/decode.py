@@ -254,6 +254,9 @@ class KvCache:
                              "131072 are wanted")
         if (k.data_ptr() | v.data_ptr()) & 15:
             raise ValueError("KvCache: 16-byte aligned buffers are wanted")
+        spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in (k, v, lens))
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("KvCache: k, v and lens share memory")
         self._k, self._v, self._lens = k, v, lens
         self._numels = (k.numel(), v.numel(), lens.numel())
         self.call = (k, v, lens, self.batch, self.heads, self.dk, self.dv, self.capacity)
@@ -289,6 +292,9 @@ class KvCache:
         mine, sizes = self.call[:3], self.call[3:]
         if any(t.numel() != n for t, n in zip(mine, self._numels)):
             raise ValueError("append: the cache's tensors have other sizes than they had")
+        if any(a.data_ptr() < b.data_ptr() + 8 * b.numel() and b.data_ptr() < a.data_ptr() + 4 * a.numel()
+               for a in mine for b in (k, v)):
+            raise ValueError("append: the rows share memory with the cache")
         check(lib.zkie2_kv_append(k.data_ptr(), k.shape[2], v.data_ptr(), v.shape[2], k.shape[1], *k_scale,
                                   *[t.data_ptr() for t in mine], *sizes, word.data_ptr(), _stream()), "zkie2_kv_append")
         if err is None:
