@@ -44,3 +44,23 @@ def test_kernels_that_start_early_wait_and_restrict_nothing():
         for m in re.finditer(r"__device__ __forceinline__ [^;{]*\{", code):
             assert "__restrict__" not in m.group(), m.group()
     assert early == 5
+
+
+def test_nothing_is_asked_for_after_a_wait_that_gave_up():
+    """A barrier whose copy never came has no arrival left in its phase: another
+    expect_tx would take its count below zero, and another copy would go to a
+    slot whose first one is still under way.  Every ring's ask, and every
+    later wait, ends at once."""
+    wait = _body(_code("q4.cuh"), _code("q4.cuh").index("void barrier_wait"))
+    assert wait.index("if (patience.failed) return;") < wait.index("mbarrier.try_wait")
+    asks = [(name, m.start()) for name in FILES for m in re.finditer(r"auto ask = ", _code(name))]
+    assert len(asks) == 4
+    for name, at in asks:
+        text = _body(_code(name), at)
+        assert re.match(r"auto ask = \[&\]\(\) \{\s*if \(patience\.failed\) return;", text), text[:120]
+    # and there is no other place that asks for a copy
+    for name in FILES[1:]:
+        code = _code(name)
+        inside = sum(_body(code, at).count("barrier_expect(") for n, at in asks if n == name)
+        assert code.count("barrier_expect(") == inside and code.count("bulk_copy(") == sum(
+            _body(code, at).count("bulk_copy(") for n, at in asks if n == name)

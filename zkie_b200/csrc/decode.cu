@@ -174,7 +174,9 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     };
     uint32_t next_batch = tile0, next_at = first_of(tile0, warp), next_end = first_of(tile0, warp + 1), next_slot = 0;
     uint32_t next_b = next_at % blocks;  // within its tile
+    Patience patience;
     auto ask = [&]() {  // lane 0 only
+        if (patience.failed) return;
         while (next_at == next_end) {
             next_batch += kProjBatch;
             if (next_batch >= tile1) {
@@ -206,7 +208,6 @@ __global__ void __launch_bounds__(kProjThreads, 1) k_q4_project(const __grid_con
     __syncthreads();
 
     const uint32_t from = shared_addr(digits) + g * p.stride + 16 * t;  // column g: digit g % 4 of row g / 4
-    Patience patience;
     uint32_t slot = 0, phase = 0;
     for (uint32_t batch = tile0; batch < tile1; batch += kProjBatch) {
         uint32_t at = first_of(batch, warp);
@@ -538,7 +539,9 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
         const uint32_t there = min((uint32_t)kKvBlock, cached - b * kKvBlock), at = i * vtokens;
         return at < there ? min(vtokens, there - at) : 0u;
     };
+    Patience patience;
     auto ask = [&]() {  // lane 0 only
+        if (patience.failed) return;
         if (next_b >= b1 - b0) {
             if (next_v || warp >= b1 - b0) return;
             next_v = true;
@@ -564,7 +567,6 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     };
     if (lane == 0)
         for (uint32_t i = 0; i < kAttDepth; i++) ask();
-    Patience patience;
     uint32_t slot = 0, phase = 0;
     auto step = [&]() {  // on to the next slot, this one being filled again
         __syncwarp();

@@ -362,7 +362,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
         next_at += next_left;
         return true;
     };
+    Patience patience;
     auto ask = [&]() {  // lane 0 only: fill the ring, up to RUN blocks of one tile to a slot
+        if (patience.failed) return;
         while (asked < taken + DEPTH) {
             if (next_left == 0 && !next_tile()) return;
             const uint32_t run = min((uint32_t)RUN, next_left), b = bar + 8 * next_slot;
@@ -412,7 +414,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_up(const __grid_constant__ 
     __syncthreads();
     cluster_arrive();  // the neighbour's logits: waited for after the first batch
 
-    Patience patience;
     uint32_t slot = 0, phase = 0;
     bool routed = false;
     auto token_of = [&](bool shared, uint32_t first, uint32_t j) { return shared ? first + j : items.token[first + j]; };
@@ -632,7 +633,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
         locate(now, at);
         next = now;
     }
+    Patience patience;
     auto ask = [&]() {  // lane 0 only
+        if (patience.failed) return;
         const uint32_t b = bar + 8 * next_slot, to = shared_addr(ring + next_slot * kSlot);
         const uint32_t run = min(kDownRun, min(end - next_at, next.len - next.b));
         barrier_expect(b, run * (2 * kBytes + 256 * next.count));
@@ -648,7 +651,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant_
     if (lane == 0)
         for (uint32_t i = 0; i < p.depth; i++)
             if (next_at < end) ask();
-    Patience patience;
     uint32_t slot = 0, phase = 0;
     while (at < end) {
         const uint32_t stop = min(end, at + now.len - now.b);

@@ -175,12 +175,12 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
 // One lane asks for a run of blocks with one instruction; a barrier in shared
 // memory counts its bytes.  The bytes in flight depend on no register, and the
 // stream of a warp's blocks runs on across tiles, sums and block-wide waits.
-// A wait gives up after a bounded number of attempts (a second or so), says so
-// in the error word, and every later one then after a few.
+// A wait gives up after a bounded number of attempts (a second or so) and says
+// so in the error word; nothing more is then asked for or waited for.
 constexpr uint32_t kErrWait = 32u;
+constexpr uint32_t kTries = 1u << 18;
 
 struct Patience {
-    uint32_t tries = 1u << 18;
     bool failed = false;
 };
 
@@ -215,7 +215,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, const void* from, uint32_
                  : "memory");
 }
 __device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, Patience& patience) {  // the whole warp
-    for (uint32_t i = 0; i < patience.tries; i++) {
+    if (patience.failed) return;
+    for (uint32_t i = 0; i < kTries; i++) {
         uint32_t done;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
@@ -225,7 +226,6 @@ __device__ __forceinline__ void barrier_wait(uint32_t bar, uint32_t parity, Pati
         if (__all_sync(0xFFFFFFFFu, done)) return;
     }
     patience.failed = true;
-    patience.tries = 64;
 }
 // At a kernel's end: a wait that gave up is told, and the copies that it was
 // for get another ten milliseconds before their shared memory is given away.
