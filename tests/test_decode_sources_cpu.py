@@ -64,3 +64,54 @@ def test_nothing_is_asked_for_after_a_wait_that_gave_up():
         inside = sum(_body(code, at).count("barrier_expect(") for n, at in asks if n == name)
         assert code.count("barrier_expect(") == inside and code.count("bulk_copy(") == sum(
             _body(code, at).count("bulk_copy(") for n, at in asks if n == name)
+
+
+# ---- the binding ----------------------------------------------------------------------------------
+def test_the_binding_is_built_again_for_another_torch(zk, monkeypatch, tmp_path):
+    from zkie_b200 import build
+    ran = []
+
+    class Done:
+        returncode, stderr = 0, ""
+
+    def run(cmd, **kw):
+        ran.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return Done()
+
+    monkeypatch.setattr(build, "CALLS", str(tmp_path / "_calls.so"))
+    monkeypatch.setattr(build, "BUILD", str(tmp_path / "_build"))
+    if hasattr(build, "CALLS_FOR"):
+        monkeypatch.setattr(build, "CALLS_FOR", str(tmp_path / "_build" / "for"))
+    monkeypatch.setattr(build.subprocess, "run", run)
+    build.build_calls()
+    assert len(ran) == 1
+    build.build_calls()
+    assert len(ran) == 1
+    import importlib.metadata
+    real = importlib.metadata.version
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "9.9" if name == "torch" else real(name))
+    build.build_calls()
+    assert len(ran) == 2
+    build.build_calls()
+    assert len(ran) == 2
+
+
+def test_the_package_imports_without_its_binding(zk):
+    """A binding that does not load stops the per-token calls, not the proofs."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.modules["zkie_b200._calls"] = None
+import zkie_b200 as zk
+import zkie_b200.deepseek
+assert zk.lib.zkie2_q4_words(1, 64, 16, 64, 0) == 136
+try:
+    zk.decode.choose_token(0, err=0)
+except ImportError as e:
+    assert "zkie_b200.build" in str(e)
+    print("refused")
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(CSRC)))
+    assert res.stdout.strip() == "refused", res.stderr

@@ -20,6 +20,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libzkie_b200.so")
 BINDING = os.path.join(HERE, "binding", "calls.cpp")
 CALLS = os.path.join(HERE, "_calls.so")
+CALLS_FOR = os.path.join(BUILD, "calls.built_for")  # the torch and the Python that it was built against
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -74,10 +75,15 @@ def _compile(src: str, obj: str, verbose_ptxas: bool) -> str:
 
 
 def build_calls(force: bool = False):
-    """The Python extension zkie_b200._calls (after the library it links)."""
+    """The Python extension zkie_b200._calls (after the library it links), again
+    when its sources, torch or Python have changed."""
+    from importlib.metadata import version
     newest = max(os.path.getmtime(f) for f in (BINDING, os.path.join(INCLUDE, "zkie2.h")))
-    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest:
-        return
+    built_for = f"torch {version('torch')}, Python {sys.version}"
+    if not force and os.path.exists(CALLS) and os.path.getmtime(CALLS) >= newest and os.path.exists(CALLS_FOR):
+        with open(CALLS_FOR) as f:
+            if f.read() == built_for:
+                return
     import sysconfig
     import torch
     base = os.path.dirname(torch.__file__)
@@ -91,6 +97,9 @@ def build_calls(force: bool = False):
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING}:\n{res.stderr}")
     os.replace(tmp, CALLS)
+    os.makedirs(BUILD, exist_ok=True)
+    with open(CALLS_FOR, "w") as f:
+        f.write(built_for)
 
 
 def build(force: bool = False, verbose_ptxas: bool = False, jobs: int = 8) -> str:

@@ -24,12 +24,12 @@ likes (``check_err``); not given, the call reads its own, which synchronises,
 and raises ValueError.  Besides the op layer's bits, 8 is a value outside the
 32-bit range the kernels take (computed on as zero) and 16 a full cache.
 """
+from importlib import import_module
 from typing import Optional, Tuple
 
 import torch
 
 from ._lib import check, lib
-from . import _calls  # after the library it links
 from .compose import _INDEX_WRITERS, _check_err, _err_word
 from .device import P, device
 
@@ -43,6 +43,23 @@ def check_err(err: torch.Tensor, what: str = "decode"):
     _check_err(err, what)
 
 
+class _Calls:
+    """The extension zkie_b200._calls, loaded with the first per-token call:
+    one built for another torch fails here and leaves the rest of the package
+    alone."""
+
+    def __getattr__(self, name: str):
+        try:
+            module = import_module(__package__ + "._calls")
+        except ImportError as e:
+            raise ImportError("zkie_b200/_calls.so is missing or does not load: build it with `python -m zkie_b200.build` "
+                              "(there is no fallback)") from e
+        for call in ("project", "attend", "moe", "choose"):
+            setattr(self, call, getattr(module, call))
+        return getattr(module, name)
+
+
+_calls = _Calls()
 _U64, _I32 = torch.uint64, torch.int32
 
 
