@@ -58,21 +58,18 @@ def moe_graph(zk, store, rng, group=32, **shape):
     return s, ops, weights, top
 
 
-def liven(store, ops):
+def liven(store, ops, weight=12000):
     """Numbers at which every part of a layer counts, in place of a builder's
     (whose norms' scales of 1 to 5 in 2^16 leave little but the biases, and
     whose weights are all positive): norms' scales about 1, weights of both
-    signs, embeddings about 1.  Zeros stay, the padding among them."""
+    signs up to ``weight``, embeddings about 1.  Zeros stay, the padding among
+    them."""
+    import torch
+    from zkie_b200 import decode
+
     def numbers(t):
         v = store.get(t)
-        return ref.signed(v if isinstance(v, np.ndarray) else v.cpu().numpy())
-
-    def put(t, v):
-        if isinstance(store.get(t), np.ndarray):
-            store.v[t] = ref.field(v)
-        else:
-            import torch
-            store.v[t] = torch.from_numpy(ref.field(v)).to(store.get(t).device)
+        return decode._signed(torch.from_numpy(v) if isinstance(v, np.ndarray) else v)
 
     written, news = {t for op in ops for t in op.writes()}, {}
     for i, op in enumerate(ops):
@@ -80,12 +77,13 @@ def liven(store, ops):
             news[op.w], news[op.b] = (lambda v: 60000 + 2000 * v), (lambda v: 3000 * v)
         elif op.kind in ("Projection", "GatherMatMul") or (op.kind == "MatMul" and op.b not in written):
             t = op.b if op.kind == "MatMul" else op.w
-            if numbers(t).min() >= 0:
-                news[t] = lambda v: (2 * v - v.max()) * 12000 // v.max()
+            if int(numbers(t).min()) >= 0:
+                news[t] = lambda v: torch.div((2 * v - v.max()) * weight, v.max(), rounding_mode="floor")
         elif i == 0 and op.kind == "Lookup":
             news[op.table] = lambda v: (v - 25) * 3000
         elif i == 1 and op.kind == "Add":
             news[op.b] = lambda v: (v - 25) * 2000
     for t, f in news.items():
         v = numbers(t)
-        put(t, np.where(v != 0, f(v), 0))
+        new = decode._field(torch.where(v != 0, f(v), torch.zeros_like(v)))
+        store.v[t] = new.numpy() if isinstance(store.get(t), np.ndarray) else new

@@ -92,6 +92,67 @@ def test_moe_layer_steps_equal_the_graph_where_attention_counts(zk, shift):
     dec.check()
 
 
+def test_gpt2_at_its_own_shape(zk):
+    """Two layers of GPT-2's graph (1024 wide, 65536 logits, 512 positions):
+    three sequences, from empty, within and at the end of the text."""
+    import torch
+    s, store = zk.gpt2.GPT2_SMALL, zk.compose.Store()
+    ops, tok, out = zk.gpt2.gpt2_model(store, s, layers=2)
+    ds_ref.liven(store, ops, 2500)
+    weights = zk.decode.quantise_weights(store, ops, ("Projection", "MatMul"))
+    zk.compose.forward_ops(store, ops)
+    logits = store.get(next(op for op in ops if op.kind == "Argmax").x).view(torch.int64).reshape(s.m, s.vocab)
+    tokens, argmax = store.get_idx(tok).view(torch.int32), store.get_idx(out).view(torch.int32)
+    dec, start = zk.gpt2.Gpt2Decoder(store, ops, s, weights, batch=3), [0, 200, 502]
+    for b in range(3):
+        dec.load(store, b, start[b])
+    for i in range(10):
+        at = [a + i for a in start]
+        dec.tokens.copy_(tokens[at].view(torch.uint32))
+        token, got = dec.step()
+        assert torch.equal(got.view(torch.int64), logits[at]) and torch.equal(token.view(torch.int32), argmax[at]), i
+    dec.check()
+    assert len(set(argmax.tolist())) > 400
+
+
+def test_moe_layer_at_its_own_shape(zk):
+    """DeepSeek-V2-Lite's layer (2048 wide, 64 experts, 512 positions), its
+    first positions past a block of the cache."""
+    import torch
+    from zkie_b200 import deepseek as ds
+    s, store = ds.DSV2_LITE, zk.compose.Store()
+    ops, x, out = ds.moe_layer(store, s)
+    ds_ref.liven(store, ops, 2500)
+    weights = zk.decode.quantise_weights(store, ops)
+    zk.compose.forward_ops(store, ops)
+    rows = lambda t: store.get(t).view(torch.int64).reshape(s.m, s.h)  # noqa: E731
+    dec = ds.MoeLayerDecoder(store, ops, s, weights, 2)
+    for i in range(40):
+        got = dec.step(rows(x)[[i, i]].view(torch.uint64))
+        assert torch.equal(got.view(torch.int64), rows(out)[[i, i]]), i
+    dec.check()
+
+
+@pytest.mark.parametrize("token", [500, 512, 517, 1023, 512 * 63, 1 << 31, (1 << 32) - 1])
+def test_gpt2_tokens_outside_the_vocabulary(zk, token):
+    """Said at the step: the embedding's last dimension, or its first, lies
+    outside the table.  (From vocab_real to vocab the graph's padding is a
+    token like any other.)"""
+    import torch
+    s, store = zk.gpt2.LayerShape(**ds_ref.GPT2), zk.compose.Store()
+    ops, _, _ = zk.gpt2.gpt2_model(store, s, layers=1)
+    dec = zk.gpt2.Gpt2Decoder(store, ops, s, zk.decode.quantise_weights(store, ops, ("Projection", "MatMul")), batch=2)
+    dec.tokens.copy_(torch.tensor([3, token], dtype=torch.int64).to(torch.uint32))
+    dec.step()
+    if token < s.vocab:
+        dec.check()
+    else:
+        with pytest.raises(ValueError, match="index outside"):
+            dec.check()
+    dec.step()  # the next tokens are its own
+    dec.check()
+
+
 # ---- what the decoders refuse -----------------------------------------------------------------------
 def test_decoders_refuse_a_table_that_does_not_begin_with_zero(zk):
     """A table of 2^19 entries begins with 22, which the graph counts for every masked column."""
