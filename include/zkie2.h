@@ -637,7 +637,7 @@ int zkie2_eq_combine(const uint64_t *h_points, const uint64_t *h_coeffs, uint32_
  * a whole sequence; every result equals the same row of the arms named with
  * it, bit for bit.  Beside the bits of *d_err above: 8, a value outside the
  * range that the kernels take (it is replaced by zero); 16, a cache without
- * room; 32, a copy that did not arrive (the call's results are void).  None of
+ * room (or with more tokens counted than it holds); 32, a copy that did not arrive (the call's results are void).  None of
  * these synchronizes; row strides (ld*) are in elements.  An output shares no
  * memory with an input, except that it may be the residual itself.
  * zkie2_q4_project and zkie2_moe_rows start to read their packed weights while

@@ -293,3 +293,19 @@ def test_caches_apart_from_their_rows(zk):
     assert not mem.any()
     d.attend(free, cache, table, k=free, v=free)  # side by side they may lie
     d.attend(u64(0), cache, table)  # and what is only read may be read twice
+
+
+def test_a_length_beyond_the_capacity_is_said(zk):
+    """Tokens that the cache does not hold were counted: the answer over those
+    it holds is not the row's."""
+    import torch
+    rng = np.random.default_rng(7)
+    _, _, cache = _cache(zk, rng, 3, 1, 8, 8, 32, [32, 5, 20])
+    q, table, err = _u(rng.integers(-99, 99, (3, 8))), _u(_exp_table()), torch.zeros(1, dtype=torch.int32, device="cuda")
+    zk.decode.attend(q, cache, table, err=err)
+    assert int(err.item()) == 0
+    cache.lens[2] = 33
+    zk.decode.attend(q, cache, table, err=err)
+    assert int(err.item()) == 16
+    with pytest.raises(ValueError, match="full"):
+        zk.decode.attend(q, cache, table)

@@ -34,7 +34,7 @@ namespace {
 
 constexpr uint32_t kErrIndex = 1u;
 constexpr uint32_t kErrDivide = 2u;
-constexpr uint32_t kErrFull = 16u;  // a cache without room for the new token
+constexpr uint32_t kErrFull = 16u;  // a cache without room for the tokens that are counted
 constexpr size_t kMaxShared = 226 * 1024;  // dynamic, next to what is declared
 
 // ---- the weight ---------------------------------------------------------------------------
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) k_kv_attend(const __grid_const
     }
     const int64_t len = p.c.lens[seq];
     const bool append = p.rows.k != nullptr && len >= 0 && len < p.c.cap;
-    if (p.rows.k != nullptr && len >= p.c.cap && threadIdx.x == 0) atomicOr(p.err, kErrFull);
+    if (len >= (int64_t)p.c.cap + (p.rows.k == nullptr) && threadIdx.x == 0) atomicOr(p.err, kErrFull);
     const uint32_t n = (uint32_t)(len < 0 ? 0 : min(len, (int64_t)p.c.cap));  // tokens in the cache
     if (n + append == 0) {  // the whole cluster's answer
         for (uint32_t i = rank * kAttThreads + threadIdx.x; i < heads * dv; i += ranks * kAttThreads) out[i] = 0;
