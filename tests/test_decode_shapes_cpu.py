@@ -142,3 +142,33 @@ def test_moe_decoder_refuses_other_rows(zk):
               torch.zeros((3, 128), dtype=torch.int64), torch.zeros((3, 64), dtype=torch.uint64), [0]):
         with pytest.raises(ValueError, match="MoeLayerDecoder: x"):
             dec.step(x)
+
+
+# ---- quantising a store --------------------------------------------------------------------------------
+def test_quantise_weights_all_or_none(zk):
+    """A weight that has no 4-bit form leaves the store as it was, with the
+    weights before it as they were."""
+    import torch
+    c = zk.compose
+
+    class Store:
+        def __init__(self):
+            self.v = []
+
+        def push(self, a):
+            self.v.append(torch.from_numpy(ref.field(np.asarray(a).reshape(-1))))
+            return len(self.v) - 1
+
+        def get(self, t):
+            return self.v[t]
+
+    rng, st = np.random.default_rng(3), Store()
+    a, b = st.push(rng.integers(-9000, 9000, (32, 8))), st.push(np.full((32, 8), 1 << 21))
+    ops = [c.Projection(0, t, 0, 2, 3, 1, 32, 8, 16) for t in (a, b)]
+    before = [t.clone() for t in st.v]
+    with pytest.raises(ValueError, match="65535"):
+        zk.decode.quantise_weights(st, ops, group=32)
+    assert all(torch.equal(x.view(torch.int64), y.view(torch.int64)) for x, y in zip(st.v, before))
+    done = zk.decode.quantise_weights(st, ops[:1], group=32)
+    assert list(done) == [a] and np.array_equal(ref.signed(st.v[a].numpy()).reshape(32, 8),
+                                                ref.dense(*[t.numpy() for t in done[a][:2]], 32))

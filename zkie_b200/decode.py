@@ -132,9 +132,11 @@ def quantise(w: torch.Tensor, group: int = 64, segment: int = 0) -> Tuple[torch.
 
 def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: int = 64) -> dict:
     """Quantise the weights that the ops of these kinds read (Projection w,
-    GatherMatMul w, MatMul b where no op writes it), in place: the Store gets
-    the dense tensor that the codes stand for, so the model that is run and
-    proven is the quantised one.  Returns {tensor id: (codes, scales, group)},
+    GatherMatMul w, MatMul b where no op writes it): the Store gets
+    the dense tensors that the codes stand for in their place (all of them, or
+    none where one raises), so the model that is run and proven is the
+    quantised one; a forward or a prover that was recorded before reads the old
+    ones.  Returns {tensor id: (codes, scales, group)},
     what QuantWeight takes."""
     written = {t for op in ops if op.kind not in _INDEX_WRITERS for t in op.writes()}
     done = {}
@@ -143,10 +145,10 @@ def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: in
         if op.kind not in kinds or t is None or t in done or t in written:
             continue
         shape = (op.n_experts, op.k, op.n) if op.kind == "GatherMatMul" else (op.k, op.n)
-        codes, scales = quantise(store.get(t).reshape(shape), group)
-        row = _group_of(op.k, group, 0, codes.device)
+        done[t] = (*quantise(store.get(t).reshape(shape), group), group)
+    for t, (codes, scales, _) in done.items():  # all of them have a 4-bit form
+        row = _group_of(codes.shape[-2], group, 0, codes.device)
         store.v[t] = _field(codes.to(torch.int64) * scales.to(torch.int64)[..., row, :]).reshape(-1)
-        done[t] = (codes, scales, group)
     return done
 
 
