@@ -145,24 +145,25 @@ def test_moe_decoder_refuses_other_rows(zk):
 
 
 # ---- quantising a store --------------------------------------------------------------------------------
+class _TorchStore:
+    def __init__(self):
+        self.v = []
+
+    def push(self, a):
+        import torch
+        self.v.append(torch.from_numpy(ref.field(np.asarray(a).reshape(-1))))
+        return len(self.v) - 1
+
+    def get(self, t):
+        return self.v[t]
+
+
 def test_quantise_weights_all_or_none(zk):
     """A weight that has no 4-bit form leaves the store as it was, with the
     weights before it as they were."""
     import torch
     c = zk.compose
-
-    class Store:
-        def __init__(self):
-            self.v = []
-
-        def push(self, a):
-            self.v.append(torch.from_numpy(ref.field(np.asarray(a).reshape(-1))))
-            return len(self.v) - 1
-
-        def get(self, t):
-            return self.v[t]
-
-    rng, st = np.random.default_rng(3), Store()
+    rng, st = np.random.default_rng(3), _TorchStore()
     a, b = st.push(rng.integers(-9000, 9000, (32, 8))), st.push(np.full((32, 8), 1 << 21))
     ops = [c.Projection(0, t, 0, 2, 3, 1, 32, 8, 16) for t in (a, b)]
     before = [t.clone() for t in st.v]
@@ -172,3 +173,22 @@ def test_quantise_weights_all_or_none(zk):
     done = zk.decode.quantise_weights(st, ops[:1], group=32)
     assert list(done) == [a] and np.array_equal(ref.signed(st.v[a].numpy()).reshape(32, 8),
                                                 ref.dense(*[t.numpy() for t in done[a][:2]], 32))
+
+
+def test_quantise_weights_in_the_stores_own_memory(zk):
+    """A recorded forward or prover has the addresses of the Store's tensors:
+    they stay, and hold the new numbers."""
+    import torch
+    c, rng, st = zk.compose, np.random.default_rng(4), _TorchStore()
+    a, b = st.push(rng.integers(-9000, 9000, (32, 8))), st.push(rng.integers(-9000, 9000, (3, 40, 8)))
+    ops = [c.Projection(9, a, 9, 7, 8, 1, 32, 8, 16), c.GatherMatMul(9, 0, b, 8, 1, 40, 8, 3)]
+    held = list(st.v)
+    done = zk.decode.quantise_weights(st, ops, group=32)
+    for t in (a, b):
+        assert st.v[t] is held[t]
+        codes, scales = (x.numpy() for x in done[t][:2])
+        want = ref.dense(codes, scales, 32) if t == a else np.stack([ref.dense(codes[e], scales[e], 32) for e in range(3)])
+        assert np.array_equal(ref.signed(held[t].numpy()), want.reshape(-1))
+    st.v.append(st.v[a][:64])  # another id for part of the same memory
+    with pytest.raises(ValueError, match="share memory"):
+        zk.decode.quantise_weights(st, [ops[0], c.Projection(9, 2, 9, 7, 8, 1, 8, 8, 16)], group=32)

@@ -309,3 +309,19 @@ def test_a_length_beyond_the_capacity_is_said(zk):
     assert int(err.item()) == 16
     with pytest.raises(ValueError, match="full"):
         zk.decode.attend(q, cache, table)
+
+
+def test_a_recorded_forward_runs_the_quantised_weights(zk):
+    """Recorded before the weights were quantised, replayed after."""
+    import torch
+    s = zk.gpt2.LayerShape(**ds_ref.GPT2)
+    store = zk.compose.Store()
+    ops, _, out = zk.gpt2.gpt2_layer(store, s)
+    ds_ref.liven(store, ops)
+    recorded = zk.compose.GraphForward(store, ops)
+    plain = store.get(out).view(torch.int64).clone()
+    zk.decode.quantise_weights(store, ops, ("Projection",), 32)
+    recorded.run()
+    got = store.get(out).view(torch.int64).clone()
+    zk.compose.forward_ops(store, ops)
+    assert torch.equal(got, store.get(out).view(torch.int64)) and not torch.equal(got, plain)

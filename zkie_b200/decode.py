@@ -132,12 +132,11 @@ def quantise(w: torch.Tensor, group: int = 64, segment: int = 0) -> Tuple[torch.
 
 def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: int = 64) -> dict:
     """Quantise the weights that the ops of these kinds read (Projection w,
-    GatherMatMul w, MatMul b where no op writes it): the Store gets
-    the dense tensors that the codes stand for in their place (all of them, or
-    none where one raises), so the model that is run and proven is the
-    quantised one; a forward or a prover that was recorded before reads the old
-    ones.  Returns {tensor id: (codes, scales, group)},
-    what QuantWeight takes."""
+    GatherMatMul w, MatMul b where no op writes it), in the Store's own tensors: they hold the
+    dense numbers that the codes stand for (all of them, or none where one
+    raises), so the model that is run and proven is the quantised one, by a
+    forward or a prover that was recorded before, too.  Returns {tensor id:
+    (codes, scales, group)}, what QuantWeight takes."""
     written = {t for op in ops if op.kind not in _INDEX_WRITERS for t in op.writes()}
     done = {}
     for op in ops:
@@ -146,9 +145,13 @@ def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: in
             continue
         shape = (op.n_experts, op.k, op.n) if op.kind == "GatherMatMul" else (op.k, op.n)
         done[t] = (*quantise(store.get(t).reshape(shape), group), group)
+    spans = sorted((store.get(t).data_ptr(), store.get(t).data_ptr() + 8 * store.get(t).numel()) for t in done)
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("quantise_weights: weights that share memory")
     for t, (codes, scales, _) in done.items():  # all of them have a 4-bit form
         row = _group_of(codes.shape[-2], group, 0, codes.device)
-        store.v[t] = _field(codes.to(torch.int64) * scales.to(torch.int64)[..., row, :]).reshape(-1)
+        dense = _field(codes.to(torch.int64) * scales.to(torch.int64)[..., row, :]).reshape(-1)
+        store.get(t).view(torch.int64).copy_(dense.view(torch.int64))
     return done
 
 
