@@ -325,3 +325,15 @@ def test_a_recorded_forward_runs_the_quantised_weights(zk):
     got = store.get(out).view(torch.int64).clone()
     zk.compose.forward_ops(store, ops)
     assert torch.equal(got, store.get(out).view(torch.int64)) and not torch.equal(got, plain)
+
+
+def test_append_refuses_factors_beyond_64_bits(zk):
+    """As attend does; they were cut to 64 bits."""
+    cache = zk.decode.KvCache.zeros(1, 1, 4, 4, 32)
+    rows = _u(np.ones((1, 1, 4), dtype=np.int64))
+    for factor in ((1 << 64) + 1, 1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="64 bits"):
+            cache.append(rows, rows, k_scale=(factor, 0))
+    assert not cache.k.any()
+    with pytest.raises(OverflowError):
+        zk.decode.attend(rows[0], cache, _u(_exp_table(8)), k=rows[0], v=rows[0], k_scale=(1 << 64, 0))

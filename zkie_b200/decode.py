@@ -310,6 +310,8 @@ class KvCache:
                 raise ValueError(f"{name}: uint64 ({self.batch}, tokens, {cols}), as many tokens of k and v, is wanted")
         if self.device != dev or k.shape[1] > 1 << 17 or not 0 <= k_scale[1] <= 62:
             raise ValueError("append: the cache's device, at most 131072 tokens and a shift 0 .. 62 are wanted")
+        if not -(1 << 63) <= k_scale[0] < 1 << 63:
+            raise ValueError("append: a factor of 64 bits is wanted")
         k, v, word = k.contiguous(), v.contiguous(), _err_word() if err is None else _flat(err, "err", _I32, dev)
         mine, sizes = self.call[:3], self.call[3:]
         if any(t.numel() != n for t, n in zip(mine, self._numels)):
