@@ -64,7 +64,9 @@ def test_a_copied_weight_has_its_own_memory(zk, how):
     w, x = ref.weight(rng, 96, 40, 32), rng.integers(-(1 << 18), 1 << 18, (3, 96))
     q = _quant(zk, w, 32)
     other = COPIES[how](q)
+    import torch
     q.packed.zero_()  # codes and scales of zero
+    torch.cuda.synchronize()
     assert not _s(zk.decode.project(_u(x), q, 9)).any()
     del q
     _i32(np.full(1 << 16, -1))  # whoever takes the memory that is free now
@@ -74,6 +76,7 @@ def test_a_copied_weight_has_its_own_memory(zk, how):
 
 @pytest.mark.parametrize("how", COPIES)
 def test_a_copied_block_has_its_own_memory(zk, how):
+    import torch
     rng = np.random.default_rng(3)
     router, w = _moe_case(rng, 64, 8, 48, 40, 32)
     x, exp, silu = rng.integers(-(1 << 17), 1 << 17, (3, 64)), _exp_table(), _silu_table()
@@ -81,6 +84,7 @@ def test_a_copied_block_has_its_own_memory(zk, how):
     other = COPIES[how](block)
     for t in (block.router, *block.packed, block.exp_table, block.silu_table):
         t.zero_()
+    torch.cuda.synchronize()
     del block
     out, gate = other.forward(_u(x))
     want, want_gate = ref.moe(x, router, w, 32, exp, silu, 3)
@@ -337,3 +341,18 @@ def test_append_refuses_factors_beyond_64_bits(zk):
     assert not cache.k.any()
     with pytest.raises(OverflowError):
         zk.decode.attend(rows[0], cache, _u(_exp_table(8)), k=rows[0], v=rows[0], k_scale=(1 << 64, 0))
+
+
+def test_a_copy_of_weights_is_complete(zk):
+    """Calls start to read weights while earlier kernels still run, so a copy's
+    are there when copying returns, whatever the stream had to do."""
+    import torch
+    rng = np.random.default_rng(9)
+    router, w = _moe_case(rng, 32, 4, 16, 16, 32)
+    for handle in (_quant(zk, w[3], 32), _moe_block(zk, router, w, 32, 2, _exp_table(12), _silu_table(12))):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(50_000_000)  # 25 ms
+            copy.deepcopy(handle)
+            assert side.query()
+        torch.cuda.synchronize()

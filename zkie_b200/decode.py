@@ -156,12 +156,22 @@ def quantise_weights(store, ops, kinds=("Projection", "GatherMatMul"), group: in
 
 
 def _kept(name: str) -> property:
-    """A handle's tensor: read, and written in place, but not replaced -- calls
-    take it from ``call``, which a copy or a pickle of the handle has its own of."""
+    """A handle's tensor: not replaced -- calls take it from ``call``, which a
+    copy or a pickle of the handle has its own of.  A cache's may be written
+    in place; a weight's are only read, unless the host waits before the next
+    call (calls start to read weights while earlier kernels still run)."""
     return property(lambda self: getattr(self, name))
 
 
-class QuantWeight:
+class _Weights:
+    """Handles of weights: those of a copy are complete before a call too."""
+
+    def __setstate__(self, state: dict):
+        self.__dict__.update(state)
+        torch.cuda.current_stream(self.device).synchronize()
+
+
+class QuantWeight(_Weights):
     """A weight w[k][n] = codes[k][n] scales[row of k][n] in 4 bits, laid out
     once for the kernels (``packed``).
 
@@ -371,7 +381,7 @@ def masked_counts_nothing(table, what: str):
 
 
 # ---- a mixture-of-experts layer -----------------------------------------------------------------------
-class MoeBlock:
+class MoeBlock(_Weights):
     """build_moe's layer for a few tokens: router (h x experts, field elements
     of at most 32639 in size), the routed experts' gate, up (experts x h x f)
     and down (experts x f x h) and the shared experts' gate, up (h x shared f)
