@@ -137,9 +137,9 @@ constexpr uint32_t kProjBatch = 16;     // tiles whose sums are held at a time
 // Bound by: for few rows and a wide weight the weight's bytes (1024 x 65536 in
 // groups of 128, one row: 36 MB in 10.2 us, of which 3 us are the launch, the
 // row's digits and the last sums: 5 TB/s in between); for eight rows what a
-// warp does per block and pair of rows, about ten cycles of the SM (17.5 us:
-// 2.1 TB/s); for a small weight the launch and three trips to memory (1024 x
-// 192: 2.9 us).  A ring's slots are of four blocks because copies of 2176
+// warp does per block and pair of rows, about ten cycles of the SM (17.8 us:
+// 2.0 TB/s); for a small weight the launch and three trips to memory (1024 x
+// 192: 2.8 us).  A ring's slots are of four blocks because copies of 2176
 // bytes reach 5.8 TB/s and single blocks 3.7 (eight blocks to a slot: within 4
 // % either way); with three slots to a ring, 24 warps of 80 registers instead
 // of 16 of 127 take 20.8 us for the eight rows instead of 18.3, 20 warps 19.9.
@@ -347,7 +347,7 @@ int project_seg(const ProjectArgs& p, cudaStream_t stream) {
 template <int G>
 int project_rows(ProjectArgs p, cudaStream_t stream) {
     // Rows to a block: as many as there are, up to eight, so that a weight is read once for them, and
-    // as their digits leave room for (1024 x 65536: eight rows 17.5 us, four 13.7, two 10.7, one 10.2,
+    // as their digits leave room for (1024 x 65536: eight rows 17.8 us, four 12.4, two 10.2, one 10.2,
     // one row with eight's kernel 16.9).  Slots of four blocks where there is room, else of two or one
     // (one row 10.6, 13.2, 18.0 us, of rings of three; a weight of 1024 x 192 in 3.0, 2.9, 2.8).
     for (uint32_t rows = p.m > 4 ? 8 : p.m > 2 ? 4 : 2;; rows /= 2)
@@ -465,12 +465,12 @@ struct AttendArgs {
 // A product is one 32 x 32 + 64 bit multiply-add, 32 a clock on an SM.
 //
 // Bound by: for one long sequence the two streams (16 heads of 192 + 128, 4096
-// tokens: 82 MB in 26.6 us, keys 10 us and values 7 at 4.5 to 5 TB/s, between
+// tokens: 82 MB in 26.7 us, keys 10 us and values 7 at 4.5 to 5 TB/s, between
 // them 7 us of meetings and table entries, the first bytes 2); for a ragged
 // batch the longest sequence's blocks, whose cluster is as large as any other
-// (eight sequences of up to 8192 tokens, four query heads to a key head: 69
+// (eight sequences of up to 8192 tokens, four query heads to a key head: 70
 // us, of which multiply-adds cost 12, table entries 10, the streams the
-// rest); for a short one the chain of latencies (512 tokens: 8.5 us).  Half
+// rest); for a short one the chain of latencies (512 tokens: 8.2 us).  Half
 // the heads' products in double precision: 69 us instead of 71, not kept; an
 // L2 prefetch of the values during the softmax: 29 to 32 us instead of 27; the
 // table's entries asked for sixteen at a time by a thread: the same 71, their
@@ -833,7 +833,7 @@ constexpr uint32_t kChooseStep = kChooseThreads * kChooseEach;
 // takes 32 neighbours, so a mask word is one load.
 //
 // Bound by the chain launch - lengths - history - logits - cluster: one row of
-// 65536 takes 5.8 us, sixteen of 50257 with histories of 4096 9.3 us (19.7 MB:
+// 65536 takes 5.9 us, sixteen of 50257 with histories of 4096 9.4 us (19.7 MB:
 // 2.1 TB/s, every block reading its row's whole history).  Histories loaded
 // before their lengths are known: 13.7 us instead of 12.8 at the time; four
 // logits to a thread, three blocks to an SM: 13.0; 1024 threads: 16.7.
@@ -1099,7 +1099,7 @@ int zkie2_choose_token(const uint64_t* d_logits, uint64_t batch, uint64_t vocab,
                        frequency, d_bias, bias_stride, d_allowed, allowed_stride, mask_value, d_out, d_token, d_err};
     // Blocks to a row: the fewest steps of the vocabulary at which the rows' clusters find room at
     // once, with up to half as many blocks again where those do too.  A second wave of clusters
-    // costs more than a second step (sixteen rows of 50257 logits: 9.3 us as clusters of thirteen,
+    // costs more than a second step (sixteen rows of 50257 logits: 9.4 us as clusters of thirteen,
     // 12.8 of sixteen; 32 rows 12.8 us as clusters of nine, 18.7 of sixteen), and clusters that
     // fill an SM's share of threads evenly more than the steps alone (24 rows: 11.2 and 12.8 us).
     static std::atomic<uint64_t> set{0};

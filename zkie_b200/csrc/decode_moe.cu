@@ -576,10 +576,10 @@ struct DownAt {
 //
 // Bound by (sizes as above): one token 6.5 us, of which 1.5 pass before the
 // items are there and 3.5 stream 10 MB; sixteen tokens some 25 us, 3 before the
-// items, 18 over 81 MB of codes (4.5 TB/s) and as many bytes of digits from the
-// second-level cache, by the number of copies: two to a slot, one of 2176 bytes
-// of codes and one of digits, where a copy to each tile and token took the layer
-// from 94 to 103 us.  Slots of more blocks but fewer tokens' digits, two or
+// items, 18 over 81 MB of codes (4.5 TB/s) and 46 MB of digits from the
+// second-level cache, by the number of copies more than by their bytes: two to a
+// slot, one of 2176 bytes of codes and one of digits, where a copy to each tile
+// and token took the layer from 94 to 103 us.  Slots of more blocks but fewer tokens' digits, two or
 // three blocks by what fits: 97 to 104 us.
 template <bool TWO>
 __global__ void __launch_bounds__(kThreads, 1) k_moe_down(const __grid_constant__ MoeArgs p) {

@@ -10,10 +10,12 @@
 // spends two instructions a block on two rows of x.  The instruction is the
 // warp-wide mma.sync (two cycles of an SM, latency 20): with up to eight rows
 // a product is bound by the weight's bytes and by what each warp does around
-// the instruction -- taking codes apart, scaling groups -- and the matrix pipe
-// is busy 19 % of the time at eight rows, so accumulators in
-// tensor memory would save nothing and cost their set-up in a call of a few
-// microseconds.
+// the instruction -- taking codes apart, scaling groups.  At eight rows the
+// matrix pipe is busy 19 % of the time and 126 registers a thread leave four
+// warps to a scheduler, too few to cover its latency and that of the
+// instructions around it.  Accumulators in tensor memory would free registers
+// and cost a set-up and a read-back of every group's sums; that form has not
+// been measured.
 //
 // The sums are exact: within a block 16 c d stays below 2^29 even with two
 // digits joined, the scaled group sums are added in 64 bits, and a padded K
