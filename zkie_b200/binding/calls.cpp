@@ -94,11 +94,10 @@ struct Handle {
     int64_t size(int i) const { return number(at(i)); }
     template <typename T>
     T* memory(PyObject* o, const char* what, at::ScalarType type, int64_t numel) const {
-        const std::string full = std::string(name) + ": " + what;
-        const at::Tensor& t = tensor(o, full.c_str());
+        const at::Tensor& t = tensor(o, what);
         if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != dev || !t.is_contiguous() || t.numel() != numel)
-            refuse(full + " is not the memory of " + std::to_string(numel) + " numbers on the call's device that it was, but " +
-                   said(t));
+            refuse(std::string(name) + ": " + what + " is not the memory of " + std::to_string(numel) +
+                   " numbers on the call's device that it was, but " + said(t));
         return static_cast<T*>(t.data_ptr());
     }
     template <typename T>
@@ -141,14 +140,18 @@ struct Apart {
         begin = static_cast<const char*>(out.data_ptr());
         end = begin + out.nbytes();
     }
-    Apart(PyObject* given, const at::Tensor& out) : Apart(given == Py_None ? at::Tensor() : out, "out") {}
+    Apart(PyObject* given, const at::Tensor& out) : what("out") {
+        if (given != Py_None) *this = Apart(out, "out");
+    }
     void from(const void* data, int64_t bytes, const char* name) const {
         const char* b = static_cast<const char*>(data);
         if (begin && b && bytes > 0 && begin < b + bytes && b < end) refuse(std::string(what) + " shares memory with " + name);
     }
-    void from(const at::Tensor& t, const char* name) const { from(t.numel() ? t.data_ptr() : nullptr, (int64_t)t.nbytes(), name); }
+    void from(const at::Tensor& t, const char* name) const {
+        if (begin && t.numel()) from(t.data_ptr(), (int64_t)t.nbytes(), name);
+    }
     void from(const Rows& in, int64_t cols, const char* name, bool same = false) const {
-        if (in.n == 0 || (same && reinterpret_cast<const char*>(in.data) == begin && (in.n == 1 || in.stride == cols))) return;
+        if (!begin || in.n == 0 || (same && reinterpret_cast<const char*>(in.data) == begin && (in.n == 1 || in.stride == cols))) return;
         from(in.data, 8 * ((in.n - 1) * in.stride + cols), name);
     }
 };
@@ -257,7 +260,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         apart.from(k, heads * dk, "k");
         apart.from(v, heads * dv, "v");
         apart.from(t, "the table");
-        for (int i = 0; i < 3; i++) apart.from(tensor(c.at(i), "cache"), "the cache");
+        for (int i = 0; apart.begin && i < 3; i++) apart.from(tensor(c.at(i), "cache"), "the cache");
         apart.from(tensor(a[11], "err"), "the error word");
         for (int i = 0; i < 2 && k.data; i++) {  // the new token is stored while other blocks read
             const Apart cache(tensor(c.at(i), "cache"), "the cache");
@@ -306,7 +309,7 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const Apart apart(a[3], out);
         apart.from(in, h, "x");
         apart.from(residual, h, "the residual (and is not it)", true);
-        for (int i = 7; i < 14; i++) apart.from(tensor(b.at(i), "MoeBlock"), "the block's weights and tables");
+        for (int i = 7; apart.begin && i < 14; i++) apart.from(tensor(b.at(i), "MoeBlock"), "the block's weights and tables");
         apart.from(tensor(a[4], "err"), "the error word");
         // this call's own: calls on other streams may run beside it
         const uint64_t elems = zkie2_moe_rows_scratch_elems(in.n, h, experts, top_k, f, shared_f, group);
