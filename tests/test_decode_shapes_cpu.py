@@ -192,3 +192,19 @@ def test_quantise_weights_in_the_stores_own_memory(zk):
     st.v.append(st.v[a][:64])  # another id for part of the same memory
     with pytest.raises(ValueError, match="share memory"):
         zk.decode.quantise_weights(st, [ops[0], c.Projection(9, 2, 9, 7, 8, 1, 8, 8, 16)], group=32)
+
+
+def test_decoders_refuse_other_graphs(zk):
+    """Graphs of other builders, and parts of their own."""
+    from zkie_b200 import deepseek as ds
+    st, ops, s = _gpt2_ops(zk)
+    _, moe, ms = _moe_ops(zk)
+    layer = zk.gpt2.gpt2_layer(co.HostStore(), s)[0]
+    reference = zk.gpt2.reference_layer_roundtrip_case(co.HostStore(), zk.XorShift64)[0]
+    kinds = sorted({op.kind for op in ops})
+    for other in (layer, reference, moe, [], *[[op for op in ops if op.kind != k] for k in kinds if k not in ("Transpose", "MatMul", "Softmax")]):
+        with pytest.raises(ValueError, match="shape"):
+            zk.gpt2.Gpt2Decoder(st, other, s, {})
+    for other in (ops, layer, [], *[[op for op in moe if op.kind != k] for k in ("Projection", "RmsNorm", "RoPE", "Scale")]):
+        with pytest.raises(ValueError, match="shape"):
+            ds.MoeLayerDecoder(st, other, ms, {})

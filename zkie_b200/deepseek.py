@@ -18,6 +18,7 @@ RoPE's cos / sin at scale 2^16.
 for a few rows, one token at a time, with the weights of such a graph in 4
 bits (``decode.quantise_weights``), bit for bit the graph's rows.
 """
+from collections import defaultdict
 from dataclasses import dataclass
 from typing import Optional
 
@@ -324,10 +325,10 @@ class MoeLayerDecoder:
     def _shaped(ops, s: MoeShape) -> bool:
         """Whether the graph is moe_layer's of this shape: the attention's sizes,
         shifts, Scales and tables (the experts are read from the graph)."""
-        of = {}
+        of = defaultdict(list)
         for op in ops:
-            of.setdefault(op.kind, []).append(op)
-        proj, norms = of.get("Projection", []), of.get("RmsNorm", [])
+            of[op.kind].append(op)
+        proj, norms = of["Projection"], of["RmsNorm"]
         if len(proj) != 2 + 5 * s.heads + 3 or len(norms) != 3:
             return False
         sizes = [(s.h, s.kv_lora), (s.h, s.qk_rope)] + [
@@ -336,7 +337,7 @@ class MoeLayerDecoder:
             [(op.m, op.d, op.n_real) for op in norms] == [(s.m, d, d) for d in (s.h, s.kv_lora, s.h)] and \
             [(op.m, op.d, op.shift) for op in of["RoPE"]] == [(s.m, s.qk_rope, s.shift)] * (1 + s.heads) and \
             [(op.factor, op.shift) for op in of["Scale"][:2 * s.heads]] == [(7519, 32), (1, 16)] * s.heads and \
-            all((op.offset, op.table_len) == (1 << s.exp_bits,) * 2 for op in of["StableSoftmaxIndex"])
+            [(op.offset, op.table_len) for op in of["StableSoftmaxIndex"]] == [(1 << s.exp_bits,) * 2] * (s.heads + 1)
 
     def _norm(self, x, i):
         w, d = self.norms[i]

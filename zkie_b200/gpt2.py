@@ -28,6 +28,7 @@ in 4 bits (``decode.quantise_weights``): its logits are the graph's rows, bit
 for bit.
 """
 import ctypes as C
+from collections import defaultdict
 from dataclasses import dataclass
 
 import numpy as np
@@ -436,12 +437,12 @@ class Gpt2Decoder:
     def _shaped(store, ops, s: LayerShape) -> bool:
         """Whether the graph is gpt2_model's of this shape: sizes, shifts, the
         Scales' factors, the tables' offsets and the vocabulary's mask."""
-        of = {}
+        of = defaultdict(list)
         for op in ops:
-            of.setdefault(op.kind, []).append(op)
-        proj, norms, per = of.get("Projection", []), of.get("LayerNormCentered", []), 4 * s.heads + 2
+            of[op.kind].append(op)
+        proj, norms, per = of["Projection"], of["LayerNormCentered"], 4 * s.heads + 2
         layers = len(proj) // per
-        if not layers or len(proj) % per or len(norms) != 2 * layers + 1 or "Argmax" not in of:
+        if not layers or len(proj) % per or len(norms) != 2 * layers + 1 or not of["Argmax"] or len(of["Lookup"]) != 1 + layers:
             return False
         sizes = [(s.d, s.dh)] * 3 + [(s.dh, s.d)]
         sizes = sizes * s.heads + [(s.d, s.ffn), (s.ffn, s.d)]
@@ -450,8 +451,8 @@ class Gpt2Decoder:
             return False
         scales = [(23170, 16)] * 2 + [(1, 16)] * 2  # queries, keys, scores, outputs
         if [(op.factor, op.shift) for op in of["Scale"]] != scales * (layers * s.heads) or \
-                any((op.offset, op.table_len) != (1 << s.exp_bits,) * 2 for op in of["StableSoftmaxIndex"]) or \
-                any((op.offset, op.table_len) != (1 << s.gelu_bits >> 1, 1 << s.gelu_bits) for op in of["GeluIndex"]):
+                [(op.offset, op.table_len) for op in of["StableSoftmaxIndex"]] != [(1 << s.exp_bits,) * 2] * (layers * s.heads) or \
+                [(op.offset, op.table_len) for op in of["GeluIndex"]] != [(1 << s.gelu_bits >> 1, 1 << s.gelu_bits)] * layers:
             return False
         last = of["Argmax"][-1]
         mask = next((store.get(op.b)[:s.vocab] for op in of["Add"] if op.c == last.x), None)
