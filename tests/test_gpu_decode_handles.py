@@ -356,3 +356,14 @@ def test_a_copy_of_weights_is_complete(zk):
             copy.deepcopy(handle)
             assert side.query()
         torch.cuda.synchronize()
+
+
+def test_an_output_without_memory(zk):
+    """Raised as torch raises it, and nothing is left behind."""
+    import torch
+    n = 1 << 22
+    q = zk.decode.QuantWeight(torch.ones((1, n), dtype=torch.int8), torch.ones((1, n), dtype=torch.int32), group=32)
+    x = torch.ones((65535, 1), dtype=torch.int64, device="cuda").view(torch.uint64)
+    with pytest.raises(torch.OutOfMemoryError):
+        zk.decode.project(x, q, 0)
+    assert _s(zk.decode.project(x[:2], q, 0)).sum() == 2 * n

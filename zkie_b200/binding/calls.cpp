@@ -9,6 +9,7 @@
 #include <Python.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -169,15 +170,16 @@ void done(int rc, const char* what) {
     }
 }
 
+// what torch itself throws -- an output that finds no memory -- is raised as torch raises it
 template <typename F>
 PyObject* guarded(F f) {
+    HANDLE_TH_ERRORS
     try {
         return f();
     } catch (const Refused&) {
-    } catch (const std::exception& e) {  // an allocation that failed
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
     }
-    return nullptr;
+    END_HANDLE_TH_ERRORS
 }
 
 // project(x, (packed, k, n, group, segment, experts), shift, bias, table, offset, residual, out, err)
