@@ -208,3 +208,47 @@ def test_decoders_refuse_other_graphs(zk):
     for other in (ops, layer, [], *[[op for op in moe if op.kind != k] for k in ("Projection", "RmsNorm", "RoPE", "Scale")]):
         with pytest.raises(ValueError, match="shape"):
             ds.MoeLayerDecoder(st, other, ms, {})
+
+
+def _changed(st, t, at):
+    """The store with one word of a tensor changed; put back by calling what it returns."""
+    old = st.v[t]
+    st.v[t] = old.copy()
+    st.v[t][at] = (int(old[at]) + 1) % ref.P
+    return lambda: st.v.__setitem__(t, old)
+
+
+def test_decoders_refuse_tensors_they_do_not_compute_with(zk, monkeypatch):
+    """Norms and biases that differ from row to row, biases where a model has
+    none, other masks than the causal one: the steps would leave them out."""
+    from zkie_b200 import deepseek as ds
+    st, ops, s = _gpt2_ops(zk)
+    first = lambda ops, kind, i=0: [op for op in ops if op.kind == kind][i]  # noqa: E731
+    assert zk.gpt2.Gpt2Decoder._filled(st, ops, s)
+    for t, at in ((first(ops, "LayerNormCentered").w, s.d), (first(ops, "LayerNormCentered", 2).b, 3), (first(ops, "Projection").bias, 20),
+                  (first(ops, "Projection", 3).bias, 0), (first(ops, "Projection", 7).bias, -1), (first(ops, "Projection", -1).bias, s.d + 1),
+                  (first(ops, "StableSoftmaxIndex").mask, 0)):
+        back = _changed(st, t, at)
+        with pytest.raises(ValueError, match="biases or masks"):
+            zk.gpt2.Gpt2Decoder(st, ops, s, {})
+        back()
+    assert zk.gpt2.Gpt2Decoder._filled(st, ops, s)
+    st, ops, s = _moe_ops(zk)
+    for t, at in ((first(ops, "RmsNorm").w, s.h), (first(ops, "RmsNorm", 2).w, 1), (first(ops, "Projection").bias, 5),
+                  (first(ops, "Projection", 6).bias, 0), (first(ops, "Projection", -1).bias, 9), (first(ops, "StableSoftmaxIndex").mask, 1)):
+        back = _changed(st, t, at)
+        with pytest.raises(ValueError, match="biases or masks"):
+            ds.MoeLayerDecoder(st, ops, s, {})
+        back()
+    monkeypatch.setattr(zk.decode, "QuantWeight", lambda *a: a)
+    monkeypatch.setattr(zk.decode, "MoeBlock", lambda *a: a)
+    top = next(i for i, op in enumerate(ops) if op.kind == "TopKSelect")
+    given = {op.w: () for op in ops if op.kind in ("GatherMatMul", "Projection")}
+    block = lambda: ds.moe_block(st, ops, given, ops[top - 1].table, ops[top - 1].table)  # noqa: E731
+    block()
+    for t, at in ((ops[top - 2].mask, 7), (first(ops, "Projection", -3).bias, 0), (first(ops, "Projection", -1).bias, -1)):
+        back = _changed(st, t, at)
+        with pytest.raises(ValueError, match="build_moe"):
+            block()
+        back()
+    block()

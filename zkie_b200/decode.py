@@ -27,6 +27,7 @@ and raises ValueError.  Besides the op layer's bits, 8 is a value outside the
 from importlib import import_module
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 
 from ._lib import check, lib
@@ -367,6 +368,27 @@ def attend(q: torch.Tensor, cache: KvCache, table: torch.Tensor, *, k: Optional[
     if err is None:
         _check_err(word, "attend")
     return out
+
+
+def _numbers(t):
+    """A store's tensor (of the device's or a host store) to compare words of."""
+    return t.view(torch.int64) if isinstance(t, torch.Tensor) else t
+
+
+def same_rows(t, n: int) -> bool:
+    """Whether a matrix of n columns is one row over and over."""
+    rows = _numbers(t).reshape(-1, n)
+    return bool((rows == rows[:1]).all())
+
+
+def all_zero(t) -> bool:
+    return not bool((_numbers(t) != 0).any())
+
+
+def masks(t, mask) -> bool:
+    """Whether a store's tensor holds the words of ``mask`` (numpy)."""
+    t = t.cpu().numpy() if isinstance(t, torch.Tensor) else t
+    return np.array_equal(t, mask)
 
 
 def masked_counts_nothing(table, what: str):

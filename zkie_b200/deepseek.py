@@ -272,11 +272,13 @@ def moe_block(store, ops, weights: dict, exp_table: int, silu_table: int, shift:
     experts = [op for op in ops[at:] if op.kind == "GatherMatMul"]
     shared = [op for op in ops[at:] if op.kind == "Projection"]
     scales = [op for op in ops[at - 3:] if op.kind in ("Scale", "ScaleVec")]
-    if router.kind != "MatMul" or len(experts) != 3 or len(shared) != 3:
+    if router.kind != "MatMul" or ops[at - 2].kind != "StableSoftmaxIndex" or len(experts) != 3 or len(shared) != 3:
         raise ValueError("moe_block: not a graph of build_moe")
     if any((op.factor, op.shift) != (1, 16) for op in scales if op.kind == "Scale") or \
             any(op.shift != 16 for op in scales if op.kind == "ScaleVec") or len({op.shift for op in shared}) != 1:
         raise ValueError("moe_block: not a graph of build_moe: Scales by 2^16 and one shift of the shared experts are wanted")
+    if not all(decode.all_zero(store.get(t)) for t in (ops[at - 2].mask, *[op.bias for op in shared])):
+        raise ValueError("moe_block: not a graph of build_moe: a mask of the experts or biases that the kernels do not have")
     if shift not in (None, shared[0].shift):
         raise ValueError(f"moe_block: shift {shift}, the graph's shared experts have {shared[0].shift}")
     quant = lambda op: decode.QuantWeight(*weights[op.w])  # noqa: E731
@@ -295,6 +297,11 @@ class MoeLayerDecoder:
     def __init__(self, store, ops, s: MoeShape, weights: dict, batch: int = 1):
         if not self._shaped(ops, s):
             raise ValueError("MoeLayerDecoder: not a graph of moe_layer with this shape")
+        causal = {op.mask for op in [op for op in ops if op.kind == "StableSoftmaxIndex"][:s.heads]}
+        if not all(decode.all_zero(store.get(op.bias)) for op in ops if op.kind == "Projection") or \
+                not all(decode.same_rows(store.get(op.w), op.d) for op in ops if op.kind == "RmsNorm") or \
+                not all(decode.masks(store.get(t), causal_mask(s.m)) for t in causal):
+            raise ValueError("MoeLayerDecoder: biases or masks that the steps do not compute with")
         soft = next(op for op in ops if op.kind == "Softmax")
         decode.masked_counts_nothing(store.get(soft.table), "MoeLayerDecoder")
         self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())

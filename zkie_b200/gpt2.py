@@ -383,6 +383,8 @@ class Gpt2Decoder:
     def __init__(self, store, ops, s: LayerShape, weights: dict, batch: int = 1):
         if not self._shaped(store, ops, s):
             raise ValueError("Gpt2Decoder: not a graph of gpt2_model with this shape")
+        if not self._filled(store, ops, s):
+            raise ValueError("Gpt2Decoder: biases or masks that the steps do not compute with")
         tables = {op.kind: op for op in ops}
         decode.masked_counts_nothing(store.get(tables["Softmax"].table), "Gpt2Decoder")
         self.s, self.batch, self.err = s, batch, torch.zeros(1, dtype=torch.int32, device=device())
@@ -412,6 +414,8 @@ class Gpt2Decoder:
             cat = lambda ids: torch.cat([rows(t, s.dh).view(torch.int64) for t in ids]).view(torch.uint64)  # noqa: E731
             # the output bias is added after the heads' sum: Add(acc, o_b)
             o_b = next(op.b for op in ops if op.kind == "Add" and op.a == self._sum_of(ops, [o.out for o in kinds[3]]))
+            if not decode.same_rows(store.get(o_b), s.d):
+                raise ValueError("Gpt2Decoder: biases or masks that the steps do not compute with")
             self.layers.append(dict(
                 ln1=(wide(norms[n].w, s.d), wide(norms[n].b, s.d)), ln2=(wide(norms[n + 1].w, s.d), wide(norms[n + 1].b, s.d)),
                 qkv=quant([o.w for j in range(3) for o in kinds[j]], 1), qkv_b=cat([o.bias for j in range(3) for o in kinds[j]]),
@@ -458,8 +462,20 @@ class Gpt2Decoder:
         mask = next((store.get(op.b)[:s.vocab] for op in of["Add"] if op.c == last.x), None)
         if mask is None or (last.m, last.n) != (s.m, s.vocab):
             return False
-        mask = mask.cpu().numpy() if isinstance(mask, torch.Tensor) else mask
-        return np.array_equal(mask, from_i64(np.where(np.arange(s.vocab) < s.vocab_real, 0, decode.MASKED)))
+        return decode.masks(mask, from_i64(np.where(np.arange(s.vocab) < s.vocab_real, 0, decode.MASKED)))
+
+    @staticmethod
+    def _filled(store, ops, s: LayerShape) -> bool:
+        """Whether the graph's tensors are what the steps compute with: norms'
+        scales and biases one row over and over, no bias of a head's output
+        projection, the causal mask."""
+        proj, per = [op for op in ops if op.kind == "Projection"], 4 * s.heads + 2
+        row = [(t, s.d) for op in ops if op.kind == "LayerNormCentered" for t in (op.w, op.b)]
+        none = [op.bias for i, op in enumerate(proj) if i % per < 4 * s.heads and i % per % 4 == 3]
+        row += [(op.bias, op.n) for op in proj if op.bias not in none]
+        causal = causal_mask(s.m)
+        return all(decode.same_rows(store.get(t), n) for t, n in row) and all(decode.all_zero(store.get(t)) for t in none) and \
+            all(decode.masks(store.get(t), causal) for t in {op.mask for op in ops if op.kind == "StableSoftmaxIndex"})
 
     @staticmethod
     def _sum_of(ops, heads):
